@@ -316,6 +316,31 @@ typedef struct jib_scan {
 // single: one token per sequence (row t = sequence t).
 JIB_EXPORT int jib_selective_scan(const jib_scan * m, int single, int f32, void * stream);
 
+// ---- microscaled 4-bit tensors (mx4.cu and its neighbours; the order of packed weights is in mx4.cuh) ------------------------------
+// codes [rows][cols / 2]: two E2M1 values a byte, the lower half first; scales [rows][cols / 32]: E8M0.  cols is a multiple of 32.
+// type: 0 bf16, 1 fp16, 2 fp32.
+JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * codes, void * scales, int rows, int cols, void * stream);
+JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, void * out, int type, long long rows, int cols, void * stream);
+JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, const int * shift, void * out, int batch, int N, int K, long long out_stride,
+                            int step, int first, void * stream);
+// Products of activations with packed weights: out[r][n] = f(sum_k x[r][k] w[n][k]) (+ residual), gated: act(x Wg^T) * (x Wu^T).
+typedef struct jib_mx4_desc {
+    const void * x;            // [rows][K], rows ldx elements apart
+    const void * w;            // packed weights; matrix e starts w_stride bytes behind matrix e - 1
+    const float * w_scale;     // [batch] power of two that goes with matrix e (gated: the gate's)
+    const float * w_scale2;    // [batch] gated: the up matrix's
+    void * out;                // [rows][N], rows ldo elements apart; fp32 with out_f32, else bf16
+    const void * residual;     // NULL or [rows][N], rows ldr elements apart (0: one row for all)
+    const int * seg;           // NULL, or device int[batch + 1]: rows seg[e] .. seg[e + 1] - 1 belong to matrix e
+    const int * src;           // with seg: row r of the result comes from row src[r] of x (NULL: row r)
+    int * status;
+    long long ldx, w_stride, ldo, ldr;
+    int T, N, K, batch, max_rows;          // T: rows of the result; max_rows: the most that one matrix can have
+    int gated, act, out_f32, res_f32;
+    int x_rows;                // rows of x
+} jib_mx4_desc;
+JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, int f32, void * stream);
+
 // ---- expert-parallel all-to-all over peer memory (ep_alltoall.cu); ctx is a JibEpCtx (ep_alltoall.h) ---------
 JIB_EXPORT int jib_ep_plan(const int * ids, int T, int k, const struct JibEpCtx * ctx, int site, int * seg, int * pair_dst, void * stream);
 JIB_EXPORT int jib_ep_push(const void * x, const int * pair_dst, int T, int k, const struct JibEpCtx * ctx, int site, const int * seg,

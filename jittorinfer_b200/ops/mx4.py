@@ -1,0 +1,304 @@
+"""Microscaled 4-bit floating point: tensors, weights laid out for the products, and the operators over them.
+
+A value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) times the power of two that its block of 32 columns shares (E8M0, a
+byte less 127; 255 makes the block NaN).  Activations stay bf16 (or fp32) in ``mx4_linear``, ``mx4_gateup`` and the MoE layers;
+``mx4_matmul`` multiplies two 4-bit operands.  CUDA tensors go to the kernels in ``csrc/kernels/mx4*.cu``, CPU tensors to plain PyTorch; fp32
+activations are multiplied in fp32.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import reference as ref
+
+BLOCK = 32                     # columns that share a scale
+ROWS, COLS, CHUNK = 16, 128, 1088      # a packed chunk: rows, columns, bytes (csrc/kernels/mx4.cuh)
+ACTS = ("silu", "gelu_tanh")
+_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _native(t: torch.Tensor):
+    from . import use_native
+    if not use_native(t):
+        return None
+    from . import nat, native_mx4
+    nat()
+    return native_mx4
+
+
+class Mx4Tensor:
+    """Rows of 4-bit values: ``codes`` uint8 [..., cols / 2] (the lower half of a byte is the even column), ``scales`` uint8 [..., cols / 32]."""
+    __slots__ = ("codes", "scales")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.device != scales.device:
+            raise ValueError("codes and scales are uint8 tensors of one device")
+        if codes.dim() < 2 or codes.shape[-1] == 0 or codes.shape[-1] % (BLOCK // 2) or \
+                tuple(scales.shape) != (*codes.shape[:-1], codes.shape[-1] * 2 // BLOCK):
+            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not blocks of {BLOCK} columns")
+        self.codes, self.scales = codes.contiguous(), scales.contiguous()
+
+    @property
+    def shape(self) -> Tuple[int, ...]:
+        return (*self.codes.shape[:-1], self.codes.shape[-1] * 2)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+class Mx4Weight:
+    """A matrix [n, k], or ``batch`` of them, or as many gated pairs, in the order in which the products read it.  On the GPU ``data`` holds the packed
+    bytes and ``scale`` / ``scale2`` the powers of two that go with each matrix; elsewhere ``plain`` holds the tensors."""
+    __slots__ = ("n", "k", "batch", "gated", "data", "scale", "scale2", "plain")
+
+    def __init__(self, n, k, batch, gated, data=None, scale=None, scale2=None, plain=None):
+        self.n, self.k, self.batch, self.gated = n, k, batch, gated
+        self.data, self.scale, self.scale2, self.plain = data, scale, scale2, plain
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device if self.data is not None else self.plain[0].device
+
+    @property
+    def matrices(self) -> int:
+        return self.batch or 1
+
+    @property
+    def stride(self) -> int:
+        """Bytes of one matrix (or pair) in ``data``."""
+        return (2 if self.gated else 1) * ((self.n + ROWS - 1) // ROWS) * ((self.k + COLS - 1) // COLS) * CHUNK
+
+    def nbytes(self) -> int:
+        if self.data is not None:
+            return self.data.numel() + 4 * self.matrices * (2 if self.gated else 1)
+        return sum(p.nbytes() for p in self.plain)
+
+    def values(self, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, ...]:
+        """The matrices [(batch,) n, k] (a pair: gate, up) as plain tensors."""
+        if self.data is None:
+            return tuple(_dequantize(p, dtype) for p in self.plain)
+        return tuple(_unpack(self, m).to(dtype) for m in range(2 if self.gated else 1))
+
+
+# ---- plain PyTorch ---------------------------------------------------------------------------------------------------------------
+def _pow2(e: torch.Tensor) -> torch.Tensor:
+    """2^e in fp64 for integers e."""
+    return torch.ldexp(torch.ones_like(e, dtype=torch.float64), e)
+
+
+def _quantize(x: torch.Tensor) -> Mx4Tensor:
+    b = x.reshape(*x.shape[:-1], x.shape[-1] // BLOCK, BLOCK).double()
+    top = b.abs().amax(-1)
+    bad = ~torch.isfinite(top)
+    top = torch.where(bad, torch.ones_like(top), top)
+    e = torch.where(top > 0, torch.frexp(top).exponent - 3, torch.full_like(top, -127, dtype=torch.int32)).clamp(-127, 127)
+    y = b * _pow2(-e)[..., None]
+    a = y.abs()
+    a = torch.where(a < 2, torch.round(a * 2), torch.where(a < 4, torch.round(a) * 2, torch.round(a / 2) * 4)).clamp(max=12)       # twice the value
+    code = torch.where(a <= 4, a, torch.where(a == 6, 5.0, torch.where(a == 8, 6.0, 7.0)))
+    code = torch.where(bad[..., None], torch.zeros_like(code), code + 8 * torch.signbit(y)).to(torch.uint8).reshape(*x.shape[:-1], x.shape[-1] // 2, 2)
+    return Mx4Tensor(code[..., 0] | (code[..., 1] << 4), torch.where(bad, torch.full_like(e, 255), e + 127).to(torch.uint8))
+
+
+def _dequantize(q: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
+    table = torch.tensor(_VALUES + tuple(-v for v in _VALUES), dtype=torch.float64, device=q.device)
+    v = torch.stack((table[(q.codes & 15).long()], table[(q.codes >> 4).long()]), -1).reshape(*q.shape[:-1], -1, BLOCK)
+    s = torch.where(q.scales == 255, torch.full_like(q.scales, 0, dtype=torch.float64).fill_(float("nan")), _pow2(q.scales.int() - 127))
+    return (v * s[..., None]).reshape(q.shape).to(dtype)
+
+
+def _unpack(w: Mx4Weight, member: int) -> torch.Tensor:
+    """fp32 [(batch,) n, k] from the packed bytes (the inverse of the kernel that lays them out)."""
+    M, E = (2 if w.gated else 1), w.matrices
+    B, C = (w.n + ROWS - 1) // ROWS, (w.k + COLS - 1) // COLS
+    ch = w.data.view(E, B, M, C, CHUNK)[:, :, member]
+    word = ch[..., :1024].contiguous().view(torch.int32).view(E, B, C, 2, 8, 4, 4).long()       # unit, g, t, i
+    out = torch.zeros(E, B, 2, 8, C, 2, 4, 2, 4, 2, dtype=torch.int64, device=w.data.device)       # half of the rows, g; unit, i, half of the columns, t, parity
+    for par in range(2):
+        h = word >> (16 * par)
+        for j in range(4):
+            if j == 3:
+                code = (h >> 11 & 8) | (h >> 11 & 4) | (h >> 10 & 3)
+            else:
+                code = (h >> (12 - 3 * j) & 8) | (h >> (6 - 3 * j) & 7)
+            # [E, B, C, u, g, t, i] -> [E, B, g, C, u, i, t]
+            out[:, :, j % 2, :, :, :, :, j // 2, :, par] = code.permute(0, 1, 4, 2, 3, 6, 5)
+    table = torch.tensor(_VALUES + tuple(-v for v in _VALUES), dtype=torch.float64, device=w.data.device)
+    v = table[out].view(E, B * ROWS, C, 4, BLOCK)
+    f = ch[..., 1024:].reshape(E, B, C, 8, 2, 4).permute(0, 1, 4, 3, 2, 5).reshape(E, B * ROWS, C, 4).int()
+    s = torch.where(f == 255, torch.full(f.shape, float("nan"), dtype=torch.float64, device=f.device), _pow2(f - 253))
+    s = s * (w.scale, w.scale2)[member].double()[:, None, None, None]
+    m = (v * s[..., None]).view(E, B * ROWS, C * COLS)[:, :w.n, :w.k].float()
+    return m if w.batch else m[0]
+
+
+def _act(z: torch.Tensor, act: str) -> torch.Tensor:
+    return torch.nn.functional.silu(z) if act == "silu" else torch.nn.functional.gelu(z, approximate="tanh")
+
+
+# ---- checks ----------------------------------------------------------------------------------------------------------------------
+def _check_rows(x: torch.Tensor, k: int, what: str) -> None:
+    if x.dim() != 2 or x.shape[1] != k:
+        raise ValueError(f"{what}: activations {tuple(x.shape)} for {k} columns")
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{what}: activations are bf16 or fp32, not {x.dtype}")
+
+
+def _check_weight(x: torch.Tensor, w: Mx4Weight, gated: bool, batched: bool, what: str) -> None:
+    if not isinstance(w, Mx4Weight) or w.gated != gated or (w.batch is not None) != batched:
+        raise ValueError(f"{what}: needs {'a batch of ' if batched else ''}{'gated pairs' if gated else 'matrices'} from mx4_weight")
+    if w.device != x.device:
+        raise ValueError(f"{what}: weights on {w.device}, activations on {x.device}")
+
+
+def _check_residual(residual: Optional[torch.Tensor], rows: int, cols: int, x: torch.Tensor, what: str) -> None:
+    if residual is not None and (tuple(residual.shape) != (rows, cols) or residual.dtype not in (torch.bfloat16, torch.float32) or residual.device != x.device):
+        raise ValueError(f"{what}: residual {tuple(residual.shape)} {residual.dtype} for a result of {(rows, cols)}")
+
+
+def _check_out(out_dtype: Optional[torch.dtype], x_dtype: torch.dtype, what: str) -> torch.dtype:
+    dtype = out_dtype or x_dtype
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{what}: results are bf16 or fp32, not {dtype}")
+    return dtype
+
+
+# ---- operators -------------------------------------------------------------------------------------------------------------------
+def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
+    """bf16, fp16 or fp32 [..., cols] to 4 bits, cols a multiple of 32.  A block's scale is 2^(floor(log2 of its largest magnitude) - 2), at least
+    2^-127; a value goes to the nearest code, ties to the even one, at most 6.  A block with an infinity or NaN becomes NaN."""
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"mx4_quantize: bf16, fp16 or fp32, not {x.dtype}")
+    if x.dim() < 2 or x.shape[-1] == 0 or x.shape[-1] % BLOCK:
+        raise ValueError(f"mx4_quantize: rows of whole blocks of {BLOCK}, not {tuple(x.shape)}")
+    n = _native(x)
+    return n.quantize(x) if n else _quantize(x)
+
+
+def mx4_dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values as bf16, fp16 or fp32 (rounded where the type cannot hold them)."""
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"mx4_dequantize: bf16, fp16 or fp32, not {dtype}")
+    n = _native(q.codes)
+    return n.dequantize(q, dtype) if n else _dequantize(q, dtype)
+
+
+def mx4_weight(q: Mx4Tensor, up: Optional[Mx4Tensor] = None) -> Mx4Weight:
+    """Lays a matrix [n, k] or a batch of them [e, n, k] out for the products, once; with ``up`` a gated pair (gate, up).  The tensors are not needed
+    afterwards (on the CPU they are kept as they are)."""
+    if len(q.shape) not in (2, 3) or 0 in q.shape or (up is not None and (up.shape != q.shape or up.device != q.device)):
+        raise ValueError(f"mx4_weight: {q.shape}" + (f" and {up.shape}" if up is not None else ""))
+    batch = q.shape[0] if len(q.shape) == 3 else None
+    w = Mx4Weight(q.shape[-2], q.shape[-1], batch, up is not None)
+    n = _native(q.codes)
+    if n:
+        n.pack(w, q, up)
+    else:
+        w.plain = (q,) if up is None else (q, up)
+    return w
+
+
+def mx4_linear(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x w^T + residual (bf16 or fp32; one row expanded over the tokens is a bias); ``out_dtype`` bf16 or fp32, default x's."""
+    _check_weight(x, w, False, False, "mx4_linear")
+    _check_rows(x, w.k, "mx4_linear")
+    _check_residual(residual, x.shape[0], w.n, x, "mx4_linear")
+    dtype = _check_out(out_dtype, x.dtype, "mx4_linear")
+    n = _native(x)
+    if n:
+        return n.product(x, w, residual, dtype, None)
+    y = x.float() @ w.values()[0].T
+    return (y if residual is None else y + residual.float()).to(dtype)
+
+
+def mx4_gateup(x: torch.Tensor, w: Mx4Weight, act: str = "silu", out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(x Wg^T) * (x Wu^T); ``act`` "silu" or "gelu_tanh"."""
+    _check_weight(x, w, True, False, "mx4_gateup")
+    _check_rows(x, w.k, "mx4_gateup")
+    if act not in ACTS:
+        raise ValueError(f"mx4_gateup: activation {act!r}, not one of {ACTS}")
+    dtype = _check_out(out_dtype, x.dtype, "mx4_gateup")
+    n = _native(x)
+    if n:
+        return n.product(x, w, None, dtype, act)
+    g, u = w.values()
+    return (_act(x.float() @ g.T, act) * (x.float() @ u.T)).to(dtype)
+
+
+def mx4_matmul(a: Mx4Tensor, b: Mx4Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a b^T for a [t, k] and b [n, k] in 4 bits; the result [t, n] is bf16 or fp32."""
+    if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[1] or a.device != b.device:
+        raise ValueError(f"mx4_matmul: {a.shape} on {a.device} and {b.shape} on {b.device}")
+    dtype = _check_out(out_dtype, torch.bfloat16, "mx4_matmul")
+    n = _native(a.codes)
+    if n:
+        return n.matmul(a, b, dtype)
+    return (_dequantize(a, torch.float32) @ _dequantize(b, torch.float32).T).to(dtype)
+
+
+def _check_moe(x, wgu, wd, residual, act, what):
+    _check_weight(x, wgu, True, True, what)
+    _check_weight(x, wd, False, True, what)
+    _check_rows(x, wgu.k, what)
+    if (wd.n, wd.k, wd.batch) != (wgu.k, wgu.n, wgu.batch):
+        raise ValueError(f"{what}: {wd.batch} down matrices {(wd.n, wd.k)} for {wgu.batch} pairs {(wgu.n, wgu.k)}")
+    if act not in ACTS:
+        raise ValueError(f"{what}: activation {act!r}, not one of {ACTS}")
+    _check_residual(residual, x.shape[0], x.shape[1], x, what)
+    if residual is not None and residual.dtype != x.dtype:
+        raise ValueError(f"{what}: residual {residual.dtype} beside activations {x.dtype}")
+
+
+def _moe_plain(x, residual, ids, wts, wgu, wd, act):
+    g, u = wgu.values()
+    d, = wd.values()
+    out = torch.zeros(x.shape, dtype=torch.float32, device=x.device) if residual is None else residual.float()
+    for e in range(wgu.batch):
+        share = torch.where(ids == e, wts, torch.zeros_like(wts)).sum(-1)
+        rows = torch.nonzero((ids == e).any(-1))[:, 0]
+        if rows.numel():
+            xr = x[rows].float()
+            h = (_act(xr @ g[e].T, act) * (xr @ u[e].T)).to(x.dtype).float()
+            out = out.index_add(0, rows, share[rows, None] * (h @ d[e].T))
+    return out.to(x.dtype)
+
+
+def mx4_moe_ffn(x: torch.Tensor, residual: Optional[torch.Tensor], ids: torch.Tensor, wts: torch.Tensor, wgu: Mx4Weight, wd: Mx4Weight,
+                act: str = "silu") -> torch.Tensor:
+    """residual + sum over the choices of a token of wts * down(act(gate) * up), x's dtype; the hidden units are rounded to x's dtype.
+
+    ``ids`` int32, ``wts`` fp32 [tokens, k]; an id outside the experts counts for nothing.  ``residual`` may be None.  Up to 16 tokens run as one launch."""
+    _check_moe(x, wgu, wd, residual, act, "mx4_moe_ffn")
+    if ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape != wts.shape or ids.dtype != torch.int32 or wts.dtype != torch.float32 or \
+            ids.device != x.device or wts.device != x.device:
+        raise ValueError(f"mx4_moe_ffn: ids {tuple(ids.shape)} {ids.dtype} and weights {tuple(wts.shape)} {wts.dtype} for {x.shape[0]} tokens")
+    n = _native(x)
+    return n.moe_ffn(x, residual, ids.contiguous(), wts.contiguous(), wgu, wd, act) if n else _moe_plain(x, residual, ids, wts, wgu, wd, act)
+
+
+def mx4_moe_layer(x: torch.Tensor, w_router: torch.Tensor, bias: Optional[torch.Tensor], k: int, n_group: int, topk_group: int, scale: float, norm: bool,
+                  sigmoid: bool, wgu: Mx4Weight, wd: Mx4Weight, n_shared: int = 0, group_top2: bool = False,
+                  residual: Optional[torch.Tensor] = None, act: str = "silu") -> torch.Tensor:
+    """A whole MoE layer: router, choice of experts, their products, weighted sum and residual.  The gate's arguments are those of ``moe_gate``; the
+    last ``n_shared`` experts of the weights take every token with weight 1.  Up to 16 bf16 tokens run as two launches."""
+    _check_moe(x, wgu, wd, residual, act, "mx4_moe_layer")
+    E = w_router.shape[0] if w_router.dim() == 2 else -1
+    if w_router.dim() != 2 or w_router.shape[1] != x.shape[1] or E + n_shared != wgu.batch or n_shared < 0 or w_router.dtype != torch.float32 or \
+            w_router.device != x.device:
+        raise ValueError(f"mx4_moe_layer: router {tuple(w_router.shape)} {w_router.dtype} and {n_shared} shared experts for {wgu.batch} of width {x.shape[1]}")
+    if bias is not None and (tuple(bias.shape) != (E,) or bias.dtype != torch.float32 or bias.device != x.device):
+        raise ValueError(f"mx4_moe_layer: bias {tuple(bias.shape)} {bias.dtype} for {E} experts")
+    if not 1 <= k <= E or n_group < 1 or E % n_group or not 1 <= topk_group <= n_group:
+        raise ValueError(f"mx4_moe_layer: {k} of {E} experts in {topk_group} of {n_group} groups")
+    n = _native(x)
+    if n:
+        return n.moe_layer(x, w_router.contiguous(), bias if bias is None else bias.contiguous(), k, n_group, topk_group, scale, norm, sigmoid, wgu, wd,
+                           n_shared, group_top2, residual, act)
+    ids, wts = ref.moe_gate(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, n_shared, group_top2)
+    return _moe_plain(x, residual, ids, wts, wgu, wd, act)

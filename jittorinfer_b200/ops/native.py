@@ -101,6 +101,12 @@ class ScanDesc(C.Structure):
                [(n, C.c_int) for n in ("ch", "N", "n_state", "n_seqs", "T")] + [("out_scale", C.c_float)]
 
 
+class Mx4Desc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "w_scale", "w_scale2", "out", "residual", "seg", "src", "status")] + \
+               [(n, C.c_longlong) for n in ("ldx", "w_stride", "ldo", "ldr")] + \
+               [(n, C.c_int) for n in ("T", "N", "K", "batch", "max_rows", "gated", "act", "out_f32", "res_f32", "x_rows")]
+
+
 def load():
     global _lib
     if _lib is not None:
@@ -153,6 +159,10 @@ def load():
     sig("jib_mla_attention", vp, vp, ip, i, ip, ip, i, i, i, i, i, i, f, i, i, i, fp, fp, vp, vp)
     sig("jib_mla_combine", fp, fp, i, i, i, i, vp, vp)
     sig("jib_mla_flash", vp, vp, ll, ip, i, ip, ip, i, i, i, f, i, i, i, fp, fp, vp, ip, vp)
+    sig("jib_mx4_quantize", vp, i, ll, vp, vp, i, i, vp)
+    sig("jib_mx4_dequantize", vp, vp, vp, i, ll, i, vp)
+    sig("jib_mx4_pack", vp, vp, ip, vp, i, i, i, ll, i, i, vp)
+    sig("jib_mx4_product_simt", C.POINTER(Mx4Desc), i, vp)
     _lib = L
     return L
 

@@ -1,0 +1,134 @@
+"""ctypes front-end of the kernels over microscaled 4-bit tensors (see ``ops.mx4`` for the operators and their checks)."""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import native as nat
+from .mx4 import CHUNK, COLS, ROWS, Mx4Tensor, Mx4Weight
+
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(t: torch.Tensor):
+    """The tensor's device as the current one: launches go to the current device's stream."""
+    return _NO_SWITCH if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def quantize(x: torch.Tensor) -> Mx4Tensor:
+    cols = x.shape[-1]
+    x2 = x if x.dim() == 2 else x.reshape(-1, cols)
+    if x2.stride(1) != 1 or x2.stride(0) < 0:
+        x2 = x2.contiguous()
+    codes = torch.empty(*x.shape[:-1], cols // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*x.shape[:-1], cols // 32, dtype=torch.uint8, device=x.device)
+    with _on(x):
+        nat._ck(nat.load().jib_mx4_quantize(x2.data_ptr(), TYPES[x.dtype], x2.stride(0), codes.data_ptr(), scales.data_ptr(), x2.shape[0], cols,
+                                            nat._stream()), "mx4_quantize")
+    return Mx4Tensor(codes, scales)
+
+
+def dequantize(q: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    with _on(out):
+        nat._ck(nat.load().jib_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), TYPES[dtype], out.numel() // q.shape[-1], q.shape[-1],
+                                              nat._stream()), "mx4_dequantize")
+    return out
+
+
+def pack(w: Mx4Weight, q: Mx4Tensor, up: Optional[Mx4Tensor]) -> None:
+    E = w.matrices
+    w.data = torch.empty(E * w.stride, dtype=torch.uint8, device=q.device)
+    for member, t in enumerate((q,) if up is None else (q, up)):
+        top = t.scales.reshape(E, -1).masked_fill(t.scales.reshape(E, -1) == 255, 0).amax(1).int()
+        shift = (top - 128).clamp(min=0)          # scales above 2 do not fit the byte with their factor of 2^126
+        scale = torch.ldexp(torch.ones(E, device=q.device), shift)
+        with _on(q.codes):
+            nat._ck(nat.load().jib_mx4_pack(t.codes.data_ptr(), t.scales.data_ptr(), shift.data_ptr(), w.data.data_ptr(), E, w.n, w.k, w.stride,
+                                            1 if up is None else 2, member, nat._stream()), "mx4_pack")
+        if member == 0:
+            w.scale = scale
+        else:
+            w.scale2 = scale
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """Rows that the kernels can read: contiguous, 16-byte steps."""
+    ok = x.stride(1) == 1 and x.stride(0) >= x.shape[1] and (x.stride(0) * x.element_size()) % 16 == 0 and x.data_ptr() % 16 == 0
+    return x if ok else x.contiguous()
+
+
+def _desc(x: torch.Tensor, w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act: Optional[str]) -> "nat.Mx4Desc":
+    d = nat.Mx4Desc()
+    d.x, d.ldx, d.x_rows = x.data_ptr(), x.stride(0), x.shape[0]
+    d.w, d.w_stride, d.w_scale, d.w_scale2 = w.data.data_ptr(), w.stride, w.scale.data_ptr(), nat._p(w.scale2)
+    d.out, d.ldo, d.out_f32 = out.data_ptr(), out.stride(0), int(out.dtype == torch.float32)
+    if residual is not None:
+        d.residual, d.ldr, d.res_f32 = residual.data_ptr(), residual.stride(0), int(residual.dtype == torch.float32)
+    d.T, d.N, d.K, d.batch, d.max_rows = out.shape[0], w.n, w.k, 1, out.shape[0]
+    d.gated, d.act = int(w.gated), nat.ACTS[act or "silu"]
+    d.status = nat.workspace(x.device).status.data_ptr()
+    return d
+
+
+def _run(d: "nat.Mx4Desc", x: torch.Tensor, what: str) -> None:
+    nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), int(x.dtype == torch.float32), nat._stream()), what)
+
+
+def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dtype: torch.dtype, act: Optional[str]) -> torch.Tensor:
+    x = _rows(x)
+    out = torch.empty(x.shape[0], w.n, dtype=dtype, device=x.device)
+    if residual is not None and residual.stride(1) != 1:
+        residual = residual.contiguous()
+    if x.shape[0]:
+        with _on(x):
+            _run(_desc(x, w, out, residual, act), x, "mx4_product")
+    return out
+
+
+def grouped(x: torch.Tensor, w: Mx4Weight, seg: torch.Tensor, src: Optional[torch.Tensor], rows: int, max_rows: int, act: Optional[str]) -> torch.Tensor:
+    """Rows sorted by expert: expert e's are seg[e] .. seg[e + 1] - 1; row r is computed from x[src[r]] (without ``src`` x[r])."""
+    out = torch.empty(rows, w.n, dtype=x.dtype, device=x.device)
+    d = _desc(x, w, out, None, act)
+    d.seg, d.src, d.batch, d.max_rows = seg.data_ptr(), nat._p(src), w.batch, max_rows
+    _run(d, x, "mx4_grouped")
+    return out
+
+
+def matmul(a: Mx4Tensor, b: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return product(dequantize(a, torch.float32), _packed(b), None, dtype, None)
+
+
+def _packed(b: Mx4Tensor) -> Mx4Weight:
+    w = Mx4Weight(b.shape[0], b.shape[1], None, False)
+    pack(w, b, None)
+    return w
+
+
+def moe_ffn(x, residual, ids, wts, wgu, wd, act):
+    x = _rows(x)
+    T, k = ids.shape
+    if T == 0:
+        return torch.empty_like(x)
+    with _on(x):
+        seg, src, dest = nat.moe_permute(ids, 0, wgu.batch)
+        h = grouped(x, wgu, seg, src, T * k, T * k, act)
+        y = grouped(h, wd, seg, None, T * k, T * k, None)
+        if x.dtype == torch.bfloat16:
+            return nat.moe_combine(y, dest, wts, None, None if residual is None else residual.contiguous())
+        ok = (dest >= 0).to(wts.dtype) * wts
+        out = (y[dest.clamp(min=0).long()] * ok[..., None]).sum(1)
+        return out if residual is None else out + residual
+
+
+def moe_layer(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, wgu, wd, n_shared, group_top2, residual, act):
+    x = _rows(x)
+    if x.shape[0] == 0:
+        return torch.empty_like(x)
+    with _on(x):
+        ids, wts = nat.moe_gate(x.contiguous(), w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, n_shared, group_top2)
+    return moe_ffn(x, residual, ids, wts, wgu, wd, act)

@@ -317,12 +317,16 @@ typedef struct jib_scan {
 JIB_EXPORT int jib_selective_scan(const jib_scan * m, int single, int f32, void * stream);
 
 // ---- microscaled 4-bit tensors (mx4.cu and its neighbours; the order of packed weights is in mx4.cuh) ------------------------------
-// codes [rows][cols / 2]: two E2M1 values a byte, the lower half first; scales [rows][cols / 32]: E8M0.  cols is a multiple of 32.
+// codes [rows][cols / 2]: two E2M1 values a byte, the lower half first; scales [rows][cols / 32], rows ld_s bytes apart: E8M0.  cols is a
+// multiple of 32.
 // type: 0 bf16, 1 fp16, 2 fp32.
-JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * codes, void * scales, int rows, int cols, void * stream);
-JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, void * out, int type, long long rows, int cols, void * stream);
-JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, const int * shift, void * out, int batch, int N, int K, long long out_stride,
-                            int step, int first, void * stream);
+JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * codes, void * scales, long long ld_s, int rows, int cols, void * stream);
+JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long long ld_s, void * out, int type, long long rows, int cols, void * stream);
+JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, const int * shift, void * out, int batch, int N, int K,
+                            long long out_stride, int step, int first, void * stream);
+// out[t][n] = sum_k a[t][k] b[n][k], both in 4 bits; scale rows are multiples of 8 bytes apart and 8-byte aligned, codes 16-byte aligned.
+JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_scales, long long a_ld, const void * b_codes, const void * b_scales, long long b_ld,
+                              void * out, long long ldo, int out_f32, int T, int N, int K, int * status, void * stream);
 // Products of activations with packed weights: out[r][n] = f(sum_k x[r][k] w[n][k]) (+ residual), gated: act(x Wg^T) * (x Wu^T).
 typedef struct jib_mx4_desc {
     const void * x;            // [rows][K], rows ldx elements apart

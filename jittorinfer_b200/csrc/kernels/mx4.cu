@@ -48,15 +48,15 @@ __device__ __forceinline__ uint32_t to_e2m1(const float (&y)[8]) {
 // 2^-e, exact.  A block with an infinity or NaN gets the scale NaN (255) and codes 0.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_kernel(const T * __restrict__ x, long long ld, uint32_t * __restrict__ codes,
-                                                       uint8_t * __restrict__ scales, long long n8, int per_row, int vec) {
+                                                       uint8_t * __restrict__ scales, long long ld_s, long long n8, int per_row, int vec) {
     PDL_TRIGGER_TOP();
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
     for (long long i0 = (long long) blockIdx.x * blockDim.x; i0 < n8; i0 += (long long) gridDim.x * blockDim.x) {
         const long long i = i0 + threadIdx.x;
+        const long long row = i / per_row;
         float y[8];
         uint32_t top = 0;
         if (i < n8) {
-            const long long row = i / per_row;
             const T * p = x + row * ld + (i - row * per_row) * 8;
             Vec8<T> in;
             if (vec) in = *(const Vec8<T> *) p;
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T * __restrict__ x,
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] *= inv;
         codes[i] = byte == 255 ? 0u : to_e2m1(y);
-        if ((i & 3) == 0) scales[i >> 2] = (uint8_t) byte;
+        if ((i & 3) == 0) scales[row * ld_s + ((i - row * per_row) >> 2)] = (uint8_t) byte;
     }
 }
 
@@ -89,12 +89,13 @@ __device__ __forceinline__ float code_value(uint32_t c) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t * __restrict__ codes, const uint8_t * __restrict__ scales,
-                                                         T * __restrict__ out, long long n8) {
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t * __restrict__ codes, const uint8_t * __restrict__ scales, long long ld_s,
+                                                         T * __restrict__ out, long long n8, int per_row) {
     PDL_TRIGGER_TOP();
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
     for (long long i = (long long) blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += (long long) gridDim.x * blockDim.x) {
-        const uint32_t w = codes[i], s = scales[i >> 2];
+        const long long row = i / per_row;
+        const uint32_t w = codes[i], s = scales[row * ld_s + ((i - row * per_row) >> 2)];
         Vec8<T> o;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -110,24 +111,24 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t * __rest
 // ---- weights: row-major codes to the order of mx4.cuh ----------------------------------------------------------------------------
 // One warp a chunk.  step, first: a gated pair's matrices take every second row block.  shift: one int per matrix.
 __global__ void __launch_bounds__(128) pack_kernel(const uint8_t * __restrict__ codes, const uint8_t * __restrict__ scales,
-                                                   const int * __restrict__ shift, uint8_t * __restrict__ out, int N, int K, long long out_stride,
-                                                   int step, int first) {
+                                                   long long ld_s, const int * __restrict__ shift, uint8_t * __restrict__ out, int N, int K,
+                                                   long long out_stride, int step, int first) {
     const int C = mx4::chunks(K), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const long long id = (long long) blockIdx.x * 4 + (threadIdx.x >> 5);
     if (id >= (long long) mx4::row_blocks(N) * C) return;
     const int b = (int) (id / C), c = (int) (id % C), m = blockIdx.y;
     codes += (size_t) m * N * (K / 2);
-    scales += (size_t) m * N * (K / 32);
+    scales += (size_t) m * N * ld_s;
     uint8_t * dst = out + (size_t) m * out_stride + ((size_t) (b * step + first) * C + c) * mx4::CHUNK;
     const int r0 = b * mx4::ROWS + g, r1 = r0 + 8, k0 = c * mx4::COLS, sh = shift[m];
     auto scale_byte = [&](int r, int blk) -> uint32_t {
         const int kb = k0 / 32 + blk;
         if (r >= N || kb >= K / 32) return 0u;
-        const int e = scales[(size_t) r * (K / 32) + kb];
+        const int e = scales[(size_t) r * ld_s + kb];
         return e == 255 ? 255u : (uint32_t) min(254, max(0, e - sh + 126));
     };
     auto pair = [&](int r, int k) -> uint32_t {       // two codes of row r, columns k and k + 1
-        if (r >= N || k >= K || scales[(size_t) r * (K / 32) + k / 32] == 255) return 0u;
+        if (r >= N || k >= K || scales[(size_t) r * ld_s + k / 32] == 255) return 0u;
         return codes[(size_t) r * (K / 2) + k / 2];
     };
     for (int u = 0; u < 2; ++u) {
@@ -247,42 +248,42 @@ unsigned grid_for(long long items, int per) {
 
 extern "C" {
 
-// x [rows][cols], rows ld elements apart; type 0 bf16, 1 fp16, 2 fp32.  codes [rows][cols / 2], scales [rows][cols / 32].
-JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * codes, void * scales, int rows, int cols, void * stream) {
+// x [rows][cols], rows ld elements apart; type 0 bf16, 1 fp16, 2 fp32.  codes [rows][cols / 2], scales [rows][cols / 32], rows ld_s bytes apart.
+JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * codes, void * scales, long long ld_s, int rows, int cols, void * stream) {
     if (rows <= 0) return 0;
-    if (cols <= 0 || cols % 32 || type < 0 || type > 2) return JIB_E_ARG;
+    if (cols <= 0 || cols % 32 || ld_s < cols / 32 || type < 0 || type > 2) return JIB_E_ARG;
     const int el = type == 2 ? 4 : 2, per_row = cols / 8;
     const long long n8 = (long long) rows * per_row;
     const int vec = ((uintptr_t) x | (uintptr_t) (ld * el)) % (size_t) 16 == 0;
     const unsigned grid = grid_for(n8, 256);
     cudaStream_t s = (cudaStream_t) stream;
-    if (type == 0) JIB_LAUNCH((quantize_kernel<bf16>), grid, 256, 0, s, (const bf16 *) x, ld, (uint32_t *) codes, (uint8_t *) scales, n8, per_row, vec);
-    if (type == 1) JIB_LAUNCH((quantize_kernel<__half>), grid, 256, 0, s, (const __half *) x, ld, (uint32_t *) codes, (uint8_t *) scales, n8, per_row, vec);
-    if (type == 2) JIB_LAUNCH((quantize_kernel<float>), grid, 256, 0, s, (const float *) x, ld, (uint32_t *) codes, (uint8_t *) scales, n8, per_row, vec);
+    if (type == 0) JIB_LAUNCH((quantize_kernel<bf16>), grid, 256, 0, s, (const bf16 *) x, ld, (uint32_t *) codes, (uint8_t *) scales, ld_s, n8, per_row, vec);
+    if (type == 1) JIB_LAUNCH((quantize_kernel<__half>), grid, 256, 0, s, (const __half *) x, ld, (uint32_t *) codes, (uint8_t *) scales, ld_s, n8, per_row, vec);
+    if (type == 2) JIB_LAUNCH((quantize_kernel<float>), grid, 256, 0, s, (const float *) x, ld, (uint32_t *) codes, (uint8_t *) scales, ld_s, n8, per_row, vec);
     return launched();
 }
 
 // The values of `rows` rows, to out [rows][cols] of the type.
-JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, void * out, int type, long long rows, int cols, void * stream) {
+JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long long ld_s, void * out, int type, long long rows, int cols, void * stream) {
     if (rows <= 0) return 0;
-    if (cols <= 0 || cols % 32 || type < 0 || type > 2) return JIB_E_ARG;
+    if (cols <= 0 || cols % 32 || ld_s < cols / 32 || type < 0 || type > 2) return JIB_E_ARG;
     const long long n8 = rows * (cols / 8);
     const unsigned grid = grid_for(n8, 256);
     cudaStream_t s = (cudaStream_t) stream;
-    if (type == 0) JIB_LAUNCH((dequantize_kernel<bf16>), grid, 256, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, (bf16 *) out, n8);
-    if (type == 1) JIB_LAUNCH((dequantize_kernel<__half>), grid, 256, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, (__half *) out, n8);
-    if (type == 2) JIB_LAUNCH((dequantize_kernel<float>), grid, 256, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, (float *) out, n8);
+    if (type == 0) JIB_LAUNCH((dequantize_kernel<bf16>), grid, 256, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, ld_s, (bf16 *) out, n8, cols / 8);
+    if (type == 1) JIB_LAUNCH((dequantize_kernel<__half>), grid, 256, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, ld_s, (__half *) out, n8, cols / 8);
+    if (type == 2) JIB_LAUNCH((dequantize_kernel<float>), grid, 256, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, ld_s, (float *) out, n8, cols / 8);
     return launched();
 }
 
 // Row-major codes and scales of `batch` matrices [N][K] to the order that the products read; shift [batch]; out_stride: bytes of a matrix.
-JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, const int * shift, void * out, int batch, int N, int K, long long out_stride,
+JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, const int * shift, void * out, int batch, int N, int K, long long out_stride,
                             int step, int first, void * stream) {
     if (batch <= 0) return 0;
-    if (N <= 0 || K <= 0 || K % 32 || batch > 65535 || step < 1 || first < 0 || first >= step) return JIB_E_ARG;
+    if (N <= 0 || K <= 0 || K % 32 || ld_s < K / 32 || batch > 65535 || step < 1 || first < 0 || first >= step) return JIB_E_ARG;
     const long long n = (long long) mx4::row_blocks(N) * mx4::chunks(K);
     if ((n + 3) / 4 > 0x7fffffffll || out_stride < n * step * mx4::CHUNK) return JIB_E_ARG;
-    pack_kernel<<<dim3((unsigned) ((n + 3) / 4), batch), 128, 0, (cudaStream_t) stream>>>((const uint8_t *) codes, (const uint8_t *) scales, shift,
+    pack_kernel<<<dim3((unsigned) ((n + 3) / 4), batch), 128, 0, (cudaStream_t) stream>>>((const uint8_t *) codes, (const uint8_t *) scales, ld_s, shift,
                                                                                         (uint8_t *) out, N, K, out_stride, step, first);
     return launched();
 }

@@ -1,0 +1,222 @@
+// Product of two microscaled 4-bit operands on the 4-bit tensor cores: out[t][n] = sum_k a[t][k] b[n][k].
+//
+// tcgen05.mma.kind::mxf4.block_scale multiplies E2M1 codes and applies the blocks' scales itself, 64 columns an instruction: nothing is
+// expanded.  b (the weights) is operand A of the instruction, 128 rows a tile, a's rows are its columns, up to 208 a tile: so few tokens cost
+// a narrow tile.  The scales live in tensor memory: column j of a slab holds, in lane l of every quarter, the four scale bytes of row 32 j + l
+// for 128 columns of K.  Four warps copy them there from global memory, a stage (256 columns, 128 bytes of codes a row) at a time.
+#include "sm100.cuh"
+#include "jib_kernels.h"
+#include "pdl.cuh"
+#include "tma_host.cuh"
+
+namespace {
+
+using namespace sm100;
+typedef __nv_bfloat16 bf16;
+
+constexpr int BM = 128, MAX_BN = 208, STAGES = 4, KS = 256;       // weights a tile, tokens at most, stages, columns a stage
+constexpr int A_BYTES = BM * 128, B_BYTES = MAX_BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int SLAB = 12;                                         // columns of the scales of 128 columns of K: 4 of A, 8 of B
+constexpr int SF0 = 2 * MAX_BN;                                  // two accumulators, then the scales of each stage
+constexpr int THREADS = 384;                                     // producer, issuer, two idle; four scale warps; four epilogue warps
+static_assert(SF0 + STAGES * 2 * SLAB <= 512, "tensor memory");
+
+struct Args {
+    const uint8_t * a_scales, * b_scales;
+    long long a_ld, b_ld;                    // bytes between rows, a multiple of 8
+    void * out;
+    long long ldo;
+    int * status;
+    int T, N, K, bn, out_f32, m_tiles, items;
+};
+
+__device__ __forceinline__ void st_cols4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t) accumulate)
+        : "memory");
+}
+// E2M1 x E2M1 with E8M0 scales, 128 x n, the scales in bytes `half` and `half` + 1 of their words.
+__device__ __forceinline__ uint32_t idesc_mxf4(int n, uint32_t half) {
+    return half << 4 | 1u << 7 | 1u << 10 | (uint32_t) (n >> 3) << 17 | 1u << 23 | (uint32_t) (BM >> 4) << 24 | half << 29;
+}
+
+__global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                                                                const Args g) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t * tiles = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
+    uint64_t * full = (uint64_t *) (tiles + STAGES * STAGE_BYTES), * empty = full + STAGES, * sf_full = empty + STAGES, * acc_full = sf_full + STAGES,
+             * acc_empty = acc_full + 2;
+    uint32_t * tmem_slot = (uint32_t *) (acc_empty + 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&sf_full[i], 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+        fence_barrier_init();
+        prefetch_tmap(&tm_a);
+        prefetch_tmap(&tm_b);
+    }
+    if (warp == 2) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    PDL_TRIGGER_TOP();
+    pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
+    const int n_stages = (g.K + KS - 1) / KS;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int it = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+                const int n0 = item % g.m_tiles * BM, t0 = item / g.m_tiles * g.bn;
+                for (int kb = 0; kb < n_stages; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait(&empty[s], (it / STAGES & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 41, item); ok = false; break; }
+                    uint8_t * st = tiles + s * STAGE_BYTES;
+                    mbar_expect_tx(&full[s], A_BYTES + g.bn * 128);
+                    tma_load_2d(st, &tm_b, &full[s], kb * 128, n0);
+                    tma_load_2d(st + A_BYTES, &tm_a, &full[s], kb * 128, t0);
+                }
+            }
+            // copies in flight end before the memory is given back
+            if (!ok)
+                for (int i = it - STAGES < 0 ? 0 : it - STAGES; i < it; ++i) mbar_wait(&full[i % STAGES], i / STAGES & 1);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t id0 = idesc_mxf4(g.bn, 0), id1 = idesc_mxf4(g.bn, 2);
+            int it = 0, j = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x, ++j) {
+                const int buf = j & 1;
+                if (!mbar_wait(&acc_empty[buf], (j >> 1 & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 42, item); break; }
+                tc_fence_after();
+                const uint32_t acc = tmem + buf * MAX_BN;
+                for (int kb = 0; kb < n_stages; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    const uint32_t ph = it / STAGES & 1;
+                    if (!mbar_wait(&full[s], ph) || !mbar_wait(&sf_full[s], ph)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 43, item); ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t a_addr = smem_u32(tiles + s * STAGE_BYTES), b_addr = a_addr + A_BYTES, sf = tmem + SF0 + s * 2 * SLAB;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        mma_mxf4(acc, desc_k_sw128(a_addr + q * 32), desc_k_sw128(b_addr + q * 32), q & 1 ? id1 : id0, sf + q / 2 * SLAB,
+                                 sf + q / 2 * SLAB + 4, (kb | q) != 0);
+                    mma_commit(&empty[s]);
+                }
+                mma_commit(&acc_full[buf]);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4 && warp < 8) {
+        // scales of a stage: eight bytes a row
+        const uint32_t mine = tmem + ((uint32_t) (warp & 3) << 21) + SF0;
+        const int valid = g.K / 32, b_words = (g.bn + 31) / 32;
+        int it = 0;
+        bool ok = true;
+        for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+            const int n0 = item % g.m_tiles * BM, t0 = item / g.m_tiles * g.bn;
+            for (int kb = 0; kb < n_stages; ++kb, ++it) {
+                const int s = it % STAGES, n = valid - kb * 8;
+                // bytes behind the last block: 1 (the codes there are zero)
+                const uint64_t keep = n >= 8 ? ~0ull : (1ull << (8 * n)) - 1, ones = 0x7f7f7f7f7f7f7f7full & ~keep;
+                uint2 v[12];
+#pragma unroll
+                for (int j = 0; j < 12; ++j) {
+                    const bool of_b = j < 4;
+                    const long long row = of_b ? min(n0 + 32 * j + lane, g.N - 1) : min(t0 + 32 * (j - 4) + lane, g.T - 1);
+                    uint64_t w = 0;
+                    if (of_b || j - 4 < b_words) w = *(const uint64_t *) ((of_b ? g.b_scales + row * g.b_ld : g.a_scales + row * g.a_ld) + kb * 8);
+                    w = (w & keep) | ones;
+                    v[j] = make_uint2((uint32_t) w, (uint32_t) (w >> 32));
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (it / STAGES & 1) ^ 1));
+                if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 44, item); break; }
+                tc_fence_after();
+                const uint32_t dst = mine + s * 2 * SLAB;
+#pragma unroll
+                for (int q = 0; q < 3; ++q) {
+                    st_cols4(dst + 4 * q, v[4 * q].x, v[4 * q + 1].x, v[4 * q + 2].x, v[4 * q + 3].x);
+                    st_cols4(dst + SLAB + 4 * q, v[4 * q].y, v[4 * q + 1].y, v[4 * q + 2].y, v[4 * q + 3].y);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sf_full[s]);
+            }
+        }
+    } else if (warp >= 8) {
+        const uint32_t mine = tmem + ((uint32_t) (warp & 3) << 21);
+        int j = 0;
+        for (int item = blockIdx.x; item < g.items; item += gridDim.x, ++j) {
+            const int n = item % g.m_tiles * BM + (warp & 3) * 32 + lane, t0 = item / g.m_tiles * g.bn, buf = j & 1, cols = min(g.bn, g.T - t0);
+            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], j >> 1 & 1))) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 45, item); break; }
+            tc_fence_after();
+            for (int c = 0; c < cols; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(mine + buf * MAX_BN + c, v);
+                tmem_ld_wait();
+                if (n < g.N)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (c + i >= cols) break;
+                        const long long at = (long long) (t0 + c + i) * g.ldo + n;
+                        if (g.out_f32) ((float *) g.out)[at] = __uint_as_float(v[i]);
+                        else ((bf16 *) g.out)[at] = __float2bfloat16(__uint_as_float(v[i]));
+                    }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace
+
+// a [T][K], b [N][K] in 4 bits: codes row-major and dense, scale rows a_ld / b_ld bytes apart (multiples of 8, the arrays 8-byte aligned).
+extern "C" JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_scales, long long a_ld, const void * b_codes, const void * b_scales,
+                                         long long b_ld, void * out, long long ldo, int out_f32, int T, int N, int K, int * status, void * stream) {
+    if (T <= 0) return 0;
+    if (N <= 0 || K <= 0 || K % 32 || a_ld < K / 32 || b_ld < K / 32) return JIB_E_ARG;
+    if (((uintptr_t) a_scales | (uintptr_t) b_scales | (uintptr_t) a_ld | (uintptr_t) b_ld) & 7) return JIB_E_ALIGN;
+    // The width of a token tile: the one whose rounds over the machine cost least (a tile's fixed part is worth some 24 tokens).
+    const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148, m_tiles = (N + BM - 1) / BM;
+    int bn = 16;
+    long long best = -1;
+    for (int w = 16; w <= MAX_BN; w += 16) {
+        const long long tiles = (long long) m_tiles * ((T + w - 1) / w), cost = (tiles + sms - 1) / sms * (w + 24);
+        if (best < 0 || cost <= best) { best = cost; bn = w; }
+        if (w >= T) break;
+    }
+    Args g;
+    g.a_scales = (const uint8_t *) a_scales; g.b_scales = (const uint8_t *) b_scales; g.a_ld = a_ld; g.b_ld = b_ld;
+    g.out = out; g.ldo = ldo; g.status = status; g.T = T; g.N = N; g.K = K; g.bn = bn; g.out_f32 = out_f32; g.m_tiles = m_tiles;
+    const long long items = (long long) m_tiles * ((T + bn - 1) / bn);
+    if (items > 0x3fffffff) return JIB_E_ARG;
+    g.items = (int) items;
+    CUtensorMap ma, mb;
+    int rc = jib::tma_rows_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a_codes, T, K / 2, K / 2, bn);
+    if (rc) return rc;
+    rc = jib::tma_rows_map(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, b_codes, N, K / 2, K / 2, BM);
+    if (rc) return rc;
+    static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
+    if (!jib::ensure_dyn_smem(mx4_matmul_kernel, SMEM, attr_done)) return JIB_E_LAUNCH;
+    JIB_LAUNCH((mx4_matmul_kernel), (unsigned) (items < sms ? items : sms), THREADS, SMEM, (cudaStream_t) stream, ma, mb, g);
+    return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH;
+}

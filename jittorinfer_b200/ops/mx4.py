@@ -28,8 +28,25 @@ def _native(t: torch.Tensor):
     return native_mx4
 
 
+def scale_rows(lead, blocks: int, device) -> torch.Tensor:
+    """Room for the scales of rows, a view: each row starts at a multiple of 8 bytes."""
+    return torch.empty(*lead, (blocks + 7) // 8 * 8, dtype=torch.uint8, device=device)[..., :blocks]
+
+
+def _laid_out(s: torch.Tensor) -> bool:
+    ld, want = s.stride(-2), s.stride(-2)
+    if s.stride(-1) != 1 or ld % 8 or ld < s.shape[-1] or s.data_ptr() % 8:
+        return False
+    for i in range(s.dim() - 2, -1, -1):
+        if s.stride(i) != want:
+            return False
+        want *= s.shape[i]
+    return True
+
+
 class Mx4Tensor:
-    """Rows of 4-bit values: ``codes`` uint8 [..., cols / 2] (the lower half of a byte is the even column), ``scales`` uint8 [..., cols / 32]."""
+    """Rows of 4-bit values: ``codes`` uint8 [..., cols / 2] (the lower half of a byte is the even column), ``scales`` uint8 [..., cols / 32].  They are kept
+    as the kernels read them: codes dense and 16-byte aligned, scale rows at multiples of 8 bytes; tensors that are otherwise are copied."""
     __slots__ = ("codes", "scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
@@ -38,7 +55,13 @@ class Mx4Tensor:
         if codes.dim() < 2 or codes.shape[-1] == 0 or codes.shape[-1] % (BLOCK // 2) or \
                 tuple(scales.shape) != (*codes.shape[:-1], codes.shape[-1] * 2 // BLOCK):
             raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not blocks of {BLOCK} columns")
-        self.codes, self.scales = codes.contiguous(), scales.contiguous()
+        codes = codes.contiguous()
+        self.codes = codes if codes.data_ptr() % 16 == 0 else codes.clone()
+        if not _laid_out(scales):
+            rows = scale_rows(scales.shape[:-1], scales.shape[-1], scales.device)
+            rows.copy_(scales)
+            scales = rows
+        self.scales = scales
 
     @property
     def shape(self) -> Tuple[int, ...]:

@@ -159,9 +159,10 @@ def load():
     sig("jib_mla_attention", vp, vp, ip, i, ip, ip, i, i, i, i, i, i, f, i, i, i, fp, fp, vp, vp)
     sig("jib_mla_combine", fp, fp, i, i, i, i, vp, vp)
     sig("jib_mla_flash", vp, vp, ll, ip, i, ip, ip, i, i, i, f, i, i, i, fp, fp, vp, ip, vp)
-    sig("jib_mx4_quantize", vp, i, ll, vp, vp, i, i, vp)
-    sig("jib_mx4_dequantize", vp, vp, vp, i, ll, i, vp)
-    sig("jib_mx4_pack", vp, vp, ip, vp, i, i, i, ll, i, i, vp)
+    sig("jib_mx4_quantize", vp, i, ll, vp, vp, ll, i, i, vp)
+    sig("jib_mx4_dequantize", vp, vp, ll, vp, i, ll, i, vp)
+    sig("jib_mx4_pack", vp, vp, ll, ip, vp, i, i, i, ll, i, i, vp)
+    sig("jib_mx4_matmul", vp, vp, ll, vp, vp, ll, vp, ll, i, i, i, i, ip, vp)
     sig("jib_mx4_product_simt", C.POINTER(Mx4Desc), i, vp)
     _lib = L
     return L

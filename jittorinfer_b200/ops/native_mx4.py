@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import native as nat
-from .mx4 import CHUNK, COLS, ROWS, Mx4Tensor, Mx4Weight
+from .mx4 import Mx4Tensor, Mx4Weight, scale_rows
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _NO_SWITCH = contextlib.nullcontext()
@@ -25,9 +25,9 @@ def quantize(x: torch.Tensor) -> Mx4Tensor:
     if x2.stride(1) != 1 or x2.stride(0) < 0:
         x2 = x2.contiguous()
     codes = torch.empty(*x.shape[:-1], cols // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(*x.shape[:-1], cols // 32, dtype=torch.uint8, device=x.device)
+    scales = scale_rows(x.shape[:-1], cols // 32, x.device)
     with _on(x):
-        nat._ck(nat.load().jib_mx4_quantize(x2.data_ptr(), TYPES[x.dtype], x2.stride(0), codes.data_ptr(), scales.data_ptr(), x2.shape[0], cols,
+        nat._ck(nat.load().jib_mx4_quantize(x2.data_ptr(), TYPES[x.dtype], x2.stride(0), codes.data_ptr(), scales.data_ptr(), scales.stride(-2), x2.shape[0], cols,
                                             nat._stream()), "mx4_quantize")
     return Mx4Tensor(codes, scales)
 
@@ -35,7 +35,7 @@ def quantize(x: torch.Tensor) -> Mx4Tensor:
 def dequantize(q: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
     with _on(out):
-        nat._ck(nat.load().jib_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), TYPES[dtype], out.numel() // q.shape[-1], q.shape[-1],
+        nat._ck(nat.load().jib_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), q.scales.stride(-2), out.data_ptr(), TYPES[dtype], out.numel() // q.shape[-1], q.shape[-1],
                                               nat._stream()), "mx4_dequantize")
     return out
 
@@ -48,7 +48,7 @@ def pack(w: Mx4Weight, q: Mx4Tensor, up: Optional[Mx4Tensor]) -> None:
         shift = (top - 128).clamp(min=0)          # scales above 2 do not fit the byte with their factor of 2^126
         scale = torch.ldexp(torch.ones(E, device=q.device), shift)
         with _on(q.codes):
-            nat._ck(nat.load().jib_mx4_pack(t.codes.data_ptr(), t.scales.data_ptr(), shift.data_ptr(), w.data.data_ptr(), E, w.n, w.k, w.stride,
+            nat._ck(nat.load().jib_mx4_pack(t.codes.data_ptr(), t.scales.data_ptr(), t.scales.stride(-2), shift.data_ptr(), w.data.data_ptr(), E, w.n, w.k, w.stride,
                                             1 if up is None else 2, member, nat._stream()), "mx4_pack")
         if member == 0:
             w.scale = scale
@@ -100,13 +100,15 @@ def grouped(x: torch.Tensor, w: Mx4Weight, seg: torch.Tensor, src: Optional[torc
 
 
 def matmul(a: Mx4Tensor, b: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
-    return product(dequantize(a, torch.float32), _packed(b), None, dtype, None)
-
-
-def _packed(b: Mx4Tensor) -> Mx4Weight:
-    w = Mx4Weight(b.shape[0], b.shape[1], None, False)
-    pack(w, b, None)
-    return w
+    T, K = a.shape
+    N = b.shape[0]
+    out = torch.empty(T, N, dtype=dtype, device=a.device)
+    if T and N:
+        with _on(out):
+            nat._ck(nat.load().jib_mx4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), a.scales.stride(0), b.codes.data_ptr(), b.scales.data_ptr(),
+                                              b.scales.stride(0), out.data_ptr(), N, int(dtype == torch.float32), T, N, K,
+                                              nat.workspace(out.device).status.data_ptr(), nat._stream()), "mx4_matmul")
+    return out
 
 
 def moe_ffn(x, residual, ids, wts, wgu, wd, act):

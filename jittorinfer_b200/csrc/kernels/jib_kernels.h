@@ -344,6 +344,25 @@ typedef struct jib_mx4_desc {
     int x_rows;                // rows of x
 } jib_mx4_desc;
 JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, int f32, void * stream);
+// A mixture-of-experts layer for up to 16 tokens (mx4_moe.cu).
+typedef struct jib_mx4_moe_desc {
+    const void * x, * residual;            // bf16 [T][d], rows ldx / ldr elements apart; residual may be NULL
+    const float * logits, * bias;          // router outputs [T][E - n_shared] and the bias of the choice (or NULL); logits NULL: ids and wts
+    const int * ids;                       // [T][k]
+    const float * wts;
+    const void * gu, * down;               // packed pairs [E][F][d], packed matrices [E][d][F]
+    const float * gu_scale, * gu_scale2, * down_scale;      // [E]
+    void * h, * out;                       // scratch; bf16 [T][d]
+    float * part;                          // scratch
+    int * sync;                            // zeros
+    int * status;
+    long long ldx, ldr, gu_stride, down_stride, h_bytes, part_floats, sync_ints;
+    int T, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act;
+    float scale;
+} jib_mx4_moe_desc;
+JIB_EXPORT int jib_mx4_moe_sizes(int T, int d, int F, int E, int k, long long * h_bytes, long long * part_floats, long long * sync_ints);
+JIB_EXPORT int jib_mx4_moe_router(const void * x, const float * w_router, float * logits, int * sync, int n_sync, int T, int d, int E, void * stream);
+JIB_EXPORT int jib_mx4_moe(const jib_mx4_moe_desc * m, void * stream);
 
 // ---- expert-parallel all-to-all over peer memory (ep_alltoall.cu); ctx is a JibEpCtx (ep_alltoall.h) ---------
 JIB_EXPORT int jib_ep_plan(const int * ids, int T, int k, const struct JibEpCtx * ctx, int site, int * seg, int * pair_dst, void * stream);

@@ -9,7 +9,7 @@
 #include <stdint.h>
 
 #include "jib_kernels.h"
-#include "mx4.cuh"
+#include "mx4_stream.cuh"
 #include "pdl.cuh"
 
 namespace {
@@ -153,11 +153,6 @@ __global__ void __launch_bounds__(128) pack_kernel(const uint8_t * __restrict__ 
 // A warp holds one row block (of a pair: two) for eight rows of x; a lane multiplies its weights of rows g and g + 8, four lanes share a row.
 constexpr int ST = 8;
 
-__device__ __forceinline__ float gated(float z, float u, int act) {
-    const float a = act == JIB_ACT_GELU_TANH ? 1.5957691216057308f * (z + 0.044715f * z * z * z) : z;
-    return z / (1.f + expf(-a)) * u;
-}
-
 template <typename T, bool PAIR>
 __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
     PDL_TRIGGER_TOP();
@@ -224,7 +219,7 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
             const int n = b * mx4::ROWS + 8 * h + g;
             if (t != 0 || j >= nt || n >= d.N) continue;
             const long long r = base + t0 + j;
-            float y = PAIR ? gated(s[0] * ws, s[M - 1] * ws2, d.act) : s[0] * ws;
+            float y = PAIR ? mx4::gated(s[0] * ws, s[M - 1] * ws2, d.act) : s[0] * ws;
             if (d.residual != nullptr) {
                 const long long ri = r * d.ldr + n;
                 y += d.res_f32 ? ((const float *) d.residual)[ri] : to_f(((const bf16 *) d.residual)[ri]);

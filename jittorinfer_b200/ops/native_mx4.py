@@ -11,6 +11,8 @@ from . import native as nat
 from .mx4 import Mx4Tensor, Mx4Weight, scale_rows
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+FEW_TOKENS = 16                              # tokens of a layer that runs as one launch behind the router's
+MAX_EXPERTS, MAX_CHOICES, ROUTER_WIDTH = 256, 32, 8192       # what the gate and the sort take (csrc/kernels/moe.cu, gate.cuh)
 _NO_SWITCH = contextlib.nullcontext()
 
 
@@ -111,12 +113,52 @@ def matmul(a: Mx4Tensor, b: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
+_few_sizes: dict = {}        # (tokens, width, hidden, experts, choices) -> bytes of h, floats of part, ints of sync, or None
+
+
+def _few(x: torch.Tensor, wgu: Mx4Weight, k: int):
+    """The buffers' sizes where a layer of few tokens runs as one launch."""
+    if x.dtype != torch.bfloat16 or x.shape[0] > FEW_TOKENS:
+        return None
+    key = (x.shape[0], wgu.k, wgu.n, wgu.batch, k)
+    if key not in _few_sizes:
+        s = [C.c_longlong() for _ in range(3)]
+        _few_sizes[key] = tuple(v.value for v in s) if nat.load().jib_mx4_moe_sizes(*key, *(C.byref(v) for v in s)) else None
+    return _few_sizes[key]
+
+
+def _few_desc(x, residual, wgu: Mx4Weight, wd: Mx4Weight, sizes, sync, act: str):
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    scratch = torch.empty(sizes[0] + 4 * sizes[1], dtype=torch.uint8, device=x.device)
+    m = nat.Mx4MoeDesc()
+    m.x, m.ldx, m.out, m.h, m.part = x.data_ptr(), x.stride(0), out.data_ptr(), scratch.data_ptr(), scratch.data_ptr() + sizes[0]
+    if residual is not None:
+        m.residual, m.ldr = residual.data_ptr(), residual.stride(0)
+    m.gu, m.gu_stride, m.gu_scale, m.gu_scale2 = wgu.data.data_ptr(), wgu.stride, wgu.scale.data_ptr(), wgu.scale2.data_ptr()
+    m.down, m.down_stride, m.down_scale = wd.data.data_ptr(), wd.stride, wd.scale.data_ptr()
+    m.sync, m.status = sync.data_ptr(), nat.workspace(x.device).status.data_ptr()
+    m.h_bytes, m.part_floats, m.sync_ints = sizes
+    m.T, m.d, m.F, m.E, m.act = x.shape[0], wgu.k, wgu.n, wgu.batch, nat.ACTS[act]
+    return m, out, scratch
+
+
 def moe_ffn(x, residual, ids, wts, wgu, wd, act):
     x = _rows(x)
     T, k = ids.shape
     if T == 0:
         return torch.empty_like(x)
+    if residual is not None and residual.stride(1) != 1:
+        residual = residual.contiguous()
+    if wgu.batch > MAX_EXPERTS:
+        raise ValueError(f"mx4_moe_ffn: {wgu.batch} experts, at most {MAX_EXPERTS}")
     with _on(x):
+        sizes = _few(x, wgu, k)
+        if sizes is not None:
+            sync = torch.zeros(sizes[2], dtype=torch.int32, device=x.device)
+            m, out, keep = _few_desc(x, residual, wgu, wd, sizes, sync, act)      # noqa: F841
+            m.ids, m.wts, m.k = ids.data_ptr(), wts.data_ptr(), k
+            nat._ck(nat.load().jib_mx4_moe(C.byref(m), nat._stream()), "mx4_moe")
+            return out
         seg, src, dest = nat.moe_permute(ids, 0, wgu.batch)
         h = grouped(x, wgu, seg, src, T * k, T * k, act)
         y = grouped(h, wd, seg, None, T * k, T * k, None)
@@ -129,8 +171,26 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act):
 
 def moe_layer(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, wgu, wd, n_shared, group_top2, residual, act):
     x = _rows(x)
-    if x.shape[0] == 0:
+    T, d = x.shape
+    if T == 0:
         return torch.empty_like(x)
+    if k + n_shared > MAX_CHOICES or wgu.batch > MAX_EXPERTS or n_group > 32:
+        raise ValueError(f"mx4_moe_layer: {k} + {n_shared} of {wgu.batch} experts in {n_group} groups; at most {MAX_CHOICES} of {MAX_EXPERTS} in 32")
     with _on(x):
+        sizes = _few(x, wgu, k + n_shared) if d <= ROUTER_WIDTH else None
+        if sizes is not None:
+            E = w_router.shape[0]
+            if residual is not None and residual.stride(1) != 1:
+                residual = residual.contiguous()
+            x = x if x.stride(0) == d else x.contiguous()
+            sync = torch.empty(sizes[2], dtype=torch.int32, device=x.device)
+            logits = torch.empty(T, E, dtype=torch.float32, device=x.device)
+            m, out, keep = _few_desc(x, residual, wgu, wd, sizes, sync, act)      # noqa: F841
+            m.logits, m.bias, m.k, m.n_group, m.topk_group, m.scale = logits.data_ptr(), nat._p(bias), k, n_group, topk_group, scale
+            m.norm, m.sigmoid, m.n_shared, m.group_top2 = int(norm), int(sigmoid), n_shared, int(group_top2)
+            L, stream = nat.load(), nat._stream()
+            nat._ck(L.jib_mx4_moe_router(x.data_ptr(), w_router.data_ptr(), logits.data_ptr(), sync.data_ptr(), sizes[2], T, d, E, stream), "mx4_moe_router")
+            nat._ck(L.jib_mx4_moe(C.byref(m), stream), "mx4_moe")
+            return out
         ids, wts = nat.moe_gate(x.contiguous(), w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, n_shared, group_top2)
     return moe_ffn(x, residual, ids, wts, wgu, wd, act)

@@ -322,7 +322,7 @@ JIB_EXPORT int jib_selective_scan(const jib_scan * m, int single, int f32, void 
 // type: 0 bf16, 1 fp16, 2 fp32.
 JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * codes, void * scales, long long ld_s, int rows, int cols, void * stream);
 JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long long ld_s, void * out, int type, long long rows, int cols, void * stream);
-JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, const int * shift, void * out, int batch, int N, int K,
+JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, int * exps, void * out, int batch, int N, int K,
                             long long out_stride, int step, int first, void * stream);
 // out[t][n] = sum_k a[t][k] b[n][k], both in 4 bits; scale rows are multiples of 8 bytes apart and 8-byte aligned, codes 16-byte aligned.
 JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_scales, long long a_ld, const void * b_codes, const void * b_scales, long long b_ld,
@@ -331,8 +331,7 @@ JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_scales, long 
 typedef struct jib_mx4_desc {
     const void * x;            // [rows][K], rows ldx elements apart
     const void * w;            // packed weights; matrix e starts w_stride bytes behind matrix e - 1
-    const float * w_scale;     // [batch] power of two that goes with matrix e (gated: the gate's)
-    const float * w_scale2;    // [batch] gated: the up matrix's
+    const int * w_exp;         // exponents of its rows, in the order of the packed row blocks
     void * out;                // [rows][N], rows ldo elements apart; fp32 with out_f32, else bf16
     const void * residual;     // NULL or [rows][N], rows ldr elements apart (0: one row for all)
     const int * seg;           // NULL, or device int[batch + 1]: rows seg[e] .. seg[e + 1] - 1 belong to matrix e
@@ -346,22 +345,24 @@ typedef struct jib_mx4_desc {
 JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, int f32, void * stream);
 // A mixture-of-experts layer for up to 16 tokens (mx4_moe.cu).
 typedef struct jib_mx4_moe_desc {
-    const void * x, * residual;            // bf16 [T][d], rows ldx / ldr elements apart; residual may be NULL
+    const void * residual;                 // NULL, or bf16 [T][d], rows ldr elements apart
     const float * logits, * bias;          // router outputs [T][E - n_shared] and the bias of the choice (or NULL); logits NULL: ids and wts
     const int * ids;                       // [T][k]
     const float * wts;
     const void * gu, * down;               // packed pairs [E][F][d], packed matrices [E][d][F]
-    const float * gu_scale, * gu_scale2, * down_scale;      // [E]
+    const int * gu_exp, * down_exp;        // exponents of their rows
+    void * xf;                             // what jib_mx4_moe_prepare made of x
     void * h, * out;                       // scratch; bf16 [T][d]
     float * part;                          // scratch
     int * sync;                            // zeros
     int * status;
-    long long ldx, ldr, gu_stride, down_stride, h_bytes, part_floats, sync_ints;
+    long long ldr, gu_stride, down_stride;
     int T, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act;
     float scale;
 } jib_mx4_moe_desc;
-JIB_EXPORT int jib_mx4_moe_sizes(int T, int d, int F, int E, int k, long long * h_bytes, long long * part_floats, long long * sync_ints);
-JIB_EXPORT int jib_mx4_moe_router(const void * x, const float * w_router, float * logits, int * sync, int n_sync, int T, int d, int E, void * stream);
+JIB_EXPORT int jib_mx4_moe_sizes(int T, int d, int F, int E, int k, long long * sizes);
+JIB_EXPORT int jib_mx4_moe_prepare(const void * x, long long ldx, const float * w_router, float * logits, void * xf, int * sync, int n_sync, int T, int d, int E,
+                                   void * stream);
 JIB_EXPORT int jib_mx4_moe(const jib_mx4_moe_desc * m, void * stream);
 
 // ---- expert-parallel all-to-all over peer memory (ep_alltoall.cu); ctx is a JibEpCtx (ep_alltoall.h) ---------

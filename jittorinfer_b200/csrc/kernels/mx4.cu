@@ -109,24 +109,35 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t * __rest
 }
 
 // ---- weights: row-major codes to the order of mx4.cuh ----------------------------------------------------------------------------
-// One warp a chunk.  step, first: a gated pair's matrices take every second row block.  shift: one int per matrix.
+// Exponents of the rows: the largest scale of a row less 127 and TOP (a row without a number: of scale 1).  One warp a row; step, first: a
+// gated pair's matrices take every second row block.
+__global__ void __launch_bounds__(128) row_exponent_kernel(const uint8_t * __restrict__ scales, long long ld_s, int * __restrict__ exps, int N, int K, int step,
+                                                           int first) {
+    const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5), m = blockIdx.y, rows = mx4::row_blocks(N) * mx4::ROWS;
+    if (r >= rows) return;
+    int top = -1;
+    if (r < N)
+        for (int i = lane; i < K / 32; i += 32) {
+            const int e = scales[((size_t) m * N + r) * ld_s + i];
+            if (e != 255) top = max(top, e);
+        }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) exps[((size_t) m * (rows / mx4::ROWS) * step + (r / mx4::ROWS) * step + first) * mx4::ROWS + r % mx4::ROWS] = (top < 0 ? 127 : top) - 127 - mx4::TOP;
+}
+
+// One warp a chunk.
 __global__ void __launch_bounds__(128) pack_kernel(const uint8_t * __restrict__ codes, const uint8_t * __restrict__ scales,
-                                                   long long ld_s, const int * __restrict__ shift, uint8_t * __restrict__ out, int N, int K,
+                                                   long long ld_s, const int * __restrict__ exps, uint8_t * __restrict__ out, int N, int K,
                                                    long long out_stride, int step, int first) {
     const int C = mx4::chunks(K), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const long long id = (long long) blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (id >= (long long) mx4::row_blocks(N) * C) return;
+    const int B = mx4::row_blocks(N);
+    if (id >= (long long) B * C) return;
     const int b = (int) (id / C), c = (int) (id % C), m = blockIdx.y;
     codes += (size_t) m * N * (K / 2);
     scales += (size_t) m * N * ld_s;
     uint8_t * dst = out + (size_t) m * out_stride + ((size_t) (b * step + first) * C + c) * mx4::CHUNK;
-    const int r0 = b * mx4::ROWS + g, r1 = r0 + 8, k0 = c * mx4::COLS, sh = shift[m];
-    auto scale_byte = [&](int r, int blk) -> uint32_t {
-        const int kb = k0 / 32 + blk;
-        if (r >= N || kb >= K / 32) return 0u;
-        const int e = scales[(size_t) r * ld_s + kb];
-        return e == 255 ? 255u : (uint32_t) min(254, max(0, e - sh + 126));
-    };
+    const int r0 = b * mx4::ROWS + g, r1 = r0 + 8, k0 = c * mx4::COLS;
     auto pair = [&](int r, int k) -> uint32_t {       // two codes of row r, columns k and k + 1
         if (r >= N || k >= K || scales[(size_t) r * ld_s + k / 32] == 255) return 0u;
         return codes[(size_t) r * (K / 2) + k / 2];
@@ -135,16 +146,19 @@ __global__ void __launch_bounds__(128) pack_kernel(const uint8_t * __restrict__ 
         uint32_t w[4];
         for (int i = 0; i < 4; ++i) {
             const int k = k0 + 64 * u + 16 * i + 2 * t;
-            const uint32_t p[4] = {pair(r0, k), pair(r1, k), pair(r0, k + 8), pair(r1, k + 8)};
-            w[i] = 0;
-            for (int j = 0; j < 4; ++j) w[i] |= mx4::place(p[j] & 15, j) | mx4::place(p[j] >> 4, j) << 16;
+            w[i] = pair(r0, k) | pair(r1, k) << 8 | pair(r0, k + 8) << 16 | pair(r1, k + 8) << 24;
         }
         ((uint4 *) dst)[u * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
     }
     if (t < 2) {
-        const int r = t == 0 ? r0 : r1;
+        const int r = t == 0 ? r0 : r1, top = exps[((size_t) m * B * step + b * step + first) * mx4::ROWS + r % mx4::ROWS] + 127 + mx4::TOP;
         uint32_t f = 0;
-        for (int blk = 0; blk < 4; ++blk) f |= scale_byte(r, blk) << (8 * blk);
+        for (int blk = 0; blk < 4; ++blk) {
+            const int kb = k0 / 32 + blk;
+            if (r >= N || kb >= K / 32) continue;
+            const int e = scales[(size_t) r * ld_s + kb];
+            f |= (uint32_t) (e == 255 ? 31 : max(0, 15 + mx4::TOP - (top - e))) << (8 * blk + 2);
+        }
         ((uint32_t *) (dst + mx4::SCALES))[g * 2 + t] = f;
     }
 }
@@ -176,6 +190,13 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
         xr[j] = (const T *) d.x + (d.src != nullptr ? (long long) d.src[r] : r) * d.ldx;
     }
     const uint8_t * w = (const uint8_t *) d.w + (size_t) e * d.w_stride + (size_t) b * M * C * mx4::CHUNK;
+    const int * ex = d.w_exp + ((size_t) e * mx4::row_blocks(d.N) + b) * M * mx4::ROWS;
+    float unit[M][2];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        unit[m][0] = mx4::pow2(ex[m * mx4::ROWS + g]);
+        unit[m][1] = mx4::pow2(ex[m * mx4::ROWS + g + 8]);
+    }
     float acc[M][2][ST] = {};
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -193,7 +214,11 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
                     mx4::decode(word[i], mx4::scale2(f.x, 2 * u + i / 2), mx4::scale2(f.y, 2 * u + i / 2), a);
                     float2 v[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = __bfloat1622float2(*(const __nv_bfloat162 *) &a[j]);
+                    for (int j = 0; j < 4; ++j) {
+                        v[j] = __half22float2(*(const __half2 *) &a[j]);
+                        v[j].x *= unit[m][j & 1];
+                        v[j].y *= unit[m][j & 1];
+                    }
 #pragma unroll
                     for (int j = 0; j < ST; ++j) {
                         if (j >= nt) break;
@@ -204,7 +229,6 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
                 }
             }
         }
-    const float ws = d.w_scale[e], ws2 = PAIR ? d.w_scale2[e] : 1.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -219,7 +243,7 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
             const int n = b * mx4::ROWS + 8 * h + g;
             if (t != 0 || j >= nt || n >= d.N) continue;
             const long long r = base + t0 + j;
-            float y = PAIR ? mx4::gated(s[0] * ws, s[M - 1] * ws2, d.act) : s[0] * ws;
+            float y = PAIR ? mx4::gated(s[0], s[M - 1], d.act) : s[0];
             if (d.residual != nullptr) {
                 const long long ri = r * d.ldr + n;
                 y += d.res_f32 ? ((const float *) d.residual)[ri] : to_f(((const bf16 *) d.residual)[ri]);
@@ -271,15 +295,18 @@ JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long 
     return launched();
 }
 
-// Row-major codes and scales of `batch` matrices [N][K] to the order that the products read; shift [batch]; out_stride: bytes of a matrix.
-JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, const int * shift, void * out, int batch, int N, int K, long long out_stride,
+// Row-major codes and scales of `batch` matrices [N][K] to the order that the products read; exps [batch][row blocks * step][16]; out_stride:
+// bytes of a matrix.
+JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, int * exps, void * out, int batch, int N, int K, long long out_stride,
                             int step, int first, void * stream) {
     if (batch <= 0) return 0;
     if (N <= 0 || K <= 0 || K % 32 || ld_s < K / 32 || batch > 65535 || step < 1 || first < 0 || first >= step) return JIB_E_ARG;
     const long long n = (long long) mx4::row_blocks(N) * mx4::chunks(K);
     if ((n + 3) / 4 > 0x7fffffffll || out_stride < n * step * mx4::CHUNK) return JIB_E_ARG;
-    pack_kernel<<<dim3((unsigned) ((n + 3) / 4), batch), 128, 0, (cudaStream_t) stream>>>((const uint8_t *) codes, (const uint8_t *) scales, ld_s, shift,
-                                                                                        (uint8_t *) out, N, K, out_stride, step, first);
+    cudaStream_t s = (cudaStream_t) stream;
+    row_exponent_kernel<<<dim3(mx4::row_blocks(N) * 4, batch), 128, 0, s>>>((const uint8_t *) scales, ld_s, exps, N, K, step, first);
+    pack_kernel<<<dim3((unsigned) ((n + 3) / 4), batch), 128, 0, s>>>((const uint8_t *) codes, (const uint8_t *) scales, ld_s, exps, (uint8_t *) out, N, K,
+                                                                     out_stride, step, first);
     return launched();
 }
 

@@ -77,12 +77,12 @@ class Mx4Tensor:
 
 class Mx4Weight:
     """A matrix [n, k], or ``batch`` of them, or as many gated pairs, in the order in which the products read it.  On the GPU ``data`` holds the packed
-    bytes and ``scale`` / ``scale2`` the powers of two that go with each matrix; elsewhere ``plain`` holds the tensors."""
-    __slots__ = ("n", "k", "batch", "gated", "data", "scale", "scale2", "plain")
+    bytes and ``exps`` the exponents of its rows; elsewhere ``plain`` holds the tensors."""
+    __slots__ = ("n", "k", "batch", "gated", "data", "exps", "plain")
 
-    def __init__(self, n, k, batch, gated, data=None, scale=None, scale2=None, plain=None):
+    def __init__(self, n, k, batch, gated):
         self.n, self.k, self.batch, self.gated = n, k, batch, gated
-        self.data, self.scale, self.scale2, self.plain = data, scale, scale2, plain
+        self.data = self.exps = self.plain = None
 
     @property
     def device(self) -> torch.device:
@@ -93,13 +93,17 @@ class Mx4Weight:
         return self.batch or 1
 
     @property
+    def row_blocks(self) -> int:
+        return (self.n + ROWS - 1) // ROWS
+
+    @property
     def stride(self) -> int:
         """Bytes of one matrix (or pair) in ``data``."""
-        return (2 if self.gated else 1) * ((self.n + ROWS - 1) // ROWS) * ((self.k + COLS - 1) // COLS) * CHUNK
+        return (2 if self.gated else 1) * self.row_blocks * ((self.k + COLS - 1) // COLS) * CHUNK
 
     def nbytes(self) -> int:
         if self.data is not None:
-            return self.data.numel() + 4 * self.matrices * (2 if self.gated else 1)
+            return self.data.numel() + 4 * self.exps.numel()
         return sum(p.nbytes() for p in self.plain)
 
     def values(self, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, ...]:
@@ -138,26 +142,16 @@ def _dequantize(q: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 def _unpack(w: Mx4Weight, member: int) -> torch.Tensor:
     """fp32 [(batch,) n, k] from the packed bytes (the inverse of the kernel that lays them out)."""
-    M, E = (2 if w.gated else 1), w.matrices
-    B, C = (w.n + ROWS - 1) // ROWS, (w.k + COLS - 1) // COLS
+    M, E, B, C = (2 if w.gated else 1), w.matrices, w.row_blocks, (w.k + COLS - 1) // COLS
     ch = w.data.view(E, B, M, C, CHUNK)[:, :, member]
-    word = ch[..., :1024].contiguous().view(torch.int32).view(E, B, C, 2, 8, 4, 4).long()       # unit, g, t, i
-    out = torch.zeros(E, B, 2, 8, C, 2, 4, 2, 4, 2, dtype=torch.int64, device=w.data.device)       # half of the rows, g; unit, i, half of the columns, t, parity
-    for par in range(2):
-        h = word >> (16 * par)
-        for j in range(4):
-            if j == 3:
-                code = (h >> 11 & 8) | (h >> 11 & 4) | (h >> 10 & 3)
-            else:
-                code = (h >> (12 - 3 * j) & 8) | (h >> (6 - 3 * j) & 7)
-            # [E, B, C, u, g, t, i] -> [E, B, g, C, u, i, t]
-            out[:, :, j % 2, :, :, :, :, j // 2, :, par] = code.permute(0, 1, 4, 2, 3, 6, 5)
+    # unit, g, t, step, half of the columns, half of the rows -> half of the rows, g; chunk, unit, step, half of the columns, t
+    byte = ch[..., :1024].reshape(E, B, C, 2, 8, 4, 4, 2, 2).permute(0, 1, 8, 4, 2, 3, 6, 7, 5)
+    code = torch.stack((byte & 15, byte >> 4), -1).reshape(E, B * ROWS, C, 4, BLOCK)
     table = torch.tensor(_VALUES + tuple(-v for v in _VALUES), dtype=torch.float64, device=w.data.device)
-    v = table[out].view(E, B * ROWS, C, 4, BLOCK)
-    f = ch[..., 1024:].reshape(E, B, C, 8, 2, 4).permute(0, 1, 4, 3, 2, 5).reshape(E, B * ROWS, C, 4).int()
-    s = torch.where(f == 255, torch.full(f.shape, float("nan"), dtype=torch.float64, device=f.device), _pow2(f - 253))
-    s = s * (w.scale, w.scale2)[member].double()[:, None, None, None]
-    m = (v * s[..., None]).view(E, B * ROWS, C * COLS)[:, :w.n, :w.k].float()
+    f = ch[..., 1024:].reshape(E, B, C, 8, 2, 4).permute(0, 1, 4, 3, 2, 5).reshape(E, B * ROWS, C, 4).int() >> 2
+    s = torch.where(f == 31, torch.full(f.shape, float("nan"), dtype=torch.float64, device=f.device), torch.where(f > 0, _pow2(f - 15), torch.zeros_like(_pow2(f))))
+    s = s * _pow2(w.exps.view(E, B, M, ROWS)[:, :, member]).reshape(E, B * ROWS, 1, 1)
+    m = (table[code.long()] * s[..., None]).view(E, B * ROWS, C * COLS)[:, :w.n, :w.k].float()
     return m if w.batch else m[0]
 
 

@@ -102,15 +102,14 @@ class ScanDesc(C.Structure):
 
 
 class Mx4Desc(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "w_scale", "w_scale2", "out", "residual", "seg", "src", "status")] + \
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "w_exp", "out", "residual", "seg", "src", "status")] + \
                [(n, C.c_longlong) for n in ("ldx", "w_stride", "ldo", "ldr")] + \
                [(n, C.c_int) for n in ("T", "N", "K", "batch", "max_rows", "gated", "act", "out_f32", "res_f32", "x_rows")]
 
 
 class Mx4MoeDesc(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("x", "residual", "logits", "bias", "ids", "wts", "gu", "down", "gu_scale", "gu_scale2", "down_scale", "h", "out", "part",
-                                          "sync", "status")] + \
-               [(n, C.c_longlong) for n in ("ldx", "ldr", "gu_stride", "down_stride", "h_bytes", "part_floats", "sync_ints")] + \
+    _fields_ = [(n, C.c_void_p) for n in ("residual", "logits", "bias", "ids", "wts", "gu", "down", "gu_exp", "down_exp", "xf", "h", "out", "part", "sync", "status")] + \
+               [(n, C.c_longlong) for n in ("ldr", "gu_stride", "down_stride")] + \
                [(n, C.c_int) for n in ("T", "d", "F", "E", "k", "n_group", "topk_group", "norm", "sigmoid", "n_shared", "group_top2", "act")] + [("scale", C.c_float)]
 
 
@@ -171,8 +170,8 @@ def load():
     sig("jib_mx4_pack", vp, vp, ll, ip, vp, i, i, i, ll, i, i, vp)
     sig("jib_mx4_matmul", vp, vp, ll, vp, vp, ll, vp, ll, i, i, i, i, ip, vp)
     sig("jib_mx4_product_simt", C.POINTER(Mx4Desc), i, vp)
-    sig("jib_mx4_moe_sizes", i, i, i, i, i, C.POINTER(ll), C.POINTER(ll), C.POINTER(ll))
-    sig("jib_mx4_moe_router", vp, fp, fp, ip, i, i, i, i, vp)
+    sig("jib_mx4_moe_sizes", i, i, i, i, i, C.POINTER(ll))
+    sig("jib_mx4_moe_prepare", vp, ll, fp, fp, vp, ip, i, i, i, i, vp)
     sig("jib_mx4_moe", C.POINTER(Mx4MoeDesc), vp)
     _lib = L
     return L

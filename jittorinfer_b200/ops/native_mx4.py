@@ -8,11 +8,11 @@ from typing import Optional
 import torch
 
 from . import native as nat
-from .mx4 import Mx4Tensor, Mx4Weight, scale_rows
+from .mx4 import ROWS, Mx4Tensor, Mx4Weight, scale_rows
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 FEW_TOKENS = 16                              # tokens of a layer that runs as one launch behind the router's
-MAX_EXPERTS, MAX_CHOICES, ROUTER_WIDTH = 256, 32, 8192       # what the gate and the sort take (csrc/kernels/moe.cu, gate.cuh)
+MAX_EXPERTS, MAX_CHOICES = 256, 32           # what the gate and the sort take (csrc/kernels/moe.cu)
 _NO_SWITCH = contextlib.nullcontext()
 
 
@@ -43,19 +43,13 @@ def dequantize(q: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 
 def pack(w: Mx4Weight, q: Mx4Tensor, up: Optional[Mx4Tensor]) -> None:
-    E = w.matrices
+    E, members = w.matrices, (q,) if up is None else (q, up)
     w.data = torch.empty(E * w.stride, dtype=torch.uint8, device=q.device)
-    for member, t in enumerate((q,) if up is None else (q, up)):
-        top = t.scales.reshape(E, -1).masked_fill(t.scales.reshape(E, -1) == 255, 0).amax(1).int()
-        shift = (top - 128).clamp(min=0)          # scales above 2 do not fit the byte with their factor of 2^126
-        scale = torch.ldexp(torch.ones(E, device=q.device), shift)
-        with _on(q.codes):
-            nat._ck(nat.load().jib_mx4_pack(t.codes.data_ptr(), t.scales.data_ptr(), t.scales.stride(-2), shift.data_ptr(), w.data.data_ptr(), E, w.n, w.k, w.stride,
-                                            1 if up is None else 2, member, nat._stream()), "mx4_pack")
-        if member == 0:
-            w.scale = scale
-        else:
-            w.scale2 = scale
+    w.exps = torch.empty(E, w.row_blocks * len(members), ROWS, dtype=torch.int32, device=q.device)
+    with _on(q.codes):
+        for m, t in enumerate(members):
+            nat._ck(nat.load().jib_mx4_pack(t.codes.data_ptr(), t.scales.data_ptr(), t.scales.stride(-2), w.exps.data_ptr(), w.data.data_ptr(), E, w.n, w.k,
+                                            w.stride, len(members), m, nat._stream()), "mx4_pack")
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -67,7 +61,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 def _desc(x: torch.Tensor, w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act: Optional[str]) -> "nat.Mx4Desc":
     d = nat.Mx4Desc()
     d.x, d.ldx, d.x_rows = x.data_ptr(), x.stride(0), x.shape[0]
-    d.w, d.w_stride, d.w_scale, d.w_scale2 = w.data.data_ptr(), w.stride, w.scale.data_ptr(), nat._p(w.scale2)
+    d.w, d.w_stride, d.w_exp = w.data.data_ptr(), w.stride, w.exps.data_ptr()
     d.out, d.ldo, d.out_f32 = out.data_ptr(), out.stride(0), int(out.dtype == torch.float32)
     if residual is not None:
         d.residual, d.ldr, d.res_f32 = residual.data_ptr(), residual.stride(0), int(residual.dtype == torch.float32)
@@ -113,33 +107,41 @@ def matmul(a: Mx4Tensor, b: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
-_few_sizes: dict = {}        # (tokens, width, hidden, experts, choices) -> bytes of h, floats of part, ints of sync, or None
+_few_sizes: dict = {}        # (tokens, width, hidden, experts, choices) -> bytes of xf and h, floats of part, ints of sync, or None
 
 
 def _few(x: torch.Tensor, wgu: Mx4Weight, k: int):
-    """The buffers' sizes where a layer of few tokens runs as one launch."""
+    """The buffers' sizes where a layer of few tokens runs as two launches."""
     if x.dtype != torch.bfloat16 or x.shape[0] > FEW_TOKENS:
         return None
     key = (x.shape[0], wgu.k, wgu.n, wgu.batch, k)
     if key not in _few_sizes:
-        s = [C.c_longlong() for _ in range(3)]
-        _few_sizes[key] = tuple(v.value for v in s) if nat.load().jib_mx4_moe_sizes(*key, *(C.byref(v) for v in s)) else None
+        s = (C.c_longlong * 4)()
+        _few_sizes[key] = tuple(s) if nat.load().jib_mx4_moe_sizes(*key, s) else None
     return _few_sizes[key]
 
 
-def _few_desc(x, residual, wgu: Mx4Weight, wd: Mx4Weight, sizes, sync, act: str):
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    scratch = torch.empty(sizes[0] + 4 * sizes[1], dtype=torch.uint8, device=x.device)
-    m = nat.Mx4MoeDesc()
-    m.x, m.ldx, m.out, m.h, m.part = x.data_ptr(), x.stride(0), out.data_ptr(), scratch.data_ptr(), scratch.data_ptr() + sizes[0]
+def _few_layer(x, residual, wgu: Mx4Weight, wd: Mx4Weight, sizes, act: str, m, w_router: Optional[torch.Tensor]) -> torch.Tensor:
+    """Both launches; ``m`` holds what says which experts."""
+    T, d = x.shape
+    xf, h, part, sync = sizes
+    out = torch.empty(T, d, dtype=x.dtype, device=x.device)
+    E = w_router.shape[0] if w_router is not None else 0
+    scratch = torch.empty(xf + h + 4 * (part + sync + T * E), dtype=torch.uint8, device=x.device)
+    m.out, m.xf = out.data_ptr(), scratch.data_ptr()
+    m.h, m.part, m.sync = m.xf + xf, m.xf + xf + h, m.xf + xf + h + 4 * part
+    if E:
+        m.logits = m.sync + 4 * sync
     if residual is not None:
         m.residual, m.ldr = residual.data_ptr(), residual.stride(0)
-    m.gu, m.gu_stride, m.gu_scale, m.gu_scale2 = wgu.data.data_ptr(), wgu.stride, wgu.scale.data_ptr(), wgu.scale2.data_ptr()
-    m.down, m.down_stride, m.down_scale = wd.data.data_ptr(), wd.stride, wd.scale.data_ptr()
-    m.sync, m.status = sync.data_ptr(), nat.workspace(x.device).status.data_ptr()
-    m.h_bytes, m.part_floats, m.sync_ints = sizes
-    m.T, m.d, m.F, m.E, m.act = x.shape[0], wgu.k, wgu.n, wgu.batch, nat.ACTS[act]
-    return m, out, scratch
+    m.gu, m.gu_stride, m.gu_exp = wgu.data.data_ptr(), wgu.stride, wgu.exps.data_ptr()
+    m.down, m.down_stride, m.down_exp = wd.data.data_ptr(), wd.stride, wd.exps.data_ptr()
+    m.status = nat.workspace(x.device).status.data_ptr()
+    m.T, m.d, m.F, m.E, m.act = T, d, wgu.n, wgu.batch, nat.ACTS[act]
+    L, stream = nat.load(), nat._stream()
+    nat._ck(L.jib_mx4_moe_prepare(x.data_ptr(), x.stride(0), nat._p(w_router), m.logits, m.xf, m.sync, sync, T, d, E, stream), "mx4_moe_prepare")
+    nat._ck(L.jib_mx4_moe(C.byref(m), stream), "mx4_moe")
+    return out
 
 
 def moe_ffn(x, residual, ids, wts, wgu, wd, act):
@@ -154,11 +156,9 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act):
     with _on(x):
         sizes = _few(x, wgu, k)
         if sizes is not None:
-            sync = torch.zeros(sizes[2], dtype=torch.int32, device=x.device)
-            m, out, keep = _few_desc(x, residual, wgu, wd, sizes, sync, act)      # noqa: F841
+            m = nat.Mx4MoeDesc()
             m.ids, m.wts, m.k = ids.data_ptr(), wts.data_ptr(), k
-            nat._ck(nat.load().jib_mx4_moe(C.byref(m), nat._stream()), "mx4_moe")
-            return out
+            return _few_layer(x, residual, wgu, wd, sizes, act, m, None)
         seg, src, dest = nat.moe_permute(ids, 0, wgu.batch)
         h = grouped(x, wgu, seg, src, T * k, T * k, act)
         y = grouped(h, wd, seg, None, T * k, T * k, None)
@@ -177,20 +177,14 @@ def moe_layer(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, w
     if k + n_shared > MAX_CHOICES or wgu.batch > MAX_EXPERTS or n_group > 32:
         raise ValueError(f"mx4_moe_layer: {k} + {n_shared} of {wgu.batch} experts in {n_group} groups; at most {MAX_CHOICES} of {MAX_EXPERTS} in 32")
     with _on(x):
-        sizes = _few(x, wgu, k + n_shared) if d <= ROUTER_WIDTH else None
+        x = x if x.stride(0) == d else x.contiguous()
+        sizes = _few(x, wgu, k + n_shared)
         if sizes is not None:
-            E = w_router.shape[0]
             if residual is not None and residual.stride(1) != 1:
                 residual = residual.contiguous()
-            x = x if x.stride(0) == d else x.contiguous()
-            sync = torch.empty(sizes[2], dtype=torch.int32, device=x.device)
-            logits = torch.empty(T, E, dtype=torch.float32, device=x.device)
-            m, out, keep = _few_desc(x, residual, wgu, wd, sizes, sync, act)      # noqa: F841
-            m.logits, m.bias, m.k, m.n_group, m.topk_group, m.scale = logits.data_ptr(), nat._p(bias), k, n_group, topk_group, scale
+            m = nat.Mx4MoeDesc()
+            m.bias, m.k, m.n_group, m.topk_group, m.scale = nat._p(bias), k, n_group, topk_group, scale
             m.norm, m.sigmoid, m.n_shared, m.group_top2 = int(norm), int(sigmoid), n_shared, int(group_top2)
-            L, stream = nat.load(), nat._stream()
-            nat._ck(L.jib_mx4_moe_router(x.data_ptr(), w_router.data_ptr(), logits.data_ptr(), sync.data_ptr(), sizes[2], T, d, E, stream), "mx4_moe_router")
-            nat._ck(L.jib_mx4_moe(C.byref(m), stream), "mx4_moe")
-            return out
-        ids, wts = nat.moe_gate(x.contiguous(), w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, n_shared, group_top2)
+            return _few_layer(x, residual, wgu, wd, sizes, act, m, w_router)
+        ids, wts = nat.moe_gate(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, n_shared, group_top2)
     return moe_ffn(x, residual, ids, wts, wgu, wd, act)

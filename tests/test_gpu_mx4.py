@@ -30,7 +30,8 @@ def weights(*shape, seed=0, scale=0.02):
 
 def within(got, want, lim):
     err = (got.double() - want).abs()
-    assert bool((err <= lim).all()), f"{float((err / lim).max()):.3g} of the limit at {tuple(torch.nonzero(err > lim)[0].tolist())}"
+    bad = ~(err <= lim)
+    assert not bool(bad.any()), f"{float((err / lim)[bad].max()):.3g} of the limit at {torch.nonzero(bad)[0].tolist()}, {int(bad.sum())} of {bad.numel()}"
 
 
 def product_limit(x, w, want, dtype):

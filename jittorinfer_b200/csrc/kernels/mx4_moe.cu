@@ -4,18 +4,17 @@
 // The reference runs router, choice, sorting, grouped products and the weighted sum as some dozen launches
 // (src/llama-graph-ffn.cpp:145-260); the bf16 path here takes five.
 //
-// The layer is bound by the stream of the chosen experts' weights, so the second launch is one stream: every CTA draws units from a counter,
-// first 32 hidden units of an expert (rows of gate and up), then 64 rows of down over a share of the chosen experts' hidden units.  A unit of the
-// second kind needs hidden units that other CTAs store: an expert's counter says how many of its gate and up units are done.  Units are drawn
-// in order and a CTA works them off in order, those of the first kind never wait, so whatever a unit waits for is being worked on: the
-// launch ends however few of its CTAs run at a time.
-// A stage is NP places along K times four row blocks (gate, up, gate, up; or four of down), and a place's activations.  Roles: 2 NP warps
-// multiply two row blocks each at one place, each with its own ring of weights that it keeps filled with asynchronous copies; one thread draws
-// units; one warp waits for hidden units and copies them to shared memory; FIN warps take turns in adding a unit's NP sums up, in the
-// order of the warps, and finishing its rows.  Sums of shares meet in memory, the share that comes last adds them up in their order.
-// Five roles in one kernel are much code, and what runs beside one another has to stay in the instruction cache: waits are short loops, what one thread
-// can work out for all (the drawing one) is worked out once, and only the products are unrolled.  (With every wait and index in line the kernel
-// was 140 KB and took twice the time.)
+// The layer is bound by the stream of the chosen experts' weights, and on the way by instructions: a weight has 2.8 issue slots at the memory's rate.  So
+// the second launch is two plain loops over chunks and a meeting of its CTAs in between; every warp is alike, and keeps a ring of weights of its
+// own filled with asynchronous copies.  (Versions with units drawn one by one, special warps for copies and sums, and waits for single
+// experts' hidden units overlapped more and took twice the time: their code did not stay in the instruction cache.)
+//
+// Gate and up: GW warps share 16 hidden units of an expert, each a part of K, and add their sums up in order in shared memory.  Hidden units go to
+// memory as fragments, fp16, each 16 of a token scaled by a power of two that is kept beside them.  A part of this loop (one part for each CTA) is
+// drawn from a counter, so that every part is done by a CTA that runs; a CTA draws until there is none left and then waits for all
+// parts: nothing waits for a CTA that has not started.
+// Down: the chunks of 64 rows x all chosen experts' hidden units are one line, cut into equal pieces, one for each CTA.  Where a piece ends inside 64
+// rows, the sums meet in memory, and the CTA that comes last adds them up in their order.
 #include "gate.cuh"
 #include "jib_kernels.h"
 #include "mx4_stream.cuh"
@@ -26,10 +25,10 @@ namespace {
 using namespace sm100;
 
 constexpr int MAX_T = 16, MAX_K = 32;                         // tokens, choices of a token
-constexpr int MAX_SHARES = 24, MOST_SMEM = 227 * 1024;
+constexpr int NW = 16, THREADS = NW * 32;                     // warps
+constexpr int MOST_SMEM = 227 * 1024, MAX_DEPTH = 4;
 constexpr int BIAS = 113;                                     // top_exponent() + BIAS is 1 .. 240
-constexpr uint64_t WAIT_NS = JIB_WAIT_NS;                     // for hidden units that another CTA stores
-constexpr int NP = 8, NW = 2 * NP;                            // places of a stage; multiplying warps
+constexpr uint64_t WAIT_NS = JIB_WAIT_NS;                     // for the other CTAs' hidden units
 
 struct MoeArgs {
     const bf16 * residual;                   // may be NULL
@@ -41,39 +40,32 @@ struct MoeArgs {
     const int * gu_exp, * down_exp;
     __half * h;                              // hidden units: [slot][chunks of F][NT] fragments, each 16 of a token scaled by a power of two ...
     uint8_t * h_exp;                         // ... [slot][chunk][token][step], BIAS more than its exponent
-    float * part;                            // [d / 64][shares][512 NT]
+    float * part;                            // [pieces][512 NT]
     bf16 * out;
-    int * sync;                              // zeros: next unit (and three more), done gate and up units of each slot [MAX_E], the largest byte of h_exp of
-                                             // each slot and token [slots][16], shares done of each 64 rows
+    int * sync;                              // zeros: parts of gate and up drawn, parts done (and two more), the largest byte of h_exp of each slot and token
+                                             // [slots][16], pieces done of each 64 rows
     int * status;
     long long ldr, gu_stride, down_stride;
-    int T, max_slots, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act, shares, ring, depth;
+    int T, max_slots, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act, gw, depth1, depth2, warm;
     float scale;
 };
 
-// A drawn unit, in shared memory.
-struct Unit {
-    const uint8_t * weights;      // of its first row block: of the expert's pairs; or of the first expert's matrix of down
-    int id, n;                    // id -1: the end; places along K
-    int slot, col;                // of down: the first place's expert and chunk
-};
-
-// Shared memory: the tokens' fragments; a ring of stages' hidden units (for each place fragments, their exponents' bytes, the exponents of 64 rows, the
-// largest bytes of 16 tokens); sums; tables; barriers.
+// Shared memory: tables; sums, twice; then for gate and up the tokens' fragments and the warps' rings of chunks, for down the warps' rings of chunks with
+// their hidden units (fragments, the exponents' bytes, the exponents of 32 rows, the largest bytes of 16 tokens).
 template <int NT>
 struct Layout {
-    static constexpr int FIN = 2;                                 // finishing warps, each with a buffer of sums
-    static constexpr int THREADS = (NW + 2 + FIN) * 32;
-    static constexpr int H_EXP = NP * NT * mx4::FRAG, H_ROW = H_EXP + NP * NT * 64, H_TOP = H_ROW + NP * 256, HID = H_TOP + NP * 64;
     static constexpr int SUMS = 8 * NT;                           // of a lane
-    static constexpr int RED = NW * 32 * SUMS * 4;                // one unit's sums of every warp
-    static constexpr int MAX_RING = 3, QUEUE = 2;                 // stages of hidden units; units drawn and not begun by all
-    static constexpr int DEEP = NW * 2 * mx4::CHUNK, MAX_DEPTH = 4;       // weights of a stage; stages asked for ahead
-    static constexpr int BARS = 16 + (2 * MAX_RING + 2 * QUEUE + 2 * FIN + 1) * 8 + QUEUE * (int) sizeof(Unit) + (FIN + 1) * 4;
-    static_assert(FIN * RED >= 8 * (MAX_E + 32) * 4, "scratch of the choice");
+    static constexpr int RED = NW * 32 * SUMS * 4;
+    static constexpr int G_SLOT = 2 * mx4::CHUNK;
+    static constexpr int H_EXP = G_SLOT + NT * mx4::FRAG, H_ROW = H_EXP + NT * 64, H_TOP = H_ROW + 128, D_SLOT = H_TOP + 64;
+    static_assert(2 * RED >= NW * (MAX_E + 32) * 4, "scratch of the choice");
     __host__ __device__ static int frags(int d) { return mx4::chunks(d) * NT * mx4::FRAG; }
-    __host__ __device__ static int tables(int slots) { return slots * 64 + MAX_E * 4 * 3 + MAX_T * MAX_K * 8; }
-    __host__ __device__ static int bytes(int d, int slots, int ring, int depth) { return 128 + depth * DEEP + ring * HID + frags(d) + FIN * RED + tables(slots) + BARS; }
+    __host__ __device__ static int tables(int slots) { return (slots * 64 + MAX_E * 4 * 3 + MAX_T * MAX_K * 8 + 64 + 127) / 128 * 128; }
+    __host__ __device__ static int base(int slots) { return 128 + tables(slots) + 2 * RED; }
+    __host__ __device__ static int bytes(int d, int slots, int depth1, int depth2) {
+        const int a = frags(d) + NW * depth1 * G_SLOT, b = NW * depth2 * D_SLOT;
+        return base(slots) + (a > b ? a : b);
+    }
 };
 
 // 2^-n in fp16, twice (n below 0, from a byte that no hidden unit goes with, counts as 0)
@@ -90,61 +82,55 @@ __device__ __forceinline__ int ld_acquire(const int * p) {
 }
 
 template <int NT>
-__global__ void __launch_bounds__(Layout<NT>::THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
+__global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     using L = Layout<NT>;
-    constexpr int FIN = L::FIN;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t * ring = (uint8_t *) (((uintptr_t) smem_raw + 127) & ~(uintptr_t) 127);
-    uint8_t * acts = ring + g.ring * L::HID, * weights = (uint8_t *) (((uintptr_t) smem_raw + L::bytes(g.d, g.max_slots, g.ring, 0) - 1) & ~(uintptr_t) 15);
-    float * red = (float *) (acts + L::frags(g.d));
-    float * wtab = red + FIN * L::RED / 4;                         // [slot][16] weight of each token, 0: not chosen
+    uint8_t * base = (uint8_t *) (((uintptr_t) smem_raw + 127) & ~(uintptr_t) 127);
+    float * wtab = (float *) base;                                 // [slot][16] weight of each token, 0: not chosen
     int * slot_of = (int *) (wtab + g.max_slots * 16), * expert_of = slot_of + MAX_E, * mask = expert_of + MAX_E;
     int * ids_s = mask + MAX_E;
     float * wts_s = (float *) (ids_s + MAX_T * MAX_K);
-    float * sel = red, * gscore = red + 8 * MAX_E;                 // the choice's scratch, before the first sums
-    uint64_t * hid_full = (uint64_t *) (wts_s + MAX_T * MAX_K), * hid_empty = hid_full + L::MAX_RING;
-    uint64_t * drawn = hid_empty + L::MAX_RING, * worked = drawn + L::QUEUE, * red_full = worked + L::QUEUE, * red_empty = red_full + FIN;
-    uint64_t * acts_full = red_empty + FIN;
-    Unit * queue = (Unit *) (acts_full + 1);
-    int * red_unit = (int *) (queue + L::QUEUE), * n_slots_s = red_unit + FIN;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = g.ring;
+    uint64_t * acts_full = (uint64_t *) (wts_s + MAX_T * MAX_K);
+    int * word = (int *) (acts_full + 1);                          // [0] slots, [1] part drawn, [2] pieces done
+    float * red = (float *) (base + L::tables(g.max_slots));
+    uint8_t * work = (uint8_t *) (red + 2 * L::RED / 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t2 = 2 * (lane & 3);
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < R; ++i) { mbar_init(&hid_full[i], 1); mbar_init(&hid_empty[i], NW); }
-        for (int i = 0; i < L::QUEUE; ++i) { mbar_init(&drawn[i], 1); mbar_init(&worked[i], NW + 1); }
         mbar_init(acts_full, 1);
-        for (int i = 0; i < FIN; ++i) { mbar_init(&red_full[i], NW); mbar_init(&red_empty[i], 1); }
         fence_barrier_init();
     }
-    for (int i = threadIdx.x; i < g.max_slots * 16; i += L::THREADS) wtab[i] = 0.f;
-    for (int i = threadIdx.x; i < MAX_E; i += L::THREADS) { slot_of[i] = 0; mask[i] = 0; }
+    for (int i = threadIdx.x; i < g.max_slots * 16; i += THREADS) wtab[i] = 0.f;
+    for (int i = threadIdx.x; i < MAX_E; i += THREADS) { slot_of[i] = 0; mask[i] = 0; }
     __syncthreads();
     PDL_TRIGGER_TOP();
+    if (g.warm && g.logits != nullptr && warp == 0)      // the choice's code (33 KB) comes to the SM while the launch before this one runs
+        gate_token(nullptr, nullptr, nullptr, nullptr, 0, g.E - g.n_shared, g.k, g.n_group, g.topk_group, g.scale, g.norm, g.sigmoid, g.n_shared, g.group_top2,
+                   red, red + MAX_E, ids_s, wts_s, true);
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
-    int first_unit = 0;
-    if (threadIdx.x == NW * 32) {          // the drawing thread: its first unit, the tokens' fragments
-        first_unit = atomicAdd(g.sync, 1);
+    if (threadIdx.x == THREADS - 1) {
+        word[1] = atomicAdd(g.sync, 1);
         mbar_expect_tx(acts_full, L::frags(g.d));
-        mx4::bulk_load(acts, g.xf, L::frags(g.d), acts_full);
+        mx4::bulk_load(work, g.xf, L::frags(g.d), acts_full);
     }
 
     // ---- which experts, for which tokens, with which weights ----
     const int kk = g.k + g.n_shared;
     if (g.logits != nullptr) {
         const int E = g.E - g.n_shared;
-        if (warp < 8)
-            for (int t = warp; t < g.T; t += 8)
-                gate_token(g.logits + (size_t) t * E, g.bias, nullptr, nullptr, t, E, g.k, g.n_group, g.topk_group, g.scale, g.norm, g.sigmoid, g.n_shared,
-                           g.group_top2, sel + warp * MAX_E, gscore + warp * 32, ids_s, wts_s);
+        if (warp < g.T)
+            gate_token(g.logits + (size_t) warp * E, g.bias, nullptr, nullptr, warp, E, g.k, g.n_group, g.topk_group, g.scale, g.norm, g.sigmoid, g.n_shared,
+                       g.group_top2, red + warp * (MAX_E + 32), red + warp * (MAX_E + 32) + MAX_E, ids_s, wts_s);
     } else {
-        for (int i = threadIdx.x; i < g.T * kk; i += L::THREADS) { ids_s[i] = g.ids[i]; wts_s[i] = g.wts[i]; }
+        for (int i = threadIdx.x; i < g.T * kk; i += THREADS) { ids_s[i] = g.ids[i]; wts_s[i] = g.wts[i]; }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < g.T * kk; i += L::THREADS)
+    for (int i = threadIdx.x; i < g.T * kk; i += THREADS)
         if ((unsigned) ids_s[i] < (unsigned) g.E) slot_of[ids_s[i]] = 1;
     __syncthreads();
     if (warp == 0) {
         int n = 0;
+#pragma unroll 1
         for (int e = lane; e < MAX_E; e += 32) {
             const bool hit = slot_of[e] != 0;
             const unsigned m = __ballot_sync(0xffffffffu, hit);
@@ -153,9 +139,10 @@ __global__ void __launch_bounds__(Layout<NT>::THREADS, 1) mx4_moe_kernel(const M
             if (hit) expert_of[s] = e;
             n += __popc(m);
         }
-        if (lane == 0) *n_slots_s = n;
+        if (lane == 0) word[0] = n;
         __syncwarp();
         if (lane < g.T)
+#pragma unroll 1
             for (int j = 0; j < kk; ++j) {
                 const int e = ids_s[lane * kk + j];
                 if ((unsigned) e >= (unsigned) g.E) continue;
@@ -164,411 +151,289 @@ __global__ void __launch_bounds__(Layout<NT>::THREADS, 1) mx4_moe_kernel(const M
             }
     }
     __syncthreads();
-    const int slots = *n_slots_s, C1 = mx4::chunks(g.d), C2 = mx4::chunks(g.F), UPE = g.F / 32, RB2 = g.d / 16, UPS = (g.d + 63) / 64;
-    const int P = slots * C2, shares = min(g.shares, max(1, (P + NP - 1) / NP));      // a share is a stage at least
-    const int U1 = slots * UPE, U = U1 + UPS * shares;
-    int * done = g.sync + 4, * h_top = done + MAX_E, * shares_done = h_top + g.max_slots * 16;
+    const int slots = word[0], C1 = mx4::chunks(g.d), C2 = mx4::chunks(g.F), RB1 = g.F / 16, RB2 = g.d / 16, G = gridDim.x;
+    int * done = g.sync + 1, * h_top = g.sync + 4, * pieces_done = h_top + g.max_slots * 16;
+    const uint64_t policy = l2_policy_evict_first();
 
-    if (warp == NW) {
-        // ---- units ----
-        if (lane == 0)
+    // ---- gate and up: a part at a time ----
+    if (!mx4::wait_all(acts_full, 0) && lane == 0) jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 51, warp);
+    {
+        const int U = slots * RB1, groups = NW / g.gw, wg = warp % g.gw, depth = g.depth1;
+        const uint8_t * ring = work + L::frags(g.d) + warp * depth * L::G_SLOT;
+        const uint32_t ring_s = smem_u32(ring);
+        const uint4 * acts = (const uint4 *) work + lane;
+        const size_t apart = (size_t) C1 * mx4::CHUNK;
+        int parity = 0;
 #pragma unroll 1
-            for (int i = 0;; ++i) {
-                const int q = i % L::QUEUE, id = i == 0 ? first_unit : atomicAdd(g.sync, 1);
-                if (!mx4::wait(&worked[q], (i / L::QUEUE & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 51, i); break; }
-                Unit & u = queue[q];
-                u.id = id < U ? id : -1;
-                if (id < U1) {
-                    u.n = C1;
-                    u.slot = u.col = 0;
-                    u.weights = g.gu + (size_t) expert_of[id / UPE] * g.gu_stride + (size_t) (id % UPE) * 4 * C1 * mx4::CHUNK;
-                } else if (id < U) {
-                    const int share = (id - U1) % shares, lo = share * P / shares;
-                    u.n = (share + 1) * P / shares - lo;
-                    u.slot = lo / C2;
-                    u.col = lo % C2;
-                    u.weights = g.down + (size_t) ((id - U1) / shares) * 4 * C2 * mx4::CHUNK;
-                }
-                mbar_arrive(&drawn[q]);
-                if (id >= U) break;
-            }
-        __syncwarp();
-        return;
-    }
-
-    if (warp == NW + 1) {
-        // ---- hidden units ----
-        int st = 0;                          // stages of down
-        bool ok = true;
-#pragma unroll 1
-        for (int i = 0; ok; ++i) {
-            ok = mx4::wait_all(&drawn[i % L::QUEUE], i / L::QUEUE & 1);
-            if (!ok) break;
-            const Unit u = queue[i % L::QUEUE];
-            if (u.id < 0) break;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&worked[i % L::QUEUE]);
-            if (u.id < U1) continue;
-            const int rb = (u.id - U1) / shares * 4, row_bytes = min(4, RB2 - rb) * 64;
-            int slot = u.slot, c = u.col + lane;             // of this lane's place
-#pragma unroll 1
-            for (int p0 = 0; p0 < u.n; p0 += NP, c += NP, ++st) {
-                const int s = st % R, n = min(NP, u.n - p0);
-                while (c >= C2) { c -= C2; ++slot; }
-                ok = mx4::wait_all(&hid_empty[s], (st / R & 1) ^ 1);
-                const uint64_t t0 = globaltimer_ns();
-#pragma unroll 1
-                for (bool there = lane >= n; ok;) {
-                    if (!there) there = ld_acquire(done + slot) >= UPE;
-                    if (__all_sync(0xffffffffu, there)) break;
-                    ok = __all_sync(0xffffffffu, globaltimer_ns() - t0 <= WAIT_NS);
-                    __nanosleep(20);
-                }
-                if (!ok) break;
-                asm volatile("fence.proxy.async.global;" ::: "memory");      // stored by ordinary stores, read by copies
-                if (lane == 0) mbar_expect_tx(&hid_full[s], n * (NT * (mx4::FRAG + 64) + row_bytes + 64));
-                __syncwarp();
-                if (lane < n) {
-                    uint8_t * hid = ring + s * L::HID;
-                    const size_t tile = (size_t) (slot * C2 + c) * NT;
-                    mx4::bulk_load(hid + lane * NT * mx4::FRAG, (const uint8_t *) g.h + tile * mx4::FRAG, NT * mx4::FRAG, &hid_full[s]);
-                    mx4::bulk_load(hid + L::H_EXP + lane * NT * 64, g.h_exp + tile * 64, NT * 64, &hid_full[s]);
-                    mx4::bulk_load(hid + L::H_ROW + lane * 256, g.down_exp + ((size_t) expert_of[slot] * RB2 + rb) * 16, row_bytes, &hid_full[s]);
-                    mx4::bulk_load(hid + L::H_TOP + lane * 64, h_top + slot * 16, 64, &hid_full[s]);
-                }
-                __syncwarp();
-            }
-        }
-        if (!ok) {
-            if (lane == 0) jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 52, st);
-            // copies in flight end before the memory is given back
-            for (int i = st - R < 0 ? 0 : st - R; i < st; ++i) mx4::wait(&hid_full[i % R], i / R & 1);
-        }
-        return;
-    }
-
-    if (warp < NW) {
-        // ---- products ----
-        float acc[2][NT][4];                 // gate and up, or two row blocks of the weighted sum
-        const int pair = warp / NP, g4 = lane >> 2, t2 = 2 * (lane & 3);
-        // Two walks over the same stages, places p0 .. p0 + n - 1 of a unit, of which this warp has p0 + j if j < n: one asks for weights, up to
-        // `depth` stages ahead of the other, which multiplies.  Places go around the warps, wherever units end.
-        const uint64_t policy = l2_policy_evict_first();
-        const int depth = g.depth;
-        const uint8_t * mine = weights + warp * depth * (2 * mx4::CHUNK);
-        Unit u;                                                   // the asking walk's unit, its place and the place in the ring
-        int u_i = -1, u_p0 = 0, u_turn = 0, at_ask = 0, ahead = 0;
-        u.id = u.n = 0;
-        int id = 0, n_places = 0, slot0 = 0, col0 = 0, now_i = -1, p0 = 0, turn = 0, at_now = 0, sums = 0, st = 0;
-        bool ok = mx4::wait_all(acts_full, 0);
-#pragma unroll 1
-        while (ok) {
-            // ask, as far as units are known (with nothing on its way: wait for one)
-#pragma unroll 1
-            while (ahead < depth && u.id >= 0) {
-                u_p0 += NP;
-                if (u_i < 0 || u_p0 >= u.n) {
-                    const int q = (u_i + 1) % L::QUEUE, ph = (u_i + 1) / L::QUEUE & 1;
-                    if (ahead > 0 && !__all_sync(0xffffffffu, mbar_test_wait(&drawn[q], ph))) {
-                        u_p0 -= NP;
-                        break;
-                    }
-                    ok = mx4::wait_all(&drawn[q], ph);
-                    if (!ok) break;
-                    ++u_i;
-                    u = queue[q];
-                    u_p0 = 0;
-                }
-                const int j = (warp - u_turn) & (NP - 1), n = min(NP, u.n - u_p0);
-                if (u.id >= 0) {
-                    u_turn += n;
-                    if (j < n) {
-                        const bool down = u.id >= U1;
-                        int slot = u.slot, c = u.col + u_p0 + j;
-                        const uint8_t * at = u.weights;
-                        if (down) {
-                            while (c >= C2) { c -= C2; ++slot; }
-                            at += (size_t) expert_of[slot] * g.down_stride;
-                        }
-                        const size_t apart = (size_t) (down ? C2 : C1) * mx4::CHUNK;
-                        if (!down || (u.id - U1) / shares * 4 + 2 * pair < RB2) at += 2 * pair * apart;      // (two row blocks behind the last: any)
-                        mx4::copy_chunks(smem_u32(mine) + at_ask * (2 * mx4::CHUNK), at + c * mx4::CHUNK, apart, policy);
-                    }
+        while (true) {
+            const int part = word[1];
+            if (part >= G) break;
+            const int u0 = part * groups + warp / g.gw, du = G * groups;
+            // asks for this warp's next chunks: units u0, u0 + du .., of each the chunks wg, wg + gw ..
+            int ua = u0, ka = wg, at = 0;
+            const uint8_t * src = nullptr;
+            auto ask = [&] {
+                if (ua < U && ka < C1) {
+                    if (src == nullptr) src = g.gu + (size_t) expert_of[ua / RB1] * g.gu_stride + (size_t) (ua % RB1) * 2 * apart;
+                    mx4::copy_chunks(ring_s + at * L::G_SLOT, src + ka * mx4::CHUNK, apart, policy);
+                    at = at + 1 == depth ? 0 : at + 1;
+                    ka += g.gw;
+                    if (ka >= C1) { ka = wg; ua += du; src = nullptr; }
                 }
                 mx4::copies_commit();
-                at_ask = at_ask + 1 == depth ? 0 : at_ask + 1;
-                ++ahead;
-            }
-            if (!ok) break;
-            // the stage to multiply
-            p0 += NP;
-            if (now_i < 0 || p0 >= n_places) {
-                ++now_i;
-                const Unit & v = queue[now_i % L::QUEUE];           // (the asking walk has seen that it is there)
-                id = v.id;
-                n_places = v.n;
-                slot0 = v.slot;
-                col0 = v.col;
-                p0 = 0;
-                if (id < 0) break;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&worked[now_i % L::QUEUE]);
-            }
-            const bool down = id >= U1, first = p0 == 0, last = p0 + NP >= n_places;
-            const int n_now = min(NP, n_places - p0), j_now = (warp - turn) & (NP - 1);
-            turn += n_now;
-            // its weights are here when at most those asked for behind them are not
-            if (ahead == 1) mx4::copies_wait<0>();
-            else if (ahead == 2) mx4::copies_wait<1>();
-            else if (ahead == 3) mx4::copies_wait<2>();
-            else mx4::copies_wait<3>();
-            __syncwarp();
-            const uint8_t * chunks = mine + at_now * (2 * mx4::CHUNK);
-            if (first) {
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[m][t][i] = 0.f;
-            }
-            if (!down) {
-                if (j_now < n_now) {
-                    const uint4 * b = (const uint4 *) acts + (p0 + j_now) * NT * 128 + lane;
-                    float y[2][NT][4];
-                    mx4::chunks_mma<NT>(chunks, y, [&](int t, int p) { return b[(t * 4 + p) * 32]; });
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[m][t][i] += y[m][t][i];
-                }
-            } else if (n_now > 0) {
-                const int s = st % R;
-                ok = mx4::wait_all(&hid_full[s], st / R & 1);
-                ++st;
-                if (!ok) break;
-                if (j_now < n_now) {
-                    const uint8_t * hid = ring + s * L::HID;
-                    int slot = slot0, c = col0 + p0 + j_now;
-                    while (c >= C2) { c -= C2; ++slot; }
-                    const uint4 * b = (const uint4 *) hid + j_now * NT * 128 + lane;
-                    const int * tops = (const int *) (hid + L::H_TOP) + j_now * 16, * rows = (const int *) (hid + L::H_ROW) + j_now * 64 + pair * 32 + g4;
-                    uint2 ex[NT];
-                    int top[NT];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        ex[t] = ((const uint2 *) (hid + L::H_EXP))[(j_now * NT + t) * 8 + g4];
-                        top[t] = tops[t * 8 + g4];
-                    }
-                    float y[2][NT][4];
-                    mx4::chunks_mma<NT>(chunks, y, [&](int t, int p) {
-                        // all hidden units of a token to the same power of two: its largest one's
-                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                        if (c * mx4::COLS + p * 32 < g.F) {
-                            v = b[(t * 4 + p) * 32];
-                            const uint32_t two = (p < 2 ? ex[t].x : ex[t].y) >> (16 * (p & 1));
-                            const uint32_t f0 = below(top[t] - (int) (two & 0xff)), f1 = below(top[t] - (int) (two >> 8 & 0xff));
-                            v.x = mx4::mul2(v.x, f0);
-                            v.y = mx4::mul2(v.y, f0);
-                            v.z = mx4::mul2(v.z, f1);
-                            v.w = mx4::mul2(v.w, f1);
-                        }
-                        return v;
-                    });
-                    int re[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) re[i] = rows[8 * i] - BIAS - 14;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const float2 wt = *(const float2 *) (wtab + slot * 16 + t * 8 + t2);
-                        const int2 te = *(const int2 *) (tops + t * 8 + t2);
-                        const int chosen = mask[slot] >> (t * 8 + t2);
-#pragma unroll
-                        for (int m = 0; m < 2; ++m)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (chosen >> (i & 1) & 1)                // else there are no hidden units
-                                    acc[m][t][i] += (i & 1 ? wt.y : wt.x) * mx4::pow2_normal(re[2 * m + (i >> 1)] + (i & 1 ? te.y : te.x)) * y[m][t][i];
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&hid_empty[s]);
-            }
-            __syncwarp();
-            at_now = at_now + 1 == depth ? 0 : at_now + 1;
-            --ahead;
-            if (last) {
-                const int buf = sums % FIN;
-                ok = mx4::wait_all(&red_empty[buf], (sums / FIN & 1) ^ 1);
-                if (!ok) break;
-                float4 * dst = (float4 *) red + (buf * NW + warp) * (L::SUMS / 4) * 32 + lane;
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) dst[(m * NT + t) * 32] = make_float4(acc[m][t][0], acc[m][t][1], acc[m][t][2], acc[m][t][3]);
-                if (warp == 0 && lane == 0) red_unit[buf] = id;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&red_full[buf]);
-                ++sums;
-            }
-        }
-        mx4::copies_wait<0>();
-        if (!ok && lane == 0) jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 53, warp);
-        // the end, for every finishing warp
+            };
 #pragma unroll 1
-        for (int i = 0; i < FIN; ++i, ++sums) {
-            const int buf = sums % FIN;
-            mx4::wait(&red_empty[buf], (sums / FIN & 1) ^ 1);
-            if (warp == 0 && lane == 0) red_unit[buf] = -1;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&red_full[buf]);
+            for (int i = 0; i < depth; ++i) ask();
+            int here = 0;
+#pragma unroll 1
+            for (int u = u0; u < U; u += du) {
+                float acc[2][NT][4];
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+#pragma unroll 1
+                for (int k = wg; k < C1; k += g.gw) {
+                    mx4::copies_wait(depth - 1);
+                    __syncwarp();
+                    const uint4 * b = acts + k * NT * 128;
+                    mx4::chunks_mma<NT>(ring + here * L::G_SLOT, acc, [&](int n, int p) { return b[(n * 4 + p) * 32]; });
+                    here = here + 1 == depth ? 0 : here + 1;
+                    __syncwarp();
+                    ask();
+                }
+                // the group's sums, in the order of its warps: [gate or up][tile][register][lane]
+                float * mine = red + parity * (L::RED / 4) + warp * L::SUMS * 32 + lane;
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mine[((m * NT + n) * 4 + i) * 32] = acc[m][n][i];
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / g.gw), "r"(g.gw * 32) : "memory");
+                if (wg < 2 * NT) {
+                    // token 8 n + col, hidden units f + row0 and f + row0 + 8
+                    const int n = wg >> 1, col = t2 + (wg & 1), slot = u / RB1, f = u % RB1 * 16;
+                    const float * src = red + parity * (L::RED / 4) + (warp - wg) * L::SUMS * 32 + (n * 4 + (wg & 1)) * 32 + lane;
+                    float z[2] = {0.f, 0.f}, v[2] = {0.f, 0.f};
+#pragma unroll 4
+                    for (int w = 0; w < g.gw; ++w)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            z[i] += src[w * L::SUMS * 32 + 64 * i];
+                            v[i] += src[w * L::SUMS * 32 + NT * 128 + 64 * i];
+                        }
+                    const int * rows = g.gu_exp + ((size_t) expert_of[slot] * RB1 + u % RB1) * 32 + g4;
+                    const int xe = ((const int *) ((const uint8_t *) g.xf + L::frags(g.d)))[n * 8 + col];
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        v[i] = mx4::gated(mx4::times_pow2(z[i], __ldg(rows + 8 * i) + xe), mx4::times_pow2(v[i], __ldg(rows + 16 + 8 * i) + xe), g.act);
+                        top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+                    }
+#pragma unroll
+                    for (int o = 4; o < 32; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    if (mask[slot] >> (n * 8 + col) & 1) {
+                        const int he = mx4::top_exponent(top);
+                        const float up = mx4::pow2_normal(14 - he);
+                        const size_t tile = ((size_t) slot * C2 + f / mx4::COLS) * NT + n;
+                        __half * to = g.h + ((tile * 4 + f % mx4::COLS / 32) * 32 + col * 4 + g4 / 2) * 8 + (f / 16 & 1) * 4 + (g4 & 1);
+                        to[0] = __float2half_rn(v[0] * up);
+                        to[2] = __float2half_rn(v[1] * up);
+                        if (g4 == 0) {
+                            g.h_exp[(tile * 8 + col) * 8 + f % mx4::COLS / 16] = (uint8_t) (he + BIAS);
+                            atomicMax(h_top + slot * 16 + n * 8 + col, he + BIAS);
+                        }
+                    }
+                }
+                parity ^= 1;
+            }
+            mx4::copies_wait(0);
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                atomicAdd(done, 1);
+                word[1] = atomicAdd(g.sync, 1);
+            }
+            __syncthreads();
+        }
+    }
+
+    // ---- down: places (64 rows, chunk of an expert's hidden units) i0 .. i1 - 1 of the line ----
+    const int P = slots * C2, groups = (g.d + 63) / 64;
+    const long long N = (long long) groups * P;
+    const int pieces = N < G ? (int) N : G;
+    if (N == 0) {                                 // no expert: the residual, or zeros
+        for (int i = blockIdx.x * THREADS + threadIdx.x; i < g.T * g.d; i += G * THREADS) {
+            const int t = i / g.d, o = i % g.d;
+            g.out[i] = g.residual != nullptr ? g.residual[t * g.ldr + o] : __float2bfloat16(0.f);
         }
         return;
     }
-
-    // ---- finished rows: a warp a unit; a lane holds row g of columns 2t, 2t + 1 and row g + 8 of the same ----
-    constexpr int AT_ONCE = NT == 1 ? 3 : 1;                 // shares
-    const int fin = warp - NW - 2, row0 = lane >> 2, col0 = 2 * (lane & 3);
-    int x_exp[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) x_exp[n][p] = ((const int *) ((const uint8_t *) g.xf + L::frags(g.d)))[n * 8 + col0 + p];
+    if ((int) blockIdx.x >= pieces) return;
+    const int i0 = (int) (blockIdx.x * N / pieces), i1 = (int) ((blockIdx.x + 1) * N / pieces);
+    const int pair = warp >> 3, wj = warp & 7, depth = g.depth2;
+    const uint8_t * ring = work + warp * depth * L::D_SLOT;
+    const uint32_t ring_s = smem_u32(ring);
+    const size_t apart = (size_t) C2 * mx4::CHUNK;
+    // the other CTAs' hidden units
+    if (threadIdx.x == 0) {
+        const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
-    for (int round = 0;; ++round) {
-        if (!mx4::wait_all(&red_full[fin], round & 1)) {
-            if (lane == 0) jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 54, round);
-            break;
-        }
-        const int unit = red_unit[fin];
-        if (unit < 0) break;
-        int ex[4][2];                        // exponents of this lane's rows of gate and up
-        const int slot = unit < U1 ? unit / UPE : 0;
-        if (unit < U1) {
-            const int * rows = g.gu_exp + ((size_t) expert_of[slot] * UPE + unit % UPE) * 64 + row0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ex[i >> 1][i & 1] = __ldg(rows + 8 * i);
-        }
-        float s[4][NT][4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[m][n][i] = 0.f;
-#pragma unroll
-                for (int w = 0; w < NP; ++w) {
-                    const float4 v = ((const float4 *) red)[((fin * NW + (m >> 1) * NP + w) * (L::SUMS / 4) + (m & 1) * NT + n) * 32 + lane];
-                    s[m][n][0] += v.x;
-                    s[m][n][1] += v.y;
-                    s[m][n][2] += v.z;
-                    s[m][n][3] += v.w;
-                }
+        while (ld_acquire(done) < G) {
+            if (globaltimer_ns() - t0 > WAIT_NS) {
+                jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 52, blockIdx.x);
+                break;
             }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&red_empty[fin]);
-        if (unit < U1) {
-            const int f0 = unit % UPE * 32, m = mask[slot];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const size_t tile = ((size_t) slot * C2 + f0 / mx4::COLS) * NT + n;
-#pragma unroll 1
-                for (int st = 0; st < 2; ++st) {             // 16 hidden units each
-                    float v[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        v[i] = mx4::gated(mx4::times_pow2(s[2 * st][n][i], ex[2 * st][i >> 1] + x_exp[n][i & 1]),
-                                          mx4::times_pow2(s[2 * st + 1][n][i], ex[2 * st + 1][i >> 1] + x_exp[n][i & 1]), g.act);
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        // those of token 8 n + col, scaled together
-                        const int col = col0 + p;
-                        uint32_t top = max(__float_as_uint(v[p]) & 0x7fffffffu, __float_as_uint(v[p + 2]) & 0x7fffffffu);
-#pragma unroll
-                        for (int o = 4; o < 32; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        if (m >> (n * 8 + col) & 1) {
-                            const int he = mx4::top_exponent(top);
-                            const float up = mx4::pow2(14 - he);
-                            // hidden unit f0 + 16 st + row in its place among the fragments
-                            __half * to = g.h + ((tile * 4 + f0 % mx4::COLS / 32) * 32 + col * 4 + row0 / 2) * 8 + st * 4 + (row0 & 1);
-                            to[0] = __float2half_rn(v[p] * up);
-                            to[2] = __float2half_rn(v[p + 2] * up);
-                            if (row0 == 0) {
-                                g.h_exp[(tile * 8 + col) * 8 + f0 % mx4::COLS / 16 + st] = (uint8_t) (he + BIAS);
-                                atomicMax(h_top + slot * 16 + n * 8 + col, he + BIAS);
-                            }
-                        }
-                    }
-                }
-            }
-            __threadfence();
-            __syncwarp();
-            if (lane == 0) atomicAdd(done + slot, 1);
-            continue;
+            __nanosleep(32);
         }
-        const int rb = (unit - U1) / shares, share = (unit - U1) % shares;
-        if (shares > 1) {
-            float4 * part = (float4 *) g.part + (size_t) rb * shares * (4 * NT * 32) + lane;
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    __stcg(part + ((share * 4 + m) * NT + n) * 32, make_float4(s[m][n][0], s[m][n][1], s[m][n][2], s[m][n][3]));
-            __threadfence();
-            __syncwarp();
-            int others = 0;
-            if (lane == 0) {
-                others = atomicAdd(shares_done + rb, 1);
-                __threadfence();
-            }
-            if (__shfl_sync(0xffffffffu, others, 0) != shares - 1) continue;
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[m][n][i] = 0.f;
-#pragma unroll 1
-            for (int i0 = 0; i0 < shares; i0 += AT_ONCE) {
-                float4 v[AT_ONCE][4 * NT];
-#pragma unroll
-                for (int i = 0; i < AT_ONCE; ++i)
-#pragma unroll
-                    for (int k = 0; k < 4 * NT; ++k)
-                        v[i][k] = i0 + i < shares ? __ldcg(part + ((i0 + i) * 4 * NT + k) * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int i = 0; i < AT_ONCE; ++i)
-#pragma unroll
-                    for (int k = 0; k < 4 * NT; ++k) {
-                        s[k / NT][k % NT][0] += v[i][k].x;
-                        s[k / NT][k % NT][1] += v[i][k].y;
-                        s[k / NT][k % NT][2] += v[i][k].z;
-                        s[k / NT][k % NT][3] += v[i][k].w;
-                    }
-            }
+    }
+    __syncthreads();
+    __threadfence();
+    // This warp's places: of each piece of 64 rows' places [a, b) those at a + wj, a + wj + 8, ..
+    int ga = i0 / P, pa = i0 % P + wj, ea = min(P, i1 - ga * P), at = 0;        // asked for: rows, place, the piece's end
+    auto ask = [&] {
+        while (pa >= ea && (ga + 1) * P < i1) {
+            ++ga;
+            pa = wj;
+            ea = min(P, i1 - ga * P);
         }
-        if (g.residual != nullptr)           // (all read before the first result is stored)
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int t = n * 8 + col0 + (i & 1), o = rb * 64 + m * 16 + row0 + 8 * (i >> 1);
-                        if (t < g.T && o < g.d) s[m][n][i] += __bfloat162float(g.residual[t * g.ldr + o]);
-                    }
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
+        if (pa < ea) {
+            const int slot = pa / C2, c = pa % C2, e = expert_of[slot], rb = ga * 4 + 2 * pair < RB2 ? ga * 4 + 2 * pair : 0;      // (rows behind the last: any)
+            const uint32_t to = ring_s + at * L::D_SLOT;
+            mx4::copy_chunks(to, g.down + (size_t) e * g.down_stride + rb * apart + c * mx4::CHUNK, apart, policy);
+            const size_t tile = (size_t) (slot * C2 + c) * NT;
+            const int m = mask[slot];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = n * 8 + col0 + (i & 1), o = rb * 64 + m * 16 + row0 + 8 * (i >> 1);
-                    if (t < g.T && o < g.d) g.out[(size_t) t * g.d + o] = __float2bfloat16(s[m][n][i]);
+                for (int p = 0; p < 4; ++p)        // zeros for tokens that have not chosen this expert, and behind the last hidden unit
+                    mx4::copy16_or_zero(to + L::G_SLOT + ((n * 4 + p) * 32 + lane) * 16, (const uint4 *) g.h + ((tile + n) * 4 + p) * 32 + lane,
+                                        (m >> (n * 8 + g4) & 1) && c * mx4::COLS + p * 32 < g.F ? 16 : 0);
+            const uint8_t * more = nullptr;
+            if (lane < 4 * NT) more = g.h_exp + tile * 64 + lane * 16;
+            else if (lane >= 8 && lane < 16) more = (const uint8_t *) (g.down_exp + ((size_t) e * RB2 + rb) * 16) + (lane - 8) * 16;
+            else if (lane >= 16 && lane < 20) more = (const uint8_t *) (h_top + slot * 16) + (lane - 16) * 16;
+            const int off = lane < 8 ? L::H_EXP + lane * 16 : lane < 16 ? L::H_ROW + (lane - 8) * 16 : L::H_TOP + (lane - 16) * 16;
+            if (more != nullptr) mx4::copy16_or_zero(to + off, more, 16);
+            at = at + 1 == depth ? 0 : at + 1;
+            pa += 8;
+        }
+        mx4::copies_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < depth; ++i) ask();
+    int here = 0;
+#pragma unroll 1
+    for (int gr = i0 / P; gr * P < i1; ++gr) {
+        const int a = max(0, i0 - gr * P), b = min(P, i1 - gr * P);
+        float acc[2][NT][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+#pragma unroll 1
+        for (int p = a + wj; p < b; p += 8) {
+            mx4::copies_wait(depth - 1);
+            __syncwarp();
+            const uint8_t * chunks = ring + here * L::D_SLOT;
+            const uint4 * frags = (const uint4 *) (chunks + L::G_SLOT) + lane;
+            const int * tops = (const int *) (chunks + L::H_TOP), * rows = (const int *) (chunks + L::H_ROW) + g4, slot = p / C2;
+            uint2 ex[NT];
+            int top[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                ex[n] = ((const uint2 *) (chunks + L::H_EXP))[n * 8 + g4];
+                top[n] = tops[n * 8 + g4];
+            }
+            float y[2][NT][4] = {};
+            mx4::chunks_mma<NT>(chunks, y, [&](int n, int q) {
+                // a token's hidden units of each step to the power of two of its largest ones
+                const uint32_t two = (q < 2 ? ex[n].x : ex[n].y) >> (16 * (q & 1));
+                const uint32_t f0 = below(top[n] - (int) (two & 0xff)), f1 = below(top[n] - (int) (two >> 8 & 0xff));
+                uint4 v = frags[(n * 4 + q) * 32];
+                v.x = mx4::mul2(v.x, f0);
+                v.y = mx4::mul2(v.y, f0);
+                v.z = mx4::mul2(v.z, f1);
+                v.w = mx4::mul2(v.w, f1);
+                return v;
+            });
+            int re[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) re[i] = rows[8 * i] - BIAS - 14;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float2 wt = *(const float2 *) (wtab + slot * 16 + n * 8 + t2);
+                const int2 te = *(const int2 *) (tops + n * 8 + t2);
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[m][n][i] += (i & 1 ? wt.y : wt.x) * mx4::pow2_normal(re[2 * m + (i >> 1)] + (i & 1 ? te.y : te.x)) * y[m][n][i];
+            }
+            here = here + 1 == depth ? 0 : here + 1;
+            __syncwarp();
+            ask();
+        }
+        float * mine = red + (gr & 1) * (L::RED / 4) + warp * L::SUMS * 32 + lane;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mine[((m * NT + n) * 4 + i) * 32] = acc[m][n][i];
+        __syncthreads();
+        // thread = (two row blocks, register, lane): its row of one row block, then of the other, for each tile
+        const int half = warp >> 3, m = warp >> 2 & 1, reg = warp & 3, o = gr * 64 + (2 * half + m) * 16 + g4 + 8 * (reg >> 1);
+        const float * src = red + (gr & 1) * (L::RED / 4) + half * 8 * L::SUMS * 32 + (m * NT * 4 + reg) * 32 + lane;
+        float v[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            v[n] = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) v[n] += src[(w * L::SUMS + n * 4) * 32];
+        }
+        if (a > 0 || b < P) {
+            // pieces first .. last hold places of these rows
+            const int first = (int) ((((long long) gr * P + 1) * pieces - 1) / N), last = (int) ((((long long) gr + 1) * P * pieces - 1) / N);
+            float * part = g.part + ((size_t) (first + 2 * gr)) * (THREADS * NT) + threadIdx.x;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) __stcg(part + ((blockIdx.x - first) * NT + n) * THREADS, v[n]);
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                word[2] = atomicAdd(pieces_done + gr, 1);
+                __threadfence();
+            }
+            __syncthreads();
+            if (word[2] != last - first) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                v[n] = 0.f;
+#pragma unroll 1
+                for (int q0 = 0; q0 <= last - first; q0 += 8) {
+                    float x[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) x[q] = q0 + q <= last - first ? __ldcg(part + ((q0 + q) * NT + n) * THREADS) : 0.f;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[n] += x[q];
                 }
+            }
+        }
+        if (o < g.d)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int t = n * 8 + t2 + (reg & 1);
+                if (t >= g.T) continue;
+                if (g.residual != nullptr) v[n] += __bfloat162float(g.residual[t * g.ldr + o]);
+                g.out[(size_t) t * g.d + o] = __float2bfloat16(v[n]);
+            }
     }
+    mx4::copies_wait(0);
 }
 
 // The layer's first launch: CTAs below E compute router outputs [T][E], the others a token's fragments each (8 NT of them, zeros from T on); zeros where
@@ -613,37 +478,33 @@ __global__ void __launch_bounds__(GATE_NT) mx4_prepare_kernel(const bf16 * __res
     }
 }
 
+// Stages of chunks that fit, at most MAX_DEPTH (0: not one).
+template <int NT>
+int depth_of(int d, int slots, bool down) {
+    using L = Layout<NT>;
+    for (int i = MAX_DEPTH; i > 0; --i)
+        if ((down ? L::bytes(0, slots, 0, i) : L::bytes(d, slots, i, 0)) <= MOST_SMEM) return i;
+    return 0;
+}
+
 template <int NT>
 int launch(const MoeArgs & a, cudaStream_t s) {
     using L = Layout<NT>;
     static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
     MoeArgs g = a;
-    g.ring = 2;
-    g.depth = (MOST_SMEM - L::bytes(g.d, g.max_slots, g.ring, 0)) / L::DEEP;
-    if (g.depth > L::MAX_DEPTH) {
-        g.depth = L::MAX_DEPTH;
-        if (L::bytes(g.d, g.max_slots, 3, g.depth) <= MOST_SMEM) g.ring = 3;
-    }
-    if (g.depth < 1) return JIB_E_SCRATCH;
-    if (!jib::ensure_dyn_smem(mx4_moe_kernel<NT>, MOST_SMEM, attr_done)) return JIB_E_LAUNCH;
+    g.depth1 = depth_of<NT>(g.d, g.max_slots, false);
+    g.depth2 = depth_of<NT>(g.d, g.max_slots, true);
+    // Warps that share 16 hidden units: as few as leave every group of warps about as many units (four are enough to finish a unit of 16 tokens).
     const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
-    JIB_LAUNCH((mx4_moe_kernel<NT>), sms, L::THREADS, L::bytes(g.d, g.max_slots, g.ring, g.depth), s, g);
-    return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH;
-}
-
-// Shares that 64 rows of down are cut into at most: two, three or four units for each SM, whichever leaves the last round fullest.
-int shares_of(int d) {
-    const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148, groups = (d + 63) / 64;
-    int best = 1;
-    double fill = 0;
-    for (int k = 2; k <= 4; ++k) {
-        int n = k * sms / groups;
-        n = n < 1 ? 1 : n > MAX_SHARES ? MAX_SHARES : n;
-        const int rounds = (groups * n + sms - 1) / sms;
-        const double f = (double) groups * n / ((double) rounds * sms);
-        if (f > fill + 0.02) { fill = f; best = n; }
+    const long long units = (long long) g.max_slots * (g.F / 16);
+    long long best = -1;
+    for (int gw = 4; gw <= NW; gw *= 2) {
+        const long long groups = (long long) sms * (NW / gw), cost = (units + groups - 1) / groups * gw;
+        if (best < 0 || cost < best) { best = cost; g.gw = gw; }
     }
-    return best;
+    if (!jib::ensure_dyn_smem(mx4_moe_kernel<NT>, MOST_SMEM, attr_done)) return JIB_E_LAUNCH;
+    JIB_LAUNCH((mx4_moe_kernel<NT>), sms, THREADS, L::bytes(g.d, g.max_slots, g.depth1, g.depth2), s, g);
+    return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH;
 }
 
 // Experts that T tokens can choose.
@@ -658,13 +519,14 @@ JIB_EXPORT int jib_mx4_moe_sizes(int T, int d, int F, int E, int k, long long * 
     if (T < 1 || T > MAX_T || k < 1 || k > MAX_K || E < 1 || E > MAX_E || d % 32 || F % 32 || d < 32 || F < 32 || d > GATE_MAXC * GATE_NT * 8) return 0;
     const int NT = T <= 8 ? 1 : 2;
     const long long slots = slots_of(T, k, E);
-    if ((NT == 1 ? Layout<1>::bytes(d, (int) slots, 2, 1) : Layout<2>::bytes(d, (int) slots, 2, 1)) > MOST_SMEM) return 0;
+    if ((NT == 1 ? depth_of<1>(d, (int) slots, false) : depth_of<2>(d, (int) slots, false)) == 0) return 0;
     const long long tiles = slots * mx4::chunks(F) * NT;
-    if (slots * (F / 32) + (long long) (d / 32) * MAX_SHARES > (1ll << 30) || tiles > (1 << 25)) return 0;
+    const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148, groups = (d + 63) / 64;
+    if (tiles * groups > (1 << 30) || slots * (F / 16) > (1 << 30)) return 0;
     sizes[0] = (NT == 1 ? Layout<1>::frags(d) : Layout<2>::frags(d)) + 64;
     sizes[1] = tiles * (mx4::FRAG + 64);
-    sizes[2] = (long long) ((d + 63) / 64) * shares_of(d) * 512 * NT;
-    sizes[3] = 4 + MAX_E + slots * 16 + (d + 63) / 64;
+    sizes[2] = (long long) (sms + 2 * groups) * THREADS * NT;
+    sizes[3] = 4 + slots * 16 + groups;
     return 1;
 }
 
@@ -699,7 +561,7 @@ JIB_EXPORT int jib_mx4_moe(const jib_mx4_moe_desc * m, void * stream) {
     a.ldr = m->ldr; a.gu_stride = m->gu_stride; a.down_stride = m->down_stride;
     a.T = m->T; a.d = m->d; a.F = m->F; a.E = m->E; a.k = m->k; a.n_group = m->n_group; a.topk_group = m->topk_group; a.norm = m->norm; a.sigmoid = m->sigmoid;
     a.n_shared = m->n_shared; a.group_top2 = m->group_top2; a.act = m->act; a.scale = m->scale;
-    a.shares = shares_of(m->d);
+    a.warm = jib::warm_enabled();
     return m->T <= 8 ? launch<1>(a, (cudaStream_t) stream) : launch<2>(a, (cudaStream_t) stream);
 }
 

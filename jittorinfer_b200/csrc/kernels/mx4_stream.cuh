@@ -37,23 +37,26 @@ __device__ __forceinline__ void copy_chunks(uint32_t dst, const uint8_t * src, s
         for (int u = 0; u < 2; ++u) copy16(dst + m * CHUNK + (u * 32 + lane) * 16, src + m * apart + (u * 32 + lane) * 16, policy);
     if (lane < 8) copy16(dst + (lane >> 2) * CHUNK + SCALES + (lane & 3) * 16, src + (lane >> 2) * apart + SCALES + (lane & 3) * 16, policy);
 }
+// The same through no cache policy; `bytes` 16, or 0: zeros.
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void * src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// All but the last n groups of copies are there (n: 0 .. 3).
+__device__ __forceinline__ void copies_wait(int n) {
+    if (n == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else if (n == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else asm volatile("cp.async.wait_group 3;" ::: "memory");
+}
 
-// y[m] (row g: columns 2t, 2t + 1; row g + 8) = chunk m x the same fragments: frag(n, pair) gives this lane's 16 bytes.
+// y[m] (row g: columns 2t, 2t + 1; row g + 8) += chunk m x the same fragments: frag(n, pair) gives this lane's 16 bytes.
 template <int NT, typename F>
 __device__ __forceinline__ void chunks_mma(const uint8_t * chunks, float (&y)[2][NT][4], F frag) {
     const int lane = threadIdx.x & 31;
     uint2 f[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) f[m] = *(const uint2 *) (chunks + m * CHUNK + SCALES + (lane >> 2) * 8);
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[m][n][i] = 0.f;
     uint4 q[2];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {          // 32 columns: two steps, one scale a row

@@ -10,9 +10,8 @@
 // experts' hidden units overlapped more and took twice the time: their code did not stay in the instruction cache.)
 //
 // Gate and up: GW warps share 16 hidden units of an expert, each a part of K, and add their sums up in order in shared memory.  Hidden units go to
-// memory as fragments, fp16, each 16 of a token scaled by a power of two that is kept beside them.  A part of this loop (one part for each CTA) is
-// drawn from a counter, so that every part is done by a CTA that runs; a CTA draws until there is none left and then waits for all
-// parts: nothing waits for a CTA that has not started.
+// memory as fragments, fp16, each 16 of a token scaled by a power of two that is kept beside them.  Groups draw their units from a counter, so every
+// unit is done by a CTA that runs; a CTA whose groups find none left waits until all are done: nothing waits for a CTA that has not started.
 // Down: the chunks of 64 rows x all chosen experts' hidden units are one line, cut into equal pieces, one for each CTA.  Where a piece ends inside 64
 // rows, the sums meet in memory, and the CTA that comes last adds them up in their order.
 #include "gate.cuh"
@@ -26,7 +25,7 @@ using namespace sm100;
 
 constexpr int MAX_T = 16, MAX_K = 32;                         // tokens, choices of a token
 constexpr int NW = 16, THREADS = NW * 32;                     // warps
-constexpr int MOST_SMEM = 227 * 1024, MAX_DEPTH = 4;
+constexpr int MOST_SMEM = 227 * 1024, MAX_DEPTH = 4, KNOWN = 8, AHEAD = 3;       // units of a group: that it remembers, that it draws ahead
 constexpr int BIAS = 113;                                     // top_exponent() + BIAS is 1 .. 240
 constexpr uint64_t WAIT_NS = JIB_WAIT_NS;                     // for the other CTAs' hidden units
 
@@ -42,7 +41,7 @@ struct MoeArgs {
     uint8_t * h_exp;                         // ... [slot][chunk][token][step], BIAS more than its exponent
     float * part;                            // [pieces][512 NT]
     bf16 * out;
-    int * sync;                              // zeros: parts of gate and up drawn, parts done (and two more), the largest byte of h_exp of each slot and token
+    int * sync;                              // zeros: units of gate and up drawn, units done (and two more), the largest byte of h_exp of each slot and token
                                              // [slots][16], pieces done of each 64 rows
     int * status;
     long long ldr, gu_stride, down_stride;
@@ -50,25 +49,25 @@ struct MoeArgs {
     float scale;
 };
 
-// Shared memory: tables; sums, twice; then for gate and up the tokens' fragments and the warps' rings of chunks, for down the warps' rings of chunks with
-// their hidden units (fragments, the exponents' bytes, the exponents of 32 rows, the largest bytes of 16 tokens).
+// Shared memory: tables; sums, twice; the warps' rings of chunks, for gate and up behind the tokens' fragments.
 template <int NT>
 struct Layout {
+    static_assert((48 + 4 * KNOWN * 8) % 16 == 0, "the exponents' place");
     static constexpr int SUMS = 8 * NT;                           // of a lane
     static constexpr int RED = NW * 32 * SUMS * 4;
-    static constexpr int G_SLOT = 2 * mx4::CHUNK;
-    static constexpr int H_EXP = G_SLOT + NT * mx4::FRAG, H_ROW = H_EXP + NT * 64, H_TOP = H_ROW + 128, D_SLOT = H_TOP + 64;
-    static_assert(2 * RED >= NW * (MAX_E + 32) * 4, "scratch of the choice");
+    static constexpr int SLOT = 2 * mx4::CHUNK;
+    static constexpr int BUFFERS = NT == 1 ? 3 : 2;               // of sums (see where a unit of gate and up is finished)
+    static_assert(BUFFERS * RED >= NW * (MAX_E + 32) * 4, "scratch of the choice");
     __host__ __device__ static int frags(int d) { return mx4::chunks(d) * NT * mx4::FRAG; }
-    __host__ __device__ static int tables(int slots) { return (slots * 64 + MAX_E * 4 * 3 + MAX_T * MAX_K * 8 + 64 + 127) / 128 * 128; }
-    __host__ __device__ static int base(int slots) { return 128 + tables(slots) + 2 * RED; }
+    __host__ __device__ static int tables(int slots) { return (slots * 64 + MAX_E * 4 * 3 + MAX_T * MAX_K * 8 + 64 + 4 * KNOWN * (8 + 128) + 127) / 128 * 128; }
+    __host__ __device__ static int base(int slots) { return 128 + tables(slots) + BUFFERS * RED; }
     __host__ __device__ static int bytes(int d, int slots, int depth1, int depth2) {
-        const int a = frags(d) + NW * depth1 * G_SLOT, b = NW * depth2 * D_SLOT;
+        const int a = frags(d) + NW * depth1 * SLOT, b = NW * depth2 * SLOT;
         return base(slots) + (a > b ? a : b);
     }
 };
 
-// 2^-n in fp16, twice (n below 0, from a byte that no hidden unit goes with, counts as 0)
+// 2^-n in fp16, twice 
 __device__ __forceinline__ uint32_t below(int n) {
     const float f = __uint_as_float((uint32_t) min(max(127 - n, 0), 127) << 23);
     const __half2 h = __floats2half2_rn(f, f);
@@ -91,9 +90,11 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     int * ids_s = mask + MAX_E;
     float * wts_s = (float *) (ids_s + MAX_T * MAX_K);
     uint64_t * acts_full = (uint64_t *) (wts_s + MAX_T * MAX_K);
-    int * word = (int *) (acts_full + 1);                          // [0] slots, [1] part drawn, [2] pieces done
+    int * word = (int *) (acts_full + 1);                          // [0] slots, [1] units done by this CTA, [2] pieces done
+    long long * drawn = (long long *) (word + 10);                 // (48 bytes behind the barrier) of each group (at most 4) the last KNOWN units: number << 32 | unit
+    int * exps = (int *) (drawn + 4 * KNOWN);                      // ... and the exponents of their 32 rows: 16-byte copies, 304 bytes behind the barrier
     float * red = (float *) (base + L::tables(g.max_slots));
-    uint8_t * work = (uint8_t *) (red + 2 * L::RED / 4);
+    uint8_t * work = (uint8_t *) (red + L::BUFFERS * L::RED / 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t2 = 2 * (lane & 3);
 
     if (threadIdx.x == 0) {
@@ -102,14 +103,16 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     }
     for (int i = threadIdx.x; i < g.max_slots * 16; i += THREADS) wtab[i] = 0.f;
     for (int i = threadIdx.x; i < MAX_E; i += THREADS) { slot_of[i] = 0; mask[i] = 0; }
+    if (threadIdx.x < 4 * KNOWN) drawn[threadIdx.x] = -1;
     __syncthreads();
     PDL_TRIGGER_TOP();
     if (g.warm && g.logits != nullptr && warp == 0)      // the choice's code (33 KB) comes to the SM while the launch before this one runs
         gate_token(nullptr, nullptr, nullptr, nullptr, 0, g.E - g.n_shared, g.k, g.n_group, g.topk_group, g.scale, g.norm, g.sigmoid, g.n_shared, g.group_top2,
                    red, red + MAX_E, ids_s, wts_s, true);
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
+    if (warp % g.gw == 0 && lane < AHEAD) drawn[warp / g.gw * KNOWN + lane] = (long long) lane << 32 | atomicAdd(g.sync, 1);
     if (threadIdx.x == THREADS - 1) {
-        word[1] = atomicAdd(g.sync, 1);
+        word[1] = 0;
         mbar_expect_tx(acts_full, L::frags(g.d));
         mx4::bulk_load(work, g.xf, L::frags(g.d), acts_full);
     }
@@ -151,114 +154,135 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
             }
     }
     __syncthreads();
-    const int slots = word[0], C1 = mx4::chunks(g.d), C2 = mx4::chunks(g.F), RB1 = g.F / 16, RB2 = g.d / 16, G = gridDim.x;
+    const int slots = word[0], C1 = mx4::chunks(g.d), C2 = mx4::chunks(g.F), RB1 = g.F / 16, RB2 = g.d / 16, G = gridDim.x, U = slots * RB1;
     int * done = g.sync + 1, * h_top = g.sync + 4, * pieces_done = h_top + g.max_slots * 16;
     const uint64_t policy = l2_policy_evict_first();
 
-    // ---- gate and up: a part at a time ----
+    // ---- gate and up ----
     if (!mx4::wait_all(acts_full, 0) && lane == 0) jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 51, warp);
     {
-        const int U = slots * RB1, groups = NW / g.gw, wg = warp % g.gw, depth = g.depth1;
-        const uint8_t * ring = work + L::frags(g.d) + warp * depth * L::G_SLOT;
+        const int group = warp / g.gw, wg = warp % g.gw, count = (C1 - wg + g.gw - 1) / g.gw, depth = min(g.depth1, max(2 * count, 1));
+        const uint8_t * ring = work + L::frags(g.d) + warp * g.depth1 * L::SLOT;
         const uint32_t ring_s = smem_u32(ring);
         const uint4 * acts = (const uint4 *) work + lane;
         const size_t apart = (size_t) C1 * mx4::CHUNK;
-        int parity = 0;
+        int * rows_of = exps + group * KNOWN * 32;
+        // The group's unit number i, once it is drawn (by the group's first warp, which draws number i + 3 before it begins with number i + 1).
+        auto unit = [&](int i) -> int {
+            volatile const long long * at = drawn + group * KNOWN + i % KNOWN;
 #pragma unroll 1
-        while (true) {
-            const int part = word[1];
-            if (part >= G) break;
-            const int u0 = part * groups + warp / g.gw, du = G * groups;
-            // asks for this warp's next chunks: units u0, u0 + du .., of each the chunks wg, wg + gw ..
-            int ua = u0, ka = wg, at = 0;
-            const uint8_t * src = nullptr;
-            auto ask = [&] {
-                if (ua < U && ka < C1) {
-                    if (src == nullptr) src = g.gu + (size_t) expert_of[ua / RB1] * g.gu_stride + (size_t) (ua % RB1) * 2 * apart;
-                    mx4::copy_chunks(ring_s + at * L::G_SLOT, src + ka * mx4::CHUNK, apart, policy);
-                    at = at + 1 == depth ? 0 : at + 1;
-                    ka += g.gw;
-                    if (ka >= C1) { ka = wg; ua += du; src = nullptr; }
+            for (int tries = 0; tries < 1 << 22; ++tries) {
+                const long long v = *at;
+                if ((int) (v >> 32) == i) return (int) v;
+            }
+            jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 53, i);
+            return U;
+        };
+        // Asks for this warp's next chunks: of unit after unit the chunks wg, wg + gw .., at most two units ahead; and for the exponents of a unit's rows.
+        int ia = 0, ka = wg, at = 0, ua = 0;
+        const uint8_t * src = nullptr;
+        auto ask = [&] {
+            if (src == nullptr && ua < U) ua = unit(ia);
+            if (ua < U && ka < C1) {
+                if (src == nullptr) {
+                    const int slot = ua / RB1, rb = ua - slot * RB1, e = expert_of[slot];
+                    src = g.gu + (size_t) e * g.gu_stride + (size_t) rb * 2 * apart;
+                    if (wg == 0 && lane < 8)
+                        mx4::copy16_or_zero(smem_u32(rows_of + (ia % KNOWN) * 32 + lane * 4), g.gu_exp + ((size_t) e * RB1 + rb) * 32 + lane * 4, 16);
                 }
-                mx4::copies_commit();
-            };
-#pragma unroll 1
-            for (int i = 0; i < depth; ++i) ask();
-            int here = 0;
-#pragma unroll 1
-            for (int u = u0; u < U; u += du) {
-                float acc[2][NT][4];
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
-#pragma unroll 1
-                for (int k = wg; k < C1; k += g.gw) {
-                    mx4::copies_wait(depth - 1);
-                    __syncwarp();
-                    const uint4 * b = acts + k * NT * 128;
-                    mx4::chunks_mma<NT>(ring + here * L::G_SLOT, acc, [&](int n, int p) { return b[(n * 4 + p) * 32]; });
-                    here = here + 1 == depth ? 0 : here + 1;
-                    __syncwarp();
-                    ask();
+                mx4::copy_chunks(ring_s + at * L::SLOT, src + ka * mx4::CHUNK, apart, policy);
+                at = at + 1 == depth ? 0 : at + 1;
+                ka += g.gw;
+                if (ka >= C1) {
+                    ka = wg;
+                    src = nullptr;
+                    ++ia;
                 }
-                // the group's sums, in the order of its warps: [gate or up][tile][register][lane]
-                float * mine = red + parity * (L::RED / 4) + warp * L::SUMS * 32 + lane;
+            }
+            mx4::copies_commit();
+        };
+#pragma unroll 1
+        for (int i = 0; i < depth; ++i) ask();
+        int here = 0, i = 0;
+        const int set = wg / (2 * NT), job = wg % (2 * NT), col = t2 + (job & 1);
+        const int xe = ((const int *) ((const uint8_t *) g.xf + L::frags(g.d)))[(job >> 1) * 8 + col];
+#pragma unroll 1
+        for (int u; (u = unit(i)) < U; ++i) {
+            const int parity = i & 1;
+            float * sums = red + i % L::BUFFERS * (L::RED / 4);
+            int next = 0;
+            if (wg == 0 && lane == 0) next = atomicAdd(g.sync, 1);
+            float acc[2][NT][4];
 #pragma unroll
-                for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) mine[((m * NT + n) * 4 + i) * 32] = acc[m][n][i];
-                asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / g.gw), "r"(g.gw * 32) : "memory");
-                if (wg < 2 * NT) {
-                    // token 8 n + col, hidden units f + row0 and f + row0 + 8
-                    const int n = wg >> 1, col = t2 + (wg & 1), slot = u / RB1, f = u % RB1 * 16;
-                    const float * src = red + parity * (L::RED / 4) + (warp - wg) * L::SUMS * 32 + (n * 4 + (wg & 1)) * 32 + lane;
-                    float z[2] = {0.f, 0.f}, v[2] = {0.f, 0.f};
+                    for (int c = 0; c < 4; ++c) acc[m][n][c] = 0.f;
+#pragma unroll 1
+            for (int k = wg; k < C1; k += g.gw) {
+                mx4::copies_wait(depth - 1);
+                __syncwarp();
+                const uint4 * b = acts + k * NT * 128;
+                mx4::chunks_mma<NT>(ring + here * L::SLOT, acc, [&](int n, int p) { return b[(n * 4 + p) * 32]; });
+                here = here + 1 == depth ? 0 : here + 1;
+                __syncwarp();
+                ask();
+            }
+            if (wg == 0 && lane == 0) *(volatile long long *) (drawn + group * KNOWN + (i + AHEAD) % KNOWN) = (long long) (i + AHEAD) << 32 | next;
+            // the group's sums, in the order of its warps: [gate or up][tile][register][lane]
+            float * mine = sums + warp * L::SUMS * 32 + lane;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) mine[((m * NT + n) * 4 + c) * 32] = acc[m][n][c];
+            // 2 NT warps finish the unit.  With 8 tokens the first two and the next two take turns, and the two whose turn it is not go on without waiting:
+            // they wait for all at the next unit, so that a buffer is free again three units later (two, where everybody waits).
+            const int barrier = 1 + group * 2 + parity, turn = NT == 1 ? parity : 0;
+            if (NT == 1 && set == (turn ^ 1)) asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "r"(g.gw * 32) : "memory");
+            else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(g.gw * 32) : "memory");
+            if (set == turn) {
+                // token 8 n + col, hidden units f + g and f + g + 8
+                const int n = job >> 1, slot = u / RB1, f = (u - slot * RB1) * 16;
+                const float * from = sums + (warp - wg) * L::SUMS * 32 + (n * 4 + (job & 1)) * 32 + lane;
+                float z[2] = {0.f, 0.f}, v[2] = {0.f, 0.f};
 #pragma unroll 4
-                    for (int w = 0; w < g.gw; ++w)
+                for (int w = 0; w < g.gw; ++w)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            z[i] += src[w * L::SUMS * 32 + 64 * i];
-                            v[i] += src[w * L::SUMS * 32 + NT * 128 + 64 * i];
-                        }
-                    const int * rows = g.gu_exp + ((size_t) expert_of[slot] * RB1 + u % RB1) * 32 + g4;
-                    const int xe = ((const int *) ((const uint8_t *) g.xf + L::frags(g.d)))[n * 8 + col];
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        v[i] = mx4::gated(mx4::times_pow2(z[i], __ldg(rows + 8 * i) + xe), mx4::times_pow2(v[i], __ldg(rows + 16 + 8 * i) + xe), g.act);
-                        top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+                    for (int c = 0; c < 2; ++c) {
+                        z[c] += from[w * L::SUMS * 32 + 64 * c];
+                        v[c] += from[w * L::SUMS * 32 + NT * 128 + 64 * c];
                     }
+                const int * rows = rows_of + i % KNOWN * 32 + g4;
+                uint32_t top = 0;
 #pragma unroll
-                    for (int o = 4; o < 32; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    if (mask[slot] >> (n * 8 + col) & 1) {
-                        const int he = mx4::top_exponent(top);
-                        const float up = mx4::pow2_normal(14 - he);
-                        const size_t tile = ((size_t) slot * C2 + f / mx4::COLS) * NT + n;
-                        __half * to = g.h + ((tile * 4 + f % mx4::COLS / 32) * 32 + col * 4 + g4 / 2) * 8 + (f / 16 & 1) * 4 + (g4 & 1);
-                        to[0] = __float2half_rn(v[0] * up);
-                        to[2] = __float2half_rn(v[1] * up);
-                        if (g4 == 0) {
-                            g.h_exp[(tile * 8 + col) * 8 + f % mx4::COLS / 16] = (uint8_t) (he + BIAS);
-                            atomicMax(h_top + slot * 16 + n * 8 + col, he + BIAS);
-                        }
+                for (int c = 0; c < 2; ++c) {
+                    v[c] = mx4::gated(mx4::times_pow2(z[c], rows[8 * c] + xe), mx4::times_pow2(v[c], rows[16 + 8 * c] + xe), g.act);
+                    top = max(top, __float_as_uint(v[c]) & 0x7fffffffu);
+                }
+#pragma unroll
+                for (int o = 4; o < 32; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                if (mask[slot] >> (n * 8 + col) & 1) {
+                    const int he = mx4::top_exponent(top);
+                    const float up = mx4::pow2_normal(14 - he);
+                    const size_t tile = ((size_t) slot * C2 + f / mx4::COLS) * NT + n;
+                    __half * to = g.h + ((tile * 4 + f % mx4::COLS / 32) * 32 + col * 4 + g4 / 2) * 8 + (f / 16 & 1) * 4 + (g4 & 1);
+                    to[0] = __float2half_rn(v[0] * up);
+                    to[2] = __float2half_rn(v[1] * up);
+                    if (g4 == 0) {
+                        g.h_exp[(tile * 8 + col) * 8 + f % mx4::COLS / 16] = (uint8_t) (he + BIAS);
+                        atomicMax(h_top + slot * 16 + n * 8 + col, he + BIAS);
                     }
                 }
-                parity ^= 1;
             }
-            mx4::copies_wait(0);
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                atomicAdd(done, 1);
-                word[1] = atomicAdd(g.sync, 1);
-            }
-            __syncthreads();
         }
+        mx4::copies_wait(0);
+        __threadfence();
+        if (wg == 0 && lane == 0) atomicAdd(&word[1], i);
+        __syncthreads();
+        if (threadIdx.x == 0) atomicAdd(done, word[1]);
     }
 
     // ---- down: places (64 rows, chunk of an expert's hidden units) i0 .. i1 - 1 of the line ----
@@ -275,14 +299,82 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     if ((int) blockIdx.x >= pieces) return;
     const int i0 = (int) (blockIdx.x * N / pieces), i1 = (int) ((blockIdx.x + 1) * N / pieces);
     const int pair = warp >> 3, wj = warp & 7, depth = g.depth2;
-    const uint8_t * ring = work + warp * depth * L::D_SLOT;
+    const uint8_t * ring = work + warp * depth * L::SLOT;
     const uint32_t ring_s = smem_u32(ring);
     const size_t apart = (size_t) C2 * mx4::CHUNK;
+    // This warp's places: of each piece of 64 rows' places [a, b) those at a + wj, a + wj + 8, ..
+    struct Place {
+        int gr, p, end, slot, c;        // rows, place (slot * C2 + c) and the piece's end there
+    };
+    auto start = [&](Place & x, int gr, int p) {
+        x.gr = gr;
+        x.p = p + wj;
+        x.end = min(P, i1 - gr * P);
+        x.slot = x.p / C2;
+        x.c = x.p - x.slot * C2;
+    };
+    auto advance = [&](Place & x) {              // past the last place: p >= end in the last rows
+        x.p += 8;
+        x.c += 8;
+#pragma unroll 1
+        while (x.c >= C2) { x.c -= C2; ++x.slot; }
+#pragma unroll 1
+        while (x.p >= x.end && (x.gr + 1) * P < i1) start(x, x.gr + 1, 0);
+    };
+    auto begin = [&](Place & x) {
+        start(x, i0 / P, i0 % P);
+#pragma unroll 1
+        while (x.p >= x.end && (x.gr + 1) * P < i1) start(x, x.gr + 1, 0);
+    };
+    Place xa, xh;                                // asked for: chunks; hidden units
+    begin(xa);
+    begin(xh);
+    int at = 0;
+    auto row_block = [&](const Place & x) { return x.gr * 4 + 2 * pair < RB2 ? x.gr * 4 + 2 * pair : 0; };      // (rows behind the last: any)
+    auto ask = [&] {
+        if (xa.p < xa.end) {
+            mx4::copy_chunks(ring_s + at * L::SLOT, g.down + (size_t) expert_of[xa.slot] * g.down_stride + row_block(xa) * apart + xa.c * mx4::CHUNK, apart, policy);
+            at = at + 1 == depth ? 0 : at + 1;
+            advance(xa);
+        }
+        mx4::copies_commit();
+    };
+    // A place's hidden units: fragments (zeros for tokens that have not chosen this expert, and behind the last hidden unit), their exponents' bytes, the
+    // largest byte of this lane's token; the exponents of this lane's rows.
+    struct Hidden {
+        uint4 b[NT][4];
+        uint2 ex[NT];
+        int top[NT], row[4];
+    } next;
+    auto fetch = [&] {
+        if (xh.p >= xh.end) return;
+        const size_t tile = (size_t) (xh.slot * C2 + xh.c) * NT;
+        const int m = mask[xh.slot], * rows = g.down_exp + ((size_t) expert_of[xh.slot] * RB2 + row_block(xh)) * 16 + g4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next.row[i] = __ldg(rows + 8 * i);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const bool chosen = m >> (n * 8 + g4) & 1;
+            next.ex[n] = make_uint2(0u, 0u);
+            next.top[n] = 0;
+            if (chosen) {
+                next.ex[n] = __ldcg((const uint2 *) g.h_exp + (tile + n) * 8 + g4);
+                next.top[n] = __ldcg(h_top + xh.slot * 16 + n * 8 + g4);
+            }
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                next.b[n][p] = make_uint4(0u, 0u, 0u, 0u);
+                if (chosen && xh.c * mx4::COLS + p * 32 < g.F) next.b[n][p] = __ldcg((const uint4 *) g.h + ((tile + n) * 4 + p) * 32 + lane);
+            }
+        }
+    };
+#pragma unroll 1
+    for (int i = 0; i < depth; ++i) ask();
     // the other CTAs' hidden units
     if (threadIdx.x == 0) {
         const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
-        while (ld_acquire(done) < G) {
+        while (ld_acquire(done) < U) {
             if (globaltimer_ns() - t0 > WAIT_NS) {
                 jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 52, blockIdx.x);
                 break;
@@ -291,40 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
         }
     }
     __syncthreads();
-    __threadfence();
-    // This warp's places: of each piece of 64 rows' places [a, b) those at a + wj, a + wj + 8, ..
-    int ga = i0 / P, pa = i0 % P + wj, ea = min(P, i1 - ga * P), at = 0;        // asked for: rows, place, the piece's end
-    auto ask = [&] {
-        while (pa >= ea && (ga + 1) * P < i1) {
-            ++ga;
-            pa = wj;
-            ea = min(P, i1 - ga * P);
-        }
-        if (pa < ea) {
-            const int slot = pa / C2, c = pa % C2, e = expert_of[slot], rb = ga * 4 + 2 * pair < RB2 ? ga * 4 + 2 * pair : 0;      // (rows behind the last: any)
-            const uint32_t to = ring_s + at * L::D_SLOT;
-            mx4::copy_chunks(to, g.down + (size_t) e * g.down_stride + rb * apart + c * mx4::CHUNK, apart, policy);
-            const size_t tile = (size_t) (slot * C2 + c) * NT;
-            const int m = mask[slot];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int p = 0; p < 4; ++p)        // zeros for tokens that have not chosen this expert, and behind the last hidden unit
-                    mx4::copy16_or_zero(to + L::G_SLOT + ((n * 4 + p) * 32 + lane) * 16, (const uint4 *) g.h + ((tile + n) * 4 + p) * 32 + lane,
-                                        (m >> (n * 8 + g4) & 1) && c * mx4::COLS + p * 32 < g.F ? 16 : 0);
-            const uint8_t * more = nullptr;
-            if (lane < 4 * NT) more = g.h_exp + tile * 64 + lane * 16;
-            else if (lane >= 8 && lane < 16) more = (const uint8_t *) (g.down_exp + ((size_t) e * RB2 + rb) * 16) + (lane - 8) * 16;
-            else if (lane >= 16 && lane < 20) more = (const uint8_t *) (h_top + slot * 16) + (lane - 16) * 16;
-            const int off = lane < 8 ? L::H_EXP + lane * 16 : lane < 16 ? L::H_ROW + (lane - 8) * 16 : L::H_TOP + (lane - 16) * 16;
-            if (more != nullptr) mx4::copy16_or_zero(to + off, more, 16);
-            at = at + 1 == depth ? 0 : at + 1;
-            pa += 8;
-        }
-        mx4::copies_commit();
-    };
-#pragma unroll 1
-    for (int i = 0; i < depth; ++i) ask();
+    fetch();
     int here = 0;
 #pragma unroll 1
     for (int gr = i0 / P; gr * P < i1; ++gr) {
@@ -337,47 +396,44 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
 #pragma unroll 1
-        for (int p = a + wj; p < b; p += 8) {
+        while (xh.gr == gr && xh.p < xh.end) {
+            Hidden h = next;
+            const int slot = xh.slot;
+            // all hidden units of a token to the power of two of its largest ones
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t two = (q < 2 ? h.ex[n].x : h.ex[n].y) >> (16 * (q & 1));
+                    const uint32_t f0 = below(h.top[n] - (int) (two & 0xff)), f1 = below(h.top[n] - (int) (two >> 8 & 0xff));
+                    uint4 & v = h.b[n][q];
+                    v.x = mx4::mul2(v.x, f0);
+                    v.y = mx4::mul2(v.y, f0);
+                    v.z = mx4::mul2(v.z, f1);
+                    v.w = mx4::mul2(v.w, f1);
+                }
+            advance(xh);
+            fetch();
             mx4::copies_wait(depth - 1);
             __syncwarp();
-            const uint8_t * chunks = ring + here * L::D_SLOT;
-            const uint4 * frags = (const uint4 *) (chunks + L::G_SLOT) + lane;
-            const int * tops = (const int *) (chunks + L::H_TOP), * rows = (const int *) (chunks + L::H_ROW) + g4, slot = p / C2;
-            uint2 ex[NT];
-            int top[NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                ex[n] = ((const uint2 *) (chunks + L::H_EXP))[n * 8 + g4];
-                top[n] = tops[n * 8 + g4];
-            }
             float y[2][NT][4] = {};
-            mx4::chunks_mma<NT>(chunks, y, [&](int n, int q) {
-                // a token's hidden units of each step to the power of two of its largest ones
-                const uint32_t two = (q < 2 ? ex[n].x : ex[n].y) >> (16 * (q & 1));
-                const uint32_t f0 = below(top[n] - (int) (two & 0xff)), f1 = below(top[n] - (int) (two >> 8 & 0xff));
-                uint4 v = frags[(n * 4 + q) * 32];
-                v.x = mx4::mul2(v.x, f0);
-                v.y = mx4::mul2(v.y, f0);
-                v.z = mx4::mul2(v.z, f1);
-                v.w = mx4::mul2(v.w, f1);
-                return v;
-            });
-            int re[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) re[i] = rows[8 * i] - BIAS - 14;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float2 wt = *(const float2 *) (wtab + slot * 16 + n * 8 + t2);
-                const int2 te = *(const int2 *) (tops + n * 8 + t2);
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[m][n][i] += (i & 1 ? wt.y : wt.x) * mx4::pow2_normal(re[2 * m + (i >> 1)] + (i & 1 ? te.y : te.x)) * y[m][n][i];
-            }
+            mx4::chunks_mma<NT>(ring + here * L::SLOT, y, [&](int n, int q) { return h.b[n][q]; });
             here = here + 1 == depth ? 0 : here + 1;
             __syncwarp();
             ask();
+            float r[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = mx4::pow2(h.row[i]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float2 wt = *(const float2 *) (wtab + slot * 16 + n * 8 + t2);
+                const int e0 = __shfl_sync(0xffffffffu, h.top[n], 4 * t2), e1 = __shfl_sync(0xffffffffu, h.top[n], 4 * t2 + 4);
+                const float w0 = wt.x * mx4::pow2_normal(e0 - BIAS - 14), w1 = wt.y * mx4::pow2_normal(e1 - BIAS - 14);
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[m][n][i] += y[m][n][i] * r[2 * m + (i >> 1)] * (i & 1 ? w1 : w0);
+            }
         }
         float * mine = red + (gr & 1) * (L::RED / 4) + warp * L::SUMS * 32 + lane;
 #pragma unroll
@@ -494,12 +550,13 @@ int launch(const MoeArgs & a, cudaStream_t s) {
     MoeArgs g = a;
     g.depth1 = depth_of<NT>(g.d, g.max_slots, false);
     g.depth2 = depth_of<NT>(g.d, g.max_slots, true);
-    // Warps that share 16 hidden units: as few as leave every group of warps about as many units (four are enough to finish a unit of 16 tokens).
+    // Warps that share 16 hidden units: whatever takes the fullest group the least time, in chunks of one warp (finishing a unit is worth one more).
+    // Four are enough to finish a unit of 16 tokens.
     const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
     const long long units = (long long) g.max_slots * (g.F / 16);
     long long best = -1;
     for (int gw = 4; gw <= NW; gw *= 2) {
-        const long long groups = (long long) sms * (NW / gw), cost = (units + groups - 1) / groups * gw;
+        const long long groups = (long long) sms * (NW / gw), cost = (units + groups - 1) / groups * ((mx4::chunks(g.d) + gw - 1) / gw + 1);
         if (best < 0 || cost < best) { best = cost; g.gw = gw; }
     }
     if (!jib::ensure_dyn_smem(mx4_moe_kernel<NT>, MOST_SMEM, attr_done)) return JIB_E_LAUNCH;

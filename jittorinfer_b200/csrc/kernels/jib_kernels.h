@@ -322,22 +322,22 @@ JIB_EXPORT int jib_selective_scan(const jib_scan * m, int single, int f32, void 
 // type: 0 bf16, 1 fp16, 2 fp32.
 JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * codes, void * scales, long long ld_s, int rows, int cols, void * stream);
 JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long long ld_s, void * out, int type, long long rows, int cols, void * stream);
-JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, int * exps, void * out, int batch, int N, int K,
-                            long long out_stride, int step, int first, void * stream);
+JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, void * out, void * out_scales, void * factors, int * exps, int batch, int N,
+                            int K, int step, int first, void * stream);
 // out[t][n] = sum_k a[t][k] b[n][k], both in 4 bits; scale rows are multiples of 8 bytes apart and 8-byte aligned, codes 16-byte aligned.
 JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_scales, long long a_ld, const void * b_codes, const void * b_scales, long long b_ld,
                               void * out, long long ldo, int out_f32, int T, int N, int K, int * status, void * stream);
 // Products of activations with packed weights: out[r][n] = f(sum_k x[r][k] w[n][k]) (+ residual), gated: act(x Wg^T) * (x Wu^T).
 typedef struct jib_mx4_desc {
     const void * x;            // [rows][K], rows ldx elements apart
-    const void * w;            // packed weights; matrix e starts w_stride bytes behind matrix e - 1
-    const int * w_exp;         // exponents of its rows, in the order of the packed row blocks
+    const void * w;            // packed codes of `batch` matrices
+    const unsigned char * w_scales;        // their scales
     void * out;                // [rows][N], rows ldo elements apart; fp32 with out_f32, else bf16
     const void * residual;     // NULL or [rows][N], rows ldr elements apart (0: one row for all)
     const int * seg;           // NULL, or device int[batch + 1]: rows seg[e] .. seg[e + 1] - 1 belong to matrix e
     const int * src;           // with seg: row r of the result comes from row src[r] of x (NULL: row r)
     int * status;
-    long long ldx, w_stride, ldo, ldr;
+    long long ldx, ldo, ldr;
     int T, N, K, batch, max_rows;          // T: rows of the result; max_rows: the most that one matrix can have
     int gated, act, out_f32, res_f32;
     int x_rows;                // rows of x
@@ -349,14 +349,15 @@ typedef struct jib_mx4_moe_desc {
     const float * logits, * bias;          // router outputs [T][E - n_shared] and the bias of the choice (or NULL); logits NULL: ids and wts
     const int * ids;                       // [T][k]
     const float * wts;
-    const void * gu, * down;               // packed pairs [E][F][d], packed matrices [E][d][F]
+    const void * gu, * down;               // packed codes of pairs [E][F][d], of matrices [E][d][F]
+    const unsigned char * gu_factors, * down_factors;
     const int * gu_exp, * down_exp;        // exponents of their rows
     void * xf;                             // what jib_mx4_moe_prepare made of x
     void * h, * out;                       // scratch; bf16 [T][d]
     float * part;                          // scratch
     int * sync;                            // zeros
     int * status;
-    long long ldr, gu_stride, down_stride;
+    long long ldr;
     int T, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act;
     float scale;
 } jib_mx4_moe_desc;

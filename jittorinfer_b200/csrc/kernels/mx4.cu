@@ -109,12 +109,14 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t * __rest
 }
 
 // ---- weights: row-major codes to the order of mx4.cuh ----------------------------------------------------------------------------
-// Exponents of the rows: the largest scale of a row less 127 and TOP (a row without a number: of scale 1).  One warp a row; step, first: a
-// gated pair's matrices take every second row block.
-__global__ void __launch_bounds__(128) row_exponent_kernel(const uint8_t * __restrict__ scales, long long ld_s, int * __restrict__ exps, int N, int K, int step,
+// Where row r of a matrix stands: of a pair's member `first` of `step` 2, in blocks of 16 rows that alternate.
+__device__ __forceinline__ int packed_row(int r, int step, int first) { return step == 1 ? r : (r / 16 * 2 + first) * 16 + r % 16; }
+
+// Exponents of the rows: the largest scale of a row (1 for one without a number) less 127 and TOP.  One warp a row.
+__global__ void __launch_bounds__(128) row_exponent_kernel(const uint8_t * __restrict__ scales, long long ld_s, int * __restrict__ exps, int N, int K, int R, int step,
                                                            int first) {
-    const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5), m = blockIdx.y, rows = mx4::row_blocks(N) * mx4::ROWS;
-    if (r >= rows) return;
+    const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5), m = blockIdx.y;
+    if (r >= R / step) return;
     int top = -1;
     if (r < N)
         for (int i = lane; i < K / 32; i += 32) {
@@ -122,49 +124,33 @@ __global__ void __launch_bounds__(128) row_exponent_kernel(const uint8_t * __res
             if (e != 255) top = max(top, e);
         }
     top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) exps[((size_t) m * (rows / mx4::ROWS) * step + (r / mx4::ROWS) * step + first) * mx4::ROWS + r % mx4::ROWS] = (top < 0 ? 127 : top) - 127 - mx4::TOP;
+    if (lane == 0) exps[(size_t) m * R + packed_row(r, step, first)] = (top < 0 ? 127 : top) - 127 - mx4::TOP;
 }
 
-// One warp a chunk.
-__global__ void __launch_bounds__(128) pack_kernel(const uint8_t * __restrict__ codes, const uint8_t * __restrict__ scales,
-                                                   long long ld_s, const int * __restrict__ exps, uint8_t * __restrict__ out, int N, int K,
-                                                   long long out_stride, int step, int first) {
-    const int C = mx4::chunks(K), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const long long id = (long long) blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int B = mx4::row_blocks(N);
-    if (id >= (long long) B * C) return;
-    const int b = (int) (id / C), c = (int) (id % C), m = blockIdx.y;
-    codes += (size_t) m * N * (K / 2);
-    scales += (size_t) m * N * ld_s;
-    uint8_t * dst = out + (size_t) m * out_stride + ((size_t) (b * step + first) * C + c) * mx4::CHUNK;
-    const int r0 = b * mx4::ROWS + g, r1 = r0 + 8, k0 = c * mx4::COLS;
-    auto pair = [&](int r, int k) -> uint32_t {       // two codes of row r, columns k and k + 1
-        if (r >= N || k >= K || scales[(size_t) r * ld_s + k / 32] == 255) return 0u;
-        return codes[(size_t) r * (K / 2) + k / 2];
-    };
-    for (int u = 0; u < 2; ++u) {
-        uint32_t w[4];
-        for (int i = 0; i < 4; ++i) {
-            const int k = k0 + 64 * u + 16 * i + 2 * t;
-            w[i] = pair(r0, k) | pair(r1, k) << 8 | pair(r0, k + 8) << 16 | pair(r1, k + 8) << 24;
-        }
-        ((uint4 *) dst)[u * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+// A thread moves 32 columns of a row: 16 bytes and a scale.
+__global__ void __launch_bounds__(256) pack_kernel(const uint8_t * __restrict__ codes, const uint8_t * __restrict__ scales, long long ld_s,
+                                                   const int * __restrict__ exps, uint4 * __restrict__ out, uint8_t * __restrict__ out_scales,
+                                                   uint8_t * __restrict__ factors, int N, int K, int R, int step, int first) {
+    const int C = mx4::chunks(K), rows = R / step, m = blockIdx.y;
+    const long long id = (long long) blockIdx.x * blockDim.x + threadIdx.x;
+    if (id >= (long long) C * rows * 4) return;
+    const int t = (int) (id & 3), r = (int) (id / 4 % rows), c = (int) (id / 4 / rows), b = c * 4 + t;
+    const int row = packed_row(r, step, first);
+    const size_t at = (((size_t) m * C + c) * R + row) * 4 + t;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    int e = 0, f = 0;
+    if (r < N && b < K / 32) {
+        e = scales[((size_t) m * N + r) * ld_s + b];
+        f = e == 255 ? 31 : max(0, 15 + e - 127 - exps[(size_t) m * R + row]);
+        if (e != 255) v = ((const uint4 *) codes)[((size_t) m * N + r) * (K / 32) + b];
     }
-    if (t < 2) {
-        const int r = t == 0 ? r0 : r1, top = exps[((size_t) m * B * step + b * step + first) * mx4::ROWS + r % mx4::ROWS] + 127 + mx4::TOP;
-        uint32_t f = 0;
-        for (int blk = 0; blk < 4; ++blk) {
-            const int kb = k0 / 32 + blk;
-            if (r >= N || kb >= K / 32) continue;
-            const int e = scales[(size_t) r * ld_s + kb];
-            f |= (uint32_t) (e == 255 ? 31 : max(0, 15 + mx4::TOP - (top - e))) << (8 * blk + 2);
-        }
-        ((uint32_t *) (dst + mx4::SCALES))[g * 2 + t] = f;
-    }
+    out[at] = v;
+    out_scales[at] = (uint8_t) e;
+    factors[at] = (uint8_t) (f << 2);
 }
 
 // ---- the product on CUDA cores: fp32 activations, and every shape ------------------------------------------------------------------
-// A warp holds one row block (of a pair: two) for eight rows of x; a lane multiplies its weights of rows g and g + 8, four lanes share a row.
+// A warp holds 16 rows (of a pair: 16 of each matrix) for eight rows of x; a lane multiplies its columns of rows g and g + 8, four lanes share a row.
 constexpr int ST = 8;
 
 template <typename T, bool PAIR>
@@ -173,8 +159,8 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
     constexpr int M = PAIR ? 2 : 1;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, e = blockIdx.z;
-    const int C = mx4::chunks(d.K), b = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (b >= mx4::row_blocks(d.N)) return;
+    const int C = mx4::chunks(d.K), R = mx4::rows_of(d.N, PAIR), b = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (b * 16 >= d.N) return;
     long long base = 0, rows = d.T;
     if (d.seg != nullptr) {
         base = d.seg[e];
@@ -189,46 +175,29 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
         const long long r = base + t0 + (j < nt ? j : 0);
         xr[j] = (const T *) d.x + (d.src != nullptr ? (long long) d.src[r] : r) * d.ldx;
     }
-    const uint8_t * w = (const uint8_t *) d.w + (size_t) e * d.w_stride + (size_t) b * M * C * mx4::CHUNK;
-    const int * ex = d.w_exp + ((size_t) e * mx4::row_blocks(d.N) + b) * M * mx4::ROWS;
-    float unit[M][2];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-        unit[m][0] = mx4::pow2(ex[m * mx4::ROWS + g]);
-        unit[m][1] = mx4::pow2(ex[m * mx4::ROWS + g + 8]);
-    }
     float acc[M][2][ST] = {};
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+        const int k = c * mx4::COLS + 32 * t;
+        if (k >= d.K) continue;
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            const uint8_t * p = w + ((size_t) m * C + c) * mx4::CHUNK;
-            const uint2 f = ((const uint2 *) (p + mx4::SCALES))[g];
-            for (int u = 0; u < 2; ++u) {
-                const uint4 q = ((const uint4 *) p)[u * 32 + lane];
-                const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = c * mx4::COLS + u * 64 + i * 16 + 2 * t;
-                    if (k >= d.K) break;
-                    uint32_t a[4];
-                    mx4::decode(word[i], mx4::scale2(f.x, 2 * u + i / 2), mx4::scale2(f.y, 2 * u + i / 2), a);
-                    float2 v[4];
+            for (int h = 0; h < 2; ++h) {
+                const size_t row = ((size_t) e * C + c) * R + (b * M + m) * 16 + h * 8 + g;
+                const uint4 q = ((const uint4 *) d.w)[row * 4 + t];
+                const uint32_t s = d.w_scales[row * 4 + t], word[4] = {q.x, q.y, q.z, q.w};
+                const float unit = s == 255 ? __uint_as_float(0x7fffffffu) : mx4::pow2((int) s - 127);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        v[j] = __half22float2(*(const __half2 *) &a[j]);
-                        v[j].x *= unit[m][j & 1];
-                        v[j].y *= unit[m][j & 1];
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float w = code_value(word[i] >> (4 * j)) * unit;
+#pragma unroll
+                        for (int n = 0; n < ST; ++n)
+                            if (n < nt) acc[m][h][n] += w * to_f(xr[n][k + 8 * i + j]);
                     }
-#pragma unroll
-                    for (int j = 0; j < ST; ++j) {
-                        if (j >= nt) break;
-                        const float x0 = to_f(xr[j][k]), x1 = to_f(xr[j][k + 1]), x2 = to_f(xr[j][k + 8]), x3 = to_f(xr[j][k + 9]);
-                        acc[m][0][j] += v[0].x * x0 + v[0].y * x1 + v[2].x * x2 + v[2].y * x3;
-                        acc[m][1][j] += v[1].x * x0 + v[1].y * x1 + v[3].x * x2 + v[3].y * x3;
-                    }
-                }
             }
-        }
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -240,7 +209,7 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
                 s[m] += __shfl_xor_sync(0xffffffffu, s[m], 1);
                 s[m] += __shfl_xor_sync(0xffffffffu, s[m], 2);
             }
-            const int n = b * mx4::ROWS + 8 * h + g;
+            const int n = b * 16 + 8 * h + g;
             if (t != 0 || j >= nt || n >= d.N) continue;
             const long long r = base + t0 + j;
             float y = PAIR ? mx4::gated(s[0], s[M - 1], d.act) : s[0];
@@ -295,18 +264,20 @@ JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long 
     return launched();
 }
 
-// Row-major codes and scales of `batch` matrices [N][K] to the order that the products read; exps [batch][row blocks * step][16]; out_stride:
-// bytes of a matrix.
-JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, int * exps, void * out, int batch, int N, int K, long long out_stride,
-                            int step, int first, void * stream) {
+// Row-major codes and scales of `batch` matrices [N][K] to the order that the products read: out, out_scales, factors and exps of all (of pairs, with step 2, the
+// member `first`).
+JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, void * out, void * out_scales, void * factors, int * exps, int batch, int N,
+                            int K, int step, int first, void * stream) {
     if (batch <= 0) return 0;
-    if (N <= 0 || K <= 0 || K % 32 || ld_s < K / 32 || batch > 65535 || step < 1 || first < 0 || first >= step) return JIB_E_ARG;
-    const long long n = (long long) mx4::row_blocks(N) * mx4::chunks(K);
-    if ((n + 3) / 4 > 0x7fffffffll || out_stride < n * step * mx4::CHUNK) return JIB_E_ARG;
+    if (N <= 0 || K <= 0 || K % 32 || ld_s < K / 32 || batch > 65535 || step < 1 || step > 2 || first < 0 || first >= step) return JIB_E_ARG;
+    if (((uintptr_t) codes | (uintptr_t) out) & 15) return JIB_E_ALIGN;
+    const int R = mx4::rows_of(N, step == 2);
+    const long long n = (long long) mx4::chunks(K) * (R / step) * 4;
+    if ((n + 255) / 256 > 0x7fffffffll) return JIB_E_ARG;
     cudaStream_t s = (cudaStream_t) stream;
-    row_exponent_kernel<<<dim3(mx4::row_blocks(N) * 4, batch), 128, 0, s>>>((const uint8_t *) scales, ld_s, exps, N, K, step, first);
-    pack_kernel<<<dim3((unsigned) ((n + 3) / 4), batch), 128, 0, s>>>((const uint8_t *) codes, (const uint8_t *) scales, ld_s, exps, (uint8_t *) out, N, K,
-                                                                     out_stride, step, first);
+    row_exponent_kernel<<<dim3((R / step + 3) / 4, batch), 128, 0, s>>>((const uint8_t *) scales, ld_s, exps, N, K, R, step, first);
+    pack_kernel<<<dim3((unsigned) ((n + 255) / 256), batch), 256, 0, s>>>((const uint8_t *) codes, (const uint8_t *) scales, ld_s, exps, (uint4 *) out,
+                                                                         (uint8_t *) out_scales, (uint8_t *) factors, N, K, R, step, first);
     return launched();
 }
 
@@ -314,7 +285,7 @@ JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, int f32, void * stre
     if (d->T <= 0) return 0;
     if (d->N <= 0 || d->K <= 0 || d->K % 32 || d->batch < 1 || d->batch > 65535) return JIB_E_ARG;
     const long long rows = d->seg != nullptr ? d->max_rows : d->T;
-    const dim3 grid((mx4::row_blocks(d->N) + 3) / 4, (unsigned) ((rows + ST - 1) / ST), d->batch);
+    const dim3 grid(((d->N + 15) / 16 + 3) / 4, (unsigned) ((rows + ST - 1) / ST), d->batch);
     if ((rows + ST - 1) / ST > 65535) return JIB_E_ARG;
     cudaStream_t s = (cudaStream_t) stream;
     if (f32) {

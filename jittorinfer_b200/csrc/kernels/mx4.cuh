@@ -1,30 +1,31 @@
 // Microscaled 4-bit weights in the order in which the products read them.
 //
-// A matrix [N][K] is cut into row blocks of 16 rows and chunks of 128 columns.  A chunk is 1088 bytes: two units of 64 columns, 16 bytes for
-// each lane of a warp (lane = 4 g + t, word i = columns 16 i .. 16 i + 15 of the unit), then 8 scale bytes for each g: the four blocks of 32
-// columns of row g, those of row g + 8.  The chunks of a row block follow one another, a gated pair alternates row blocks (gate, up), and
-// everything behind the last row or column is zero.  A word's bytes are what one lane feeds mma.m16n8k16 as the fragment of A: row g
-// columns 2t, 2t + 1; row g + 8 the same; row g columns 2t + 8, 2t + 9; row g + 8 the same.
+// A matrix [N][K] is cut into chunks of 128 columns.  codes [chunk][row][64 bytes], scales [chunk][row][4 bytes], rows padded to a multiple of 32, all
+// zeros behind the last row or column; codes two to a byte, the lower half first, scales E8M0.  A gated pair is one matrix in which 16 rows of the
+// gate alternate with 16 of the up matrix.  So a tile of rows is one block of memory for the tensor maps of the tiled products, and 32
+// rows of a chunk are 2048 + 128 bytes in a row for the products of a few tokens.  Those read `factors` in place of the scales (below).
 //
-// Decoding is one conversion instruction a byte (E2M1 pair to fp16 pair) and one product with the block's scale.  (Masks and shifts to bf16 took
-// eleven integer instructions a word; 16 warps of an SM decoded and multiplied 38 weights a clock so, 66 with the conversion.)  fp16 cannot
-// hold every scale, so scales are kept relative to the largest of their row: the scale byte is the upper byte of 2^(13 - (largest - scale)) in fp16,
-// exact up to 27 binades below the largest and 0 beyond, where a weight is less than 2^-25 of the row's largest; and a row has an exponent
-// (int, next to the packed bytes) that its sum is multiplied with.  Infinity times the code 0 makes a block NaN.
+// The latter feed mma.m16n8k16 in fp16.  The order of columns within a chunk is free as long as the activations share it: lane 4 g + t
+// holds the 32 columns 32 t .. of rows g and g + 8, that is 16 bytes and one scale each, and step s of the chunk's eight multiplies its columns 4 s
+// .. 4 s + 3.  Decoding is one conversion instruction a byte (E2M1 pair to fp16 pair) and one product with the block's scale.  (Masks and shifts to
+// bf16 took eleven integer instructions for eight weights; 16 warps of an SM decoded and multiplied 38 weights a clock so, 66 with the
+// conversion.)  fp16 cannot hold every scale, so a factor is relative to the largest scale of its row: the upper byte of 2^(13 - (largest -
+// scale)) in fp16, exact up to 27 binades below the largest and 0 beyond, where a weight is less than 2^-25 of the row's largest; and a row has an
+// exponent (int) that its sum is multiplied with.  A block without a number (scale 255) has codes 0 and a factor of infinity.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
 
 namespace mx4 {
 
-constexpr int ROWS = 16;              // rows of a block
 constexpr int COLS = 128;             // columns of a chunk
-constexpr int CHUNK = 1088;           // bytes of a chunk: 2 * 512 + 8 * 8
-constexpr int SCALES = 1024;          // offset of the scales in a chunk
+constexpr int CODES = 64, SCALES = 4; // bytes of a row in it
+constexpr int ROWS = 32;              // rows are padded to
 constexpr int TOP = 13;               // the largest scale of a row is 2^TOP: 6 * 2^13 is a number in fp16
 
 __host__ __device__ inline int chunks(int K) { return (K + COLS - 1) / COLS; }
-__host__ __device__ inline int row_blocks(int N) { return (N + ROWS - 1) / ROWS; }
+// Rows of a matrix, of a gated pair.
+__host__ __device__ inline int rows_of(int N, bool pair) { return pair ? (N + 15) / 16 * 32 : (N + ROWS - 1) / ROWS * ROWS; }
 
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t s) {
     __half2 x, y;
@@ -34,24 +35,32 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t s) {
     return *(uint32_t *) &x;
 }
 
-// The fragment (four registers of two fp16) of a word; s0, s1: scales of row g and row g + 8, twice in a register.
-__device__ __forceinline__ void decode(uint32_t w, uint32_t s0, uint32_t s1, uint32_t (&a)[4]) {
-    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+// The fragments (four registers of two fp16) of two steps from four bytes of row g and of row g + 8; s0, s1: their scales, twice in a register.
+__device__ __forceinline__ void decode(uint32_t w0, uint32_t w1, uint32_t s0, uint32_t s1, uint32_t (&a)[2][4]) {
+    asm("{\n\t.reg .b8 b0, b1, b2, b3, c0, c1, c2, c3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %8;\n\t"
+        "mov.b32 {c0, c1, c2, c3}, %9;\n\t"
         "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-        : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-        : "r"(w));
-    a[0] = mul2(a[0], s0);
-    a[1] = mul2(a[1], s1);
-    a[2] = mul2(a[2], s0);
-    a[3] = mul2(a[3], s1);
+        "cvt.rn.f16x2.e2m1x2 %1, c0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, c1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %4, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %5, c2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %6, b3;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %7, c3;\n\t}"
+        : "=r"(a[0][0]), "=r"(a[0][1]), "=r"(a[0][2]), "=r"(a[0][3]), "=r"(a[1][0]), "=r"(a[1][1]), "=r"(a[1][2]), "=r"(a[1][3])
+        : "r"(w0), "r"(w1));
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        a[s][0] = mul2(a[s][0], s0);
+        a[s][1] = mul2(a[s][1], s1);
+        a[s][2] = mul2(a[s][2], s0);
+        a[s][3] = mul2(a[s][3], s1);
+    }
 }
 
-// Scale byte `j` of a word as a pair of fp16.
-__device__ __forceinline__ uint32_t scale2(uint32_t f, int j) { return __byte_perm(f, 0u, 0x0404u | (uint32_t) j << 4 | (uint32_t) j << 12); }
+// A factor's byte as a pair of fp16.
+__device__ __forceinline__ uint32_t factor2(uint32_t f) { return f * 0x01000100u; }
 
 // 2^e in fp32 for -126 <= e <= 127; 0 or infinity outside
 __device__ __forceinline__ float pow2_normal(int e) { return __uint_as_float((uint32_t) (min(max(e, -127), 128) + 127) << 23); }

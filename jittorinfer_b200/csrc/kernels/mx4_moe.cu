@@ -35,16 +35,16 @@ struct MoeArgs {
     const float * logits, * bias;            // logits NULL: ids and weights are given
     const int * ids;
     const float * wts;
-    const uint8_t * gu, * down;
+    const uint8_t * gu, * down, * gu_factors, * down_factors;
     const int * gu_exp, * down_exp;
     __half * h;                              // hidden units: [slot][chunks of F][NT] fragments, each 16 of a token scaled by a power of two ...
-    uint8_t * h_exp;                         // ... [slot][chunk][token][step], BIAS more than its exponent
+    uint8_t * h_exp;                         // ... [slot][chunk][token][16 units], BIAS more than its exponent
     float * part;                            // [pieces][512 NT]
     bf16 * out;
     int * sync;                              // zeros: units of gate and up drawn, units done (and two more), the largest byte of h_exp of each slot and token
                                              // [slots][16], pieces done of each 64 rows
     int * status;
-    long long ldr, gu_stride, down_stride;
+    long long ldr;
     int T, max_slots, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act, gw, depth1, depth2, warm;
     float scale;
 };
@@ -55,14 +55,13 @@ struct Layout {
     static_assert((48 + 4 * KNOWN * 8) % 16 == 0, "the exponents' place");
     static constexpr int SUMS = 8 * NT;                           // of a lane
     static constexpr int RED = NW * 32 * SUMS * 4;
-    static constexpr int SLOT = 2 * mx4::CHUNK;
     static constexpr int BUFFERS = NT == 1 ? 3 : 2;               // of sums (see where a unit of gate and up is finished)
     static_assert(BUFFERS * RED >= NW * (MAX_E + 32) * 4, "scratch of the choice");
     __host__ __device__ static int frags(int d) { return mx4::chunks(d) * NT * mx4::FRAG; }
     __host__ __device__ static int tables(int slots) { return (slots * 64 + MAX_E * 4 * 3 + MAX_T * MAX_K * 8 + 64 + 4 * KNOWN * (8 + 128) + 127) / 128 * 128; }
     __host__ __device__ static int base(int slots) { return 128 + tables(slots) + BUFFERS * RED; }
     __host__ __device__ static int bytes(int d, int slots, int depth1, int depth2) {
-        const int a = frags(d) + NW * depth1 * SLOT, b = NW * depth2 * SLOT;
+        const int a = frags(d) + NW * depth1 * mx4::SLOT, b = NW * depth2 * mx4::SLOT;
         return base(slots) + (a > b ? a : b);
     }
 };
@@ -154,7 +153,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
             }
     }
     __syncthreads();
-    const int slots = word[0], C1 = mx4::chunks(g.d), C2 = mx4::chunks(g.F), RB1 = g.F / 16, RB2 = g.d / 16, G = gridDim.x, U = slots * RB1;
+    const int slots = word[0], C1 = mx4::chunks(g.d), C2 = mx4::chunks(g.F), RB1 = g.F / 16, G = gridDim.x, U = slots * RB1;
     int * done = g.sync + 1, * h_top = g.sync + 4, * pieces_done = h_top + g.max_slots * 16;
     const uint64_t policy = l2_policy_evict_first();
 
@@ -162,10 +161,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     if (!mx4::wait_all(acts_full, 0) && lane == 0) jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 51, warp);
     {
         const int group = warp / g.gw, wg = warp % g.gw, count = (C1 - wg + g.gw - 1) / g.gw, depth = min(g.depth1, max(2 * count, 1));
-        const uint8_t * ring = work + L::frags(g.d) + warp * g.depth1 * L::SLOT;
+        const uint8_t * ring = work + L::frags(g.d) + warp * g.depth1 * mx4::SLOT;
         const uint32_t ring_s = smem_u32(ring);
         const uint4 * acts = (const uint4 *) work + lane;
-        const size_t apart = (size_t) C1 * mx4::CHUNK;
+        const int R1 = 2 * g.F;
         int * rows_of = exps + group * KNOWN * 32;
         // The group's unit number i, once it is drawn (by the group's first warp, which draws number i + 3 before it begins with number i + 1).
         auto unit = [&](int i) -> int {
@@ -180,22 +179,22 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
         };
         // Asks for this warp's next chunks: of unit after unit the chunks wg, wg + gw .., at most two units ahead; and for the exponents of a unit's rows.
         int ia = 0, ka = wg, at = 0, ua = 0;
-        const uint8_t * src = nullptr;
+        long long src = -1;                 // the first chunk's row among all
         auto ask = [&] {
-            if (src == nullptr && ua < U) ua = unit(ia);
+            if (src < 0 && ua < U) ua = unit(ia);
             if (ua < U && ka < C1) {
-                if (src == nullptr) {
+                if (src < 0) {
                     const int slot = ua / RB1, rb = ua - slot * RB1, e = expert_of[slot];
-                    src = g.gu + (size_t) e * g.gu_stride + (size_t) rb * 2 * apart;
-                    if (wg == 0 && lane < 8)
-                        mx4::copy16_or_zero(smem_u32(rows_of + (ia % KNOWN) * 32 + lane * 4), g.gu_exp + ((size_t) e * RB1 + rb) * 32 + lane * 4, 16);
+                    src = (long long) e * C1 * R1 + rb * 32;
+                    if (lane < 8 && wg < 1)
+                        mx4::copy16(smem_u32(rows_of + (ia % KNOWN) * 32 + lane * 4), g.gu_exp + (size_t) e * R1 + rb * 32 + lane * 4, policy);
                 }
-                mx4::copy_chunks(ring_s + at * L::SLOT, src + ka * mx4::CHUNK, apart, policy);
+                mx4::copy_chunk(ring_s + at * mx4::SLOT, g.gu, g.gu_factors, (size_t) (src + (long long) ka * R1), policy);
                 at = at + 1 == depth ? 0 : at + 1;
                 ka += g.gw;
                 if (ka >= C1) {
                     ka = wg;
-                    src = nullptr;
+                    src = -1;
                     ++ia;
                 }
             }
@@ -224,7 +223,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
                 mx4::copies_wait(depth - 1);
                 __syncwarp();
                 const uint4 * b = acts + k * NT * 128;
-                mx4::chunks_mma<NT>(ring + here * L::SLOT, acc, [&](int n, int p) { return b[(n * 4 + p) * 32]; });
+                mx4::chunk_mma<NT>(ring + here * mx4::SLOT, acc, [&](int n, int p) { return b[(n * 4 + p) * 32]; });
                 here = here + 1 == depth ? 0 : here + 1;
                 __syncwarp();
                 ask();
@@ -256,21 +255,21 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
                         v[c] += from[w * L::SUMS * 32 + NT * 128 + 64 * c];
                     }
                 const int * rows = rows_of + i % KNOWN * 32 + g4;
-                uint32_t top = 0;
+                uint32_t most = 0;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     v[c] = mx4::gated(mx4::times_pow2(z[c], rows[8 * c] + xe), mx4::times_pow2(v[c], rows[16 + 8 * c] + xe), g.act);
-                    top = max(top, __float_as_uint(v[c]) & 0x7fffffffu);
+                    most = max(most, __float_as_uint(v[c]) & 0x7fffffffu);
                 }
 #pragma unroll
-                for (int o = 4; o < 32; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                for (int o = 4; o < 32; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
                 if (mask[slot] >> (n * 8 + col) & 1) {
-                    const int he = mx4::top_exponent(top);
+                    const int he = mx4::top_exponent(most);
                     const float up = mx4::pow2_normal(14 - he);
                     const size_t tile = ((size_t) slot * C2 + f / mx4::COLS) * NT + n;
-                    __half * to = g.h + ((tile * 4 + f % mx4::COLS / 32) * 32 + col * 4 + g4 / 2) * 8 + (f / 16 & 1) * 4 + (g4 & 1);
+                    __half * to = g.h + ((tile * 4 + f % 32 / 8) * 32 + col * 4 + f % mx4::COLS / 32) * 8 + g4;
                     to[0] = __float2half_rn(v[0] * up);
-                    to[2] = __float2half_rn(v[1] * up);
+                    to[32 * 8] = __float2half_rn(v[1] * up);
                     if (g4 == 0) {
                         g.h_exp[(tile * 8 + col) * 8 + f % mx4::COLS / 16] = (uint8_t) (he + BIAS);
                         atomicMax(h_top + slot * 16 + n * 8 + col, he + BIAS);
@@ -299,9 +298,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     if ((int) blockIdx.x >= pieces) return;
     const int i0 = (int) (blockIdx.x * N / pieces), i1 = (int) ((blockIdx.x + 1) * N / pieces);
     const int pair = warp >> 3, wj = warp & 7, depth = g.depth2;
-    const uint8_t * ring = work + warp * depth * L::SLOT;
+    const uint8_t * ring = work + warp * depth * mx4::SLOT;
     const uint32_t ring_s = smem_u32(ring);
-    const size_t apart = (size_t) C2 * mx4::CHUNK;
     // This warp's places: of each piece of 64 rows' places [a, b) those at a + wj, a + wj + 8, ..
     struct Place {
         int gr, p, end, slot, c;        // rows, place (slot * C2 + c) and the piece's end there
@@ -330,10 +328,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     begin(xa);
     begin(xh);
     int at = 0;
-    auto row_block = [&](const Place & x) { return x.gr * 4 + 2 * pair < RB2 ? x.gr * 4 + 2 * pair : 0; };      // (rows behind the last: any)
+    auto first_row = [&](const Place & x) { return x.gr * 64 + pair * 32 < g.d ? x.gr * 64 + pair * 32 : 0; };      // (rows behind the last: any)
     auto ask = [&] {
         if (xa.p < xa.end) {
-            mx4::copy_chunks(ring_s + at * L::SLOT, g.down + (size_t) expert_of[xa.slot] * g.down_stride + row_block(xa) * apart + xa.c * mx4::CHUNK, apart, policy);
+            mx4::copy_chunk(ring_s + at * mx4::SLOT, g.down, g.down_factors, ((size_t) expert_of[xa.slot] * C2 + xa.c) * g.d + first_row(xa), policy);
             at = at + 1 == depth ? 0 : at + 1;
             advance(xa);
         }
@@ -343,28 +341,29 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     // largest byte of this lane's token; the exponents of this lane's rows.
     struct Hidden {
         uint4 b[NT][4];
-        uint2 ex[NT];
+        uint32_t ex[NT];
         int top[NT], row[4];
     } next;
     auto fetch = [&] {
         if (xh.p >= xh.end) return;
         const size_t tile = (size_t) (xh.slot * C2 + xh.c) * NT;
-        const int m = mask[xh.slot], * rows = g.down_exp + ((size_t) expert_of[xh.slot] * RB2 + row_block(xh)) * 16 + g4;
+        const int m = mask[xh.slot], * rows = g.down_exp + (size_t) expert_of[xh.slot] * g.d + first_row(xh) + g4;
+        const bool units = xh.c * mx4::COLS + 32 * (lane & 3) < g.F;
 #pragma unroll
         for (int i = 0; i < 4; ++i) next.row[i] = __ldg(rows + 8 * i);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const bool chosen = m >> (n * 8 + g4) & 1;
-            next.ex[n] = make_uint2(0u, 0u);
+            next.ex[n] = 0u;
             next.top[n] = 0;
             if (chosen) {
-                next.ex[n] = __ldcg((const uint2 *) g.h_exp + (tile + n) * 8 + g4);
+                next.ex[n] = __ldcg((const unsigned short *) g.h_exp + ((tile + n) * 8 + g4) * 4 + (lane & 3));
                 next.top[n] = __ldcg(h_top + xh.slot * 16 + n * 8 + g4);
             }
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 next.b[n][p] = make_uint4(0u, 0u, 0u, 0u);
-                if (chosen && xh.c * mx4::COLS + p * 32 < g.F) next.b[n][p] = __ldcg((const uint4 *) g.h + ((tile + n) * 4 + p) * 32 + lane);
+                if (chosen && units) next.b[n][p] = __ldcg((const uint4 *) g.h + ((tile + n) * 4 + p) * 32 + lane);
             }
         }
     };
@@ -401,23 +400,23 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
             const int slot = xh.slot;
             // all hidden units of a token to the power of two of its largest ones
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                const uint32_t f0 = below(h.top[n] - (int) (h.ex[n] & 0xff)), f1 = below(h.top[n] - (int) (h.ex[n] >> 8));
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const uint32_t two = (q < 2 ? h.ex[n].x : h.ex[n].y) >> (16 * (q & 1));
-                    const uint32_t f0 = below(h.top[n] - (int) (two & 0xff)), f1 = below(h.top[n] - (int) (two >> 8 & 0xff));
                     uint4 & v = h.b[n][q];
-                    v.x = mx4::mul2(v.x, f0);
-                    v.y = mx4::mul2(v.y, f0);
-                    v.z = mx4::mul2(v.z, f1);
-                    v.w = mx4::mul2(v.w, f1);
+                    v.x = mx4::mul2(v.x, q < 2 ? f0 : f1);
+                    v.y = mx4::mul2(v.y, q < 2 ? f0 : f1);
+                    v.z = mx4::mul2(v.z, q < 2 ? f0 : f1);
+                    v.w = mx4::mul2(v.w, q < 2 ? f0 : f1);
                 }
+            }
             advance(xh);
             fetch();
             mx4::copies_wait(depth - 1);
             __syncwarp();
             float y[2][NT][4] = {};
-            mx4::chunks_mma<NT>(ring + here * L::SLOT, y, [&](int n, int q) { return h.b[n][q]; });
+            mx4::chunk_mma<NT>(ring + here * mx4::SLOT, y, [&](int n, int q) { return h.b[n][q]; });
             here = here + 1 == depth ? 0 : here + 1;
             __syncwarp();
             ask();
@@ -523,14 +522,9 @@ __global__ void __launch_bounds__(GATE_NT) mx4_prepare_kernel(const bf16 * __res
     const int ex = mx4::top_exponent(top);
     const float unit = mx4::pow2(14 - ex);
     if (threadIdx.x == 0) ((int *) (xf + (size_t) C * NT * 128))[n] = ex - 14;
-    for (int i = threadIdx.x; i < C * 16; i += GATE_NT) {          // chunk, pair of steps, quarter of a step
-        const int t = i & 3, pair = i >> 2 & 3, c = i >> 4;
-        uint2 a = make_uint2(0u, 0u), b = a;
-        if (n < T) {
-            a = mx4::frag_step(row, c * 8 + pair * 2, t, d, unit);
-            b = mx4::frag_step(row, c * 8 + pair * 2 + 1, t, d, unit);
-        }
-        xf[((c * NT + (n >> 3)) * 4 + pair) * 32 + (n & 7) * 4 + t] = make_uint4(a.x, a.y, b.x, b.y);
+    for (int i = threadIdx.x; i < C * 16; i += GATE_NT) {          // eight columns
+        const int p = i & 3, t = i >> 2 & 3, c = i >> 4;
+        xf[((c * NT + (n >> 3)) * 4 + p) * 32 + (n & 7) * 4 + t] = n < T ? mx4::frag_of(row, c * mx4::COLS + 32 * t + 8 * p, d, unit) : make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
@@ -608,14 +602,14 @@ JIB_EXPORT int jib_mx4_moe(const jib_mx4_moe_desc * m, void * stream) {
     if (m->logits == nullptr ? (m->ids == nullptr || m->wts == nullptr || m->n_shared != 0)
                              : (m->n_shared >= m->E || m->k > m->E - m->n_shared || m->n_group < 1 || m->n_group > 32 || (m->E - m->n_shared) % m->n_group))
         return JIB_E_ARG;
-    if (((uintptr_t) m->gu | (uintptr_t) m->down | (uintptr_t) m->gu_stride | (uintptr_t) m->down_stride | (uintptr_t) m->h | (uintptr_t) m->xf | (uintptr_t) m->part | (uintptr_t) m->sync | (uintptr_t) m->down_exp) & 15)
+    if (((uintptr_t) m->gu | (uintptr_t) m->down | (uintptr_t) m->gu_factors | (uintptr_t) m->down_factors | (uintptr_t) m->gu_exp | (uintptr_t) m->h | (uintptr_t) m->xf | (uintptr_t) m->part | (uintptr_t) m->sync | (uintptr_t) m->down_exp) & 15)
         return JIB_E_ALIGN;
     MoeArgs a;
     a.xf = (const uint4 *) m->xf; a.residual = (const bf16 *) m->residual; a.logits = m->logits; a.bias = m->bias; a.ids = m->ids; a.wts = m->wts;
     a.gu = (const uint8_t *) m->gu; a.down = (const uint8_t *) m->down; a.gu_exp = m->gu_exp; a.down_exp = m->down_exp;
     a.max_slots = slots_of(m->T, m->k + m->n_shared, m->E);
     a.h = (__half *) m->h; a.h_exp = (uint8_t *) m->h + (long long) a.max_slots * mx4::chunks(m->F) * (m->T <= 8 ? 1 : 2) * mx4::FRAG; a.part = m->part; a.out = (bf16 *) m->out; a.sync = m->sync; a.status = m->status;
-    a.ldr = m->ldr; a.gu_stride = m->gu_stride; a.down_stride = m->down_stride;
+    a.ldr = m->ldr; a.gu_factors = m->gu_factors; a.down_factors = m->down_factors;
     a.T = m->T; a.d = m->d; a.F = m->F; a.E = m->E; a.k = m->k; a.n_group = m->n_group; a.topk_group = m->topk_group; a.norm = m->norm; a.sigmoid = m->sigmoid;
     a.n_shared = m->n_shared; a.group_top2 = m->group_top2; a.act = m->act; a.scale = m->scale;
     a.warm = jib::warm_enabled();

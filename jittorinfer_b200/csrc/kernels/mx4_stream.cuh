@@ -1,13 +1,13 @@
-// What the products of a few rows of activations with packed 4-bit weights share: a chunk of weights times tiles of 8 rows by mma, the loads
-// that bring chunks, and the order in which a warp reads activations.
+// What the products of a few rows of activations with packed 4-bit weights share: 32 rows of a chunk of weights times tiles of 8 rows of activations by
+// mma, the copies that bring chunks, and the order in which a warp reads activations.
 //
-// Up to 16 rows the stream of weights counts, 2048 weights in 1088 bytes.  A weight is decoded once for all rows: per eight weights of a lane four
-// conversions, four products and an mma for each tile of 8 rows.  The mma bound it: 14 clocks each on a quarter of an SM, 70 weights a
-// clock and SM for one tile (the memory delivers 43), 35 for two.
+// Up to 16 rows the stream of weights counts, 4096 weights in 2176 bytes, and the instructions on its way: at the memory's rate an SM gets 43
+// weights a clock, 2.8 issue slots (of 32 lanes) a weight.  A weight is decoded once for all rows.  The mma bound it in the end: 14 clocks each
+// on a quarter of an SM, 70 weights a clock and SM for one tile, 35 for two.
 //
 // Activations are fp16, each row scaled by a power of two to a largest magnitude in [2^14, 2^15): exact for bf16 values down to 2^-29 of
-// the row's largest, and within 2^-39 of it below.  They are read as fragments of B: for a chunk, a tile of 8 rows and a pair of 16-column
-// steps, lane 4 n + t holds 16 bytes, columns 2t, 2t + 1, 2t + 8, 2t + 9 of the first step and of the second of row n.
+// the row's largest, and within 2^-39 of it below.  They are read as fragments of B: for a chunk, a tile of 8 rows and two steps 2 p, 2 p + 1, lane 4 n + t
+// holds the eight columns 32 t + 8 p .. of row n.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -24,22 +24,18 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two chunks, `apart` bytes from one another in memory, side by side to this warp's shared memory: read once, so past the L1 and first to leave the
-// L2 (with sm100::l2_policy_evict_first).
+constexpr int SLOT = 32 * (CODES + SCALES);      // 32 rows of a chunk in shared memory: codes, then factors
+
+// Read once: first to leave the L2 (with sm100::l2_policy_evict_first).
 __device__ __forceinline__ void copy16(uint32_t dst, const void * src, uint64_t policy) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
-__device__ __forceinline__ void copy_chunks(uint32_t dst, const uint8_t * src, size_t apart, uint64_t policy) {
+// 32 rows of a chunk: row `row` of codes and factors on.
+__device__ __forceinline__ void copy_chunk(uint32_t dst, const uint8_t * codes, const uint8_t * factors, size_t row, uint64_t policy) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) copy16(dst + m * CHUNK + (u * 32 + lane) * 16, src + m * apart + (u * 32 + lane) * 16, policy);
-    if (lane < 8) copy16(dst + (lane >> 2) * CHUNK + SCALES + (lane & 3) * 16, src + (lane >> 2) * apart + SCALES + (lane & 3) * 16, policy);
-}
-// The same through no cache policy; `bytes` 16, or 0: zeros.
-__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void * src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    for (int i = 0; i < 4; ++i) copy16(dst + (i * 32 + lane) * 16, codes + row * CODES + (i * 32 + lane) * 16, policy);
+    if (lane < 8) copy16(dst + 32 * CODES + lane * 16, factors + row * SCALES + lane * 16, policy);
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // All but the last n groups of copies are there (n: 0 .. 3).
@@ -50,32 +46,35 @@ __device__ __forceinline__ void copies_wait(int n) {
     else asm volatile("cp.async.wait_group 3;" ::: "memory");
 }
 
-// y[m] (row g: columns 2t, 2t + 1; row g + 8) += chunk m x the same fragments: frag(n, pair) gives this lane's 16 bytes.
+// y[m] (row g: columns 2t, 2t + 1; row g + 8) += rows 16 m .. of a chunk x the same fragments: frag(n, p) gives this lane's 16 bytes.
 template <int NT, typename F>
-__device__ __forceinline__ void chunks_mma(const uint8_t * chunks, float (&y)[2][NT][4], F frag) {
+__device__ __forceinline__ void chunk_mma(const uint8_t * chunk, float (&y)[2][NT][4], F frag) {
     const int lane = threadIdx.x & 31;
-    uint2 f[2];
+    uint32_t s[2][2];
+    uint4 q[2][2];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) f[m] = *(const uint2 *) (chunks + m * CHUNK + SCALES + (lane >> 2) * 8);
-    uint4 q[2];
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {          // 32 columns: two steps, one scale a row
-        if ((p & 1) == 0)
+        for (int h = 0; h < 2; ++h) {
+            const int at = (m * 16 + h * 8) * 4 + lane;          // 4 (row) + t
+            s[m][h] = factor2(chunk[32 * CODES + at]);
+            q[m][h] = ((const uint4 *) chunk)[at];
+        }
 #pragma unroll
-            for (int m = 0; m < 2; ++m) q[m] = *(const uint4 *) (chunks + m * CHUNK + ((p >> 1) * 32 + lane) * 16);
+    for (int p = 0; p < 4; ++p) {
         uint4 v[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) v[n] = frag(n, p);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            const uint32_t s0 = scale2(f[m].x, p), s1 = scale2(f[m].y, p);
-            uint32_t a[4];
-            decode(p & 1 ? q[m].z : q[m].x, s0, s1, a);
+            const uint4 & a = q[m][0], & b = q[m][1];
+            uint32_t f[2][4];
+            decode(p == 0 ? a.x : p == 1 ? a.y : p == 2 ? a.z : a.w, p == 0 ? b.x : p == 1 ? b.y : p == 2 ? b.z : b.w, s[m][0], s[m][1], f);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816(y[m][n], a, v[n].x, v[n].y);
-            decode(p & 1 ? q[m].w : q[m].y, s0, s1, a);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816(y[m][n], a, v[n].z, v[n].w);
+            for (int n = 0; n < NT; ++n) {
+                mma16816(y[m][n], f[0], v[n].x, v[n].y);
+                mma16816(y[m][n], f[1], v[n].z, v[n].w);
+            }
         }
     }
 }
@@ -98,12 +97,20 @@ __device__ __forceinline__ bool wait_all(uint64_t * bar, uint32_t parity) { retu
 // The exponent of a largest magnitude (bits of the fp32 value): values times 2^(14 - exponent) fit fp16.  0 and what is below 2^-112 count as that.
 __device__ __forceinline__ int top_exponent(uint32_t bits) { return max(min((int) (bits >> 23), 254) - 127, -112); }
 
-// Columns 16 s + 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a row, scaled, as two registers of fp16 (zeros from column K on; K a multiple of 16).
-__device__ __forceinline__ uint2 frag_step(const __nv_bfloat16 * row, int s, int t, int K, float unit) {
-    if (16 * s >= K) return make_uint2(0u, 0u);
-    const float2 a = __bfloat1622float2(*(const __nv_bfloat162 *) (row + 16 * s + 2 * t)), b = __bfloat1622float2(*(const __nv_bfloat162 *) (row + 16 * s + 2 * t + 8));
-    const __half2 x = __floats2half2_rn(a.x * unit, a.y * unit), y = __floats2half2_rn(b.x * unit, b.y * unit);
-    return make_uint2(*(const uint32_t *) &x, *(const uint32_t *) &y);
+// Eight columns of a row from k on, scaled, as fp16 (zeros from column K on; K a multiple of 32).
+__device__ __forceinline__ uint4 frag_of(const __nv_bfloat16 * row, int k, int K, float unit) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (k >= K) return v;
+    const uint4 in = *(const uint4 *) (row + k);
+    const uint32_t w[4] = {in.x, in.y, in.z, in.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __bfloat1622float2(*(const __nv_bfloat162 *) &w[i]);
+        const __half2 h = __floats2half2_rn(f.x * unit, f.y * unit);
+        o[i] = *(const uint32_t *) &h;
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // `bytes` (a multiple of 16) to shared memory.

@@ -14,7 +14,7 @@ import torch
 from . import reference as ref
 
 BLOCK = 32                     # columns that share a scale
-ROWS, COLS, CHUNK = 16, 128, 1088      # a packed chunk: rows, columns, bytes (csrc/kernels/mx4.cuh)
+COLS = 128                     # columns of a packed chunk (csrc/kernels/mx4.cuh)
 ACTS = ("silu", "gelu_tanh")
 _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
@@ -76,39 +76,40 @@ class Mx4Tensor:
 
 
 class Mx4Weight:
-    """A matrix [n, k], or ``batch`` of them, or as many gated pairs, in the order in which the products read it.  On the GPU ``data`` holds the packed
-    bytes and ``exps`` the exponents of its rows; elsewhere ``plain`` holds the tensors."""
-    __slots__ = ("n", "k", "batch", "gated", "data", "exps", "plain")
+    """A matrix [n, k], or ``batch`` of them, or as many gated pairs, in the order in which the products read it.  On the GPU ``codes`` and ``scales`` hold
+    chunks of 128 columns, rows within them (of a pair 16 of each matrix in turn), ``factors`` and ``exps`` the scales again as the products of a few
+    tokens need them; elsewhere ``plain`` holds the tensors."""
+    __slots__ = ("n", "k", "batch", "gated", "codes", "scales", "factors", "exps", "plain")
 
     def __init__(self, n, k, batch, gated):
         self.n, self.k, self.batch, self.gated = n, k, batch, gated
-        self.data = self.exps = self.plain = None
+        self.codes = self.scales = self.factors = self.exps = self.plain = None
 
     @property
     def device(self) -> torch.device:
-        return self.data.device if self.data is not None else self.plain[0].device
+        return self.codes.device if self.codes is not None else self.plain[0].device
 
     @property
     def matrices(self) -> int:
         return self.batch or 1
 
     @property
-    def row_blocks(self) -> int:
-        return (self.n + ROWS - 1) // ROWS
+    def chunks(self) -> int:
+        return (self.k + COLS - 1) // COLS
 
     @property
-    def stride(self) -> int:
-        """Bytes of one matrix (or pair) in ``data``."""
-        return (2 if self.gated else 1) * self.row_blocks * ((self.k + COLS - 1) // COLS) * CHUNK
+    def rows(self) -> int:
+        """Rows of a matrix or pair as they are laid out."""
+        return (self.n + 15) // 16 * 32 if self.gated else (self.n + 31) // 32 * 32
 
     def nbytes(self) -> int:
-        if self.data is not None:
-            return self.data.numel() + 4 * self.exps.numel()
+        if self.codes is not None:
+            return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.factors, self.exps))
         return sum(p.nbytes() for p in self.plain)
 
     def values(self, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, ...]:
         """The matrices [(batch,) n, k] (a pair: gate, up) as plain tensors."""
-        if self.data is None:
+        if self.codes is None:
             return tuple(_dequantize(p, dtype) for p in self.plain)
         return tuple(_unpack(self, m).to(dtype) for m in range(2 if self.gated else 1))
 
@@ -142,17 +143,28 @@ def _dequantize(q: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 def _unpack(w: Mx4Weight, member: int) -> torch.Tensor:
     """fp32 [(batch,) n, k] from the packed bytes (the inverse of the kernel that lays them out)."""
-    M, E, B, C = (2 if w.gated else 1), w.matrices, w.row_blocks, (w.k + COLS - 1) // COLS
-    ch = w.data.view(E, B, M, C, CHUNK)[:, :, member]
-    # unit, g, t, step, half of the columns, half of the rows -> half of the rows, g; chunk, unit, step, half of the columns, t
-    byte = ch[..., :1024].reshape(E, B, C, 2, 8, 4, 4, 2, 2).permute(0, 1, 8, 4, 2, 3, 6, 7, 5)
-    code = torch.stack((byte & 15, byte >> 4), -1).reshape(E, B * ROWS, C, 4, BLOCK)
-    table = torch.tensor(_VALUES + tuple(-v for v in _VALUES), dtype=torch.float64, device=w.data.device)
-    f = ch[..., 1024:].reshape(E, B, C, 8, 2, 4).permute(0, 1, 4, 3, 2, 5).reshape(E, B * ROWS, C, 4).int() >> 2
-    s = torch.where(f == 31, torch.full(f.shape, float("nan"), dtype=torch.float64, device=f.device), torch.where(f > 0, _pow2(f - 15), torch.zeros_like(_pow2(f))))
-    s = s * _pow2(w.exps.view(E, B, M, ROWS)[:, :, member]).reshape(E, B * ROWS, 1, 1)
-    m = (table[code.long()] * s[..., None]).view(E, B * ROWS, C * COLS)[:, :w.n, :w.k].float()
-    return m if w.batch else m[0]
+    def rows(x):           # [e, chunks, rows, columns] -> [e, n, chunks, columns]
+        x = x.transpose(1, 2)
+        if w.gated:
+            x = x.reshape(w.matrices, -1, 2, 16, *x.shape[2:])[:, :, member].flatten(1, 2)
+        return x[:, :w.n]
+    code = rows(w.codes)
+    table = torch.tensor(_VALUES + tuple(-v for v in _VALUES), dtype=torch.float64, device=w.device)
+    v = torch.stack((table[(code & 15).long()], table[(code >> 4).long()]), -1).reshape(*code.shape[:3], COLS // BLOCK, BLOCK)
+
+    def scaled(s):
+        return (v * s[..., None]).reshape(w.matrices, w.n, -1)[..., :w.k]
+    e, f = rows(w.scales).int(), rows(w.factors).int() >> 2
+    nan = torch.full(e.shape, float("nan"), dtype=torch.float64, device=w.device)
+    out = scaled(torch.where(e == 255, nan, _pow2(e - 127)))
+    unit = _pow2(rows(w.exps[:, None, :, None]))
+    again = scaled(torch.where(f == 31, nan, torch.where(f > 0, _pow2(f - 15), torch.zeros_like(nan))) * unit)
+    lost = rows(w.exps[:, None, :, None]).double()          # scales more than 27 binades below the largest are 0 in the second form
+    same = (out == again) | (out.isnan() & again.isnan()) | (out.abs() <= 6 * _pow2((lost - 14).int()).reshape(w.matrices, w.n, 1))
+    if not bool(same.all()):
+        raise RuntimeError("the two forms of a packed weight's scales differ")
+    out = out.float()
+    return out if w.batch else out[0]
 
 
 def _act(z: torch.Tensor, act: str) -> torch.Tensor:

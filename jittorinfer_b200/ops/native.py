@@ -102,14 +102,15 @@ class ScanDesc(C.Structure):
 
 
 class Mx4Desc(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "w_exp", "out", "residual", "seg", "src", "status")] + \
-               [(n, C.c_longlong) for n in ("ldx", "w_stride", "ldo", "ldr")] + \
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "w_scales", "out", "residual", "seg", "src", "status")] + \
+               [(n, C.c_longlong) for n in ("ldx", "ldo", "ldr")] + \
                [(n, C.c_int) for n in ("T", "N", "K", "batch", "max_rows", "gated", "act", "out_f32", "res_f32", "x_rows")]
 
 
 class Mx4MoeDesc(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("residual", "logits", "bias", "ids", "wts", "gu", "down", "gu_exp", "down_exp", "xf", "h", "out", "part", "sync", "status")] + \
-               [(n, C.c_longlong) for n in ("ldr", "gu_stride", "down_stride")] + \
+    _fields_ = [(n, C.c_void_p) for n in ("residual", "logits", "bias", "ids", "wts", "gu", "down", "gu_factors", "down_factors", "gu_exp", "down_exp",
+                                          "xf", "h", "out", "part", "sync", "status")] + \
+               [(n, C.c_longlong) for n in ("ldr",)] + \
                [(n, C.c_int) for n in ("T", "d", "F", "E", "k", "n_group", "topk_group", "norm", "sigmoid", "n_shared", "group_top2", "act")] + [("scale", C.c_float)]
 
 
@@ -167,7 +168,7 @@ def load():
     sig("jib_mla_flash", vp, vp, ll, ip, i, ip, ip, i, i, i, f, i, i, i, fp, fp, vp, ip, vp)
     sig("jib_mx4_quantize", vp, i, ll, vp, vp, ll, i, i, vp)
     sig("jib_mx4_dequantize", vp, vp, ll, vp, i, ll, i, vp)
-    sig("jib_mx4_pack", vp, vp, ll, ip, vp, i, i, i, ll, i, i, vp)
+    sig("jib_mx4_pack", vp, vp, ll, vp, vp, vp, ip, i, i, i, i, i, vp)
     sig("jib_mx4_matmul", vp, vp, ll, vp, vp, ll, vp, ll, i, i, i, i, ip, vp)
     sig("jib_mx4_product_simt", C.POINTER(Mx4Desc), i, vp)
     sig("jib_mx4_moe_sizes", i, i, i, i, i, C.POINTER(ll))

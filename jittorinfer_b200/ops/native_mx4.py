@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import native as nat
-from .mx4 import ROWS, Mx4Tensor, Mx4Weight, scale_rows
+from .mx4 import COLS, Mx4Tensor, Mx4Weight, scale_rows
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 FEW_TOKENS = 16                              # tokens of a layer that runs as one launch behind the router's
@@ -43,13 +43,15 @@ def dequantize(q: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 
 def pack(w: Mx4Weight, q: Mx4Tensor, up: Optional[Mx4Tensor]) -> None:
-    E, members = w.matrices, (q,) if up is None else (q, up)
-    w.data = torch.empty(E * w.stride, dtype=torch.uint8, device=q.device)
-    w.exps = torch.empty(E, w.row_blocks * len(members), ROWS, dtype=torch.int32, device=q.device)
+    E, R, members = w.matrices, w.rows, (q,) if up is None else (q, up)
+    w.codes = torch.empty(E, w.chunks, R, COLS // 2, dtype=torch.uint8, device=q.device)
+    w.scales = torch.empty(E, w.chunks, R, COLS // 32, dtype=torch.uint8, device=q.device)
+    w.factors = torch.empty_like(w.scales)
+    w.exps = torch.empty(E, R, dtype=torch.int32, device=q.device)
     with _on(q.codes):
         for m, t in enumerate(members):
-            nat._ck(nat.load().jib_mx4_pack(t.codes.data_ptr(), t.scales.data_ptr(), t.scales.stride(-2), w.exps.data_ptr(), w.data.data_ptr(), E, w.n, w.k,
-                                            w.stride, len(members), m, nat._stream()), "mx4_pack")
+            nat._ck(nat.load().jib_mx4_pack(t.codes.data_ptr(), t.scales.data_ptr(), t.scales.stride(-2), w.codes.data_ptr(), w.scales.data_ptr(),
+                                            w.factors.data_ptr(), w.exps.data_ptr(), E, w.n, w.k, len(members), m, nat._stream()), "mx4_pack")
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -61,7 +63,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 def _desc(x: torch.Tensor, w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act: Optional[str]) -> "nat.Mx4Desc":
     d = nat.Mx4Desc()
     d.x, d.ldx, d.x_rows = x.data_ptr(), x.stride(0), x.shape[0]
-    d.w, d.w_stride, d.w_exp = w.data.data_ptr(), w.stride, w.exps.data_ptr()
+    d.w, d.w_scales = w.codes.data_ptr(), w.scales.data_ptr()
     d.out, d.ldo, d.out_f32 = out.data_ptr(), out.stride(0), int(out.dtype == torch.float32)
     if residual is not None:
         d.residual, d.ldr, d.res_f32 = residual.data_ptr(), residual.stride(0), int(residual.dtype == torch.float32)
@@ -134,8 +136,8 @@ def _few_layer(x, residual, wgu: Mx4Weight, wd: Mx4Weight, sizes, act: str, m, w
         m.logits = m.sync + 4 * sync
     if residual is not None:
         m.residual, m.ldr = residual.data_ptr(), residual.stride(0)
-    m.gu, m.gu_stride, m.gu_exp = wgu.data.data_ptr(), wgu.stride, wgu.exps.data_ptr()
-    m.down, m.down_stride, m.down_exp = wd.data.data_ptr(), wd.stride, wd.exps.data_ptr()
+    m.gu, m.gu_factors, m.gu_exp = wgu.codes.data_ptr(), wgu.factors.data_ptr(), wgu.exps.data_ptr()
+    m.down, m.down_factors, m.down_exp = wd.codes.data_ptr(), wd.factors.data_ptr(), wd.exps.data_ptr()
     m.status = nat.workspace(x.device).status.data_ptr()
     m.T, m.d, m.F, m.E, m.act = T, d, wgu.n, wgu.batch, nat.ACTS[act]
     L, stream = nat.load(), nat._stream()

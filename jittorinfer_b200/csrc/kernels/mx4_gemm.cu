@@ -1,0 +1,586 @@
+// Products of bf16 activations with packed 4-bit weights on the block-scaled tensor cores: out[r][n] = f(sum_k x[r][k] w[n][k]) (+ residual), dense or
+// grouped by expert.
+//
+// The weights go to the tensor cores as they are: the tensor map of type 16U4_ALIGN16B spreads 4-bit codes over bytes in shared memory and
+// tcgen05.mma.kind::mxf8f6f4 takes them as E2M1 with their block's scale, 128 rows a tile.  So no instruction touches a weight.  Its other operand can have 8
+// bits at most; a bf16 activation is the sum of two E4M3 numbers, the first its value rounded to four significant bits, the second what is left, each
+// with a scale for 32 columns.  That sum is the bf16 value down to 2^-11 of the block's largest magnitude and within 2^-21 of the largest below.  Two
+// instructions multiply both planes into one accumulator; at twice the rate of bf16 that costs what a bf16 product costs.
+//
+// A stage is a chunk of 128 columns: codes (16 KB in shared memory, 8 KB from memory), both planes of up to 192 rows of x, and scales, which four warps move from
+// shared memory to tensor memory (column j of an operand: lane l of every quarter holds the four scale bytes of row 32 j + l).  With few tiles K is split
+// among CTAs; their sums meet in memory, and the one that comes last adds them up in the order of K.
+#include <cuda_fp8.h>
+
+#include "jib_kernels.h"
+#include "mx4_stream.cuh"
+#include "pdl.cuh"
+#include "sm100.cuh"
+#include "tma_host.cuh"
+
+namespace {
+
+using namespace sm100;
+typedef __nv_bfloat16 bf16;
+
+constexpr int BM = 128, MAX_BN = 192, MAX_STAGES = 8, MAX_E = 256, PAD = 32;
+constexpr int A_BYTES = BM * 128, SA_BYTES = BM * 4;
+constexpr int THREADS = 384;                       // producer, issuer, two idle; four scale warps; four epilogue warps
+constexpr int MOST_SMEM = 227 * 1024;
+// Rows of the planes' scales: a tile reads up to MAX_BN behind the last one, 16 bytes (four rows) at a time.
+__host__ __device__ inline long long scale_rows_of(long long rows) { return (rows + MAX_BN + 31) / 32 * 32; }
+
+__host__ __device__ inline int stage_bytes(int bn) { return (A_BYTES + 2 * bn * 128 + SA_BYTES + 2 * bn * 4 + 1023) / 1024 * 1024; }
+__host__ __device__ inline int scale_cols(int bn) { return (bn + 127) / 128 * 4; }          // of one plane
+
+struct Args {
+    const uint8_t * w_scales;                // [matrix][chunk][R][4]
+    const uint8_t * x_scales;                // [plane][chunk][x_rows][4], x_rows as scale_rows_of says
+    void * out;
+    const void * residual;
+    const int * seg;                         // grouped: first row of each expert's rows, multiples of PAD; device int[E + 1]
+    const int * count;                       // ... and how many there are
+    float * part;                            // [tile][split][bn][128]
+    int * counters;                          // zeros, one a tile
+    int * status;
+    long long ldo, ldr, x_rows;
+    int T, N, R, C, E, bn, m_tiles, t_tiles, splits, stages, gated, act, out_f32, res_f32;
+};
+
+__device__ __forceinline__ void st_cols4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void mma_mxf8f6f4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t) accumulate)
+        : "memory");
+}
+// E2M1 x E4M3 with E8M0 scales, 128 x n, the scales in byte k of their words.
+__device__ __forceinline__ uint32_t idesc_e2m1_e4m3(int n, uint32_t k) {
+    return k << 4 | 5u << 7 | 0u << 10 | (uint32_t) (n >> 3) << 17 | 1u << 23 | (uint32_t) (BM >> 4) << 24 | k << 29;
+}
+
+// What item i is: row tile m, first row of x, how many, chunks c0 .. c1 - 1, matrix, tile (for sums that meet).
+struct Item {
+    int m, row0, rows, c0, c1, e, tile, split;
+};
+
+__device__ __forceinline__ Item item_of(const Args & g, const int * first_tile, int i) {
+    Item t;
+    t.m = i % g.m_tiles;
+    int rest = i / g.m_tiles;
+    t.e = 0;
+    t.split = 0;
+    t.c0 = 0;
+    t.c1 = g.C;
+    if (g.seg != nullptr) {                  // the expert whose tiles hold tile `rest`
+        int lo = 0, hi = g.E;
+#pragma unroll 1
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (first_tile[mid] <= rest) lo = mid;
+            else hi = mid;
+        }
+        t.e = lo;
+        const int at = (rest - first_tile[lo]) * g.bn;
+        t.row0 = g.seg[lo] + at;
+        t.rows = min(g.bn, g.count[lo] - at);
+    } else {
+        const int tt = rest % g.t_tiles;
+        t.split = rest / g.t_tiles;
+        t.row0 = tt * g.bn;
+        t.rows = min(g.bn, g.T - t.row0);
+        t.c0 = t.split * g.C / g.splits;
+        t.c1 = (t.split + 1) * g.C / g.splits;
+        rest = tt;
+    }
+    t.tile = rest * g.m_tiles + t.m;
+    return t;
+}
+
+__global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Args g) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int first_tile[MAX_E + 1], last_s;
+    __shared__ uint64_t bars[3 * MAX_STAGES + 4];
+    __shared__ uint32_t tmem_slot;
+    uint8_t * tiles = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
+    uint64_t * full = bars, * empty = full + MAX_STAGES, * sf_full = empty + MAX_STAGES, * acc_full = sf_full + MAX_STAGES, * acc_empty = acc_full + 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = g.stages, bn = g.bn;
+    const int SB = stage_bytes(bn), plane = bn * 128, sfc = scale_cols(bn), slab = 4 + 2 * sfc;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&sf_full[i], 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+        fence_barrier_init();
+        prefetch_tmap(&tm_w);
+        prefetch_tmap(&tm_x);
+    }
+    if (warp == 2) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    PDL_TRIGGER_TOP();
+    pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
+    int items = g.m_tiles * g.t_tiles * g.splits;
+    if (g.seg != nullptr) {
+        if (warp == 0) {                     // tiles of the experts before each
+            int sum = 0;
+#pragma unroll 1
+            for (int e0 = 0; e0 < g.E; e0 += 32) {
+                const int mine = e0 + lane < g.E ? (g.count[e0 + lane] + bn - 1) / bn : 0;
+                int s = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) {
+                    const int v = __shfl_up_sync(0xffffffffu, s, o);
+                    if (lane >= o) s += v;
+                }
+                if (e0 + lane < g.E) first_tile[e0 + lane] = sum + s - mine;
+                sum += __shfl_sync(0xffffffffu, s, 31);
+            }
+            if (lane == 0) first_tile[g.E] = sum;
+        }
+        __syncthreads();
+        items = first_tile[g.E] * g.m_tiles;
+    }
+    const uint32_t sf0 = tmem + 2 * bn;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int it = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+                const Item t = item_of(g, first_tile, i);
+                const int w_rows = min(BM, g.R - t.m * BM);
+#pragma unroll 1
+                for (int c = t.c0; c < t.c1; ++c, ++it) {
+                    const int s = it % S;
+                    if (!mbar_wait(&empty[s], (it / S & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 61, i); ok = false; break; }
+                    uint8_t * st = tiles + s * SB;
+                    const int z = t.e * g.C + c;
+                    mbar_expect_tx(&full[s], A_BYTES / 2 + 2 * plane + w_rows * 4 + 2 * bn * 4);      // (codes count as they are in memory)
+                    tma_load_3d(st, &tm_w, &full[s], 0, t.m * BM, z);
+                    tma_load_3d(st + A_BYTES, &tm_x, &full[s], c * 128, t.row0, 0);
+                    tma_load_3d(st + A_BYTES + plane, &tm_x, &full[s], c * 128, t.row0, 1);
+                    uint8_t * sc = st + A_BYTES + 2 * plane;
+                    mx4::bulk_load(sc, g.w_scales + ((size_t) z * g.R + t.m * BM) * 4, w_rows * 4, &full[s]);
+                    mx4::bulk_load(sc + SA_BYTES, g.x_scales + ((size_t) c * g.x_rows + t.row0) * 4, bn * 4, &full[s]);
+                    mx4::bulk_load(sc + SA_BYTES + bn * 4, g.x_scales + ((size_t) (g.C + c) * g.x_rows + t.row0) * 4, bn * 4, &full[s]);
+                }
+            }
+            // copies in flight end before the memory is given back
+            if (!ok)
+                for (int i = it - S < 0 ? 0 : it - S; i < it; ++i) mbar_wait(&full[i % S], i / S & 1);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (elect_one()) {
+            int it = 0, j = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int i = blockIdx.x; i < items && ok; i += gridDim.x, ++j) {
+                const Item t = item_of(g, first_tile, i);
+                const int buf = j & 1;
+                if (!mbar_wait(&acc_empty[buf], (j >> 1 & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 62, i); break; }
+                tc_fence_after();
+                const uint32_t acc = tmem + buf * bn;
+#pragma unroll 1
+                for (int c = t.c0; c < t.c1; ++c, ++it) {
+                    const int s = it % S;
+                    if (!mbar_wait(&sf_full[s], it / S & 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 63, i); ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(tiles + s * SB), sf = sf0 + s * slab;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int p = 0; p < 2; ++p)
+                            mma_mxf8f6f4(acc, desc_k_sw128(a + k * 32), desc_k_sw128(a + A_BYTES + p * plane + k * 32), idesc_e2m1_e4m3(bn, k), sf,
+                                         sf + 4 + p * sfc, c != t.c0 || k != 0 || p != 0);
+                    mma_commit(&empty[s]);
+                }
+                mma_commit(&acc_full[buf]);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4 && warp < 8) {
+        // scales to tensor memory
+        const uint32_t mine = sf0 + ((uint32_t) (warp & 3) << 21);
+        int it = 0;
+        bool ok = true;
+#pragma unroll 1
+        for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+            const Item t = item_of(g, first_tile, i);
+#pragma unroll 1
+            for (int c = t.c0; c < t.c1; ++c, ++it) {
+                const int s = it % S;
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], it / S & 1));
+                if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 64, i); break; }
+                tc_fence_after();
+                const uint32_t * sc = (const uint32_t *) (tiles + s * SB + A_BYTES + 2 * plane) + lane;
+                const uint32_t dst = mine + s * slab;
+                st_cols4(dst, sc[0], sc[32], sc[64], sc[96]);
+#pragma unroll 1
+                for (int p = 0; p < 2; ++p) {
+                    const uint32_t * sx = sc + SA_BYTES / 4 + p * bn;
+                    for (int q = 0; q < sfc; q += 4) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] = (q + k) * 32 + lane < bn ? sx[(q + k) * 32] : 0u;
+                        st_cols4(dst + 4 + p * sfc + q, v[0], v[1], v[2], v[3]);
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sf_full[s]);
+            }
+        }
+    } else if (warp >= 8) {
+        const int q = warp & 3;
+        const uint32_t mine = tmem + ((uint32_t) q << 21);
+        int j = 0;
+#pragma unroll 1
+        for (int i = blockIdx.x; i < items; i += gridDim.x, ++j) {
+            const Item t = item_of(g, first_tile, i);
+            const int buf = j & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], j >> 1 & 1))) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 65, i); break; }
+            tc_fence_after();
+            const uint32_t acc = mine + buf * bn;
+            bool finish = true;
+            float * part = g.part + ((size_t) t.tile * g.splits * bn) * BM + q * 32 + lane;
+            if (g.splits > 1) {
+                float * to = part + (size_t) t.split * bn * BM;
+#pragma unroll 1
+                for (int c = 0; c < t.rows; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(acc + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (c + k < t.rows) __stcg(to + (size_t) (c + k) * BM, __uint_as_float(v[k]));
+                }
+                __threadfence();
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (threadIdx.x == 256) {
+                    last_s = atomicAdd(g.counters + t.tile, 1) == g.splits - 1;
+                    __threadfence();
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                finish = last_s != 0;
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            // lane = row n of the tile (of pairs: 16 of the gate, 16 of the up matrix), 16 rows of x at a time
+            const int n = g.gated ? t.m * 64 + q * 16 + (lane & 15) : t.m * BM + q * 32 + lane;
+            const bool writes = n < g.N && (!g.gated || lane < 16);
+#pragma unroll 1
+            for (int c = 0; c < t.rows && finish; c += 16) {
+                float y[16];
+                if (g.splits > 1) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) y[k] = 0.f;
+#pragma unroll 1
+                    for (int s = 0; s < g.splits; ++s)
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            if (c + k < t.rows) y[k] += __ldcg(part + ((size_t) s * bn + c + k) * BM);
+                } else {
+                    uint32_t v[16];
+                    tmem_ld16(acc + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) y[k] = __uint_as_float(v[k]);
+                }
+                if (g.gated)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) y[k] = mx4::gated(y[k], __shfl_down_sync(0xffffffffu, y[k], 16), g.act);
+                if (!writes) continue;
+                if (g.residual != nullptr)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (c + k < t.rows) {
+                            const long long at = (long long) (t.row0 + c + k) * g.ldr + n;
+                            y[k] += g.res_f32 ? ((const float *) g.residual)[at] : __bfloat162float(((const bf16 *) g.residual)[at]);
+                        }
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (c + k < t.rows) {
+                        const long long at = (long long) (t.row0 + c + k) * g.ldo + n;
+                        if (g.out_f32) ((float *) g.out)[at] = y[k];
+                        else ((bf16 *) g.out)[at] = __float2bfloat16(y[k]);
+                    }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+// ---- bf16 rows as two E4M3 planes ------------------------------------------------------------------------------------------------
+// Four lanes a block of 32 columns.  Scale 2^e with e = floor(log2 max) - 7, at least -123: the largest magnitude becomes 128 .. 256, rounded to hi; what is left, at
+// most 8, times 16 is rounded to lo, whose scale is 2^(e - 4).  src: row r is x[src[r]] (zeros where that is negative); limit: rows from *limit on are
+// left alone.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
+__device__ __forceinline__ float e4m3_value(uint32_t w, int i) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t) (w >> (8 * i) & 0xff), __NV_E4M3)));
+}
+
+__global__ void __launch_bounds__(256) planes_kernel(const bf16 * __restrict__ x, long long ldx, const int * __restrict__ src, const int * __restrict__ limit,
+                                                     uint8_t * __restrict__ planes, uint8_t * __restrict__ scales, long long rows, long long scale_rows, int K, int C,
+                                                     int * __restrict__ zeros, int n_zeros) {
+    PDL_TRIGGER_TOP();
+    pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
+    const int per_row = C * 16;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n_zeros; i += gridDim.x * blockDim.x) zeros[i] = 0;
+    const long long most = limit != nullptr ? min(rows, (long long) *limit) : rows, n = most * per_row;
+    for (long long i0 = (long long) blockIdx.x * blockDim.x; i0 < n; i0 += (long long) gridDim.x * blockDim.x) {
+        const long long i = i0 + threadIdx.x;
+        const long long r = i < n ? i / per_row : most - 1;
+        const int k = (int) (i - r * per_row) * 8;
+        const long long from = src != nullptr ? src[r] : r;
+        float y[8] = {};
+        uint32_t top = 0;
+        if (i < n && k < K && from >= 0) {
+            const uint4 in = *(const uint4 *) (x + from * ldx + k);
+            const uint32_t w[4] = {in.x, in.y, in.z, in.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = __bfloat1622float2(*(const __nv_bfloat162 *) &w[j]);
+                y[2 * j] = f.x;
+                y[2 * j + 1] = f.y;
+                top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+            }
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (i >= n) continue;
+        const int field = (int) (top >> 23), byte = field == 255 ? 255 : max(field - 7, 4);          // e + 127
+        const float unit = field == 255 ? 0.f : __uint_as_float((uint32_t) (254 - byte) << 23);
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = field == 255 ? 0.f : y[j] * unit;
+        uint2 hi, lo;
+        hi.x = e4m3x4(z[0], z[1], z[2], z[3]);
+        hi.y = e4m3x4(z[4], z[5], z[6], z[7]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            z[j] = (z[j] - e4m3_value(hi.x, j)) * 16.f;
+            z[4 + j] = (z[4 + j] - e4m3_value(hi.y, j)) * 16.f;
+        }
+        lo.x = e4m3x4(z[0], z[1], z[2], z[3]);
+        lo.y = e4m3x4(z[4], z[5], z[6], z[7]);
+        uint8_t * to = planes + r * (long long) (C * 128) + k;
+        *(uint2 *) to = hi;
+        *(uint2 *) (to + rows * (long long) (C * 128)) = lo;
+        if ((i & 3) == 0) {
+            uint8_t * sc = scales + ((long long) (k >> 7) * scale_rows + r) * 4 + (k >> 5 & 3);
+            sc[0] = (uint8_t) byte;
+            sc[(long long) C * scale_rows * 4] = (uint8_t) (byte == 255 ? 255 : byte - 4);
+        }
+    }
+}
+
+// ---- experts' rows at multiples of PAD ------------------------------------------------------------------------------------------------
+// From the sorted order (seg, src, dest of jib_moe_permute): first[e] and count[e] of the padded order (first[E]: its end), the token of each of its rows (-1: none) and
+// the row of each pair (-1: none).
+__global__ void __launch_bounds__(256) pad_kernel(const int * __restrict__ seg, const int * __restrict__ src, const int * __restrict__ dest, int E, int n_pairs, int cap,
+                                                  int * __restrict__ first, int * __restrict__ count, int * __restrict__ row_src, int * __restrict__ pair_row) {
+    __shared__ int seg_s[MAX_E + 1], pad_s[MAX_E + 1];
+    PDL_TRIGGER_TOP();
+    pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
+    for (int e = threadIdx.x; e <= E; e += blockDim.x) seg_s[e] = seg[e];
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        int sum = 0;
+#pragma unroll 1
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            const int e = e0 + lane, mine = e < E ? (seg_s[e + 1] - seg_s[e] + PAD - 1) / PAD * PAD : 0;
+            int s = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int v = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += v;
+            }
+            if (e < E) pad_s[e] = sum + s - mine;
+            sum += __shfl_sync(0xffffffffu, s, 31);
+        }
+        if (lane == 0) pad_s[E] = sum;
+    }
+    __syncthreads();
+    auto find = [&](const int * at, int v) {             // the last e with at[e] <= v that has rows
+        int lo = 0, hi = E;
+#pragma unroll 1
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (at[mid] <= v) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    if (blockIdx.x == 0)
+        for (int e = threadIdx.x; e <= E; e += blockDim.x) {
+            first[e] = pad_s[e];
+            if (e < E) count[e] = seg_s[e + 1] - seg_s[e];
+        }
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < cap || i < n_pairs; i += gridDim.x * blockDim.x) {
+        if (i < cap && i < pad_s[E]) {
+            const int e = find(pad_s, i), at = i - pad_s[e];
+            row_src[i] = at < seg_s[e + 1] - seg_s[e] ? src[seg_s[e] + at] : -1;
+        }
+        if (i < n_pairs) {
+            const int r = dest[i];
+            int to = -1;
+            if (r >= 0) {
+                const int e = find(seg_s, r);
+                to = pad_s[e] + r - seg_s[e];
+            }
+            pair_row[i] = to;
+        }
+    }
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH; }
+
+// Tensor map of the packed codes: 4-bit elements spread over bytes, boxes of 128 rows of a chunk.
+int weights_map(CUtensorMap * out, const void * codes, long long R, long long z) {
+    jib::TmaEncodeFn fn = jib::tma_encode_fn();
+    if (!fn) return JIB_E_DRIVER;
+    if ((uintptr_t) codes & 31) return JIB_E_ALIGN;
+    const cuuint64_t dims[3] = {128, (cuuint64_t) R, (cuuint64_t) z}, strides[2] = {mx4::CODES, (cuuint64_t) R * mx4::CODES};
+    const cuuint32_t box[3] = {128, BM, 1}, step[3] = {1, 1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 3, const_cast<void *>(codes), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0
+               : JIB_E_TENSORMAP;
+}
+
+int planes_map(CUtensorMap * out, const void * planes, long long rows, long long bytes, int bn) {
+    jib::TmaEncodeFn fn = jib::tma_encode_fn();
+    if (!fn) return JIB_E_DRIVER;
+    if ((uintptr_t) planes & 15) return JIB_E_ALIGN;
+    const cuuint64_t dims[3] = {(cuuint64_t) bytes, (cuuint64_t) rows, 2}, strides[2] = {(cuuint64_t) bytes, (cuuint64_t) (bytes * rows)};
+    const cuuint32_t box[3] = {128, (cuuint32_t) bn, 1}, step[3] = {1, 1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(planes), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0
+               : JIB_E_TENSORMAP;
+}
+
+// Rows of x in a tile and splits of K of a dense product.  A tile's fixed part is worth some 24 rows; the rounds over the machine count.  Where the tiles leave SMs
+// idle, K is split, four chunks a split at least.
+void shape_of(long long T, int m_tiles, int C, int * bn, int * splits) {
+    const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
+    long long best = -1;
+    for (int w = T > 16 ? 32 : 16; w <= MAX_BN; w += 32) {
+        const long long tiles = (long long) m_tiles * ((T + w - 1) / w), cost = (tiles + sms - 1) / sms * (w + 24);
+        if (best < 0 || cost <= best) { best = cost; *bn = w; }
+        if (w >= T) break;
+        if (w == 16) w = 0;
+    }
+    const long long tiles = (long long) m_tiles * ((T + *bn - 1) / *bn);
+    int s = (int) (sms / tiles);
+    if (s > C / 4) s = C / 4;
+    if (s > 16) s = 16;
+    *splits = s < 1 ? 1 : s;
+}
+
+}  // namespace
+
+extern "C" {
+
+// Sizes of what a tiled product of `rows` rows needs: bytes of the planes, of their scales, floats of part and ints of counters (grouped: 0).
+JIB_EXPORT void jib_mx4_gemm_sizes(long long rows, int N, int K, int gated, int grouped, long long * sizes) {
+    const int C = mx4::chunks(K), m_tiles = (mx4::rows_of(N, gated != 0) + BM - 1) / BM;
+    sizes[0] = 2 * rows * C * 128;
+    sizes[1] = 2ll * C * scale_rows_of(rows) * 4;
+    sizes[2] = sizes[3] = 0;
+    if (!grouped) {
+        int bn, splits;
+        shape_of(rows, m_tiles, C, &bn, &splits);
+        const long long tiles = (long long) m_tiles * ((rows + bn - 1) / bn);
+        if (splits > 1) {
+            sizes[2] = tiles * splits * bn * BM;
+            sizes[3] = tiles;
+        }
+    }
+}
+
+// x [..][K] bf16 (rows ldx elements apart) as planes and scales of `rows` rows; zeros: n_zeros ints.
+JIB_EXPORT int jib_mx4_planes(const void * x, long long ldx, const int * src, const int * limit, void * planes, void * scales, long long rows, int K, int * zeros,
+                              int n_zeros, void * stream) {
+    if (rows <= 0) return 0;
+    if (K <= 0 || K % 32 || n_zeros < 0) return JIB_E_ARG;
+    if (((uintptr_t) x | (uintptr_t) (ldx * 2) | (uintptr_t) planes) & 15) return JIB_E_ALIGN;
+    const int C = mx4::chunks(K);
+    const long long ctas = (rows * C * 16 + 255) / 256, most = 32ll * (jib::sm_count() > 0 ? jib::sm_count() : 148);
+    JIB_LAUNCH((planes_kernel), (unsigned) (ctas < most ? ctas : most), 256, 0, (cudaStream_t) stream, (const bf16 *) x, ldx, src, limit, (uint8_t *) planes,
+               (uint8_t *) scales, rows, scale_rows_of(rows), K, C, zeros, n_zeros);
+    return launched();
+}
+
+JIB_EXPORT int jib_mx4_pad(const int * seg, const int * src, const int * dest, int E, int n_pairs, int cap, int * first, int * count, int * row_src, int * pair_row,
+                           void * stream) {
+    if (E < 1 || E > MAX_E || n_pairs < 1 || cap < 1) return JIB_E_ARG;
+    const int n = cap > n_pairs ? cap : n_pairs, ctas = (n + 255) / 256;
+    JIB_LAUNCH((pad_kernel), ctas < 148 ? ctas : 148, 256, 0, (cudaStream_t) stream, seg, src, dest, E, n_pairs, cap, first, count, row_src, pair_row);
+    return launched();
+}
+
+// The tiled product: d->x are the planes (d->x_rows rows), x_scales their scales; grouped: d->seg = first, count (see jib_mx4_pad); part and counters (zeros) as
+// jib_mx4_gemm_sizes says.
+JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const int * count, float * part, int * counters, void * stream) {
+    if (d->T <= 0) return 0;
+    if (d->N <= 0 || d->K <= 0 || d->K % 32 || d->batch < 1 || d->batch > MAX_E || d->T > d->x_rows || (d->seg != nullptr && (count == nullptr || d->residual != nullptr)))
+        return JIB_E_ARG;
+    if (((uintptr_t) x_scales | (uintptr_t) d->w_scales) & 15) return JIB_E_ALIGN;
+    const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
+    Args g;
+    g.w_scales = d->w_scales; g.x_scales = (const uint8_t *) x_scales; g.out = d->out; g.residual = d->residual; g.seg = d->seg; g.count = count;
+    g.part = part; g.counters = counters; g.status = d->status; g.ldo = d->ldo; g.ldr = d->ldr; g.x_rows = scale_rows_of(d->x_rows);
+    g.T = d->T; g.N = d->N; g.R = mx4::rows_of(d->N, d->gated != 0); g.C = mx4::chunks(d->K); g.E = d->batch;
+    g.gated = d->gated; g.act = d->act; g.out_f32 = d->out_f32; g.res_f32 = d->res_f32;
+    g.m_tiles = (g.R + BM - 1) / BM;
+    long long items;
+    if (d->seg != nullptr) {
+        // an expert's rows on average, and a quarter more: most experts then take one tile
+        const int avg = (d->max_rows + d->batch - 1) / d->batch, w = (avg + avg / 4 + 31) / 32 * 32;
+        g.bn = w < 32 ? 32 : w > MAX_BN ? MAX_BN : w;
+        g.splits = 1;
+        g.t_tiles = 1;
+        items = sms;
+    } else {
+        shape_of(d->T, g.m_tiles, g.C, &g.bn, &g.splits);
+        g.t_tiles = (d->T + g.bn - 1) / g.bn;
+        items = (long long) g.m_tiles * g.t_tiles * g.splits;
+        if (g.splits > 1 && (part == nullptr || counters == nullptr)) return JIB_E_SCRATCH;
+    }
+    if (items > 0x3fffffff) return JIB_E_ARG;
+    g.stages = (MOST_SMEM - 4096 - 1024) / stage_bytes(g.bn);        // (4 KB: barriers and tables)
+    const int slab = 4 + 2 * scale_cols(g.bn);
+    if (g.stages > (512 - 2 * g.bn) / slab) g.stages = (512 - 2 * g.bn) / slab;
+    if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
+    CUtensorMap mw, mx;
+    int rc = weights_map(&mw, d->w, g.R, (long long) g.C * d->batch);
+    if (rc) return rc;
+    rc = planes_map(&mx, d->x, d->x_rows, (long long) g.C * 128, g.bn);
+    if (rc) return rc;
+    static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
+    if (!jib::ensure_dyn_smem(mx4_gemm_kernel, MOST_SMEM - 4096, attr_done)) return JIB_E_LAUNCH;
+    JIB_LAUNCH((mx4_gemm_kernel), (unsigned) (items < sms ? items : sms), THREADS, g.stages * stage_bytes(g.bn) + 1024, (cudaStream_t) stream, mw, mx, g);
+    return launched();
+}
+
+}  // extern "C"

@@ -12,6 +12,7 @@ from .mx4 import COLS, Mx4Tensor, Mx4Weight, scale_rows
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 FEW_TOKENS = 16                              # tokens of a layer that runs as one launch behind the router's
+PAD = 32                                     # rows of an expert are padded to in grouped products (csrc/kernels/mx4_gemm.cu)
 MAX_EXPERTS, MAX_CHOICES = 256, 32           # what the gate and the sort take (csrc/kernels/moe.cu)
 _NO_SWITCH = contextlib.nullcontext()
 
@@ -57,24 +58,45 @@ def pack(w: Mx4Weight, q: Mx4Tensor, up: Optional[Mx4Tensor]) -> None:
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """Rows that the kernels can read: contiguous, 16-byte steps."""
     ok = x.stride(1) == 1 and x.stride(0) >= x.shape[1] and (x.stride(0) * x.element_size()) % 16 == 0 and x.data_ptr() % 16 == 0
-    return x if ok else x.contiguous()
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
-def _desc(x: torch.Tensor, w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act: Optional[str]) -> "nat.Mx4Desc":
+def _desc(x_rows: int, w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act: Optional[str]) -> "nat.Mx4Desc":
     d = nat.Mx4Desc()
-    d.x, d.ldx, d.x_rows = x.data_ptr(), x.stride(0), x.shape[0]
-    d.w, d.w_scales = w.codes.data_ptr(), w.scales.data_ptr()
+    d.x_rows, d.w, d.w_scales = x_rows, w.codes.data_ptr(), w.scales.data_ptr()
     d.out, d.ldo, d.out_f32 = out.data_ptr(), out.stride(0), int(out.dtype == torch.float32)
     if residual is not None:
         d.residual, d.ldr, d.res_f32 = residual.data_ptr(), residual.stride(0), int(residual.dtype == torch.float32)
     d.T, d.N, d.K, d.batch, d.max_rows = out.shape[0], w.n, w.k, 1, out.shape[0]
     d.gated, d.act = int(w.gated), nat.ACTS[act or "silu"]
-    d.status = nat.workspace(x.device).status.data_ptr()
+    d.status = nat.workspace(out.device).status.data_ptr()
     return d
 
 
-def _run(d: "nat.Mx4Desc", x: torch.Tensor, what: str) -> None:
-    nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), int(x.dtype == torch.float32), nat._stream()), what)
+_gemm_sizes: dict = {}        # (rows, n, k, gated, grouped) -> bytes of planes and of their scales, floats of part, ints of counters
+
+
+def _sizes(*key: int):
+    if key not in _gemm_sizes:
+        if len(_gemm_sizes) > 4096:
+            _gemm_sizes.clear()
+        s = (C.c_longlong * 4)()
+        nat.load().jib_mx4_gemm_sizes(*key, s)
+        _gemm_sizes[key] = tuple(s)
+    return _gemm_sizes[key]
+
+
+def _tiled(d: "nat.Mx4Desc", x: torch.Tensor, rows: int, src: Optional[int], limit: Optional[int], count: Optional[int], what: str) -> None:
+    """bf16 activations as planes, then the tiled product.  ``src``, ``limit``, ``count``: addresses, of grouped rows."""
+    planes, scales, part, counters = _sizes(rows, d.N, d.K, d.gated, int(count is not None))
+    scratch = torch.empty(planes + scales + 4 * (part + counters), dtype=torch.uint8, device=x.device)
+    at = scratch.data_ptr()
+    L, stream = nat.load(), nat._stream()
+    at_scales, at_part = at + planes, at + planes + scales
+    at_counters = at_part + 4 * part
+    nat._ck(L.jib_mx4_planes(x.data_ptr(), x.stride(0), src, limit, at, at_scales, rows, d.K, at_counters, counters, stream), "mx4_planes")
+    d.x = at
+    nat._ck(L.jib_mx4_gemm(C.byref(d), at_scales, count, at_part, at_counters, stream), what)
 
 
 def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dtype: torch.dtype, act: Optional[str]) -> torch.Tensor:
@@ -84,16 +106,31 @@ def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dty
         residual = residual.contiguous()
     if x.shape[0]:
         with _on(x):
-            _run(_desc(x, w, out, residual, act), x, "mx4_product")
+            d = _desc(x.shape[0], w, out, residual, act)
+            if x.dtype == torch.bfloat16:
+                _tiled(d, x, x.shape[0], None, None, None, "mx4_gemm")
+            else:
+                d.x, d.ldx = x.data_ptr(), x.stride(0)
+                nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), 1, nat._stream()), "mx4_product_simt")
     return out
 
 
-def grouped(x: torch.Tensor, w: Mx4Weight, seg: torch.Tensor, src: Optional[torch.Tensor], rows: int, max_rows: int, act: Optional[str]) -> torch.Tensor:
-    """Rows sorted by expert: expert e's are seg[e] .. seg[e + 1] - 1; row r is computed from x[src[r]] (without ``src`` x[r])."""
+def _grouped_simt(x: torch.Tensor, w: Mx4Weight, seg: torch.Tensor, src: Optional[torch.Tensor], rows: int, act: Optional[str]) -> torch.Tensor:
+    """fp32 rows sorted by expert: expert e's are seg[e] .. seg[e + 1] - 1; row r is computed from x[src[r]] (without ``src`` x[r])."""
     out = torch.empty(rows, w.n, dtype=x.dtype, device=x.device)
-    d = _desc(x, w, out, None, act)
-    d.seg, d.src, d.batch, d.max_rows = seg.data_ptr(), nat._p(src), w.batch, max_rows
-    _run(d, x, "mx4_grouped")
+    d = _desc(x.shape[0], w, out, None, act)
+    d.x, d.ldx, d.seg, d.src, d.batch, d.max_rows = x.data_ptr(), x.stride(0), seg.data_ptr(), nat._p(src), w.batch, rows
+    nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), 1, nat._stream()), "mx4_grouped_simt")
+    return out
+
+
+def _grouped(x: torch.Tensor, w: Mx4Weight, pad, src: Optional[int], pairs: int, act: Optional[str]) -> torch.Tensor:
+    """bf16 rows in the padded order ``pad`` = (first, count, capacity); row r is computed from x[src[r]] (without ``src`` x[r])."""
+    first, count, cap = pad
+    out = torch.empty(cap, w.n, dtype=torch.bfloat16, device=x.device)
+    d = _desc(cap, w, out, None, act)
+    d.seg, d.batch, d.max_rows = first, w.batch, pairs
+    _tiled(d, x, cap, src, first + 4 * w.batch, count, "mx4_grouped")
     return out
 
 
@@ -162,10 +199,18 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act):
             m.ids, m.wts, m.k = ids.data_ptr(), wts.data_ptr(), k
             return _few_layer(x, residual, wgu, wd, sizes, act, m, None)
         seg, src, dest = nat.moe_permute(ids, 0, wgu.batch)
-        h = grouped(x, wgu, seg, src, T * k, T * k, act)
-        y = grouped(h, wd, seg, None, T * k, T * k, None)
+        E, n = wgu.batch, T * k
         if x.dtype == torch.bfloat16:
-            return nat.moe_combine(y, dest, wts, None, None if residual is None else residual.contiguous())
+            cap = (n + min(E, n) * (PAD - 1) + PAD - 1) // PAD * PAD
+            table = torch.empty(2 * E + 1 + cap + n, dtype=torch.int32, device=x.device)       # first, count, token of each row, row of each pair
+            first = table.data_ptr()
+            count, row_src, pair_row = first + 4 * (E + 1), first + 4 * (2 * E + 1), first + 4 * (2 * E + 1 + cap)
+            nat._ck(nat.load().jib_mx4_pad(seg.data_ptr(), src.data_ptr(), dest.data_ptr(), E, n, cap, first, count, row_src, pair_row, nat._stream()), "mx4_pad")
+            h = _grouped(x, wgu, (first, count, cap), row_src, n, act)
+            y = _grouped(h, wd, (first, count, cap), None, n, None)
+            return nat.moe_combine(y, table[2 * E + 1 + cap:].view(T, k), wts, None, None if residual is None else residual.contiguous())
+        h = _grouped_simt(x, wgu, seg, src, n, act)
+        y = _grouped_simt(h, wd, seg, None, n, None)
         ok = (dest >= 0).to(wts.dtype) * wts
         out = (y[dest.clamp(min=0).long()] * ok[..., None]).sum(1)
         return out if residual is None else out + residual

@@ -7,9 +7,11 @@
 // with a scale for 32 columns.  That sum is the bf16 value down to 2^-11 of the block's largest magnitude and within 2^-21 of the largest below.  Two
 // instructions multiply both planes into one accumulator; at twice the rate of bf16 that costs what a bf16 product costs.
 //
-// A stage is a chunk of 128 columns: codes (16 KB in shared memory, 8 KB from memory), both planes of up to 192 rows of x, and scales, which four warps move from
-// shared memory to tensor memory (column j of an operand: lane l of every quarter holds the four scale bytes of row 32 j + l).  With few tiles K is split
-// among CTAs; their sums meet in memory, and the one that comes last adds them up in the order of K.
+// A stage is a chunk of 128 columns (two for up to 64 rows of x: the issuing thread's waits cost as much as the products of a small chunk): codes (16 KB
+// in shared memory, 8 KB from memory) and both planes of up to 192 rows of x.  Scales have a longer ring of their own:
+// four warps move them from shared memory to tensor memory (column j of an operand: lane l of every quarter holds the four scale bytes of row 32 j + l)
+// while the stage they belong to is still on its way.  With few tiles K is split among CTAs; their sums meet in memory, and the one that comes last
+// adds them up in the order of K.
 #include <cuda_fp8.h>
 
 #include "jib_kernels.h"
@@ -23,14 +25,15 @@ namespace {
 using namespace sm100;
 typedef __nv_bfloat16 bf16;
 
-constexpr int BM = 128, MAX_BN = 192, MAX_STAGES = 8, MAX_E = 256, PAD = 32;
+constexpr int BM = 128, MAX_BN = 192, MAX_STAGES = 8, MAX_SLOTS = 8, MAX_E = 256, PAD = 32;
 constexpr int A_BYTES = BM * 128, SA_BYTES = BM * 4;
-constexpr int THREADS = 384;                       // producer, issuer, two idle; four scale warps; four epilogue warps
+constexpr int THREADS = 512;                       // producer, issuer, one idle, producer of scales; four scale warps; eight epilogue warps
 constexpr int MOST_SMEM = 227 * 1024;
 // Rows of the planes' scales: a tile reads up to MAX_BN behind the last one, 16 bytes (four rows) at a time.
 __host__ __device__ inline long long scale_rows_of(long long rows) { return (rows + MAX_BN + 31) / 32 * 32; }
 
-__host__ __device__ inline int stage_bytes(int bn) { return (A_BYTES + 2 * bn * 128 + SA_BYTES + 2 * bn * 4 + 1023) / 1024 * 1024; }
+__host__ __device__ inline int stage_bytes(int bn) { return A_BYTES + 2 * bn * 128; }
+__host__ __device__ inline int slot_bytes(int bn) { return SA_BYTES + 2 * bn * 4; }              // scales of a stage
 __host__ __device__ inline int scale_cols(int bn) { return (bn + 127) / 128 * 4; }          // of one plane
 
 struct Args {
@@ -44,7 +47,7 @@ struct Args {
     int * counters;                          // zeros, one a tile
     int * status;
     long long ldo, ldr, x_rows;
-    int T, N, R, C, E, bn, m_tiles, t_tiles, splits, stages, gated, act, out_f32, res_f32;
+    int T, N, R, C, E, bn, m_tiles, t_tiles, splits, stages, slots, cps, gated, act, out_f32, res_f32;
 };
 
 __device__ __forceinline__ void st_cols4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -62,6 +65,15 @@ __device__ __forceinline__ void mma_mxf8f6f4(uint32_t d, uint64_t a, uint64_t b,
 __device__ __forceinline__ uint32_t idesc_e2m1_e4m3(int n, uint32_t k) {
     return k << 4 | 5u << 7 | 0u << 10 | (uint32_t) (n >> 3) << 17 | 1u << 23 | (uint32_t) (BM >> 4) << 24 | k << 29;
 }
+
+// A place in a ring of n and the parity of its round (divisions by the number of stages took the issuing thread as long as the products).
+struct Ring {
+    int at = 0;
+    uint32_t round = 0;
+    __device__ __forceinline__ void next(int n) {
+        if (++at == n) { at = 0; round ^= 1; }
+    }
+};
 
 // What item i is: row tile m, first row of x, how many, chunks c0 .. c1 - 1, matrix, tile (for sums that meet).
 struct Item {
@@ -104,15 +116,18 @@ __device__ __forceinline__ Item item_of(const Args & g, const int * first_tile, 
 __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Args g) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ int first_tile[MAX_E + 1], last_s;
-    __shared__ uint64_t bars[3 * MAX_STAGES + 4];
+    __shared__ uint64_t bars[2 * MAX_STAGES + 3 * MAX_SLOTS + 4];
     __shared__ uint32_t tmem_slot;
     uint8_t * tiles = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
-    uint64_t * full = bars, * empty = full + MAX_STAGES, * sf_full = empty + MAX_STAGES, * acc_full = sf_full + MAX_STAGES, * acc_empty = acc_full + 2;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = g.stages, bn = g.bn;
-    const int SB = stage_bytes(bn), plane = bn * 128, sfc = scale_cols(bn), slab = 4 + 2 * sfc;
+    uint64_t * full = bars, * empty = full + MAX_STAGES, * sl_full = empty + MAX_STAGES, * sf_full = sl_full + MAX_SLOTS, * sf_empty = sf_full + MAX_SLOTS,
+             * acc_full = sf_empty + MAX_SLOTS, * acc_empty = acc_full + 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = g.stages, Q = g.slots, bn = g.bn, cps = g.cps;
+    uint8_t * scale_slots = tiles + S * cps * stage_bytes(bn);
+    const int SB = stage_bytes(bn), QB = slot_bytes(bn), plane = bn * 128, sfc = scale_cols(bn), slab = 4 + 2 * sfc;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&sf_full[i], 4); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+        for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < Q; ++i) { mbar_init(&sl_full[i], 1); mbar_init(&sf_full[i], 4); mbar_init(&sf_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 8); }
         fence_barrier_init();
         prefetch_tmap(&tm_w);
         prefetch_tmap(&tm_x);
@@ -152,37 +167,63 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 
     if (warp == 0) {
         if (elect_one()) {
-            int it = 0;
+            Ring r;
+            bool ok = true;
+#pragma unroll 1
+            for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+                const Item t = item_of(g, first_tile, i);
+#pragma unroll 1
+                for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(S)) {
+                    const int s = r.at, n = min(cps, t.c1 - c0);
+                    if (!mbar_wait(&empty[s], r.round ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 61, i); ok = false; break; }
+                    mbar_expect_tx(&full[s], n * (A_BYTES / 2 + 2 * plane));      // (codes count as they are in memory)
+#pragma unroll 1
+                    for (int j = 0; j < n; ++j) {
+                        uint8_t * st = tiles + (s * cps + j) * SB;
+                        tma_load_3d(st, &tm_w, &full[s], 0, t.m * BM, t.e * g.C + c0 + j);
+                        tma_load_3d(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0, 0);
+                        tma_load_3d(st + A_BYTES + plane, &tm_x, &full[s], (c0 + j) * 128, t.row0, 1);
+                    }
+                }
+            }
+            // copies in flight end before the memory is given back (the last round's; a stage that was not asked for is not waited for long)
+            if (!ok)
+                for (int i = 0; i < S; ++i) mbar_wait(&full[i], i < r.at ? r.round : r.round ^ 1);
+        }
+        __syncwarp();
+    } else if (warp == 3) {
+        if (elect_one()) {
+            Ring r;
             bool ok = true;
 #pragma unroll 1
             for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
                 const Item t = item_of(g, first_tile, i);
                 const int w_rows = min(BM, g.R - t.m * BM);
 #pragma unroll 1
-                for (int c = t.c0; c < t.c1; ++c, ++it) {
-                    const int s = it % S;
-                    if (!mbar_wait(&empty[s], (it / S & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 61, i); ok = false; break; }
-                    uint8_t * st = tiles + s * SB;
-                    const int z = t.e * g.C + c;
-                    mbar_expect_tx(&full[s], A_BYTES / 2 + 2 * plane + w_rows * 4 + 2 * bn * 4);      // (codes count as they are in memory)
-                    tma_load_3d(st, &tm_w, &full[s], 0, t.m * BM, z);
-                    tma_load_3d(st + A_BYTES, &tm_x, &full[s], c * 128, t.row0, 0);
-                    tma_load_3d(st + A_BYTES + plane, &tm_x, &full[s], c * 128, t.row0, 1);
-                    uint8_t * sc = st + A_BYTES + 2 * plane;
-                    mx4::bulk_load(sc, g.w_scales + ((size_t) z * g.R + t.m * BM) * 4, w_rows * 4, &full[s]);
-                    mx4::bulk_load(sc + SA_BYTES, g.x_scales + ((size_t) c * g.x_rows + t.row0) * 4, bn * 4, &full[s]);
-                    mx4::bulk_load(sc + SA_BYTES + bn * 4, g.x_scales + ((size_t) (g.C + c) * g.x_rows + t.row0) * 4, bn * 4, &full[s]);
+                for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(Q)) {
+                    const int q = r.at, n = min(cps, t.c1 - c0);
+                    if (!mbar_wait(&sf_empty[q], r.round ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 66, i); ok = false; break; }
+                    mbar_expect_tx(&sl_full[q], n * (w_rows * 4 + 2 * bn * 4));
+#pragma unroll 1
+                    for (int c = c0; c < c0 + n; ++c) {
+                        uint8_t * sc = scale_slots + (q * cps + c - c0) * QB;
+                        mx4::bulk_load(sc, g.w_scales + ((size_t) (t.e * g.C + c) * g.R + t.m * BM) * 4, w_rows * 4, &sl_full[q]);
+                        mx4::bulk_load(sc + SA_BYTES, g.x_scales + ((size_t) c * g.x_rows + t.row0) * 4, bn * 4, &sl_full[q]);
+                        mx4::bulk_load(sc + SA_BYTES + bn * 4, g.x_scales + ((size_t) (g.C + c) * g.x_rows + t.row0) * 4, bn * 4, &sl_full[q]);
+                    }
                 }
             }
-            // copies in flight end before the memory is given back
             if (!ok)
-                for (int i = it - S < 0 ? 0 : it - S; i < it; ++i) mbar_wait(&full[i % S], i / S & 1);
+                for (int i = 0; i < Q; ++i) mbar_wait(&sl_full[i], i < r.at ? r.round : r.round ^ 1);
         }
         __syncwarp();
     } else if (warp == 1) {
         if (elect_one()) {
-            int it = 0, j = 0;
+            Ring r, rq;
+            int j = 0;
             bool ok = true;
+            const uint64_t desc0 = desc_k_sw128(smem_u32(tiles));
+            const uint32_t id0 = idesc_e2m1_e4m3(bn, 0), lo = (uint32_t) plane >> 4;
 #pragma unroll 1
             for (int i = blockIdx.x; i < items && ok; i += gridDim.x, ++j) {
                 const Item t = item_of(g, first_tile, i);
@@ -190,19 +231,30 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                 if (!mbar_wait(&acc_empty[buf], (j >> 1 & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 62, i); break; }
                 tc_fence_after();
                 const uint32_t acc = tmem + buf * bn;
+                bool more = false;
 #pragma unroll 1
-                for (int c = t.c0; c < t.c1; ++c, ++it) {
-                    const int s = it % S;
-                    if (!mbar_wait(&sf_full[s], it / S & 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 63, i); ok = false; break; }
+                for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(S), rq.next(Q)) {
+                    if (!mbar_wait(&sf_full[rq.at], rq.round) || !mbar_wait(&full[r.at], r.round)) {
+                        jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 63, i);
+                        ok = false;
+                        break;
+                    }
                     tc_fence_after();
-                    const uint32_t a = smem_u32(tiles + s * SB), sf = sf0 + s * slab;
+                    // descriptors count in 16 bytes, a step of 32 columns is two of them; the scales' byte is in bits 4 and 29 of the other
+#pragma unroll 1
+                    for (int j = 0; j < min(cps, t.c1 - c0); ++j) {
+                        const uint64_t a = desc0 + (uint32_t) ((r.at * cps + j) * SB >> 4), b = a + (A_BYTES >> 4);
+                        const uint32_t sf = sf0 + (rq.at * cps + j) * slab;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-#pragma unroll
-                        for (int p = 0; p < 2; ++p)
-                            mma_mxf8f6f4(acc, desc_k_sw128(a + k * 32), desc_k_sw128(a + A_BYTES + p * plane + k * 32), idesc_e2m1_e4m3(bn, k), sf,
-                                         sf + 4 + p * sfc, c != t.c0 || k != 0 || p != 0);
-                    mma_commit(&empty[s]);
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t id = id0 + (k << 4) + ((uint32_t) k << 29);
+                            mma_mxf8f6f4(acc, a + 2 * k, b + 2 * k, id, sf, sf + 4, more || k != 0);
+                            mma_mxf8f6f4(acc, a + 2 * k, b + lo + 2 * k, id, sf, sf + 4 + sfc, true);
+                        }
+                        more = true;
+                    }
+                    mma_commit(&empty[r.at]);
+                    mma_commit(&sf_empty[rq.at]);
                 }
                 mma_commit(&acc_full[buf]);
             }
@@ -211,38 +263,42 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
     } else if (warp >= 4 && warp < 8) {
         // scales to tensor memory
         const uint32_t mine = sf0 + ((uint32_t) (warp & 3) << 21);
-        int it = 0;
+        Ring r;
         bool ok = true;
 #pragma unroll 1
         for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
             const Item t = item_of(g, first_tile, i);
 #pragma unroll 1
-            for (int c = t.c0; c < t.c1; ++c, ++it) {
-                const int s = it % S;
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], it / S & 1));
+            for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(Q)) {
+                const int q = r.at;
+                ok = __all_sync(0xffffffffu, mbar_wait(&sl_full[q], r.round));
                 if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 64, i); break; }
                 tc_fence_after();
-                const uint32_t * sc = (const uint32_t *) (tiles + s * SB + A_BYTES + 2 * plane) + lane;
-                const uint32_t dst = mine + s * slab;
-                st_cols4(dst, sc[0], sc[32], sc[64], sc[96]);
 #pragma unroll 1
-                for (int p = 0; p < 2; ++p) {
-                    const uint32_t * sx = sc + SA_BYTES / 4 + p * bn;
-                    for (int q = 0; q < sfc; q += 4) {
-                        uint32_t v[4];
+                for (int c = 0; c < min(cps, t.c1 - c0); ++c) {
+                    const uint32_t * sc = (const uint32_t *) (scale_slots + (q * cps + c) * QB) + lane;
+                    const uint32_t dst = mine + (q * cps + c) * slab;
+                    st_cols4(dst, sc[0], sc[32], sc[64], sc[96]);
+#pragma unroll 1
+                    for (int p = 0; p < 2; ++p) {
+                        const uint32_t * sx = sc + SA_BYTES / 4 + p * bn;
+                        for (int j = 0; j < sfc; j += 4) {
+                            uint32_t v[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) v[k] = (q + k) * 32 + lane < bn ? sx[(q + k) * 32] : 0u;
-                        st_cols4(dst + 4 + p * sfc + q, v[0], v[1], v[2], v[3]);
+                            for (int k = 0; k < 4; ++k) v[k] = (j + k) * 32 + lane < bn ? sx[(j + k) * 32] : 0u;
+                            st_cols4(dst + 4 + p * sfc + j, v[0], v[1], v[2], v[3]);
+                        }
                     }
                 }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sf_full[s]);
+                if (lane == 0) mbar_arrive(&sf_full[q]);
             }
         }
     } else if (warp >= 8) {
-        const int q = warp & 3;
+        // two warps a quarter of the rows, they take every second 16 rows of x
+        const int q = warp & 3, half = (warp - 8) >> 2;
         const uint32_t mine = tmem + ((uint32_t) q << 21);
         int j = 0;
 #pragma unroll 1
@@ -257,7 +313,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             if (g.splits > 1) {
                 float * to = part + (size_t) t.split * bn * BM;
 #pragma unroll 1
-                for (int c = 0; c < t.rows; c += 16) {
+                for (int c = 16 * half; c < t.rows; c += 32) {
                     uint32_t v[16];
                     tmem_ld16(acc + c, v);
                     tmem_ld_wait();
@@ -266,29 +322,36 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                         if (c + k < t.rows) __stcg(to + (size_t) (c + k) * BM, __uint_as_float(v[k]));
                 }
                 __threadfence();
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (threadIdx.x == 256) {
                     last_s = atomicAdd(g.counters + t.tile, 1) == g.splits - 1;
                     __threadfence();
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                asm volatile("bar.sync 1, 256;" ::: "memory");
                 finish = last_s != 0;
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                asm volatile("bar.sync 1, 256;" ::: "memory");
             }
             // lane = row n of the tile (of pairs: 16 of the gate, 16 of the up matrix), 16 rows of x at a time
             const int n = g.gated ? t.m * 64 + q * 16 + (lane & 15) : t.m * BM + q * 32 + lane;
-            const bool writes = n < g.N && (!g.gated || lane < 16);
 #pragma unroll 1
-            for (int c = 0; c < t.rows && finish; c += 16) {
+            for (int c = 16 * half; c < t.rows && finish; c += 32) {
                 float y[16];
                 if (g.splits > 1) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) y[k] = 0.f;
 #pragma unroll 1
-                    for (int s = 0; s < g.splits; ++s)
+                    for (int s = 0; s < g.splits; s += 2) {
+                        float v[2][16];
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            if (c + k < t.rows) y[k] += __ldcg(part + ((size_t) s * bn + c + k) * BM);
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                v[h][k] = c + k < t.rows && s + h < g.splits ? __ldcg(part + ((size_t) (s + h) * bn + c + k) * BM) : 0.f;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) y[k] += v[h][k];
+                    }
                 } else {
                     uint32_t v[16];
                     tmem_ld16(acc + c, v);
@@ -296,10 +359,22 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 #pragma unroll
                     for (int k = 0; k < 16; ++k) y[k] = __uint_as_float(v[k]);
                 }
-                if (g.gated)
+                if (g.gated) {
+                    // a gate's lane takes the even rows of x, the up matrix's lane 16 above it the odd ones
+                    bf16 * to = (bf16 *) g.out + (long long) (t.row0 + c + (lane >> 4)) * g.ldo + n;
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) y[k] = mx4::gated(y[k], __shfl_down_sync(0xffffffffu, y[k], 16), g.act);
-                if (!writes) continue;
+                    for (int k = 0; k < 16; k += 2) {
+                        const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? y[k + 1] : y[k], 16);
+                        const float v = mx4::gated(lane < 16 ? y[k] : other, lane < 16 ? other : y[k + 1], g.act);
+                        if (n < g.N && c + k + (lane >> 4) < t.rows) {
+                            if (g.out_f32) ((float *) g.out)[(long long) (t.row0 + c + k + (lane >> 4)) * g.ldo + n] = v;
+                            else *to = __float2bfloat16(v);
+                        }
+                        to += 2 * g.ldo;
+                    }
+                    continue;
+                }
+                if (n >= g.N) continue;
                 if (g.residual != nullptr)
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
@@ -307,13 +382,15 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                             const long long at = (long long) (t.row0 + c + k) * g.ldr + n;
                             y[k] += g.res_f32 ? ((const float *) g.residual)[at] : __bfloat162float(((const bf16 *) g.residual)[at]);
                         }
+                bf16 * to = (bf16 *) g.out + (long long) (t.row0 + c) * g.ldo + n;
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
+                for (int k = 0; k < 16; ++k) {
                     if (c + k < t.rows) {
-                        const long long at = (long long) (t.row0 + c + k) * g.ldo + n;
-                        if (g.out_f32) ((float *) g.out)[at] = y[k];
-                        else ((bf16 *) g.out)[at] = __float2bfloat16(y[k]);
+                        if (g.out_f32) ((float *) g.out)[(long long) (t.row0 + c + k) * g.ldo + n] = y[k];
+                        else *to = __float2bfloat16(y[k]);
                     }
+                    to += g.ldo;
+                }
             }
             tc_fence_before();
             __syncwarp();
@@ -568,9 +645,10 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const
         if (g.splits > 1 && (part == nullptr || counters == nullptr)) return JIB_E_SCRATCH;
     }
     if (items > 0x3fffffff) return JIB_E_ARG;
-    g.stages = (MOST_SMEM - 4096 - 1024) / stage_bytes(g.bn);        // (4 KB: barriers and tables)
-    const int slab = 4 + 2 * scale_cols(g.bn);
-    if (g.stages > (512 - 2 * g.bn) / slab) g.stages = (512 - 2 * g.bn) / slab;
+    g.cps = g.bn <= 64 ? 2 : 1;
+    g.slots = (512 - 2 * g.bn) / (g.cps * (4 + 2 * scale_cols(g.bn)));
+    if (g.slots > MAX_SLOTS) g.slots = MAX_SLOTS;
+    g.stages = (MOST_SMEM - 4096 - 1024 - g.slots * g.cps * slot_bytes(g.bn)) / (g.cps * stage_bytes(g.bn));        // (4 KB: barriers and tables)
     if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
     CUtensorMap mw, mx;
     int rc = weights_map(&mw, d->w, g.R, (long long) g.C * d->batch);
@@ -579,7 +657,7 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const
     if (rc) return rc;
     static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
     if (!jib::ensure_dyn_smem(mx4_gemm_kernel, MOST_SMEM - 4096, attr_done)) return JIB_E_LAUNCH;
-    JIB_LAUNCH((mx4_gemm_kernel), (unsigned) (items < sms ? items : sms), THREADS, g.stages * stage_bytes(g.bn) + 1024, (cudaStream_t) stream, mw, mx, g);
+    JIB_LAUNCH((mx4_gemm_kernel), (unsigned) (items < sms ? items : sms), THREADS, g.cps * (g.stages * stage_bytes(g.bn) + g.slots * slot_bytes(g.bn)) + 1024, (cudaStream_t) stream, mw, mx, g);
     return launched();
 }
 

@@ -3,7 +3,8 @@
 // tcgen05.mma.kind::mxf4.block_scale multiplies E2M1 codes and applies the blocks' scales itself, 64 columns an instruction: nothing is
 // expanded.  b (the weights) is operand A of the instruction, 128 rows a tile, a's rows are its columns, up to 208 a tile: so few tokens cost
 // a narrow tile.  The scales live in tensor memory: column j of a slab holds, in lane l of every quarter, the four scale bytes of row 32 j + l
-// for 128 columns of K.  Four warps copy them there from global memory, a stage (256 columns, 128 bytes of codes a row) at a time.
+// for 128 columns of K.  They come in boxes of 16 bytes a row (512 columns, two stages) in a ring of their own, and four warps move them to tensor
+// memory ahead of their stage.  (Read from global memory by those warps, stage by stage, they took 1200 clocks a stage, three times the products.)
 #include "sm100.cuh"
 #include "jib_kernels.h"
 #include "pdl.cuh"
@@ -16,15 +17,14 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int BM = 128, MAX_BN = 208, STAGES = 4, KS = 256;       // weights a tile, tokens at most, stages, columns a stage
 constexpr int A_BYTES = BM * 128, B_BYTES = MAX_BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int BOXES = 3, BOX_BYTES = (BM + MAX_BN) * 16;         // scales of two stages
+constexpr int SMEM = STAGES * STAGE_BYTES + BOXES * BOX_BYTES + 1024 + 256;
 constexpr int SLAB = 12;                                         // columns of the scales of 128 columns of K: 4 of A, 8 of B
 constexpr int SF0 = 2 * MAX_BN;                                  // two accumulators, then the scales of each stage
-constexpr int THREADS = 384;                                     // producer, issuer, two idle; four scale warps; four epilogue warps
+constexpr int THREADS = 384;                                     // producer, issuer, one idle, producer of scales; four scale warps; four epilogue warps
 static_assert(SF0 + STAGES * 2 * SLAB <= 512, "tensor memory");
 
 struct Args {
-    const uint8_t * a_scales, * b_scales;
-    long long a_ld, b_ld;                    // bytes between rows, a multiple of 8
     void * out;
     long long ldo;
     int * status;
@@ -48,17 +48,21 @@ __device__ __forceinline__ uint32_t idesc_mxf4(int n, uint32_t half) {
 }
 
 __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                                                                const Args g) {
+                                                                const __grid_constant__ CUtensorMap tm_as, const __grid_constant__ CUtensorMap tm_bs, const Args g) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t * tiles = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
-    uint64_t * full = (uint64_t *) (tiles + STAGES * STAGE_BYTES), * empty = full + STAGES, * sf_full = empty + STAGES, * acc_full = sf_full + STAGES,
-             * acc_empty = acc_full + 2;
-    uint32_t * tmem_slot = (uint32_t *) (acc_empty + 2);
+    uint8_t * boxes = tiles + STAGES * STAGE_BYTES;
+    uint64_t * full = (uint64_t *) (boxes + BOXES * BOX_BYTES), * empty = full + STAGES, * sf_full = empty + STAGES, * acc_full = sf_full + STAGES,
+             * acc_empty = acc_full + 2, * box_full = acc_empty + 2, * box_empty = box_full + BOXES;
+    uint32_t * tmem_slot = (uint32_t *) (box_empty + BOXES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&sf_full[i], 4); }
         for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+        for (int i = 0; i < BOXES; ++i) { mbar_init(&box_full[i], 1); mbar_init(&box_empty[i], 4); }
         fence_barrier_init();
+        prefetch_tmap(&tm_as);
+        prefetch_tmap(&tm_bs);
         prefetch_tmap(&tm_a);
         prefetch_tmap(&tm_b);
     }
@@ -120,27 +124,52 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
             }
         }
         __syncwarp();
+    } else if (warp == 3) {
+        if (elect_one()) {
+            int it = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+                const int n0 = item % g.m_tiles * BM, t0 = item / g.m_tiles * g.bn;
+                for (int kb = 0; kb < n_stages; kb += 2, ++it) {
+                    const int s = it % BOXES;
+                    if (!mbar_wait(&box_empty[s], (it / BOXES & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 46, item); ok = false; break; }
+                    mbar_expect_tx(&box_full[s], (BM + g.bn) * 16);
+                    tma_load_2d(boxes + s * BOX_BYTES, &tm_bs, &box_full[s], kb * 8, n0);
+                    tma_load_2d(boxes + s * BOX_BYTES + BM * 16, &tm_as, &box_full[s], kb * 8, t0);
+                }
+            }
+            if (!ok)
+                for (int i = it - BOXES < 0 ? 0 : it - BOXES; i < it; ++i) mbar_wait(&box_full[i % BOXES], i / BOXES & 1);
+        }
+        __syncwarp();
     } else if (warp >= 4 && warp < 8) {
         // scales of a stage: eight bytes a row
         const uint32_t mine = tmem + ((uint32_t) (warp & 3) << 21) + SF0;
-        const int valid = g.K / 32, b_words = (g.bn + 31) / 32;
-        int it = 0;
+        const int valid = g.K / 32;
+        int it = 0, box = -1;
         bool ok = true;
-        for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
-            const int n0 = item % g.m_tiles * BM, t0 = item / g.m_tiles * g.bn;
+        for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x)
             for (int kb = 0; kb < n_stages; ++kb, ++it) {
                 const int s = it % STAGES, n = valid - kb * 8;
+                if ((kb & 1) == 0) {
+                    ++box;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&box_full[box % BOXES], box / BOXES & 1));
+                    if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 47, item); break; }
+                }
                 // bytes behind the last block: 1 (the codes there are zero)
                 const uint64_t keep = n >= 8 ? ~0ull : (1ull << (8 * n)) - 1, ones = 0x7f7f7f7f7f7f7f7full & ~keep;
+                const uint8_t * rows = boxes + box % BOXES * BOX_BYTES + (kb & 1) * 8 + lane * 16;
                 uint2 v[12];
 #pragma unroll
                 for (int j = 0; j < 12; ++j) {
-                    const bool of_b = j < 4;
-                    const long long row = of_b ? min(n0 + 32 * j + lane, g.N - 1) : min(t0 + 32 * (j - 4) + lane, g.T - 1);
                     uint64_t w = 0;
-                    if (of_b || j - 4 < b_words) w = *(const uint64_t *) ((of_b ? g.b_scales + row * g.b_ld : g.a_scales + row * g.a_ld) + kb * 8);
+                    if (j < 4 || (j - 4) * 32 + lane < g.bn) w = *(const uint64_t *) (rows + j * 512);
                     w = (w & keep) | ones;
                     v[j] = make_uint2((uint32_t) w, (uint32_t) (w >> 32));
+                }
+                if ((kb & 1) != 0 || kb == n_stages - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&box_empty[box % BOXES]);
                 }
                 ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (it / STAGES & 1) ^ 1));
                 if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 44, item); break; }
@@ -156,7 +185,6 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sf_full[s]);
             }
-        }
     } else if (warp >= 8) {
         const uint32_t mine = tmem + ((uint32_t) (warp & 3) << 21);
         int j = 0;
@@ -189,12 +217,12 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
 
 }  // namespace
 
-// a [T][K], b [N][K] in 4 bits: codes row-major and dense, scale rows a_ld / b_ld bytes apart (multiples of 8, the arrays 8-byte aligned).
+// a [T][K], b [N][K] in 4 bits: codes row-major and dense, scale rows a_ld / b_ld bytes apart (multiples of 16, the arrays 16-byte aligned).
 extern "C" JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_scales, long long a_ld, const void * b_codes, const void * b_scales,
                                          long long b_ld, void * out, long long ldo, int out_f32, int T, int N, int K, int * status, void * stream) {
     if (T <= 0) return 0;
     if (N <= 0 || K <= 0 || K % 32 || a_ld < K / 32 || b_ld < K / 32) return JIB_E_ARG;
-    if (((uintptr_t) a_scales | (uintptr_t) b_scales | (uintptr_t) a_ld | (uintptr_t) b_ld) & 7) return JIB_E_ALIGN;
+    if (((uintptr_t) a_scales | (uintptr_t) b_scales | (uintptr_t) a_ld | (uintptr_t) b_ld) & 15) return JIB_E_ALIGN;
     // The width of a token tile: the one whose rounds over the machine cost least (a tile's fixed part is worth some 24 tokens).
     const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148, m_tiles = (N + BM - 1) / BM;
     int bn = 16;
@@ -205,7 +233,6 @@ extern "C" JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_sc
         if (w >= T) break;
     }
     Args g;
-    g.a_scales = (const uint8_t *) a_scales; g.b_scales = (const uint8_t *) b_scales; g.a_ld = a_ld; g.b_ld = b_ld;
     g.out = out; g.ldo = ldo; g.status = status; g.T = T; g.N = N; g.K = K; g.bn = bn; g.out_f32 = out_f32; g.m_tiles = m_tiles;
     const long long items = (long long) m_tiles * ((T + bn - 1) / bn);
     if (items > 0x3fffffff) return JIB_E_ARG;
@@ -215,8 +242,13 @@ extern "C" JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_sc
     if (rc) return rc;
     rc = jib::tma_rows_map(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, b_codes, N, K / 2, K / 2, BM);
     if (rc) return rc;
+    CUtensorMap mas, mbs;
+    rc = jib::tma_bytes_map(&mas, a_scales, T, a_ld, 16, bn);
+    if (rc) return rc;
+    rc = jib::tma_bytes_map(&mbs, b_scales, N, b_ld, 16, BM);
+    if (rc) return rc;
     static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
     if (!jib::ensure_dyn_smem(mx4_matmul_kernel, SMEM, attr_done)) return JIB_E_LAUNCH;
-    JIB_LAUNCH((mx4_matmul_kernel), (unsigned) (items < sms ? items : sms), THREADS, SMEM, (cudaStream_t) stream, ma, mb, g);
+    JIB_LAUNCH((mx4_matmul_kernel), (unsigned) (items < sms ? items : sms), THREADS, SMEM, (cudaStream_t) stream, ma, mb, mas, mbs, g);
     return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH;
 }

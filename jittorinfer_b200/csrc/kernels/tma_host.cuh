@@ -39,4 +39,17 @@ inline int tma_rows_map(CUtensorMap * out, CUtensorMapDataType type, const void 
                : JIB_E_TENSORMAP;
 }
 
+// rows of row_bytes bytes as they are, in boxes box_bytes wide and box_rows high, not swizzled, zeros outside.
+inline int tma_bytes_map(CUtensorMap * out, const void * ptr, long long rows, long long row_bytes, int box_bytes, int box_rows) {
+    TmaEncodeFn fn = tma_encode_fn();
+    if (!fn) return JIB_E_DRIVER;
+    if (((uintptr_t) ptr & 15) || row_bytes % 16) return JIB_E_ALIGN;
+    const cuuint64_t dims[2] = {(cuuint64_t) row_bytes, (cuuint64_t) rows}, strides[1] = {(cuuint64_t) row_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t) box_bytes, (cuuint32_t) box_rows}, step[2] = {1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0
+               : JIB_E_TENSORMAP;
+}
+
 }  // namespace jib

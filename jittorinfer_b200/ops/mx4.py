@@ -16,26 +16,39 @@ from . import reference as ref
 BLOCK = 32                     # columns that share a scale
 COLS = 128                     # columns of a packed chunk (csrc/kernels/mx4.cuh)
 ACTS = ("silu", "gelu_tanh")
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
+_kernels = _front = None          # native_mx4 once its library is loaded; the package
+
+
 def _native(t: torch.Tensor):
-    from . import use_native
-    if not use_native(t):
+    """The kernels' bindings for a tensor that goes to them, else None."""
+    global _kernels, _front
+    if not t.is_cuda:
         return None
-    from . import nat, native_mx4
-    nat()
-    return native_mx4
+    if _kernels is None:
+        from .. import ops
+        _front = ops
+        if ops.force_torch():
+            return None
+        ops.nat()
+        from . import native_mx4
+        _kernels = native_mx4
+    return None if _front._FORCE_TORCH else _kernels
 
 
 def scale_rows(lead, blocks: int, device) -> torch.Tensor:
-    """Room for the scales of rows, a view: each row starts at a multiple of 8 bytes."""
-    return torch.empty(*lead, (blocks + 7) // 8 * 8, dtype=torch.uint8, device=device)[..., :blocks]
+    """Room for the scales of rows, a view: each row starts at a multiple of 16 bytes."""
+    if blocks % 16 == 0:
+        return torch.empty(*lead, blocks, dtype=torch.uint8, device=device)
+    return torch.empty(*lead, (blocks + 15) // 16 * 16, dtype=torch.uint8, device=device)[..., :blocks]
 
 
 def _laid_out(s: torch.Tensor) -> bool:
     ld, want = s.stride(-2), s.stride(-2)
-    if s.stride(-1) != 1 or ld % 8 or ld < s.shape[-1] or s.data_ptr() % 8:
+    if s.stride(-1) != 1 or ld % 16 or ld < s.shape[-1] or s.data_ptr() % 16:
         return False
     for i in range(s.dim() - 2, -1, -1):
         if s.stride(i) != want:
@@ -46,7 +59,7 @@ def _laid_out(s: torch.Tensor) -> bool:
 
 class Mx4Tensor:
     """Rows of 4-bit values: ``codes`` uint8 [..., cols / 2] (the lower half of a byte is the even column), ``scales`` uint8 [..., cols / 32].  They are kept
-    as the kernels read them: codes dense and 16-byte aligned, scale rows at multiples of 8 bytes; tensors that are otherwise are copied."""
+    as the kernels read them: codes dense and 16-byte aligned, scale rows at multiples of 16 bytes; tensors that are otherwise are copied."""
     __slots__ = ("codes", "scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
@@ -62,6 +75,13 @@ class Mx4Tensor:
             rows.copy_(scales)
             scales = rows
         self.scales = scales
+
+    @classmethod
+    def _of(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Mx4Tensor":
+        """From tensors that are laid out as they have to be."""
+        q = cls.__new__(cls)
+        q.codes, q.scales = codes, scales
+        return q
 
     @property
     def shape(self) -> Tuple[int, ...]:
@@ -202,7 +222,7 @@ def _check_out(out_dtype: Optional[torch.dtype], x_dtype: torch.dtype, what: str
 def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
     """bf16, fp16 or fp32 [..., cols] to 4 bits, cols a multiple of 32.  A block's scale is 2^(floor(log2 of its largest magnitude) - 2), at least
     2^-127; a value goes to the nearest code, ties to the even one, at most 6.  A block with an infinity or NaN becomes NaN."""
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if x.dtype not in _TYPES:
         raise ValueError(f"mx4_quantize: bf16, fp16 or fp32, not {x.dtype}")
     if x.dim() < 2 or x.shape[-1] == 0 or x.shape[-1] % BLOCK:
         raise ValueError(f"mx4_quantize: rows of whole blocks of {BLOCK}, not {tuple(x.shape)}")
@@ -212,7 +232,7 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
 
 def mx4_dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values as bf16, fp16 or fp32 (rounded where the type cannot hold them)."""
-    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if dtype not in _TYPES:
         raise ValueError(f"mx4_dequantize: bf16, fp16 or fp32, not {dtype}")
     n = _native(q.codes)
     return n.dequantize(q, dtype) if n else _dequantize(q, dtype)

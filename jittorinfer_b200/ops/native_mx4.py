@@ -15,30 +15,32 @@ FEW_TOKENS = 16                              # tokens of a layer that runs as on
 PAD = 32                                     # rows of an expert are padded to in grouped products (csrc/kernels/mx4_gemm.cu)
 MAX_EXPERTS, MAX_CHOICES = 256, 32           # what the gate and the sort take (csrc/kernels/moe.cu)
 _NO_SWITCH = contextlib.nullcontext()
+_current = nat._device or torch.cuda.current_device
 
 
 def _on(t: torch.Tensor):
     """The tensor's device as the current one: launches go to the current device's stream."""
-    return _NO_SWITCH if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NO_SWITCH if t.get_device() == _current() else torch.cuda.device(t.device)
 
 
 def quantize(x: torch.Tensor) -> Mx4Tensor:
-    cols = x.shape[-1]
-    x2 = x if x.dim() == 2 else x.reshape(-1, cols)
-    if x2.stride(1) != 1 or x2.stride(0) < 0:
+    *lead, cols = x.shape
+    x2 = x if len(lead) == 1 else x.reshape(-1, cols)
+    if x2.stride(1) != 1:
         x2 = x2.contiguous()
-    codes = torch.empty(*x.shape[:-1], cols // 2, dtype=torch.uint8, device=x.device)
-    scales = scale_rows(x.shape[:-1], cols // 32, x.device)
+    codes = torch.empty(*lead, cols // 2, dtype=torch.uint8, device=x.device)
+    scales = scale_rows(lead, cols // 32, x.device)
     with _on(x):
         nat._ck(nat.load().jib_mx4_quantize(x2.data_ptr(), TYPES[x.dtype], x2.stride(0), codes.data_ptr(), scales.data_ptr(), scales.stride(-2), x2.shape[0], cols,
                                             nat._stream()), "mx4_quantize")
-    return Mx4Tensor(codes, scales)
+    return Mx4Tensor._of(codes, scales)
 
 
 def dequantize(q: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    out = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
+    cols = out.shape[-1]
     with _on(out):
-        nat._ck(nat.load().jib_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), q.scales.stride(-2), out.data_ptr(), TYPES[dtype], out.numel() // q.shape[-1], q.shape[-1],
+        nat._ck(nat.load().jib_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), q.scales.stride(-2), out.data_ptr(), TYPES[dtype], out.numel() // cols, cols,
                                               nat._stream()), "mx4_dequantize")
     return out
 

@@ -338,7 +338,7 @@ typedef struct jib_mx4_desc {
     const int * src;           // with seg: row r of the result comes from row src[r] of x (NULL: row r)
     int * status;
     long long ldx, ldo, ldr;
-    int T, N, K, batch, max_rows;          // T: rows of the result; max_rows: the most that one matrix can have
+    int T, N, K, batch, max_rows;          // T: rows of the result; max_rows: the most that one matrix can have (tiled and grouped: the rows of all)
     int gated, act, out_f32, res_f32;
     int x_rows;                // rows of x
 } jib_mx4_desc;

@@ -46,39 +46,49 @@ __device__ __forceinline__ uint32_t to_e2m1(const float (&y)[8]) {
 // Scale 2^e with e = floor(log2 max) - 2, so that the largest value lies in [4, 8) and the largest code is 6; the exponent field of
 // the largest value is floor(log2) + 127, hence the byte e + 127 = field - 2, at least 0.  Dividing by 2^e is a product with
 // 2^-e, exact.  A block with an infinity or NaN gets the scale NaN (255) and codes 0.
+// A thread keeps its eight columns and walks down the rows (no division by the row's length), ROWS loads in flight.
+constexpr int ROWS = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_kernel(const T * __restrict__ x, long long ld, uint32_t * __restrict__ codes,
-                                                       uint8_t * __restrict__ scales, long long ld_s, long long n8, int per_row, int vec) {
+                                                       uint8_t * __restrict__ scales, long long ld_s, int rows, int per_row, int vec) {
     PDL_TRIGGER_TOP();
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
-    for (long long i0 = (long long) blockIdx.x * blockDim.x; i0 < n8; i0 += (long long) gridDim.x * blockDim.x) {
-        const long long i = i0 + threadIdx.x;
-        const long long row = i / per_row;
-        float y[8];
-        uint32_t top = 0;
-        if (i < n8) {
-            const T * p = x + row * ld + (i - row * per_row) * 8;
-            Vec8<T> in;
-            if (vec) in = *(const Vec8<T> *) p;
+    const int col = blockIdx.x * blockDim.x + threadIdx.x;
+#pragma unroll 1
+    for (long long r0 = (long long) blockIdx.y * ROWS; r0 < rows; r0 += (long long) gridDim.y * ROWS) {
+        Vec8<T> in[ROWS];
+#pragma unroll
+        for (int h = 0; h < ROWS; ++h) {
+            const T * p = x + (r0 + h) * ld + (long long) col * 8;
+            if (r0 + h >= rows || col >= per_row)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) from_f(0.f, in[h].v[j]);
+            else if (vec) in[h] = *(const Vec8<T> *) p;
             else
 #pragma unroll
-                for (int j = 0; j < 8; ++j) in.v[j] = p[j];
+                for (int j = 0; j < 8; ++j) in[h].v[j] = p[j];
+        }
+#pragma unroll
+        for (int h = 0; h < ROWS; ++h) {
+            float y[8];
+            uint32_t top = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                y[j] = to_f(in.v[j]);
+                y[j] = to_f(in[h].v[j]);
                 top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
             }
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (i >= n8) continue;
-        const int field = (int) (top >> 23);
-        const int byte = field == 255 ? 255 : max(field - 2, 0);
-        const float inv = __uint_as_float((uint32_t) (254 - byte) << 23);          // 2^(127 - byte)
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (r0 + h >= rows || col >= per_row) continue;
+            const int field = (int) (top >> 23);
+            const int byte = field == 255 ? 255 : max(field - 2, 0);
+            const float inv = __uint_as_float((uint32_t) (254 - byte) << 23);          // 2^(127 - byte)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] *= inv;
-        codes[i] = byte == 255 ? 0u : to_e2m1(y);
-        if ((i & 3) == 0) scales[row * ld_s + ((i - row * per_row) >> 2)] = (uint8_t) byte;
+            for (int j = 0; j < 8; ++j) y[j] *= inv;
+            codes[(r0 + h) * per_row + col] = byte == 255 ? 0u : to_e2m1(y);
+            if ((col & 3) == 0) scales[(r0 + h) * ld_s + (col >> 2)] = (uint8_t) byte;
+        }
     }
 }
 
@@ -90,21 +100,35 @@ __device__ __forceinline__ float code_value(uint32_t c) {
 
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t * __restrict__ codes, const uint8_t * __restrict__ scales, long long ld_s,
-                                                         T * __restrict__ out, long long n8, int per_row) {
+                                                         T * __restrict__ out, long long rows, int per_row) {
     PDL_TRIGGER_TOP();
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
-    for (long long i = (long long) blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += (long long) gridDim.x * blockDim.x) {
-        const long long row = i / per_row;
-        const uint32_t w = codes[i], s = scales[row * ld_s + ((i - row * per_row) >> 2)];
-        Vec8<T> o;
+    const int col = blockIdx.x * blockDim.x + threadIdx.x;
+    if (col >= per_row) return;
+#pragma unroll 1
+    for (long long r0 = (long long) blockIdx.y * ROWS; r0 < rows; r0 += (long long) gridDim.y * ROWS) {
+        uint32_t w[ROWS], s[ROWS];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            // 2^(s - 127) in two steps: s = 0 is below the normal numbers
-            const float v = s == 255 ? __uint_as_float(0x7fffffffu)
-                                     : code_value(w >> (4 * j)) * __uint_as_float((s > 0 ? s : 1u) << 23) * (s > 0 ? 1.f : 0.5f);
-            from_f(v, o.v[j]);
+        for (int h = 0; h < ROWS; ++h) {
+            w[h] = r0 + h < rows ? codes[(r0 + h) * per_row + col] : 0u;
+            s[h] = r0 + h < rows ? scales[(r0 + h) * ld_s + (col >> 2)] : 0u;
         }
-        *(Vec8<T> *) (out + i * 8) = o;
+#pragma unroll
+        for (int h = 0; h < ROWS; ++h) {
+            if (r0 + h >= rows) break;
+            // 2^(s - 127), of s = 0 below the normal numbers
+            const float unit = __uint_as_float(s[h] == 255 ? 0x7fffffffu : s[h] == 0 ? 0x00400000u : s[h] << 23);
+            Vec8<T> o;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                uint32_t two;
+                asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(two) : "r"(w[h] >> (4 * j)));
+                const float2 f = __half22float2(*(const __half2 *) &two);
+                from_f(f.x * unit, o.v[j]);
+                from_f(f.y * unit, o.v[j + 1]);
+            }
+            *(Vec8<T> *) (out + ((r0 + h) * per_row + col) * 8) = o;
+        }
     }
 }
 
@@ -224,12 +248,13 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
 
 int launched() { return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH; }
 
-// CTAs of `per` items each, at most a few waves (the kernels stride on).
-unsigned grid_for(long long items, int per) {
-    const long long n = (items + per - 1) / per;
+// Threads of a CTA and a grid for `per_row` threads a row and ROWS rows a step: x along a row, y down the rows, a few waves at most (the kernels stride on).
+dim3 grid_for(long long rows, int per_row, int * threads) {
+    const int nx = (per_row + 255) / 256;
+    *threads = ((per_row + nx - 1) / nx + 31) / 32 * 32;
     const int sms = jib::sm_count();
-    const long long most = (long long) (sms > 0 ? sms : 148) * 32;
-    return (unsigned) (n < most ? n : most);
+    const long long most = ((long long) (sms > 0 ? sms : 148) * 4096 / *threads + nx - 1) / nx, ny = (rows + ROWS - 1) / ROWS;
+    return dim3((unsigned) nx, (unsigned) (ny < most ? ny : most < 65535 ? most : 65535));
 }
 
 }  // namespace
@@ -240,14 +265,13 @@ extern "C" {
 JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * codes, void * scales, long long ld_s, int rows, int cols, void * stream) {
     if (rows <= 0) return 0;
     if (cols <= 0 || cols % 32 || ld_s < cols / 32 || type < 0 || type > 2) return JIB_E_ARG;
-    const int el = type == 2 ? 4 : 2, per_row = cols / 8;
-    const long long n8 = (long long) rows * per_row;
-    const int vec = ((uintptr_t) x | (uintptr_t) (ld * el)) % (size_t) 16 == 0;
-    const unsigned grid = grid_for(n8, 256);
+    const int el = type == 2 ? 4 : 2, per_row = cols / 8, vec = ((uintptr_t) x | (uintptr_t) (ld * el)) % (size_t) 16 == 0;
+    int th;
+    const dim3 grid = grid_for(rows, per_row, &th);
     cudaStream_t s = (cudaStream_t) stream;
-    if (type == 0) JIB_LAUNCH((quantize_kernel<bf16>), grid, 256, 0, s, (const bf16 *) x, ld, (uint32_t *) codes, (uint8_t *) scales, ld_s, n8, per_row, vec);
-    if (type == 1) JIB_LAUNCH((quantize_kernel<__half>), grid, 256, 0, s, (const __half *) x, ld, (uint32_t *) codes, (uint8_t *) scales, ld_s, n8, per_row, vec);
-    if (type == 2) JIB_LAUNCH((quantize_kernel<float>), grid, 256, 0, s, (const float *) x, ld, (uint32_t *) codes, (uint8_t *) scales, ld_s, n8, per_row, vec);
+    if (type == 0) JIB_LAUNCH((quantize_kernel<bf16>), grid, th, 0, s, (const bf16 *) x, ld, (uint32_t *) codes, (uint8_t *) scales, ld_s, rows, per_row, vec);
+    if (type == 1) JIB_LAUNCH((quantize_kernel<__half>), grid, th, 0, s, (const __half *) x, ld, (uint32_t *) codes, (uint8_t *) scales, ld_s, rows, per_row, vec);
+    if (type == 2) JIB_LAUNCH((quantize_kernel<float>), grid, th, 0, s, (const float *) x, ld, (uint32_t *) codes, (uint8_t *) scales, ld_s, rows, per_row, vec);
     return launched();
 }
 
@@ -255,12 +279,12 @@ JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * c
 JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long long ld_s, void * out, int type, long long rows, int cols, void * stream) {
     if (rows <= 0) return 0;
     if (cols <= 0 || cols % 32 || ld_s < cols / 32 || type < 0 || type > 2) return JIB_E_ARG;
-    const long long n8 = rows * (cols / 8);
-    const unsigned grid = grid_for(n8, 256);
+    int th;
+    const dim3 grid = grid_for(rows, cols / 8, &th);
     cudaStream_t s = (cudaStream_t) stream;
-    if (type == 0) JIB_LAUNCH((dequantize_kernel<bf16>), grid, 256, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, ld_s, (bf16 *) out, n8, cols / 8);
-    if (type == 1) JIB_LAUNCH((dequantize_kernel<__half>), grid, 256, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, ld_s, (__half *) out, n8, cols / 8);
-    if (type == 2) JIB_LAUNCH((dequantize_kernel<float>), grid, 256, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, ld_s, (float *) out, n8, cols / 8);
+    if (type == 0) JIB_LAUNCH((dequantize_kernel<bf16>), grid, th, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, ld_s, (bf16 *) out, rows, cols / 8);
+    if (type == 1) JIB_LAUNCH((dequantize_kernel<__half>), grid, th, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, ld_s, (__half *) out, rows, cols / 8);
+    if (type == 2) JIB_LAUNCH((dequantize_kernel<float>), grid, th, 0, s, (const uint32_t *) codes, (const uint8_t *) scales, ld_s, (float *) out, rows, cols / 8);
     return launched();
 }
 

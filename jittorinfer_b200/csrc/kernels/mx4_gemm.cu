@@ -5,7 +5,8 @@
 // tcgen05.mma.kind::mxf8f6f4 takes them as E2M1 with their block's scale, 128 rows a tile.  So no instruction touches a weight.  Its other operand can have 8
 // bits at most; a bf16 activation is the sum of two E4M3 numbers, the first its value rounded to four significant bits, the second what is left, each
 // with a scale for 32 columns.  That sum is the bf16 value down to 2^-11 of the block's largest magnitude and within 2^-21 of the largest below.  Two
-// instructions multiply both planes into one accumulator; at twice the rate of bf16 that costs what a bf16 product costs.
+// instructions multiply both planes into one accumulator; at twice the rate of bf16 that costs what a bf16 product costs.  Up to 96 rows of x both planes are one
+// operand of twice the rows, and the sums of the two meet in the epilogue: the weights' tile, the larger operand then, is read once.
 //
 // A stage is a chunk of 128 columns (two for up to 64 rows of x: the issuing thread's waits cost as much as the products of a small chunk): codes (16 KB
 // in shared memory, 8 KB from memory) and both planes of up to 192 rows of x.  Scales have a longer ring of their own:
@@ -13,6 +14,7 @@
 // while the stage they belong to is still on its way.  With few tiles K is split among CTAs; their sums meet in memory, and the one that comes last
 // adds them up in the order of K.
 #include <cuda_fp8.h>
+#include <math.h>
 
 #include "jib_kernels.h"
 #include "mx4_stream.cuh"
@@ -34,7 +36,7 @@ __host__ __device__ inline long long scale_rows_of(long long rows) { return (row
 
 __host__ __device__ inline int stage_bytes(int bn) { return A_BYTES + 2 * bn * 128; }
 __host__ __device__ inline int slot_bytes(int bn) { return SA_BYTES + 2 * bn * 4; }              // scales of a stage
-__host__ __device__ inline int scale_cols(int bn) { return (bn + 127) / 128 * 4; }          // of one plane
+__host__ __device__ inline int scale_cols(int n) { return (n + 127) / 128 * 4; }          // of n rows
 
 struct Args {
     const uint8_t * w_scales;                // [matrix][chunk][R][4]
@@ -47,7 +49,7 @@ struct Args {
     int * counters;                          // zeros, one a tile
     int * status;
     long long ldo, ldr, x_rows;
-    int T, N, R, C, E, bn, m_tiles, t_tiles, splits, stages, slots, cps, gated, act, out_f32, res_f32;
+    int T, N, R, C, E, bn, m_tiles, t_tiles, splits, stages, slots, cps, wide, gated, act, out_f32, res_f32;
 };
 
 __device__ __forceinline__ void st_cols4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -75,12 +77,26 @@ struct Ring {
     }
 };
 
+// Sixteen columns of sums; with the planes side by side the other plane's stand `other` columns on.
+__device__ __forceinline__ void sums16(uint32_t at, int other, uint32_t (&v)[16]) {
+    tmem_ld16(at, v);
+    if (other != 0) {
+        uint32_t u[16];
+        tmem_ld16(at + other, u);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) + __uint_as_float(u[k]));
+    } else {
+        tmem_ld_wait();
+    }
+}
+
 // What item i is: row tile m, first row of x, how many, chunks c0 .. c1 - 1, matrix, tile (for sums that meet).
 struct Item {
     int m, row0, rows, c0, c1, e, tile, split;
 };
 
-__device__ __forceinline__ Item item_of(const Args & g, const int * first_tile, int i) {
+__device__ __forceinline__ Item item_of(const Args & g, const int * first_tile, const int2 * experts, int i) {
     Item t;
     t.m = i % g.m_tiles;
     int rest = i / g.m_tiles;
@@ -98,8 +114,8 @@ __device__ __forceinline__ Item item_of(const Args & g, const int * first_tile, 
         }
         t.e = lo;
         const int at = (rest - first_tile[lo]) * g.bn;
-        t.row0 = g.seg[lo] + at;
-        t.rows = min(g.bn, g.count[lo] - at);
+        t.row0 = experts[lo].x + at;
+        t.rows = min(g.bn, experts[lo].y - at);
     } else {
         const int tt = rest % g.t_tiles;
         t.split = rest / g.t_tiles;
@@ -113,9 +129,17 @@ __device__ __forceinline__ Item item_of(const Args & g, const int * first_tile, 
     return t;
 }
 
+// How many chunks item i has.
+__device__ __forceinline__ int chunks_of(const Args & g, int i) {
+    if (g.splits == 1) return g.C;
+    const int split = i / (g.m_tiles * g.t_tiles);
+    return (split + 1) * g.C / g.splits - split * g.C / g.splits;
+}
+
 __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Args g) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ int first_tile[MAX_E + 1], last_s;
+    __shared__ int2 experts[MAX_E];            // first row, rows
     __shared__ uint64_t bars[2 * MAX_STAGES + 3 * MAX_SLOTS + 4];
     __shared__ uint32_t tmem_slot;
     uint8_t * tiles = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
@@ -123,7 +147,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
              * acc_full = sf_empty + MAX_SLOTS, * acc_empty = acc_full + 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = g.stages, Q = g.slots, bn = g.bn, cps = g.cps;
     uint8_t * scale_slots = tiles + S * cps * stage_bytes(bn);
-    const int SB = stage_bytes(bn), QB = slot_bytes(bn), plane = bn * 128, sfc = scale_cols(bn), slab = 4 + 2 * sfc;
+    const int SB = stage_bytes(bn), QB = slot_bytes(bn), plane = bn * 128, mn = g.wide ? 2 * bn : bn, sfc = scale_cols(mn), slab = 4 + (g.wide ? sfc : 2 * sfc);
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < Q; ++i) { mbar_init(&sl_full[i], 1); mbar_init(&sf_full[i], 4); mbar_init(&sf_empty[i], 1); }
@@ -148,7 +172,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             int sum = 0;
 #pragma unroll 1
             for (int e0 = 0; e0 < g.E; e0 += 32) {
-                const int mine = e0 + lane < g.E ? (g.count[e0 + lane] + bn - 1) / bn : 0;
+                const int have = e0 + lane < g.E ? g.count[e0 + lane] : 0, mine = (have + bn - 1) / bn;
+                if (e0 + lane < g.E) experts[e0 + lane] = make_int2(g.seg[e0 + lane], have);
                 int s = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o *= 2) {
@@ -163,7 +188,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         __syncthreads();
         items = first_tile[g.E] * g.m_tiles;
     }
-    const uint32_t sf0 = tmem + 2 * bn;
+    const uint32_t sf0 = tmem + 2 * mn;
 
     if (warp == 0) {
         if (elect_one()) {
@@ -171,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             bool ok = true;
 #pragma unroll 1
             for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
-                const Item t = item_of(g, first_tile, i);
+                const Item t = item_of(g, first_tile, experts, i);
 #pragma unroll 1
                 for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(S)) {
                     const int s = r.at, n = min(cps, t.c1 - c0);
@@ -197,7 +222,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             bool ok = true;
 #pragma unroll 1
             for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
-                const Item t = item_of(g, first_tile, i);
+                const Item t = item_of(g, first_tile, experts, i);
                 const int w_rows = min(BM, g.R - t.m * BM);
 #pragma unroll 1
                 for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(Q)) {
@@ -223,18 +248,18 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             int j = 0;
             bool ok = true;
             const uint64_t desc0 = desc_k_sw128(smem_u32(tiles));
-            const uint32_t id0 = idesc_e2m1_e4m3(bn, 0), lo = (uint32_t) plane >> 4;
+            const uint32_t id0 = idesc_e2m1_e4m3(mn, 0), lo = (uint32_t) plane >> 4;
 #pragma unroll 1
             for (int i = blockIdx.x; i < items && ok; i += gridDim.x, ++j) {
-                const Item t = item_of(g, first_tile, i);
+                const int n = chunks_of(g, i);
                 const int buf = j & 1;
                 if (!mbar_wait(&acc_empty[buf], (j >> 1 & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 62, i); break; }
                 tc_fence_after();
-                const uint32_t acc = tmem + buf * bn;
+                const uint32_t acc = tmem + buf * mn;
                 bool more = false;
 #pragma unroll 1
-                for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(S), rq.next(Q)) {
-                    if (!mbar_wait(&sf_full[rq.at], rq.round) || !mbar_wait(&full[r.at], r.round)) {
+                for (int c0 = 0; c0 < n; c0 += cps, r.next(S), rq.next(Q)) {
+                    if (!mbar_wait(&sf_full[rq.at], rq.round)) {      // the stage's tiles are there too
                         jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 63, i);
                         ok = false;
                         break;
@@ -242,14 +267,19 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     tc_fence_after();
                     // descriptors count in 16 bytes, a step of 32 columns is two of them; the scales' byte is in bits 4 and 29 of the other
 #pragma unroll 1
-                    for (int j = 0; j < min(cps, t.c1 - c0); ++j) {
+                    for (int j = 0; j < min(cps, n - c0); ++j) {
                         const uint64_t a = desc0 + (uint32_t) ((r.at * cps + j) * SB >> 4), b = a + (A_BYTES >> 4);
                         const uint32_t sf = sf0 + (rq.at * cps + j) * slab;
+                        if (g.wide) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t id = id0 + (k << 4) + ((uint32_t) k << 29);
-                            mma_mxf8f6f4(acc, a + 2 * k, b + 2 * k, id, sf, sf + 4, more || k != 0);
-                            mma_mxf8f6f4(acc, a + 2 * k, b + lo + 2 * k, id, sf, sf + 4 + sfc, true);
+                            for (int k = 0; k < 4; ++k) mma_mxf8f6f4(acc, a + 2 * k, b + 2 * k, id0 + (k << 4) + ((uint32_t) k << 29), sf, sf + 4, more || k != 0);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t id = id0 + (k << 4) + ((uint32_t) k << 29);
+                                mma_mxf8f6f4(acc, a + 2 * k, b + 2 * k, id, sf, sf + 4, more || k != 0);
+                                mma_mxf8f6f4(acc, a + 2 * k, b + lo + 2 * k, id, sf, sf + 4 + sfc, true);
+                            }
                         }
                         more = true;
                     }
@@ -261,36 +291,38 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         }
         __syncwarp();
     } else if (warp >= 4 && warp < 8) {
-        // scales to tensor memory
+        // scales to tensor memory; these warps also wait for the stage's tiles, so that the issuing thread waits once a stage
         const uint32_t mine = sf0 + ((uint32_t) (warp & 3) << 21);
-        Ring r;
+        Ring r, rs;
         bool ok = true;
 #pragma unroll 1
         for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
-            const Item t = item_of(g, first_tile, i);
+            const int n = chunks_of(g, i);
 #pragma unroll 1
-            for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(Q)) {
+            for (int c0 = 0; c0 < n; c0 += cps, r.next(Q), rs.next(S)) {
                 const int q = r.at;
                 ok = __all_sync(0xffffffffu, mbar_wait(&sl_full[q], r.round));
                 if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 64, i); break; }
                 tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < min(cps, t.c1 - c0); ++c) {
+                for (int c = 0; c < min(cps, n - c0); ++c) {
                     const uint32_t * sc = (const uint32_t *) (scale_slots + (q * cps + c) * QB) + lane;
                     const uint32_t dst = mine + (q * cps + c) * slab;
                     st_cols4(dst, sc[0], sc[32], sc[64], sc[96]);
 #pragma unroll 1
-                    for (int p = 0; p < 2; ++p) {
+                    for (int p = 0; p < 2 - g.wide; ++p) {
                         const uint32_t * sx = sc + SA_BYTES / 4 + p * bn;
                         for (int j = 0; j < sfc; j += 4) {
                             uint32_t v[4];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) v[k] = (j + k) * 32 + lane < bn ? sx[(j + k) * 32] : 0u;
+                            for (int k = 0; k < 4; ++k) v[k] = (j + k) * 32 + lane < mn ? sx[(j + k) * 32] : 0u;
                             st_cols4(dst + 4 + p * sfc + j, v[0], v[1], v[2], v[3]);
                         }
                     }
                 }
                 tmem_st_wait();
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[rs.at], rs.round));
+                if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 67, i); break; }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sf_full[q]);
@@ -303,11 +335,11 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         int j = 0;
 #pragma unroll 1
         for (int i = blockIdx.x; i < items; i += gridDim.x, ++j) {
-            const Item t = item_of(g, first_tile, i);
+            const Item t = item_of(g, first_tile, experts, i);
             const int buf = j & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], j >> 1 & 1))) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 65, i); break; }
             tc_fence_after();
-            const uint32_t acc = mine + buf * bn;
+            const uint32_t acc = mine + buf * mn;
             bool finish = true;
             float * part = g.part + ((size_t) t.tile * g.splits * bn) * BM + q * 32 + lane;
             if (g.splits > 1) {
@@ -315,8 +347,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 #pragma unroll 1
                 for (int c = 16 * half; c < t.rows; c += 32) {
                     uint32_t v[16];
-                    tmem_ld16(acc + c, v);
-                    tmem_ld_wait();
+                    sums16(acc + c, g.wide ? bn : 0, v);
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
                         if (c + k < t.rows) __stcg(to + (size_t) (c + k) * BM, __uint_as_float(v[k]));
@@ -354,8 +385,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     }
                 } else {
                     uint32_t v[16];
-                    tmem_ld16(acc + c, v);
-                    tmem_ld_wait();
+                    sums16(acc + c, g.wide ? bn : 0, v);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) y[k] = __uint_as_float(v[k]);
                 }
@@ -414,57 +444,61 @@ __device__ __forceinline__ float e4m3_value(uint32_t w, int i) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t) (w >> (8 * i) & 0xff), __NV_E4M3)));
 }
 
+constexpr int ROWS = 2;                             // of a thread's columns, their loads in flight together
+
 __global__ void __launch_bounds__(256) planes_kernel(const bf16 * __restrict__ x, long long ldx, const int * __restrict__ src, const int * __restrict__ limit,
                                                      uint8_t * __restrict__ planes, uint8_t * __restrict__ scales, long long rows, long long scale_rows, int K, int C,
                                                      int * __restrict__ zeros, int n_zeros) {
     PDL_TRIGGER_TOP();
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
-    const int per_row = C * 16;
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n_zeros; i += gridDim.x * blockDim.x) zeros[i] = 0;
-    const long long most = limit != nullptr ? min(rows, (long long) *limit) : rows, n = most * per_row;
-    for (long long i0 = (long long) blockIdx.x * blockDim.x; i0 < n; i0 += (long long) gridDim.x * blockDim.x) {
-        const long long i = i0 + threadIdx.x;
-        const long long r = i < n ? i / per_row : most - 1;
-        const int k = (int) (i - r * per_row) * 8;
-        const long long from = src != nullptr ? src[r] : r;
-        float y[8] = {};
-        uint32_t top = 0;
-        if (i < n && k < K && from >= 0) {
-            const uint4 in = *(const uint4 *) (x + from * ldx + k);
-            const uint32_t w[4] = {in.x, in.y, in.z, in.w};
+    const int id = (blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x, k = (blockIdx.x * blockDim.x + threadIdx.x) * 8;
+    for (int i = id; i < n_zeros; i += gridDim.x * gridDim.y * blockDim.x) zeros[i] = 0;
+    const long long most = limit != nullptr ? min(rows, (long long) *limit) : rows;
+#pragma unroll 1
+    for (long long r0 = (long long) blockIdx.y * ROWS; r0 < most; r0 += (long long) gridDim.y * ROWS) {
+        uint4 in[ROWS];
+#pragma unroll
+        for (int h = 0; h < ROWS; ++h) {
+            const long long from = r0 + h >= most ? -1 : src != nullptr ? src[r0 + h] : r0 + h;
+            in[h] = from >= 0 && k < K ? *(const uint4 *) (x + from * ldx + k) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int h = 0; h < ROWS; ++h) {
+            const uint32_t w[4] = {in[h].x, in[h].y, in[h].z, in[h].w};
+            float z[8];
+            uint32_t top = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float2 f = __bfloat1622float2(*(const __nv_bfloat162 *) &w[j]);
-                y[2 * j] = f.x;
-                y[2 * j + 1] = f.y;
+                z[2 * j] = f.x;
+                z[2 * j + 1] = f.y;
                 top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
             }
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (i >= n) continue;
-        const int field = (int) (top >> 23), byte = field == 255 ? 255 : max(field - 7, 4);          // e + 127
-        const float unit = field == 255 ? 0.f : __uint_as_float((uint32_t) (254 - byte) << 23);
-        float z[8];
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (r0 + h >= most || k >= C * 128) continue;
+            const int field = (int) (top >> 23), byte = field == 255 ? 255 : max(field - 7, 4);          // e + 127
+            const float unit = field == 255 ? 0.f : __uint_as_float((uint32_t) (254 - byte) << 23);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = field == 255 ? 0.f : y[j] * unit;
-        uint2 hi, lo;
-        hi.x = e4m3x4(z[0], z[1], z[2], z[3]);
-        hi.y = e4m3x4(z[4], z[5], z[6], z[7]);
+            for (int j = 0; j < 8; ++j) z[j] = field == 255 ? 0.f : z[j] * unit;
+            uint2 hi, lo;
+            hi.x = e4m3x4(z[0], z[1], z[2], z[3]);
+            hi.y = e4m3x4(z[4], z[5], z[6], z[7]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            z[j] = (z[j] - e4m3_value(hi.x, j)) * 16.f;
-            z[4 + j] = (z[4 + j] - e4m3_value(hi.y, j)) * 16.f;
-        }
-        lo.x = e4m3x4(z[0], z[1], z[2], z[3]);
-        lo.y = e4m3x4(z[4], z[5], z[6], z[7]);
-        uint8_t * to = planes + r * (long long) (C * 128) + k;
-        *(uint2 *) to = hi;
-        *(uint2 *) (to + rows * (long long) (C * 128)) = lo;
-        if ((i & 3) == 0) {
-            uint8_t * sc = scales + ((long long) (k >> 7) * scale_rows + r) * 4 + (k >> 5 & 3);
-            sc[0] = (uint8_t) byte;
-            sc[(long long) C * scale_rows * 4] = (uint8_t) (byte == 255 ? 255 : byte - 4);
+            for (int j = 0; j < 4; ++j) {
+                z[j] = (z[j] - e4m3_value(hi.x, j)) * 16.f;
+                z[4 + j] = (z[4 + j] - e4m3_value(hi.y, j)) * 16.f;
+            }
+            lo.x = e4m3x4(z[0], z[1], z[2], z[3]);
+            lo.y = e4m3x4(z[4], z[5], z[6], z[7]);
+            uint8_t * to = planes + (r0 + h) * (long long) (C * 128) + k;
+            *(uint2 *) to = hi;
+            *(uint2 *) (to + rows * (long long) (C * 128)) = lo;
+            if ((k >> 3 & 3) == 0) {
+                uint8_t * sc = scales + ((long long) (k >> 7) * scale_rows + r0 + h) * 4 + (k >> 5 & 3);
+                sc[0] = (uint8_t) byte;
+                sc[(long long) C * scale_rows * 4] = (uint8_t) (byte == 255 ? 255 : byte - 4);
+            }
         }
     }
 }
@@ -556,13 +590,17 @@ int planes_map(CUtensorMap * out, const void * planes, long long rows, long long
                : JIB_E_TENSORMAP;
 }
 
-// Rows of x in a tile and splits of K of a dense product.  A tile's fixed part is worth some 24 rows; the rounds over the machine count.  Where the tiles leave SMs
-// idle, K is split, four chunks a split at least.
+// Up to this many rows of x the planes are one operand (two buffers of sums and the scales fit in tensor memory).
+constexpr int MAX_WIDE = 96;
+
+// Rows of x in a tile and splits of K of a dense product.  What a chunk costs is its traffic with shared memory: 128 bytes written a row of either operand and
+// plane, and as many read by each instruction: in rows of x (512 bytes) w, and for the weights' tile 64, 96 where it is read for each plane.  1531 rows to
+// 2 x 10944, K 2048: 137 us with 192 rows, 139 us with 128.  Where the tiles leave SMs idle, K is split, four chunks a split at least.
 void shape_of(long long T, int m_tiles, int C, int * bn, int * splits) {
     const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
     long long best = -1;
     for (int w = T > 16 ? 32 : 16; w <= MAX_BN; w += 32) {
-        const long long tiles = (long long) m_tiles * ((T + w - 1) / w), cost = (tiles + sms - 1) / sms * (w + 24);
+        const long long tiles = (long long) m_tiles * ((T + w - 1) / w), cost = (tiles + sms - 1) / sms * (w + (w <= MAX_WIDE ? 64 : 96));
         if (best < 0 || cost <= best) { best = cost; *bn = w; }
         if (w >= T) break;
         if (w == 16) w = 0;
@@ -602,8 +640,9 @@ JIB_EXPORT int jib_mx4_planes(const void * x, long long ldx, const int * src, co
     if (K <= 0 || K % 32 || n_zeros < 0) return JIB_E_ARG;
     if (((uintptr_t) x | (uintptr_t) (ldx * 2) | (uintptr_t) planes) & 15) return JIB_E_ALIGN;
     const int C = mx4::chunks(K);
-    const long long ctas = (rows * C * 16 + 255) / 256, most = 32ll * (jib::sm_count() > 0 ? jib::sm_count() : 148);
-    JIB_LAUNCH((planes_kernel), (unsigned) (ctas < most ? ctas : most), 256, 0, (cudaStream_t) stream, (const bf16 *) x, ldx, src, limit, (uint8_t *) planes,
+    const int nx = (C * 16 + 255) / 256, th = ((C * 16 + nx - 1) / nx + 31) / 32 * 32, sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
+    const long long ny = (rows + ROWS - 1) / ROWS, most = ((long long) sms * 4096 / th + nx - 1) / nx;
+    JIB_LAUNCH((planes_kernel), dim3(nx, (unsigned) (ny < most ? ny : most < 65535 ? most : 65535)), th, 0, (cudaStream_t) stream, (const bf16 *) x, ldx, src, limit, (uint8_t *) planes,
                (uint8_t *) scales, rows, scale_rows_of(rows), K, C, zeros, n_zeros);
     return launched();
 }
@@ -632,8 +671,9 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const
     g.m_tiles = (g.R + BM - 1) / BM;
     long long items;
     if (d->seg != nullptr) {
-        // an expert's rows on average, and a quarter more: most experts then take one tile
-        const int avg = (d->max_rows + d->batch - 1) / d->batch, w = (avg + avg / 4 + 31) / 32 * 32;
+        // an expert's rows on average and twice their spread: most experts then take one tile
+        const float avg = (float) d->max_rows / d->batch;
+        const int w = ((int) (avg + 2.f * sqrtf(avg)) + 31) / 32 * 32;
         g.bn = w < 32 ? 32 : w > MAX_BN ? MAX_BN : w;
         g.splits = 1;
         g.t_tiles = 1;
@@ -646,9 +686,10 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const
     }
     if (items > 0x3fffffff) return JIB_E_ARG;
     g.cps = g.bn <= 64 ? 2 : 1;
-    g.slots = (512 - 2 * g.bn) / (g.cps * (4 + 2 * scale_cols(g.bn)));
+    g.wide = g.bn <= MAX_WIDE;
+    g.slots = (512 - (g.wide ? 4 : 2) * g.bn) / (g.cps * (4 + (g.wide ? scale_cols(2 * g.bn) : 2 * scale_cols(g.bn))));
     if (g.slots > MAX_SLOTS) g.slots = MAX_SLOTS;
-    g.stages = (MOST_SMEM - 4096 - 1024 - g.slots * g.cps * slot_bytes(g.bn)) / (g.cps * stage_bytes(g.bn));        // (4 KB: barriers and tables)
+    g.stages = (MOST_SMEM - 5120 - 1024 - g.slots * g.cps * slot_bytes(g.bn)) / (g.cps * stage_bytes(g.bn));        // (5 KB: barriers and tables)
     if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
     CUtensorMap mw, mx;
     int rc = weights_map(&mw, d->w, g.R, (long long) g.C * d->batch);
@@ -656,7 +697,7 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const
     rc = planes_map(&mx, d->x, d->x_rows, (long long) g.C * 128, g.bn);
     if (rc) return rc;
     static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
-    if (!jib::ensure_dyn_smem(mx4_gemm_kernel, MOST_SMEM - 4096, attr_done)) return JIB_E_LAUNCH;
+    if (!jib::ensure_dyn_smem(mx4_gemm_kernel, MOST_SMEM - 5120, attr_done)) return JIB_E_LAUNCH;
     JIB_LAUNCH((mx4_gemm_kernel), (unsigned) (items < sms ? items : sms), THREADS, g.cps * (g.stages * stage_bytes(g.bn) + g.slots * slot_bytes(g.bn)) + 1024, (cudaStream_t) stream, mw, mx, g);
     return launched();
 }

@@ -185,7 +185,7 @@ def _few_layer(x, residual, wgu: Mx4Weight, wd: Mx4Weight, sizes, act: str, m, w
     return out
 
 
-def moe_ffn(x, residual, ids, wts, wgu, wd, act):
+def moe_ffn(x, residual, ids, wts, wgu, wd, act, n_shared=0):
     x = _rows(x)
     T, k = ids.shape
     if T == 0:
@@ -208,8 +208,9 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act):
             first = table.data_ptr()
             count, row_src, pair_row = first + 4 * (E + 1), first + 4 * (2 * E + 1), first + 4 * (2 * E + 1 + cap)
             nat._ck(nat.load().jib_mx4_pad(seg.data_ptr(), src.data_ptr(), dest.data_ptr(), E, n, cap, first, count, row_src, pair_row, nat._stream()), "mx4_pad")
-            h = _grouped(x, wgu, (first, count, cap), row_src, n, act)
-            y = _grouped(h, wd, (first, count, cap), None, n, None)
+            routed = T * (k - n_shared) * E // (E - n_shared)       # the rows were there no shared experts: what the tiles are chosen for
+            h = _grouped(x, wgu, (first, count, cap), row_src, routed, act)
+            y = _grouped(h, wd, (first, count, cap), None, routed, None)
             return nat.moe_combine(y, table[2 * E + 1 + cap:].view(T, k), wts, None, None if residual is None else residual.contiguous())
         h = _grouped_simt(x, wgu, seg, src, n, act)
         y = _grouped_simt(h, wd, seg, None, n, None)
@@ -236,4 +237,4 @@ def moe_layer(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, w
             m.norm, m.sigmoid, m.n_shared, m.group_top2 = int(norm), int(sigmoid), n_shared, int(group_top2)
             return _few_layer(x, residual, wgu, wd, sizes, act, m, w_router)
         ids, wts = nat.moe_gate(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, n_shared, group_top2)
-    return moe_ffn(x, residual, ids, wts, wgu, wd, act)
+    return moe_ffn(x, residual, ids, wts, wgu, wd, act, n_shared)

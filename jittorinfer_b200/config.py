@@ -73,6 +73,7 @@ class ServerConfig:
     device_sampling: bool = False      # sample on the device when a request needs only top-k / top-p / min-p / temperature
     run_ahead: bool = False            # greedy requests: launch decode step k+1 before the ids of step k reach the host
     enforce_response_format: bool = True   # chat response_format (json_object / json_schema) constrains sampling with a grammar
+    ffn_format: str = ""               # "mxfp4": feed-forward weights in 4 bits (one GPU, GGUF models); empty: as loaded
     random_init: str = ""              # preset name ("lite", "v2", "tiny"): serve random weights instead of a GGUF file
     ignored: Dict[str, Any] = field(default_factory=dict)
 
@@ -93,6 +94,10 @@ class ServerConfig:
             raise ValueError(f"split_mode must be one of {SPLIT_MODES}")
         if self.reasoning_format not in REASONING_FORMATS:
             raise ValueError(f"reasoning_format must be one of {REASONING_FORMATS}")
+        if self.ffn_format not in ("", "mxfp4"):
+            raise ValueError("ffn_format must be empty or mxfp4")
+        if self.ffn_format and self.world_size > 1:
+            raise ValueError("ffn_format runs on one GPU: tp_size and ep_size must be 1")
         if self.tp_size not in (1, 2, 4, 8) or self.ep_size not in (1, 2, 4, 8):
             raise ValueError("tp_size / ep_size must be 1, 2, 4 or 8")       # reference: llama-model.cpp:467-476
         if self.ep_size > 1 and self.tp_size > 1 and self.ep_size != self.tp_size:

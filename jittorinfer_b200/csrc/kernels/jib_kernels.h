@@ -342,7 +342,7 @@ typedef struct jib_mx4_desc {
     int gated, act, out_f32, res_f32;
     int x_rows;                // rows of x
 } jib_mx4_desc;
-JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, int f32, void * stream);
+JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, void * stream);
 // The same on the tensor cores, bf16 activations (mx4_gemm.cu): as planes first; grouped rows at padded places.
 JIB_EXPORT void jib_mx4_gemm_sizes(long long rows, int N, int K, int gated, int grouped, long long * sizes);
 JIB_EXPORT int jib_mx4_planes(const void * x, long long ldx, const int * src, const int * limit, void * planes, void * scales, long long rows, int K, int * zeros,

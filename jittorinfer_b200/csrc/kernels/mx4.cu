@@ -173,11 +173,11 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t * __restrict__ 
     factors[at] = (uint8_t) (f << 2);
 }
 
-// ---- the product on CUDA cores: fp32 activations, and every shape ------------------------------------------------------------------
+// ---- the product of fp32 activations, on CUDA cores ------------------------------------------------------------------
 // A warp holds 16 rows (of a pair: 16 of each matrix) for eight rows of x; a lane multiplies its columns of rows g and g + 8, four lanes share a row.
 constexpr int ST = 8;
 
-template <typename T, bool PAIR>
+template <bool PAIR>
 __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
     PDL_TRIGGER_TOP();
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
@@ -193,11 +193,11 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
     const long long t0 = (long long) blockIdx.y * ST;
     if (t0 >= rows) return;
     const int nt = (int) (rows - t0 < ST ? rows - t0 : ST);
-    const T * xr[ST];
+    const float * xr[ST];
 #pragma unroll
     for (int j = 0; j < ST; ++j) {
         const long long r = base + t0 + (j < nt ? j : 0);
-        xr[j] = (const T *) d.x + (d.src != nullptr ? (long long) d.src[r] : r) * d.ldx;
+        xr[j] = (const float *) d.x + (d.src != nullptr ? (long long) d.src[r] : r) * d.ldx;
     }
     float acc[M][2][ST] = {};
     for (int c = 0; c < C; ++c) {
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
                         const float w = code_value(word[i] >> (4 * j)) * unit;
 #pragma unroll
                         for (int n = 0; n < ST; ++n)
-                            if (n < nt) acc[m][h][n] += w * to_f(xr[n][k + 8 * i + j]);
+                            if (n < nt) acc[m][h][n] += w * xr[n][k + 8 * i + j];
                     }
             }
     }
@@ -305,20 +305,15 @@ JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long l
     return launched();
 }
 
-JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, int f32, void * stream) {
+JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, void * stream) {
     if (d->T <= 0) return 0;
     if (d->N <= 0 || d->K <= 0 || d->K % 32 || d->batch < 1 || d->batch > 65535) return JIB_E_ARG;
     const long long rows = d->seg != nullptr ? d->max_rows : d->T;
     const dim3 grid(((d->N + 15) / 16 + 3) / 4, (unsigned) ((rows + ST - 1) / ST), d->batch);
     if ((rows + ST - 1) / ST > 65535) return JIB_E_ARG;
     cudaStream_t s = (cudaStream_t) stream;
-    if (f32) {
-        if (d->gated) JIB_LAUNCH((product_kernel<float, true>), grid, 128, 0, s, *d);
-        else JIB_LAUNCH((product_kernel<float, false>), grid, 128, 0, s, *d);
-    } else {
-        if (d->gated) JIB_LAUNCH((product_kernel<bf16, true>), grid, 128, 0, s, *d);
-        else JIB_LAUNCH((product_kernel<bf16, false>), grid, 128, 0, s, *d);
-    }
+    if (d->gated) JIB_LAUNCH((product_kernel<true>), grid, 128, 0, s, *d);
+    else JIB_LAUNCH((product_kernel<false>), grid, 128, 0, s, *d);
     return launched();
 }
 

@@ -499,7 +499,8 @@ __global__ void __launch_bounds__(GATE_NT) mx4_prepare_kernel(const bf16 * __res
     __shared__ float red[GATE_NT / 32][GATE_TG];
     const bool router = (int) blockIdx.x < E;
     PDL_TRIGGER_TOP();
-    if (warm && router) router_rows(x, w_router, nullptr, 0.f, nullptr, logits, 0, min(T, GATE_TG), T, d, E, blockIdx.x, red, nullptr, true);
+    // the code and this expert's row come to the SM; x is not there yet, the router's first values stand in for it
+    if (warm && router) router_rows((const bf16 *) w_router, w_router, nullptr, 0.f, nullptr, logits, 0, 1, 1, d, E, blockIdx.x, red, nullptr, true);
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
     for (int i = blockIdx.x * GATE_NT + threadIdx.x; i < n_sync; i += gridDim.x * GATE_NT) sync[i] = 0;
     if (router) {

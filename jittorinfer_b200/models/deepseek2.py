@@ -83,7 +83,8 @@ def assign_layers(n_layer: int, devices, tensor_split=None):
 class _Layer:
     __slots__ = ("attn_norm", "w_qkv_a", "q_a_norm", "w_q_b", "kv_a_norm", "w_uk", "w_uv", "w_kv_b", "w_o", "ffn_norm",
                  "w_gate", "w_up", "w_down", "w_router", "router_bias", "w_gate_exps", "w_up_exps", "w_down_exps",
-                 "w_gate_sh", "w_up_sh", "w_down_sh", "is_moe", "n_shared_merged")
+                 "w_gate_sh", "w_up_sh", "w_down_sh", "is_moe", "n_shared_merged",
+                 "ffn_gu", "ffn_d", "shared_gu", "shared_d")       # ffn_format "mxfp4": the block, or its experts, and shared experts apart from them
 
     def __init__(self):
         for s in self.__slots__:
@@ -95,7 +96,8 @@ class DeepSeek2Model:
 
     def __init__(self, hp: DeepSeek2HParams, weights: Iterable[Tuple[str, torch.Tensor]],
                  dtype: torch.dtype = torch.bfloat16, device="cpu", spec: ShardSpec = ShardSpec(),
-                 comm=None, max_positions: int = 8192, block_size: int = 64, ep=None, layer_devices=None):
+                 comm=None, max_positions: int = 8192, block_size: int = 64, ep=None, layer_devices=None,
+                 ffn_format: Optional[str] = None):
         self.hp = hp
         self.dtype = dtype
         self.device = torch.device(device)
@@ -110,6 +112,13 @@ class DeepSeek2Model:
         self.split = any(d != self.device for d in self.layer_dev)
         if self.split and spec.sharded:
             raise ValueError("layer split and tensor / expert parallelism are separate modes")
+        # "mxfp4": the feed-forward weights (dense blocks, routed and shared experts) are quantised to 4 bits as they arrive and the blocks run on the 4-bit
+        # operators; router, attention, embeddings and output stay as they are
+        if ffn_format not in (None, "mxfp4"):
+            raise ValueError(f"ffn_format {ffn_format!r}: None or \"mxfp4\"")
+        if ffn_format is not None and (spec.sharded or self.split):
+            raise ValueError("ffn_format runs on one GPU: no tensor, expert or layer parallelism")
+        self.ffn_format = ffn_format
         self.out_device = self.layer_dev[-1]
         self._cur_dev = self.device
         self._uploaders = {}
@@ -165,6 +174,38 @@ class DeepSeek2Model:
             return up.upload(t, dtype or self.dtype)          # large tensors go through pinned staging buffers
         return t.to(device=self._cur_dev, dtype=dtype or self.dtype).contiguous()
 
+    def _ffn(self, t: torch.Tensor):
+        """A feed-forward weight in the model's format for them."""
+        if self.ffn_format is None:
+            return self._dev(t)
+        # from the values as they come: a rounding to the model's type in between would move some of them to a neighbouring code
+        return ops.mx4_quantize(self._dev(t, t.dtype if t.dtype in (torch.bfloat16, torch.float16, torch.float32) else torch.float32))
+
+    def _lay_out_ffn(self, L: _Layer) -> None:
+        """The 4-bit weights of a layer in the order of the products; shared experts become experts behind the routed ones where they fit."""
+        if not L.is_moe:
+            L.ffn_gu, L.ffn_d = ops.mx4_weight(L.w_gate, L.w_up), ops.mx4_weight(L.w_down)
+            L.w_gate = L.w_up = L.w_down = None
+            return
+        gate, up, down = L.w_gate_exps, L.w_up_exps, L.w_down_exps
+        L.n_shared_merged = 0
+        if L.w_gate_sh is not None:
+            E, F, d = gate.shape
+            ns = L.w_gate_sh.shape[0] // F
+            if L.w_gate_sh.shape[0] == ns * F and E + ns <= ops.MX4_MAX_EXPERTS:
+                def rows(q, s):
+                    return ops.Mx4Tensor(*(torch.cat([a, b.reshape(ns, F, -1)]) for a, b in ((q.codes, s.codes), (q.scales, s.scales))))
+
+                def columns(q, s):
+                    return ops.Mx4Tensor(*(torch.cat([a, b.reshape(d, ns, -1).transpose(0, 1)]) for a, b in ((q.codes, s.codes), (q.scales, s.scales))))
+
+                gate, up, down = rows(gate, L.w_gate_sh), rows(up, L.w_up_sh), columns(down, L.w_down_sh)
+                L.n_shared_merged = ns
+            else:
+                L.shared_gu, L.shared_d = ops.mx4_weight(L.w_gate_sh, L.w_up_sh), ops.mx4_weight(L.w_down_sh)
+        L.ffn_gu, L.ffn_d = ops.mx4_weight(gate, up), ops.mx4_weight(down)
+        L.w_gate_exps = L.w_up_exps = L.w_down_exps = L.w_gate_sh = L.w_up_sh = L.w_down_sh = None
+
     def _load(self, weights: Iterable[Tuple[str, torch.Tensor]]):
         hp = self.hp
         H, dn, dv, r = self.n_head_local, hp.qk_nope_head_dim, hp.v_head_dim, hp.kv_lora_rank
@@ -211,28 +252,28 @@ class DeepSeek2Model:
                 elif base == "attn_output":
                     L.w_o = self._dev(t)
                 elif base == "ffn_gate":
-                    L.w_gate = self._dev(t)
+                    L.w_gate = self._ffn(t)
                 elif base == "ffn_up":
-                    L.w_up = self._dev(t)
+                    L.w_up = self._ffn(t)
                 elif base == "ffn_down":
-                    L.w_down = self._dev(t)
+                    L.w_down = self._ffn(t)
                 elif base == "ffn_gate_inp":
                     L.w_router = self._dev(t, torch.float32)
                     L.is_moe = True
                 elif base == "exp_probs_b":
                     L.router_bias = self._dev(t, torch.float32)
                 elif base == "ffn_gate_exps":
-                    L.w_gate_exps = self._dev(t)
+                    L.w_gate_exps = self._ffn(t)
                 elif base == "ffn_up_exps":
-                    L.w_up_exps = self._dev(t)
+                    L.w_up_exps = self._ffn(t)
                 elif base == "ffn_down_exps":
-                    L.w_down_exps = self._dev(t)
+                    L.w_down_exps = self._ffn(t)
                 elif base == "ffn_gate_shexp":
-                    L.w_gate_sh = self._dev(t)
+                    L.w_gate_sh = self._ffn(t)
                 elif base == "ffn_up_shexp":
-                    L.w_up_sh = self._dev(t)
+                    L.w_up_sh = self._ffn(t)
                 elif base == "ffn_down_shexp":
-                    L.w_down_sh = self._dev(t)
+                    L.w_down_sh = self._ffn(t)
                 else:
                     raise KeyError(f"unknown tensor {name}")
             else:
@@ -241,7 +282,7 @@ class DeepSeek2Model:
         self._uploaders.clear()               # release the pinned staging buffers
         if self.w_out is None:
             self.w_out = self.tok_embd if self.out_device == self.device else self.tok_embd.to(self.out_device)
-        if not self.spec.sharded or not (self.spec.expert_parallel or self.spec.dp_attention):
+        if self.ffn_format is None and (not self.spec.sharded or not (self.spec.expert_parallel or self.spec.dp_attention)):
             # single GPU, or every expert's FFN columns sharded over the ranks: the (local part of the) shared experts has
             # the (local) routed experts' shape, so it becomes experts E, E+1, ... of the grouped GEMMs (two fewer launches
             # per layer, better fill); the router appends them to every token.  Any split of the shared FFN's hidden units
@@ -262,6 +303,8 @@ class DeepSeek2Model:
             missing = [n for n in need if getattr(L, n) is None]
             if missing:
                 raise ValueError(f"layer {il}: missing tensors {missing}")
+            if self.ffn_format is not None:
+                self._lay_out_ffn(L)
 
     def cache_bytes_per_token(self) -> int:
         return self.hp.n_layer * self.hp.kv_row * torch.empty(0, dtype=self.dtype).element_size()
@@ -283,6 +326,8 @@ class DeepSeek2Model:
                 if isinstance(t, torch.Tensor) and t.data_ptr() not in seen:
                     seen.add(t.data_ptr())
                     n += t.numel() * t.element_size()
+                elif isinstance(t, ops.Mx4Weight):
+                    n += t.nbytes()
         return n
 
     # ---- forward ---------------------------------------------------------------------------
@@ -337,6 +382,8 @@ class DeepSeek2Model:
         """The feed-forward block on ``residual`` (its input norm included): returns residual + ffn(rmsnorm(residual)).
         ``norm=(weight, eps)`` (MoE blocks): returns (x, rmsnorm(x) * weight), the next block's input norm."""
         hp = self.hp
+        if self.ffn_format is not None:
+            return self._mlp_mx4(L, residual, norm)
         if not L.is_moe:
             g, _ = ops.rmsnorm(residual, L.ffn_norm, hp.rms_eps)
             hmid = ops.gateup_silu(g, L.w_gate, L.w_up)
@@ -364,6 +411,18 @@ class DeepSeek2Model:
             return self.comm.all_reduce(part, residual)
         return ops.moe_ffn(g, residual, ids, wts, L.w_gate_exps, L.w_up_exps, L.w_down_exps, L.w_gate_sh, L.w_up_sh,
                            L.w_down_sh, base, n_expert=hp.n_expert, norm=norm, route=route)
+
+    def _mlp_mx4(self, L: _Layer, residual: torch.Tensor, norm):
+        """_mlp on 4-bit weights."""
+        hp = self.hp
+        g, _ = ops.rmsnorm(residual, L.ffn_norm, hp.rms_eps)
+        if not L.is_moe:
+            return ops.mx4_linear(ops.mx4_gateup(g, L.ffn_gu), L.ffn_d, residual=residual)
+        if L.shared_gu is not None:
+            residual = ops.mx4_linear(ops.mx4_gateup(g, L.shared_gu), L.shared_d, residual=residual)
+        x = ops.mx4_moe_layer(g, L.w_router, L.router_bias, hp.n_expert_used, hp.n_group, hp.topk_group, hp.expert_weights_scale, hp.expert_weights_norm,
+                              hp.expert_gating_func == "sigmoid", L.ffn_gu, L.ffn_d, L.n_shared_merged, hp.group_score_top2, residual)
+        return x if norm is None else (x, ops.rmsnorm(x, *norm)[0])
 
     def _forward_sp(self, batch: ForwardBatch, kv_cache) -> torch.Tensor:
         """Tensor-parallel forward with a sequence-parallel residual stream (large prefill batches): every rank keeps

@@ -13,7 +13,7 @@ import os
 import torch
 
 from . import reference as ref
-from .mx4 import (Mx4Tensor, Mx4Weight, mx4_dequantize, mx4_gateup, mx4_linear, mx4_matmul, mx4_moe_ffn, mx4_moe_layer,  # noqa: F401
+from .mx4 import (MX4_MAX_EXPERTS, Mx4Tensor, Mx4Weight, mx4_dequantize, mx4_gateup, mx4_linear, mx4_matmul, mx4_moe_ffn, mx4_moe_layer,  # noqa: F401
                   mx4_quantize, mx4_weight)
 from .specs import ExpertRoute
 

@@ -170,7 +170,7 @@ def load():
     sig("jib_mx4_dequantize", vp, vp, ll, vp, i, ll, i, vp)
     sig("jib_mx4_pack", vp, vp, ll, vp, vp, vp, ip, i, i, i, i, i, vp)
     sig("jib_mx4_matmul", vp, vp, ll, vp, vp, ll, vp, ll, i, i, i, i, ip, vp)
-    sig("jib_mx4_product_simt", C.POINTER(Mx4Desc), i, vp)
+    sig("jib_mx4_product_simt", C.POINTER(Mx4Desc), vp)
     sig("jib_mx4_gemm_sizes", ll, i, i, i, i, C.POINTER(ll))
     L.jib_mx4_gemm_sizes.restype = None
     sig("jib_mx4_planes", vp, ll, ip, ip, vp, vp, ll, i, ip, i, vp)

@@ -8,12 +8,12 @@ from typing import Optional
 import torch
 
 from . import native as nat
-from .mx4 import COLS, Mx4Tensor, Mx4Weight, scale_rows
+from .mx4 import COLS, MX4_MAX_EXPERTS as MAX_EXPERTS, Mx4Tensor, Mx4Weight, scale_rows
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 FEW_TOKENS = 16                              # tokens of a layer that runs as one launch behind the router's
 PAD = 32                                     # rows of an expert are padded to in grouped products (csrc/kernels/mx4_gemm.cu)
-MAX_EXPERTS, MAX_CHOICES = 256, 32           # what the gate and the sort take (csrc/kernels/moe.cu)
+MAX_CHOICES = 32                             # of a token: what the gate takes (csrc/kernels/moe.cu)
 _NO_SWITCH = contextlib.nullcontext()
 _current = nat._device or torch.cuda.current_device
 
@@ -113,7 +113,7 @@ def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dty
                 _tiled(d, x, x.shape[0], None, None, None, "mx4_gemm")
             else:
                 d.x, d.ldx = x.data_ptr(), x.stride(0)
-                nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), 1, nat._stream()), "mx4_product_simt")
+                nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), nat._stream()), "mx4_product_simt")
     return out
 
 
@@ -122,7 +122,7 @@ def _grouped_simt(x: torch.Tensor, w: Mx4Weight, seg: torch.Tensor, src: Optiona
     out = torch.empty(rows, w.n, dtype=x.dtype, device=x.device)
     d = _desc(x.shape[0], w, out, None, act)
     d.x, d.ldx, d.seg, d.src, d.batch, d.max_rows = x.data_ptr(), x.stride(0), seg.data_ptr(), nat._p(src), w.batch, rows
-    nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), 1, nat._stream()), "mx4_grouped_simt")
+    nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), nat._stream()), "mx4_grouped_simt")
     return out
 
 

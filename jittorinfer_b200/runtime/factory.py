@@ -37,10 +37,13 @@ def build_model(hp: Optional[DeepSeek2HParams] = None, gguf_path: Optional[str] 
                 dtype: torch.dtype = torch.bfloat16, world: int = 1, rank: int = 0, expert_parallel: bool = True,
                 comm=None, seed: int = 0, std: float = 0.02, max_positions: int = 8192, fast_random: bool = True,
                 dp_attention: bool = False, ep_max_tokens: int = 256, layer_devices=None,
-                tensor_split=None, kv_overrides=None, check_tensors: bool = False):
+                tensor_split=None, kv_overrides=None, check_tensors: bool = False, ffn_format: Optional[str] = None):
     """``gguf_path``: a GGUF file, or the folder of an architecture that comes as config.json + safetensors.  ``dp_attention``: attention data-parallel (every rank serves its own requests), routed experts sharded over the
-    ranks and reached through the all-to-all dispatcher; ``ep_max_tokens`` bounds the tokens of one rank per step."""
+    ranks and reached through the all-to-all dispatcher; ``ep_max_tokens`` bounds the tokens of one rank per step.  ``ffn_format="mxfp4"`` (one GPU): feed-forward
+    weights are quantised to 4 bits while loading and run on the 4-bit operators."""
     arch = registry.for_path(gguf_path) if gguf_path is not None else registry.for_hparams(hp)
+    if ffn_format is not None and (arch.load_config is not None or world > 1 or layer_devices is not None):
+        raise ValueError("ffn_format: GGUF architectures on one GPU, without tensor, expert or layer parallelism")
     if arch.load_config is not None:
         return _build_folder_arch(arch, hp, gguf_path, device, dtype, world, seed, max_positions, check_tensors, layer_devices)
     dp_attention = dp_attention and world > 1
@@ -80,7 +83,7 @@ def build_model(hp: Optional[DeepSeek2HParams] = None, gguf_path: Optional[str] 
         from ..models.deepseek2 import assign_layers
         layer_devices = assign_layers(hp.n_layer, layer_devices, tensor_split)   # a device list: contiguous layer ranges
     return DeepSeek2Model(hp, weights, dtype=dtype, device=device, spec=spec, comm=comm, max_positions=max_positions, ep=ep,
-                          layer_devices=layer_devices)
+                          layer_devices=layer_devices, ffn_format=ffn_format)
 
 
 def kv_tokens_for_budget(total_bytes: int, free_bytes: int, utilization: float, n_layer: int, kv_row: int, elem_bytes: int,
@@ -103,14 +106,16 @@ def build_engine(hp: Optional[DeepSeek2HParams] = None, gguf_path: Optional[str]
                  n_ctx_slot: int = 2048, n_batch: int = 2048, seed: int = 0, graph_buckets: Sequence[int] = (1, 2, 4, 8),
                  cuda_graphs: bool = True, expert_parallel: bool = True, comm=None, n_ctx: Optional[int] = None,
                  dp_attention: bool = False, ep_max_tokens: int = 256, layer_devices=None, tensor_split=None,
-                 gpu_memory_utilization: Optional[float] = None, check_tensors: bool = False, **engine_kw) -> LLMEngine:
+                 gpu_memory_utilization: Optional[float] = None, check_tensors: bool = False,
+                 ffn_format: Optional[str] = None, **engine_kw) -> LLMEngine:
     """``gpu_memory_utilization`` (with ``n_ctx`` None or 0): size the latent cache from the memory left after the weights
     are loaded, so that the process fills that share of the GPU."""
     if dp_attention and world > 1:
         n_batch = min(n_batch, ep_max_tokens)          # a step's tokens must fit the dispatcher's buffers
     model = build_model(hp, gguf_path, device, dtype, world, rank, expert_parallel, comm, seed,
                         max_positions=max(n_ctx_slot, 64), dp_attention=dp_attention, ep_max_tokens=ep_max_tokens,
-                        layer_devices=layer_devices, tensor_split=tensor_split, check_tensors=check_tensors)
+                        layer_devices=layer_devices, tensor_split=tensor_split, check_tensors=check_tensors,
+                        ffn_format=ffn_format)
     dev = torch.device(device)
     if not n_ctx and gpu_memory_utilization and dev.type == "cuda":
         free, total = torch.cuda.mem_get_info(dev)

@@ -28,10 +28,10 @@ def build_from_config(cfg, device=None, world: int = 1, rank: int = 0):
                   dp_attention=bool(getattr(cfg, "attention_dp", False)) and world > 1, ep_max_tokens=getattr(cfg, "ep_max_tokens", 256),
                   run_ahead=bool(getattr(cfg, "run_ahead", False)), device_sampling=bool(getattr(cfg, "device_sampling", False)),
                   mixed_prompt_budget=int(getattr(cfg, "mixed_prompt_budget", 0)),
-                  check_tensors=bool(getattr(cfg, "check_tensors", False)))
+                  check_tensors=bool(getattr(cfg, "check_tensors", False)), ffn_format=getattr(cfg, "ffn_format", "") or None)
     hp_known = preset(cfg.random_init) if cfg.random_init else None
     folder = is_folder_model(cfg.model) and not cfg.random_init
-    if world == 1 and device.type == "cuda" and not folder and (hp_known is None or hasattr(hp_known, "kv_row")) and cfg.split_mode == "LLAMA_SPLIT_MODE_LAYER":
+    if world == 1 and device.type == "cuda" and not folder and (hp_known is None or hasattr(hp_known, "kv_row")) and cfg.split_mode == "LLAMA_SPLIT_MODE_LAYER" and not common["ffn_format"]:
         n = int(getattr(cfg, "layer_split_gpus", 1))
         if n <= 0:          # automatic, as the reference spreads layers over all devices by free memory (src/llama-model.cpp:495-540)
             if hp_known is None:

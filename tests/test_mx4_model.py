@@ -1,0 +1,126 @@
+"""``ffn_format="mxfp4"``: a model whose feed-forward weights are held in 4 bits is the model with those weights' values, served the same way."""
+import pytest
+import torch
+
+from jittorinfer_b200 import ops
+from jittorinfer_b200.config import ServerConfig, load_yaml
+from jittorinfer_b200.models import registry
+from jittorinfer_b200.models.deepseek2 import DeepSeek2Model, ForwardBatch
+from jittorinfer_b200.models.hparams import preset
+from jittorinfer_b200.models.oracle import OracleModel
+from jittorinfer_b200.models.weights import random_weights
+from jittorinfer_b200.runtime.engine import EngineConfig, LLMEngine
+from jittorinfer_b200.runtime.factory import build_engine, build_model
+from jittorinfer_b200.runtime.sampling import SamplingParams
+
+PRESETS = ("tiny", "tiny-v2", "tiny-v3")
+
+
+def _in_4_bits(w):
+    """The weights with the feed-forward matrices replaced by their 4-bit values."""
+    def is_ffn(name):
+        return ".ffn_" in name and "norm" not in name and "gate_inp" not in name
+    return {n: ops.mx4_dequantize(ops.mx4_quantize(t.float().cpu()), torch.float32).to(t.dtype) if is_ffn(n) else t for n, t in w.items()}
+
+
+def _batch(toks, n_past, device="cpu", bs=64):
+    T, S = len(toks), n_past + len(toks)
+    bt = torch.arange(1, 1 + (S + bs - 1) // bs).int()[None]
+    pos = torch.arange(n_past, S).int()
+    slots = (bt[0][(pos // bs).long()] * bs + pos % bs).int()
+    t = [torch.tensor(toks).int(), pos, slots, bt, torch.tensor([S]).int(), torch.tensor([0, T]).int(), torch.arange(T).int()]
+    tokens, pos, slots, bt, lens, start, rows = (v.to(device) for v in t)
+    return ForwardBatch(tokens=tokens, positions=pos, slot_mapping=slots, block_tables=bt, seq_lens=lens, q_start=start, out_rows=rows, max_q_len=T)
+
+
+@pytest.mark.parametrize("name", PRESETS)
+def test_a_4_bit_model_is_the_model_with_the_4_bit_values(name):
+    hp = preset(name)
+    w = random_weights(hp, seed=0, std=0.05)
+    o = OracleModel(hp, _in_4_bits(w))
+    m = DeepSeek2Model(hp, w.items(), dtype=torch.float32, ffn_format="mxfp4")
+    toks = torch.randint(0, hp.n_vocab, (40,), generator=torch.Generator().manual_seed(7)).tolist()
+    cache = torch.zeros(hp.n_layer, 4 * 64, hp.kv_row)
+    ref = o.forward(torch.tensor(toks))
+    # the same fp32 sums in another order: the bound that the plain model is held to
+    assert (m.forward(_batch(toks, 0), cache) - ref).abs().max() < 1e-4
+    plain = DeepSeek2Model(hp, w.items(), dtype=torch.float32)
+    assert m.weight_bytes() < plain.weight_bytes()
+    assert all(L.w_gate is None and L.w_gate_exps is None and L.w_gate_sh is None for L in m.layers)
+
+
+def test_shared_experts_that_do_not_fit_behind_the_routed_ones_run_apart(monkeypatch):
+    hp = preset("tiny-v2")
+    w = random_weights(hp, seed=0, std=0.05)
+    monkeypatch.setattr(ops, "MX4_MAX_EXPERTS", hp.n_expert)
+    m = DeepSeek2Model(hp, w.items(), dtype=torch.float32, ffn_format="mxfp4")
+    assert m.layers[1].shared_gu is not None and m.layers[1].ffn_gu.batch == hp.n_expert
+    toks = list(range(30, 61))
+    cache = torch.zeros(hp.n_layer, 4 * 64, hp.kv_row)
+    ref = OracleModel(hp, _in_4_bits(w)).forward(torch.tensor(toks))
+    assert (m.forward(_batch(toks, 0), cache) - ref).abs().max() < 1e-4
+
+
+def test_engine_and_configuration_take_the_format(tmp_path):
+    hp = preset("tiny")
+    eng = build_engine(hp, device="cpu", dtype=torch.float32, n_parallel=2, n_ctx_slot=128, n_batch=32, cuda_graphs=False, ffn_format="mxfp4")
+    w = {n: t for n, t in random_weights(hp, seed=0).items()}
+    m = DeepSeek2Model(hp, _in_4_bits(w).items(), dtype=torch.float32)
+    ref = LLMEngine(m, EngineConfig(n_ctx=256, n_batch=32, n_parallel=2, n_ctx_slot=128, cuda_graphs=False))
+    prompts = [[5, 9, 300, 17], list(range(100, 150))]
+    sp = SamplingParams(ignore_eos=True)
+    assert eng.generate(prompts, sp, max_new_tokens=6) == ref.generate(prompts, sp, max_new_tokens=6)
+    p = tmp_path / "c.yaml"
+    p.write_text("random_init: tiny\nffn_format: mxfp4\n")
+    assert load_yaml(str(p)).ffn_format == "mxfp4" and ServerConfig().ffn_format == ""
+
+
+def test_refusals(tmp_path):
+    hp = preset("tiny")
+    w = random_weights(hp, seed=0)
+    with pytest.raises(ValueError, match="ffn_format"):
+        DeepSeek2Model(hp, w.items(), dtype=torch.float32, ffn_format="int4")
+    with pytest.raises(ValueError, match="one GPU"):
+        build_model(hp, device="cpu", world=2, ffn_format="mxfp4")
+    with pytest.raises(ValueError, match="one GPU"):
+        build_model(hp, device="cpu", layer_devices=["cpu"] * hp.n_layer, ffn_format="mxfp4")
+    with pytest.raises(ValueError, match="GGUF"):
+        build_model(registry.preset("zomavik-tiny"), device="cpu", ffn_format="mxfp4")
+    for body in ("ffn_format: fp4\n", "ffn_format: mxfp4\ntp_size: 2\n"):
+        p = tmp_path / "bad.yaml"
+        p.write_text(body)
+        with pytest.raises(ValueError, match="ffn_format"):
+            load_yaml(str(p))
+
+
+@pytest.mark.gpu
+def test_model_on_the_kernels_and_engine_under_graphs():
+    """The benchmark's layer shapes in three layers: prompt rows and decoding rows against the fp32 oracle of the 4-bit values, then sequences under CUDA
+    graphs.  The bounds are those that the bf16 model is held to: activations are bf16 in both, and what the 4-bit products round besides (two planes
+    of 8 bits: 2^-11 of a block's largest; hidden units in fp16 or bf16) is no coarser than its bf16 products."""
+    hp = preset("lite-2l")
+    w = random_weights(hp, seed=0, std=0.02)
+    o = OracleModel(hp, _in_4_bits(w))
+    m = DeepSeek2Model(hp, w.items(), dtype=torch.bfloat16, device="cuda", ffn_format="mxfp4")
+    cache = torch.zeros(hp.n_layer, 8 * 64, hp.kv_row, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator().manual_seed(2)
+    toks, nxt, one = (torch.randint(0, hp.n_vocab, (n,), generator=g).tolist() for n in (70, 9, 1))
+    nat = ops.nat()
+    n0 = dict(nat.launches_by_name)
+    got = torch.cat([m.forward(_batch(t, p, "cuda"), cache).float().cpu() for t, p in ((toks, 0), (nxt, 70), (one, 79))])
+    nat.check_status()
+    ran = {k: nat.launches_by_name.get(k, 0) - n0.get(k, 0) for k in ("mx4_linear", "mx4_gateup", "mx4_moe", "mx4_grouped", "gemm_grouped")}
+    assert ran["mx4_moe"] == 4 and ran["mx4_grouped"] >= 2 and ran["gemm_grouped"] == 0, ran
+    ref = torch.cat([o.forward(torch.tensor(t)) for t in (toks, nxt, one)])
+    err = (got - ref).abs().amax(-1) / ref.abs().amax(-1)
+    print(f"median row error {err.median().item():.4f}, rows within 3e-2 {(err <= 3e-2).float().mean().item():.3f}, worst {err.max().item():.3f}")
+    assert err.median().item() <= 2e-2 and (err <= 3e-2).float().mean().item() >= 0.95 and err.max().item() < 0.5
+
+    prompts = [torch.randint(0, hp.n_vocab, (n,), generator=g).tolist() for n in (70, 33, 8, 100, 64, 65, 17, 5)]
+    outs = []
+    for graphs in (True, False):
+        eng = LLMEngine(m, EngineConfig(n_ctx=8 * 256, n_batch=256, n_parallel=8, graph_buckets=(1, 2, 4, 8), cuda_graphs=graphs))
+        outs.append(eng.generate(prompts, SamplingParams(ignore_eos=True), max_new_tokens=6))
+        nat.check_status()
+        assert not graphs or eng.stats["graph_steps"] >= 5
+    assert outs[0] == outs[1]                       # a replayed step computes what an eager one does

@@ -347,10 +347,9 @@ JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, void * stream);
 JIB_EXPORT void jib_mx4_gemm_sizes(long long rows, int N, int K, int gated, int grouped, long long * sizes);
 JIB_EXPORT int jib_mx4_planes(const void * x, long long ldx, const int * src, const int * limit, void * planes, void * scales, long long rows, int K, int * zeros,
                               int n_zeros, void * stream);
-JIB_EXPORT int jib_mx4_pad(const int * seg, const int * src, const int * dest, int E, int n_pairs, int cap, int * first, int * count, int * row_src, int * pair_row,
-                           void * stream);
+JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, int * count, int * row_src, int * pair_row, void * stream);
 JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const int * count, float * part, int * counters, void * stream);
-// A mixture-of-experts layer for up to 16 tokens (mx4_moe.cu).
+// A mixture-of-experts layer for up to 8 tokens (mx4_moe.cu).
 typedef struct jib_mx4_moe_desc {
     const void * residual;                 // NULL, or bf16 [T][d], rows ldr elements apart
     const float * logits, * bias;          // router outputs [T][E - n_shared] and the bias of the choice (or NULL); logits NULL: ids and wts

@@ -503,62 +503,84 @@ __global__ void __launch_bounds__(256) planes_kernel(const bf16 * __restrict__ x
     }
 }
 
-// ---- experts' rows at multiples of PAD ------------------------------------------------------------------------------------------------
-// From the sorted order (seg, src, dest of jib_moe_permute): first[e] and count[e] of the padded order (first[E]: its end), the token of each of its rows (-1: none) and
-// the row of each pair (-1: none).
-__global__ void __launch_bounds__(256) pad_kernel(const int * __restrict__ seg, const int * __restrict__ src, const int * __restrict__ dest, int E, int n_pairs, int cap,
-                                                  int * __restrict__ first, int * __restrict__ count, int * __restrict__ row_src, int * __restrict__ pair_row) {
-    __shared__ int seg_s[MAX_E + 1], pad_s[MAX_E + 1];
+// ---- pairs by expert, each expert's rows at a multiple of PAD -------------------------------------------------------------------------
+// first[e] and count[e] of the padded order (first[E]: its end), the token of each of its rows (-1: none) and the row of each pair (-1: an id outside the experts).
+// One CTA: counts, their sums, places, with a table for each warp (tokens that choose alike would queue for one).  Which of its warp's rows a pair gets is left
+// to chance; what is computed from a row does not depend on where it stands.
+constexpr int SORT_NT = 1024, SORT_AHEAD = 4;
+
+__global__ void __launch_bounds__(SORT_NT) sort_kernel(const int * __restrict__ ids, int n, int k, int E, int * __restrict__ first, int * __restrict__ count,
+                                                       int * __restrict__ row_src, int * __restrict__ pair_row) {
+    __shared__ int places[SORT_NT / 32][MAX_E], count_s[MAX_E], first_s[MAX_E + 1];
+    const int tid = threadIdx.x, lane = tid & 31;
+    int * mine = places[tid >> 5];
+    auto ask = [&](int b, int (&e)[SORT_AHEAD]) {        // -1: none
+#pragma unroll
+        for (int j = 0; j < SORT_AHEAD; ++j) {
+            const int i = b + j * SORT_NT + tid, id = i < n ? ids[i] : -1;
+            e[j] = (unsigned) id < (unsigned) E ? id : -1;
+        }
+    };
+    for (int i = tid; i < SORT_NT / 32 * MAX_E; i += SORT_NT) (&places[0][0])[i] = 0;
+    __syncthreads();
     PDL_TRIGGER_TOP();
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
-    for (int e = threadIdx.x; e <= E; e += blockDim.x) seg_s[e] = seg[e];
+    for (int b = 0; b < n; b += SORT_NT * SORT_AHEAD) {
+        int e[SORT_AHEAD];
+        ask(b, e);
+#pragma unroll
+        for (int j = 0; j < SORT_AHEAD; ++j)
+            if (e[j] >= 0) atomicAdd(&mine[e[j]], 1);
+    }
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
+    if (tid < E) {                       // each warp's first place among its expert's rows
+        int sum = 0;
+#pragma unroll 8
+        for (int w = 0; w < SORT_NT / 32; ++w) {
+            const int have = places[w][tid];
+            places[w][tid] = sum;
+            sum += have;
+        }
+        count_s[tid] = sum;
+    }
+    __syncthreads();
+    if (tid < 32) {
         int sum = 0;
 #pragma unroll 1
         for (int e0 = 0; e0 < E; e0 += 32) {
-            const int e = e0 + lane, mine = e < E ? (seg_s[e + 1] - seg_s[e] + PAD - 1) / PAD * PAD : 0;
-            int s = mine;
+            const int e = e0 + lane, rows = e < E ? (count_s[e] + PAD - 1) / PAD * PAD : 0;
+            int s = rows;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
                 const int v = __shfl_up_sync(0xffffffffu, s, o);
                 if (lane >= o) s += v;
             }
-            if (e < E) pad_s[e] = sum + s - mine;
+            if (e < E) first_s[e] = sum + s - rows;
             sum += __shfl_sync(0xffffffffu, s, 31);
         }
-        if (lane == 0) pad_s[E] = sum;
+        if (lane == 0) first_s[E] = sum;
     }
     __syncthreads();
-    auto find = [&](const int * at, int v) {             // the last e with at[e] <= v that has rows
-        int lo = 0, hi = E;
-#pragma unroll 1
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (at[mid] <= v) lo = mid;
-            else hi = mid;
-        }
-        return lo;
-    };
-    if (blockIdx.x == 0)
-        for (int e = threadIdx.x; e <= E; e += blockDim.x) {
-            first[e] = pad_s[e];
-            if (e < E) count[e] = seg_s[e + 1] - seg_s[e];
-        }
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < cap || i < n_pairs; i += gridDim.x * blockDim.x) {
-        if (i < cap && i < pad_s[E]) {
-            const int e = find(pad_s, i), at = i - pad_s[e];
-            row_src[i] = at < seg_s[e + 1] - seg_s[e] ? src[seg_s[e] + at] : -1;
-        }
-        if (i < n_pairs) {
-            const int r = dest[i];
-            int to = -1;
-            if (r >= 0) {
-                const int e = find(seg_s, r);
-                to = pad_s[e] + r - seg_s[e];
+    for (int e = tid; e <= E; e += SORT_NT) {
+        first[e] = first_s[e];
+        if (e < E) count[e] = count_s[e];
+    }
+    for (int i = tid; i < E * PAD; i += SORT_NT) {       // rows behind an expert's last
+        const int e = i / PAD, r = first_s[e] + count_s[e] + i % PAD;
+        if (r < first_s[e + 1]) row_src[r] = -1;
+    }
+    for (int b = 0; b < n; b += SORT_NT * SORT_AHEAD) {
+        int e[SORT_AHEAD];
+        ask(b, e);
+#pragma unroll
+        for (int j = 0; j < SORT_AHEAD; ++j) {
+            const int i = b + j * SORT_NT + tid;
+            int r = -1;
+            if (e[j] >= 0) {
+                r = first_s[e[j]] + atomicAdd(&mine[e[j]], 1);
+                row_src[r] = i / k;
             }
-            pair_row[i] = to;
+            if (i < n) pair_row[i] = r;
         }
     }
 }
@@ -647,15 +669,14 @@ JIB_EXPORT int jib_mx4_planes(const void * x, long long ldx, const int * src, co
     return launched();
 }
 
-JIB_EXPORT int jib_mx4_pad(const int * seg, const int * src, const int * dest, int E, int n_pairs, int cap, int * first, int * count, int * row_src, int * pair_row,
-                           void * stream) {
-    if (E < 1 || E > MAX_E || n_pairs < 1 || cap < 1) return JIB_E_ARG;
-    const int n = cap > n_pairs ? cap : n_pairs, ctas = (n + 255) / 256;
-    JIB_LAUNCH((pad_kernel), ctas < 148 ? ctas : 148, 256, 0, (cudaStream_t) stream, seg, src, dest, E, n_pairs, cap, first, count, row_src, pair_row);
+// ids [n / k][k]; first: E + 1 ints, count: E, row_src: room for n pairs and PAD - 1 more rows of each expert that has any, pair_row: n.
+JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, int * count, int * row_src, int * pair_row, void * stream) {
+    if (E < 1 || E > MAX_E || n < 1 || k < 1) return JIB_E_ARG;
+    JIB_LAUNCH((sort_kernel), 1, SORT_NT, 0, (cudaStream_t) stream, ids, n, k, E, first, count, row_src, pair_row);
     return launched();
 }
 
-// The tiled product: d->x are the planes (d->x_rows rows), x_scales their scales; grouped: d->seg = first, count (see jib_mx4_pad); part and counters (zeros) as
+// The tiled product: d->x are the planes (d->x_rows rows), x_scales their scales; grouped: d->seg = first, count (see jib_mx4_sort); part and counters (zeros) as
 // jib_mx4_gemm_sizes says.
 JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const int * count, float * part, int * counters, void * stream) {
     if (d->T <= 0) return 0;

@@ -1,4 +1,4 @@
-// A mixture-of-experts layer over packed 4-bit experts for up to 16 tokens, in two launches: the router's outputs, then everything else --
+// A mixture-of-experts layer over packed 4-bit experts for up to 8 tokens, in two launches: the router's outputs, then everything else --
 // choice of experts, gate and up products, activation, down products, weighted sum, residual.
 //
 // The reference runs router, choice, sorting, grouped products and the weighted sum as some dozen launches
@@ -23,7 +23,7 @@ namespace {
 
 using namespace sm100;
 
-constexpr int MAX_T = 16, MAX_K = 32;                         // tokens, choices of a token
+constexpr int MAX_T = 8, MAX_K = 32;                          // tokens, choices of a token
 constexpr int NW = 16, THREADS = NW * 32;                     // warps
 constexpr int MOST_SMEM = 227 * 1024, MAX_DEPTH = 4, KNOWN = 8, AHEAD = 3;       // units of a group: that it remembers, that it draws ahead
 constexpr int BIAS = 113;                                     // top_exponent() + BIAS is 1 .. 240
@@ -31,34 +31,33 @@ constexpr uint64_t WAIT_NS = JIB_WAIT_NS;                     // for the other C
 
 struct MoeArgs {
     const bf16 * residual;                   // may be NULL
-    const uint4 * xf;                        // fragments of x, then the exponents of its 16 rows
+    const uint4 * xf;                        // fragments of x, then the exponents of its 8 rows
     const float * logits, * bias;            // logits NULL: ids and weights are given
     const int * ids;
     const float * wts;
     const uint8_t * gu, * down, * gu_factors, * down_factors;
     const int * gu_exp, * down_exp;
-    __half * h;                              // hidden units: [slot][chunks of F][NT] fragments, each 16 of a token scaled by a power of two ...
+    __half * h;                              // hidden units: [slot][chunks of F] fragments, each 16 of a token scaled by a power of two ...
     uint8_t * h_exp;                         // ... [slot][chunk][token][16 units], BIAS more than its exponent
-    float * part;                            // [pieces][512 NT]
+    float * part;                            // [pieces][512]
     bf16 * out;
     int * sync;                              // zeros: units of gate and up drawn, units done (and two more), the largest byte of h_exp of each slot and token
-                                             // [slots][16], pieces done of each 64 rows
+                                             // [slots][8], pieces done of each 64 rows
     int * status;
     long long ldr;
     int T, max_slots, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act, gw, depth1, depth2, warm;
     float scale;
 };
 
-// Shared memory: tables; sums, twice; the warps' rings of chunks, for gate and up behind the tokens' fragments.
-template <int NT>
+// Shared memory: tables; sums, three times; the warps' rings of chunks, for gate and up behind the tokens' fragments.
 struct Layout {
     static_assert((48 + 4 * KNOWN * 8) % 16 == 0, "the exponents' place");
-    static constexpr int SUMS = 8 * NT;                           // of a lane
+    static constexpr int SUMS = 8;                                // of a lane
     static constexpr int RED = NW * 32 * SUMS * 4;
-    static constexpr int BUFFERS = NT == 1 ? 3 : 2;               // of sums (see where a unit of gate and up is finished)
+    static constexpr int BUFFERS = 3;                             // of sums (see where a unit of gate and up is finished)
     static_assert(BUFFERS * RED >= NW * (MAX_E + 32) * 4, "scratch of the choice");
-    __host__ __device__ static int frags(int d) { return mx4::chunks(d) * NT * mx4::FRAG; }
-    __host__ __device__ static int tables(int slots) { return (slots * 64 + MAX_E * 4 * 3 + MAX_T * MAX_K * 8 + 64 + 4 * KNOWN * (8 + 128) + 127) / 128 * 128; }
+    __host__ __device__ static int frags(int d) { return mx4::chunks(d) * mx4::FRAG; }
+    __host__ __device__ static int tables(int slots) { return (slots * 32 + MAX_E * 4 * 3 + MAX_T * MAX_K * 8 + 64 + 4 * KNOWN * (8 + 128) + 127) / 128 * 128; }
     __host__ __device__ static int base(int slots) { return 128 + tables(slots) + BUFFERS * RED; }
     __host__ __device__ static int bytes(int d, int slots, int depth1, int depth2) {
         const int a = frags(d) + NW * depth1 * mx4::SLOT, b = NW * depth2 * mx4::SLOT;
@@ -79,13 +78,12 @@ __device__ __forceinline__ int ld_acquire(const int * p) {
     return v;
 }
 
-template <int NT>
 __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
-    using L = Layout<NT>;
+    using L = Layout;
     extern __shared__ uint8_t smem_raw[];
     uint8_t * base = (uint8_t *) (((uintptr_t) smem_raw + 127) & ~(uintptr_t) 127);
-    float * wtab = (float *) base;                                 // [slot][16] weight of each token, 0: not chosen
-    int * slot_of = (int *) (wtab + g.max_slots * 16), * expert_of = slot_of + MAX_E, * mask = expert_of + MAX_E;
+    float * wtab = (float *) base;                                 // [slot][8] weight of each token, 0: not chosen
+    int * slot_of = (int *) (wtab + g.max_slots * 8), * expert_of = slot_of + MAX_E, * mask = expert_of + MAX_E;
     int * ids_s = mask + MAX_E;
     float * wts_s = (float *) (ids_s + MAX_T * MAX_K);
     uint64_t * acts_full = (uint64_t *) (wts_s + MAX_T * MAX_K);
@@ -100,7 +98,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
         mbar_init(acts_full, 1);
         fence_barrier_init();
     }
-    for (int i = threadIdx.x; i < g.max_slots * 16; i += THREADS) wtab[i] = 0.f;
+    for (int i = threadIdx.x; i < g.max_slots * 8; i += THREADS) wtab[i] = 0.f;
     for (int i = threadIdx.x; i < MAX_E; i += THREADS) { slot_of[i] = 0; mask[i] = 0; }
     if (threadIdx.x < 4 * KNOWN) drawn[threadIdx.x] = -1;
     __syncthreads();
@@ -148,13 +146,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
             for (int j = 0; j < kk; ++j) {
                 const int e = ids_s[lane * kk + j];
                 if ((unsigned) e >= (unsigned) g.E) continue;
-                wtab[slot_of[e] * 16 + lane] += wts_s[lane * kk + j];
+                wtab[slot_of[e] * 8 + lane] += wts_s[lane * kk + j];
                 atomicOr(&mask[slot_of[e]], 1 << lane);
             }
     }
     __syncthreads();
     const int slots = word[0], C1 = mx4::chunks(g.d), C2 = mx4::chunks(g.F), RB1 = g.F / 16, G = gridDim.x, U = slots * RB1;
-    int * done = g.sync + 1, * h_top = g.sync + 4, * pieces_done = h_top + g.max_slots * 16;
+    int * done = g.sync + 1, * h_top = g.sync + 4, * pieces_done = h_top + g.max_slots * 8;
     const uint64_t policy = l2_policy_evict_first();
 
     // ---- gate and up ----
@@ -203,56 +201,48 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
 #pragma unroll 1
         for (int i = 0; i < depth; ++i) ask();
         int here = 0, i = 0;
-        const int set = wg / (2 * NT), job = wg % (2 * NT), col = t2 + (job & 1);
-        const int xe = ((const int *) ((const uint8_t *) g.xf + L::frags(g.d)))[(job >> 1) * 8 + col];
+        const int set = wg >> 1, job = wg & 1, col = t2 + job;
+        const int xe = ((const int *) ((const uint8_t *) g.xf + L::frags(g.d)))[col];
 #pragma unroll 1
         for (int u; (u = unit(i)) < U; ++i) {
             const int parity = i & 1;
             float * sums = red + i % L::BUFFERS * (L::RED / 4);
             int next = 0;
             if (wg == 0 && lane == 0) next = atomicAdd(g.sync, 1);
-            float acc[2][NT][4];
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[m][n][c] = 0.f;
+            float acc[2][4] = {};
 #pragma unroll 1
             for (int k = wg; k < C1; k += g.gw) {
                 mx4::copies_wait(depth - 1);
                 __syncwarp();
-                const uint4 * b = acts + k * NT * 128;
-                mx4::chunk_mma<NT>(ring + here * mx4::SLOT, acc, [&](int n, int p) { return b[(n * 4 + p) * 32]; });
+                const uint4 * b = acts + k * 128;
+                mx4::chunk_mma(ring + here * mx4::SLOT, acc, [&](int p) { return b[p * 32]; });
                 here = here + 1 == depth ? 0 : here + 1;
                 __syncwarp();
                 ask();
             }
             if (wg == 0 && lane == 0) *(volatile long long *) (drawn + group * KNOWN + (i + AHEAD) % KNOWN) = (long long) (i + AHEAD) << 32 | next;
-            // the group's sums, in the order of its warps: [gate or up][tile][register][lane]
+            // the group's sums, in the order of its warps: [gate or up][register][lane]
             float * mine = sums + warp * L::SUMS * 32 + lane;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) mine[((m * NT + n) * 4 + c) * 32] = acc[m][n][c];
-            // 2 NT warps finish the unit.  With 8 tokens the first two and the next two take turns, and the two whose turn it is not go on without waiting:
-            // they wait for all at the next unit, so that a buffer is free again three units later (two, where everybody waits).
-            const int barrier = 1 + group * 2 + parity, turn = NT == 1 ? parity : 0;
-            if (NT == 1 && set == (turn ^ 1)) asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "r"(g.gw * 32) : "memory");
+                for (int c = 0; c < 4; ++c) mine[(m * 4 + c) * 32] = acc[m][c];
+            // Two warps finish the unit: the first two and the next two take turns, and the two whose turn it is not go on without waiting: they wait for all
+            // at the next unit, so that a buffer is free again three units later.
+            const int barrier = 1 + group * 2 + parity;
+            if (set == (parity ^ 1)) asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "r"(g.gw * 32) : "memory");
             else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(g.gw * 32) : "memory");
-            if (set == turn) {
-                // token 8 n + col, hidden units f + g and f + g + 8
-                const int n = job >> 1, slot = u / RB1, f = (u - slot * RB1) * 16;
-                const float * from = sums + (warp - wg) * L::SUMS * 32 + (n * 4 + (job & 1)) * 32 + lane;
+            if (set == parity) {
+                // token col, hidden units f + g and f + g + 8
+                const int slot = u / RB1, f = (u - slot * RB1) * 16;
+                const float * from = sums + (warp - wg) * L::SUMS * 32 + job * 32 + lane;
                 float z[2] = {0.f, 0.f}, v[2] = {0.f, 0.f};
 #pragma unroll 4
                 for (int w = 0; w < g.gw; ++w)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         z[c] += from[w * L::SUMS * 32 + 64 * c];
-                        v[c] += from[w * L::SUMS * 32 + NT * 128 + 64 * c];
+                        v[c] += from[w * L::SUMS * 32 + 128 + 64 * c];
                     }
                 const int * rows = rows_of + i % KNOWN * 32 + g4;
                 uint32_t most = 0;
@@ -263,16 +253,16 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
                 }
 #pragma unroll
                 for (int o = 4; o < 32; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                if (mask[slot] >> (n * 8 + col) & 1) {
+                if (mask[slot] >> col & 1) {
                     const int he = mx4::top_exponent(most);
                     const float up = mx4::pow2_normal(14 - he);
-                    const size_t tile = ((size_t) slot * C2 + f / mx4::COLS) * NT + n;
+                    const size_t tile = (size_t) slot * C2 + f / mx4::COLS;
                     __half * to = g.h + ((tile * 4 + f % 32 / 8) * 32 + col * 4 + f % mx4::COLS / 32) * 8 + g4;
                     to[0] = __float2half_rn(v[0] * up);
                     to[32 * 8] = __float2half_rn(v[1] * up);
                     if (g4 == 0) {
                         g.h_exp[(tile * 8 + col) * 8 + f % mx4::COLS / 16] = (uint8_t) (he + BIAS);
-                        atomicMax(h_top + slot * 16 + n * 8 + col, he + BIAS);
+                        atomicMax(h_top + slot * 8 + col, he + BIAS);
                     }
                 }
             }
@@ -340,31 +330,28 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     // A place's hidden units: fragments (zeros for tokens that have not chosen this expert, and behind the last hidden unit), their exponents' bytes, the
     // largest byte of this lane's token; the exponents of this lane's rows.
     struct Hidden {
-        uint4 b[NT][4];
-        uint32_t ex[NT];
-        int top[NT], row[4];
+        uint4 b[4];
+        uint32_t ex;
+        int top, row[4];
     } next;
     auto fetch = [&] {
         if (xh.p >= xh.end) return;
-        const size_t tile = (size_t) (xh.slot * C2 + xh.c) * NT;
+        const size_t tile = xh.slot * C2 + xh.c;
         const int m = mask[xh.slot], * rows = g.down_exp + (size_t) expert_of[xh.slot] * g.d + first_row(xh) + g4;
         const bool units = xh.c * mx4::COLS + 32 * (lane & 3) < g.F;
 #pragma unroll
         for (int i = 0; i < 4; ++i) next.row[i] = __ldg(rows + 8 * i);
+        const bool chosen = m >> g4 & 1;
+        next.ex = 0u;
+        next.top = 0;
+        if (chosen) {
+            next.ex = __ldcg((const unsigned short *) g.h_exp + (tile * 8 + g4) * 4 + (lane & 3));
+            next.top = __ldcg(h_top + xh.slot * 8 + g4);
+        }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const bool chosen = m >> (n * 8 + g4) & 1;
-            next.ex[n] = 0u;
-            next.top[n] = 0;
-            if (chosen) {
-                next.ex[n] = __ldcg((const unsigned short *) g.h_exp + ((tile + n) * 8 + g4) * 4 + (lane & 3));
-                next.top[n] = __ldcg(h_top + xh.slot * 16 + n * 8 + g4);
-            }
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                next.b[n][p] = make_uint4(0u, 0u, 0u, 0u);
-                if (chosen && units) next.b[n][p] = __ldcg((const uint4 *) g.h + ((tile + n) * 4 + p) * 32 + lane);
-            }
+        for (int p = 0; p < 4; ++p) {
+            next.b[p] = make_uint4(0u, 0u, 0u, 0u);
+            if (chosen && units) next.b[p] = __ldcg((const uint4 *) g.h + (tile * 4 + p) * 32 + lane);
         }
     };
 #pragma unroll 1
@@ -387,77 +374,58 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
 #pragma unroll 1
     for (int gr = i0 / P; gr * P < i1; ++gr) {
         const int a = max(0, i0 - gr * P), b = min(P, i1 - gr * P);
-        float acc[2][NT][4];
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+        float acc[2][4] = {};
 #pragma unroll 1
         while (xh.gr == gr && xh.p < xh.end) {
             Hidden h = next;
             const int slot = xh.slot;
             // all hidden units of a token to the power of two of its largest ones
+            const uint32_t f0 = below(h.top - (int) (h.ex & 0xff)), f1 = below(h.top - (int) (h.ex >> 8));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const uint32_t f0 = below(h.top[n] - (int) (h.ex[n] & 0xff)), f1 = below(h.top[n] - (int) (h.ex[n] >> 8));
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint4 & v = h.b[n][q];
-                    v.x = mx4::mul2(v.x, q < 2 ? f0 : f1);
-                    v.y = mx4::mul2(v.y, q < 2 ? f0 : f1);
-                    v.z = mx4::mul2(v.z, q < 2 ? f0 : f1);
-                    v.w = mx4::mul2(v.w, q < 2 ? f0 : f1);
-                }
+            for (int q = 0; q < 4; ++q) {
+                uint4 & v = h.b[q];
+                v.x = mx4::mul2(v.x, q < 2 ? f0 : f1);
+                v.y = mx4::mul2(v.y, q < 2 ? f0 : f1);
+                v.z = mx4::mul2(v.z, q < 2 ? f0 : f1);
+                v.w = mx4::mul2(v.w, q < 2 ? f0 : f1);
             }
             advance(xh);
             fetch();
             mx4::copies_wait(depth - 1);
             __syncwarp();
-            float y[2][NT][4] = {};
-            mx4::chunk_mma<NT>(ring + here * mx4::SLOT, y, [&](int n, int q) { return h.b[n][q]; });
+            float y[2][4] = {};
+            mx4::chunk_mma(ring + here * mx4::SLOT, y, [&](int q) { return h.b[q]; });
             here = here + 1 == depth ? 0 : here + 1;
             __syncwarp();
             ask();
             float r[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = mx4::pow2(h.row[i]);
+            const float2 wt = *(const float2 *) (wtab + slot * 8 + t2);
+            const int e0 = __shfl_sync(0xffffffffu, h.top, 4 * t2), e1 = __shfl_sync(0xffffffffu, h.top, 4 * t2 + 4);
+            const float w0 = wt.x * mx4::pow2_normal(e0 - BIAS - 14), w1 = wt.y * mx4::pow2_normal(e1 - BIAS - 14);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float2 wt = *(const float2 *) (wtab + slot * 16 + n * 8 + t2);
-                const int e0 = __shfl_sync(0xffffffffu, h.top[n], 4 * t2), e1 = __shfl_sync(0xffffffffu, h.top[n], 4 * t2 + 4);
-                const float w0 = wt.x * mx4::pow2_normal(e0 - BIAS - 14), w1 = wt.y * mx4::pow2_normal(e1 - BIAS - 14);
+            for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[m][n][i] += y[m][n][i] * r[2 * m + (i >> 1)] * (i & 1 ? w1 : w0);
-            }
+                for (int i = 0; i < 4; ++i) acc[m][i] += y[m][i] * r[2 * m + (i >> 1)] * (i & 1 ? w1 : w0);
         }
         float * mine = red + (gr & 1) * (L::RED / 4) + warp * L::SUMS * 32 + lane;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mine[((m * NT + n) * 4 + i) * 32] = acc[m][n][i];
+            for (int i = 0; i < 4; ++i) mine[(m * 4 + i) * 32] = acc[m][i];
         __syncthreads();
-        // thread = (two row blocks, register, lane): its row of one row block, then of the other, for each tile
+        // thread = (two row blocks, register, lane): its row of one row block, then of the other
         const int half = warp >> 3, m = warp >> 2 & 1, reg = warp & 3, o = gr * 64 + (2 * half + m) * 16 + g4 + 8 * (reg >> 1);
-        const float * src = red + (gr & 1) * (L::RED / 4) + half * 8 * L::SUMS * 32 + (m * NT * 4 + reg) * 32 + lane;
-        float v[NT];
+        const float * src = red + (gr & 1) * (L::RED / 4) + half * 8 * L::SUMS * 32 + (m * 4 + reg) * 32 + lane;
+        float v = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            v[n] = 0.f;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) v[n] += src[(w * L::SUMS + n * 4) * 32];
-        }
+        for (int w = 0; w < 8; ++w) v += src[w * L::SUMS * 32];
         if (a > 0 || b < P) {
             // pieces first .. last hold places of these rows
             const int first = (int) ((((long long) gr * P + 1) * pieces - 1) / N), last = (int) ((((long long) gr + 1) * P * pieces - 1) / N);
-            float * part = g.part + ((size_t) (first + 2 * gr)) * (THREADS * NT) + threadIdx.x;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) __stcg(part + ((blockIdx.x - first) * NT + n) * THREADS, v[n]);
+            float * part = g.part + ((size_t) (first + 2 * gr)) * THREADS + threadIdx.x;
+            __stcg(part + (blockIdx.x - first) * THREADS, v);
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
@@ -466,36 +434,30 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
             }
             __syncthreads();
             if (word[2] != last - first) continue;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                v[n] = 0.f;
+            v = 0.f;
 #pragma unroll 1
-                for (int q0 = 0; q0 <= last - first; q0 += 8) {
-                    float x[8];
+            for (int q0 = 0; q0 <= last - first; q0 += 8) {
+                float x[8];
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) x[q] = q0 + q <= last - first ? __ldcg(part + ((q0 + q) * NT + n) * THREADS) : 0.f;
+                for (int q = 0; q < 8; ++q) x[q] = q0 + q <= last - first ? __ldcg(part + (q0 + q) * THREADS) : 0.f;
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) v[n] += x[q];
-                }
+                for (int q = 0; q < 8; ++q) v += x[q];
             }
         }
-        if (o < g.d)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int t = n * 8 + t2 + (reg & 1);
-                if (t >= g.T) continue;
-                if (g.residual != nullptr) v[n] += __bfloat162float(g.residual[t * g.ldr + o]);
-                g.out[(size_t) t * g.d + o] = __float2bfloat16(v[n]);
-            }
+        const int t = t2 + (reg & 1);
+        if (o < g.d && t < g.T) {
+            if (g.residual != nullptr) v += __bfloat162float(g.residual[t * g.ldr + o]);
+            g.out[(size_t) t * g.d + o] = __float2bfloat16(v);
+        }
     }
     mx4::copies_wait(0);
 }
 
-// The layer's first launch: CTAs below E compute router outputs [T][E], the others a token's fragments each (8 NT of them, zeros from T on); zeros where
+// The layer's first launch: CTAs below E compute router outputs [T][E], the others a token's fragments each (8 of them, zeros from T on); zeros where
 // the next launch counts.
 __global__ void __launch_bounds__(GATE_NT) mx4_prepare_kernel(const bf16 * __restrict__ x, long long ldx, const float * __restrict__ w_router,
                                                               float * __restrict__ logits, uint4 * __restrict__ xf, int * __restrict__ sync, int n_sync, int T,
-                                                              int d, int E, int NT, int warm) {
+                                                              int d, int E, int warm) {
     __shared__ float red[GATE_NT / 32][GATE_TG];
     const bool router = (int) blockIdx.x < E;
     PDL_TRIGGER_TOP();
@@ -522,31 +484,29 @@ __global__ void __launch_bounds__(GATE_NT) mx4_prepare_kernel(const bf16 * __res
     for (int w = 0; w < GATE_NT / 32; ++w) top = max(top, __float_as_uint(red[w][0]));
     const int ex = mx4::top_exponent(top);
     const float unit = mx4::pow2(14 - ex);
-    if (threadIdx.x == 0) ((int *) (xf + (size_t) C * NT * 128))[n] = ex - 14;
+    if (threadIdx.x == 0) ((int *) (xf + (size_t) C * 128))[n] = ex - 14;
     for (int i = threadIdx.x; i < C * 16; i += GATE_NT) {          // eight columns
         const int p = i & 3, t = i >> 2 & 3, c = i >> 4;
-        xf[((c * NT + (n >> 3)) * 4 + p) * 32 + (n & 7) * 4 + t] = n < T ? mx4::frag_of(row, c * mx4::COLS + 32 * t + 8 * p, d, unit) : make_uint4(0u, 0u, 0u, 0u);
+        xf[(c * 4 + p) * 32 + n * 4 + t] = n < T ? mx4::frag_of(row, c * mx4::COLS + 32 * t + 8 * p, d, unit) : make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
 // Stages of chunks that fit, at most MAX_DEPTH (0: not one).
-template <int NT>
 int depth_of(int d, int slots, bool down) {
-    using L = Layout<NT>;
+    using L = Layout;
     for (int i = MAX_DEPTH; i > 0; --i)
         if ((down ? L::bytes(0, slots, 0, i) : L::bytes(d, slots, i, 0)) <= MOST_SMEM) return i;
     return 0;
 }
 
-template <int NT>
 int launch(const MoeArgs & a, cudaStream_t s) {
-    using L = Layout<NT>;
+    using L = Layout;
     static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
     MoeArgs g = a;
-    g.depth1 = depth_of<NT>(g.d, g.max_slots, false);
-    g.depth2 = depth_of<NT>(g.d, g.max_slots, true);
+    g.depth1 = depth_of(g.d, g.max_slots, false);
+    g.depth2 = depth_of(g.d, g.max_slots, true);
     // Warps that share 16 hidden units: whatever takes the fullest group the least time, in chunks of one warp (finishing a unit is worth one more).
-    // Four are enough to finish a unit of 16 tokens.
+    // Two finish a unit, and two more take turns with them.
     const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
     const long long units = (long long) g.max_slots * (g.F / 16);
     long long best = -1;
@@ -554,8 +514,8 @@ int launch(const MoeArgs & a, cudaStream_t s) {
         const long long groups = (long long) sms * (NW / gw), cost = (units + groups - 1) / groups * ((mx4::chunks(g.d) + gw - 1) / gw + 1);
         if (best < 0 || cost < best) { best = cost; g.gw = gw; }
     }
-    if (!jib::ensure_dyn_smem(mx4_moe_kernel<NT>, MOST_SMEM, attr_done)) return JIB_E_LAUNCH;
-    JIB_LAUNCH((mx4_moe_kernel<NT>), sms, THREADS, L::bytes(g.d, g.max_slots, g.depth1, g.depth2), s, g);
+    if (!jib::ensure_dyn_smem(mx4_moe_kernel, MOST_SMEM, attr_done)) return JIB_E_LAUNCH;
+    JIB_LAUNCH(mx4_moe_kernel, sms, THREADS, L::bytes(g.d, g.max_slots, g.depth1, g.depth2), s, g);
     return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH;
 }
 
@@ -569,16 +529,15 @@ extern "C" {
 // Whether the two-launch form takes a layer (else 0), and the sizes of its buffers: bytes of xf and of h, floats of part, ints of sync.
 JIB_EXPORT int jib_mx4_moe_sizes(int T, int d, int F, int E, int k, long long * sizes) {
     if (T < 1 || T > MAX_T || k < 1 || k > MAX_K || E < 1 || E > MAX_E || d % 32 || F % 32 || d < 32 || F < 32 || d > GATE_MAXC * GATE_NT * 8) return 0;
-    const int NT = T <= 8 ? 1 : 2;
     const long long slots = slots_of(T, k, E);
-    if ((NT == 1 ? depth_of<1>(d, (int) slots, false) : depth_of<2>(d, (int) slots, false)) == 0) return 0;
-    const long long tiles = slots * mx4::chunks(F) * NT;
+    if (depth_of(d, (int) slots, false) == 0) return 0;
+    const long long tiles = slots * mx4::chunks(F);
     const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148, groups = (d + 63) / 64;
     if (tiles * groups > (1 << 30) || slots * (F / 16) > (1 << 30)) return 0;
-    sizes[0] = (NT == 1 ? Layout<1>::frags(d) : Layout<2>::frags(d)) + 64;
+    sizes[0] = Layout::frags(d) + 32;
     sizes[1] = tiles * (mx4::FRAG + 64);
-    sizes[2] = (long long) (sms + 2 * groups) * THREADS * NT;
-    sizes[3] = 4 + slots * 16 + groups;
+    sizes[2] = (long long) (sms + 2 * groups) * THREADS;
+    sizes[3] = 4 + slots * 8 + groups;
     return 1;
 }
 
@@ -588,8 +547,7 @@ JIB_EXPORT int jib_mx4_moe_prepare(const void * x, long long ldx, const float * 
     if (w_router == nullptr) E = 0;
     if (T < 1 || T > MAX_T || E < 0 || E > MAX_E || d % 32 || d > GATE_MAXC * GATE_NT * 8 || (E > 0 && ldx != d)) return JIB_E_ARG;
     if (((uintptr_t) x | (uintptr_t) (ldx * 2) | (uintptr_t) xf) & 15) return JIB_E_ALIGN;
-    const int NT = T <= 8 ? 1 : 2;
-    JIB_LAUNCH((mx4_prepare_kernel), E + 8 * NT, GATE_NT, 0, (cudaStream_t) stream, (const bf16 *) x, ldx, w_router, logits, (uint4 *) xf, sync, n_sync, T, d, E, NT,
+    JIB_LAUNCH((mx4_prepare_kernel), E + 8, GATE_NT, 0, (cudaStream_t) stream, (const bf16 *) x, ldx, w_router, logits, (uint4 *) xf, sync, n_sync, T, d, E,
                jib::warm_for(T));
     return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH;
 }
@@ -609,12 +567,12 @@ JIB_EXPORT int jib_mx4_moe(const jib_mx4_moe_desc * m, void * stream) {
     a.xf = (const uint4 *) m->xf; a.residual = (const bf16 *) m->residual; a.logits = m->logits; a.bias = m->bias; a.ids = m->ids; a.wts = m->wts;
     a.gu = (const uint8_t *) m->gu; a.down = (const uint8_t *) m->down; a.gu_exp = m->gu_exp; a.down_exp = m->down_exp;
     a.max_slots = slots_of(m->T, m->k + m->n_shared, m->E);
-    a.h = (__half *) m->h; a.h_exp = (uint8_t *) m->h + (long long) a.max_slots * mx4::chunks(m->F) * (m->T <= 8 ? 1 : 2) * mx4::FRAG; a.part = m->part; a.out = (bf16 *) m->out; a.sync = m->sync; a.status = m->status;
+    a.h = (__half *) m->h; a.h_exp = (uint8_t *) m->h + (long long) a.max_slots * mx4::chunks(m->F) * mx4::FRAG; a.part = m->part; a.out = (bf16 *) m->out; a.sync = m->sync; a.status = m->status;
     a.ldr = m->ldr; a.gu_factors = m->gu_factors; a.down_factors = m->down_factors;
     a.T = m->T; a.d = m->d; a.F = m->F; a.E = m->E; a.k = m->k; a.n_group = m->n_group; a.topk_group = m->topk_group; a.norm = m->norm; a.sigmoid = m->sigmoid;
     a.n_shared = m->n_shared; a.group_top2 = m->group_top2; a.act = m->act; a.scale = m->scale;
     a.warm = jib::warm_enabled();
-    return m->T <= 8 ? launch<1>(a, (cudaStream_t) stream) : launch<2>(a, (cudaStream_t) stream);
+    return launch(a, (cudaStream_t) stream);
 }
 
 }  // extern "C"

@@ -46,9 +46,9 @@ __device__ __forceinline__ void copies_wait(int n) {
     else asm volatile("cp.async.wait_group 3;" ::: "memory");
 }
 
-// y[m] (row g: columns 2t, 2t + 1; row g + 8) += rows 16 m .. of a chunk x the same fragments: frag(n, p) gives this lane's 16 bytes.
-template <int NT, typename F>
-__device__ __forceinline__ void chunk_mma(const uint8_t * chunk, float (&y)[2][NT][4], F frag) {
+// y[m] (row g: columns 2t, 2t + 1; row g + 8) += rows 16 m .. of a chunk x the same fragments: frag(p) gives this lane's 16 bytes.
+template <typename F>
+__device__ __forceinline__ void chunk_mma(const uint8_t * chunk, float (&y)[2][4], F frag) {
     const int lane = threadIdx.x & 31;
     uint32_t s[2][2];
     uint4 q[2][2];
@@ -62,19 +62,14 @@ __device__ __forceinline__ void chunk_mma(const uint8_t * chunk, float (&y)[2][N
         }
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        uint4 v[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) v[n] = frag(n, p);
+        const uint4 v = frag(p);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             const uint4 & a = q[m][0], & b = q[m][1];
             uint32_t f[2][4];
             decode(p == 0 ? a.x : p == 1 ? a.y : p == 2 ? a.z : a.w, p == 0 ? b.x : p == 1 ? b.y : p == 2 ? b.z : b.w, s[m][0], s[m][1], f);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mma16816(y[m][n], f[0], v[n].x, v[n].y);
-                mma16816(y[m][n], f[1], v[n].z, v[n].w);
-            }
+            mma16816(y[m], f[0], v.x, v.y);
+            mma16816(y[m], f[1], v.z, v.w);
         }
     }
 }

@@ -323,7 +323,7 @@ def mx4_moe_ffn(x: torch.Tensor, residual: Optional[torch.Tensor], ids: torch.Te
                 act: str = "silu") -> torch.Tensor:
     """residual + sum over the choices of a token of wts * down(act(gate) * up), x's dtype; the hidden units are rounded to x's dtype.
 
-    ``ids`` int32, ``wts`` fp32 [tokens, k]; an id outside the experts counts for nothing.  ``residual`` may be None.  Up to 16 tokens run as one launch."""
+    ``ids`` int32, ``wts`` fp32 [tokens, k]; an id outside the experts counts for nothing.  ``residual`` may be None.  Up to 8 bf16 tokens run as two launches."""
     _check_moe(x, wgu, wd, residual, act, "mx4_moe_ffn")
     if ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape != wts.shape or ids.dtype != torch.int32 or wts.dtype != torch.float32 or \
             ids.device != x.device or wts.device != x.device:
@@ -336,7 +336,7 @@ def mx4_moe_layer(x: torch.Tensor, w_router: torch.Tensor, bias: Optional[torch.
                   sigmoid: bool, wgu: Mx4Weight, wd: Mx4Weight, n_shared: int = 0, group_top2: bool = False,
                   residual: Optional[torch.Tensor] = None, act: str = "silu") -> torch.Tensor:
     """A whole MoE layer: router, choice of experts, their products, weighted sum and residual.  The gate's arguments are those of ``moe_gate``; the
-    last ``n_shared`` experts of the weights take every token with weight 1.  Up to 16 bf16 tokens run as two launches."""
+    last ``n_shared`` experts of the weights take every token with weight 1.  Up to 8 bf16 tokens run as two launches."""
     _check_moe(x, wgu, wd, residual, act, "mx4_moe_layer")
     E = w_router.shape[0] if w_router.dim() == 2 else -1
     if w_router.dim() != 2 or w_router.shape[1] != x.shape[1] or E + n_shared != wgu.batch or n_shared < 0 or w_router.dtype != torch.float32 or \

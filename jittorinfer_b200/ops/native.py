@@ -174,7 +174,7 @@ def load():
     sig("jib_mx4_gemm_sizes", ll, i, i, i, i, C.POINTER(ll))
     L.jib_mx4_gemm_sizes.restype = None
     sig("jib_mx4_planes", vp, ll, ip, ip, vp, vp, ll, i, ip, i, vp)
-    sig("jib_mx4_pad", ip, ip, ip, i, i, i, ip, ip, ip, ip, vp)
+    sig("jib_mx4_sort", ip, i, i, i, ip, ip, ip, ip, vp)
     sig("jib_mx4_gemm", C.POINTER(Mx4Desc), vp, ip, fp, ip, vp)
     sig("jib_mx4_moe_sizes", i, i, i, i, i, C.POINTER(ll))
     sig("jib_mx4_moe_prepare", vp, ll, fp, fp, vp, ip, i, i, i, i, vp)

@@ -11,7 +11,7 @@ from . import native as nat
 from .mx4 import COLS, MX4_MAX_EXPERTS as MAX_EXPERTS, Mx4Tensor, Mx4Weight, scale_rows
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-FEW_TOKENS = 16                              # tokens of a layer that runs as one launch behind the router's
+FEW_TOKENS = 8                               # tokens of a layer that runs as one launch behind the router's
 PAD = 32                                     # rows of an expert are padded to in grouped products (csrc/kernels/mx4_gemm.cu)
 MAX_CHOICES = 32                             # of a token: what the gate takes (csrc/kernels/moe.cu)
 _NO_SWITCH = contextlib.nullcontext()
@@ -200,18 +200,18 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act, n_shared=0):
             m = nat.Mx4MoeDesc()
             m.ids, m.wts, m.k = ids.data_ptr(), wts.data_ptr(), k
             return _few_layer(x, residual, wgu, wd, sizes, act, m, None)
-        seg, src, dest = nat.moe_permute(ids, 0, wgu.batch)
         E, n = wgu.batch, T * k
         if x.dtype == torch.bfloat16:
             cap = (n + min(E, n) * (PAD - 1) + PAD - 1) // PAD * PAD
             table = torch.empty(2 * E + 1 + cap + n, dtype=torch.int32, device=x.device)       # first, count, token of each row, row of each pair
             first = table.data_ptr()
             count, row_src, pair_row = first + 4 * (E + 1), first + 4 * (2 * E + 1), first + 4 * (2 * E + 1 + cap)
-            nat._ck(nat.load().jib_mx4_pad(seg.data_ptr(), src.data_ptr(), dest.data_ptr(), E, n, cap, first, count, row_src, pair_row, nat._stream()), "mx4_pad")
+            nat._ck(nat.load().jib_mx4_sort(ids.data_ptr(), n, k, E, first, count, row_src, pair_row, nat._stream()), "mx4_sort")
             routed = T * (k - n_shared) * E // (E - n_shared)       # the rows were there no shared experts: what the tiles are chosen for
             h = _grouped(x, wgu, (first, count, cap), row_src, routed, act)
             y = _grouped(h, wd, (first, count, cap), None, routed, None)
             return nat.moe_combine(y, table[2 * E + 1 + cap:].view(T, k), wts, None, None if residual is None else residual.contiguous())
+        seg, src, dest = nat.moe_permute(ids, 0, E)
         h = _grouped_simt(x, wgu, seg, src, n, act)
         y = _grouped_simt(h, wd, seg, None, n, None)
         ok = (dest >= 0).to(wts.dtype) * wts

@@ -110,7 +110,7 @@ def test_model_on_the_kernels_and_engine_under_graphs():
     got = torch.cat([m.forward(_batch(t, p, "cuda"), cache).float().cpu() for t, p in ((toks, 0), (nxt, 70), (one, 79))])
     nat.check_status()
     ran = {k: nat.launches_by_name.get(k, 0) - n0.get(k, 0) for k in ("mx4_linear", "mx4_gateup", "mx4_moe", "mx4_grouped", "gemm_grouped")}
-    assert ran["mx4_moe"] == 4 and ran["mx4_grouped"] >= 2 and ran["gemm_grouped"] == 0, ran
+    assert ran["mx4_moe"] >= 2 and ran["mx4_grouped"] >= 4 and ran["gemm_grouped"] == 0, ran
     ref = torch.cat([o.forward(torch.tensor(t)) for t in (toks, nxt, one)])
     err = (got - ref).abs().amax(-1) / ref.abs().amax(-1)
     print(f"median row error {err.median().item():.4f}, rows within 3e-2 {(err <= 3e-2).float().mean().item():.3f}, worst {err.max().item():.3f}")

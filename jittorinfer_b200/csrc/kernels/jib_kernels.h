@@ -340,15 +340,12 @@ typedef struct jib_mx4_desc {
     long long ldx, ldo, ldr;
     int T, N, K, batch, max_rows;          // T: rows of the result; max_rows: the most that one matrix can have (tiled and grouped: the rows of all)
     int gated, act, out_f32, res_f32;
-    int x_rows;                // rows of x
 } jib_mx4_desc;
 JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, void * stream);
 // The same on the tensor cores, bf16 activations (mx4_gemm.cu): as planes first; grouped rows at padded places.
-JIB_EXPORT void jib_mx4_gemm_sizes(long long rows, int N, int K, int gated, int grouped, long long * sizes);
-JIB_EXPORT int jib_mx4_planes(const void * x, long long ldx, const int * src, const int * limit, void * planes, void * scales, long long rows, int K, int * zeros,
-                              int n_zeros, void * stream);
+JIB_EXPORT long long jib_mx4_gemm_scratch(long long rows, int N, int K, int gated, int grouped);
 JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, int * count, int * row_src, int * pair_row, void * stream);
-JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const int * count, float * part, int * counters, void * stream);
+JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, void * stream);
 // A mixture-of-experts layer for up to 8 tokens (mx4_moe.cu).
 typedef struct jib_mx4_moe_desc {
     const void * residual;                 // NULL, or bf16 [T][d], rows ldr elements apart

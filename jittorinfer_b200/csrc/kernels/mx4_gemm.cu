@@ -634,40 +634,32 @@ void shape_of(long long T, int m_tiles, int C, int * bn, int * splits) {
     *splits = s < 1 ? 1 : s;
 }
 
+// What a product needs besides its operands: planes and their scales; sums and counters of splits.
+struct Scratch {
+    long long scales, part, counters, bytes;             // (planes come first)
+    int bn = 0, splits = 1, tiles = 0;                   // of a dense product
+    Scratch(long long rows, int N, int K, bool gated, bool grouped) {
+        const int C = mx4::chunks(K), m_tiles = (mx4::rows_of(N, gated) + BM - 1) / BM;
+        scales = 2 * rows * C * 128;
+        part = scales + 2ll * C * scale_rows_of(rows) * 4;
+        counters = part;
+        if (!grouped) {
+            shape_of(rows, m_tiles, C, &bn, &splits);
+            if (splits > 1) {
+                tiles = (int) (m_tiles * ((rows + bn - 1) / bn));
+                counters = part + 4ll * tiles * splits * bn * BM;
+            }
+        }
+        bytes = counters + 4ll * tiles;
+    }
+};
+
 }  // namespace
 
 extern "C" {
 
-// Sizes of what a tiled product of `rows` rows needs: bytes of the planes, of their scales, floats of part and ints of counters (grouped: 0).
-JIB_EXPORT void jib_mx4_gemm_sizes(long long rows, int N, int K, int gated, int grouped, long long * sizes) {
-    const int C = mx4::chunks(K), m_tiles = (mx4::rows_of(N, gated != 0) + BM - 1) / BM;
-    sizes[0] = 2 * rows * C * 128;
-    sizes[1] = 2ll * C * scale_rows_of(rows) * 4;
-    sizes[2] = sizes[3] = 0;
-    if (!grouped) {
-        int bn, splits;
-        shape_of(rows, m_tiles, C, &bn, &splits);
-        const long long tiles = (long long) m_tiles * ((rows + bn - 1) / bn);
-        if (splits > 1) {
-            sizes[2] = tiles * splits * bn * BM;
-            sizes[3] = tiles;
-        }
-    }
-}
-
-// x [..][K] bf16 (rows ldx elements apart) as planes and scales of `rows` rows; zeros: n_zeros ints.
-JIB_EXPORT int jib_mx4_planes(const void * x, long long ldx, const int * src, const int * limit, void * planes, void * scales, long long rows, int K, int * zeros,
-                              int n_zeros, void * stream) {
-    if (rows <= 0) return 0;
-    if (K <= 0 || K % 32 || n_zeros < 0) return JIB_E_ARG;
-    if (((uintptr_t) x | (uintptr_t) (ldx * 2) | (uintptr_t) planes) & 15) return JIB_E_ALIGN;
-    const int C = mx4::chunks(K);
-    const int nx = (C * 16 + 255) / 256, th = ((C * 16 + nx - 1) / nx + 31) / 32 * 32, sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
-    const long long ny = (rows + ROWS - 1) / ROWS, most = ((long long) sms * 4096 / th + nx - 1) / nx;
-    JIB_LAUNCH((planes_kernel), dim3(nx, (unsigned) (ny < most ? ny : most < 65535 ? most : 65535)), th, 0, (cudaStream_t) stream, (const bf16 *) x, ldx, src, limit, (uint8_t *) planes,
-               (uint8_t *) scales, rows, scale_rows_of(rows), K, C, zeros, n_zeros);
-    return launched();
-}
+// Bytes that jib_mx4_gemm needs for `rows` rows.
+JIB_EXPORT long long jib_mx4_gemm_scratch(long long rows, int N, int K, int gated, int grouped) { return Scratch(rows, N, K, gated != 0, grouped != 0).bytes; }
 
 // ids [n / k][k]; first: E + 1 ints, count: E, row_src: room for n pairs and PAD - 1 more rows of each expert that has any, pair_row: n.
 JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, int * count, int * row_src, int * pair_row, void * stream) {
@@ -676,17 +668,18 @@ JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, i
     return launched();
 }
 
-// The tiled product: d->x are the planes (d->x_rows rows), x_scales their scales; grouped: d->seg = first, count (see jib_mx4_sort); part and counters (zeros) as
-// jib_mx4_gemm_sizes says.
-JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const int * count, float * part, int * counters, void * stream) {
+// The tiled product of bf16 rows d->x: as planes, then multiplied.  Grouped: d->seg = first, count, d->src = row_src of jib_mx4_sort (NULL: x in that order), T
+// rows at most.  scratch: jib_mx4_gemm_scratch(T, ..) bytes.
+JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, void * stream) {
     if (d->T <= 0) return 0;
-    if (d->N <= 0 || d->K <= 0 || d->K % 32 || d->batch < 1 || d->batch > MAX_E || d->T > d->x_rows || (d->seg != nullptr && (count == nullptr || d->residual != nullptr)))
-        return JIB_E_ARG;
-    if (((uintptr_t) x_scales | (uintptr_t) d->w_scales) & 15) return JIB_E_ALIGN;
+    if (d->N <= 0 || d->K <= 0 || d->K % 32 || d->batch < 1 || d->batch > MAX_E || (d->seg != nullptr && (count == nullptr || d->residual != nullptr))) return JIB_E_ARG;
+    if (((uintptr_t) d->x | (uintptr_t) (d->ldx * 2) | (uintptr_t) scratch | (uintptr_t) d->w_scales) & 15) return JIB_E_ALIGN;
+    const Scratch sc(d->T, d->N, d->K, d->gated != 0, d->seg != nullptr);
+    uint8_t * planes = (uint8_t *) scratch, * x_scales = planes + sc.scales;
     const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
     Args g;
-    g.w_scales = d->w_scales; g.x_scales = (const uint8_t *) x_scales; g.out = d->out; g.residual = d->residual; g.seg = d->seg; g.count = count;
-    g.part = part; g.counters = counters; g.status = d->status; g.ldo = d->ldo; g.ldr = d->ldr; g.x_rows = scale_rows_of(d->x_rows);
+    g.w_scales = d->w_scales; g.x_scales = x_scales; g.out = d->out; g.residual = d->residual; g.seg = d->seg; g.count = count;
+    g.part = (float *) (planes + sc.part); g.counters = (int *) (planes + sc.counters); g.status = d->status; g.ldo = d->ldo; g.ldr = d->ldr; g.x_rows = scale_rows_of(d->T);
     g.T = d->T; g.N = d->N; g.R = mx4::rows_of(d->N, d->gated != 0); g.C = mx4::chunks(d->K); g.E = d->batch;
     g.gated = d->gated; g.act = d->act; g.out_f32 = d->out_f32; g.res_f32 = d->res_f32;
     g.m_tiles = (g.R + BM - 1) / BM;
@@ -700,10 +693,10 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const
         g.t_tiles = 1;
         items = sms;
     } else {
-        shape_of(d->T, g.m_tiles, g.C, &g.bn, &g.splits);
+        g.bn = sc.bn;
+        g.splits = sc.splits;
         g.t_tiles = (d->T + g.bn - 1) / g.bn;
         items = (long long) g.m_tiles * g.t_tiles * g.splits;
-        if (g.splits > 1 && (part == nullptr || counters == nullptr)) return JIB_E_SCRATCH;
     }
     if (items > 0x3fffffff) return JIB_E_ARG;
     g.cps = g.bn <= 64 ? 2 : 1;
@@ -715,10 +708,15 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const void * x_scales, const
     CUtensorMap mw, mx;
     int rc = weights_map(&mw, d->w, g.R, (long long) g.C * d->batch);
     if (rc) return rc;
-    rc = planes_map(&mx, d->x, d->x_rows, (long long) g.C * 128, g.bn);
+    rc = planes_map(&mx, planes, d->T, (long long) g.C * 128, g.bn);
     if (rc) return rc;
     static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
     if (!jib::ensure_dyn_smem(mx4_gemm_kernel, MOST_SMEM - 5120, attr_done)) return JIB_E_LAUNCH;
+    // a thread keeps its eight columns and walks down the rows
+    const int nx = (g.C * 16 + 255) / 256, th = ((g.C * 16 + nx - 1) / nx + 31) / 32 * 32;
+    const long long ny = (d->T + ROWS - 1) / ROWS, most = ((long long) sms * 4096 / th + nx - 1) / nx;
+    JIB_LAUNCH((planes_kernel), dim3(nx, (unsigned) (ny < most ? ny : most < 65535 ? most : 65535)), th, 0, (cudaStream_t) stream, (const bf16 *) d->x, d->ldx, d->src,
+               d->seg != nullptr ? d->seg + d->batch : nullptr, planes, x_scales, (long long) d->T, g.x_rows, d->K, g.C, g.counters, sc.tiles);
     JIB_LAUNCH((mx4_gemm_kernel), (unsigned) (items < sms ? items : sms), THREADS, g.cps * (g.stages * stage_bytes(g.bn) + g.slots * slot_bytes(g.bn)) + 1024, (cudaStream_t) stream, mw, mx, g);
     return launched();
 }

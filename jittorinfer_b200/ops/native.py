@@ -104,7 +104,7 @@ class ScanDesc(C.Structure):
 class Mx4Desc(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("x", "w", "w_scales", "out", "residual", "seg", "src", "status")] + \
                [(n, C.c_longlong) for n in ("ldx", "ldo", "ldr")] + \
-               [(n, C.c_int) for n in ("T", "N", "K", "batch", "max_rows", "gated", "act", "out_f32", "res_f32", "x_rows")]
+               [(n, C.c_int) for n in ("T", "N", "K", "batch", "max_rows", "gated", "act", "out_f32", "res_f32")]
 
 
 class Mx4MoeDesc(C.Structure):
@@ -171,11 +171,10 @@ def load():
     sig("jib_mx4_pack", vp, vp, ll, vp, vp, vp, ip, i, i, i, i, i, vp)
     sig("jib_mx4_matmul", vp, vp, ll, vp, vp, ll, vp, ll, i, i, i, i, ip, vp)
     sig("jib_mx4_product_simt", C.POINTER(Mx4Desc), vp)
-    sig("jib_mx4_gemm_sizes", ll, i, i, i, i, C.POINTER(ll))
-    L.jib_mx4_gemm_sizes.restype = None
-    sig("jib_mx4_planes", vp, ll, ip, ip, vp, vp, ll, i, ip, i, vp)
+    sig("jib_mx4_gemm_scratch", ll, i, i, i, i)
+    L.jib_mx4_gemm_scratch.restype = ll
     sig("jib_mx4_sort", ip, i, i, i, ip, ip, ip, ip, vp)
-    sig("jib_mx4_gemm", C.POINTER(Mx4Desc), vp, ip, fp, ip, vp)
+    sig("jib_mx4_gemm", C.POINTER(Mx4Desc), ip, vp, vp)
     sig("jib_mx4_moe_sizes", i, i, i, i, i, C.POINTER(ll))
     sig("jib_mx4_moe_prepare", vp, ll, fp, fp, vp, ip, i, i, i, i, vp)
     sig("jib_mx4_moe", C.POINTER(Mx4MoeDesc), vp)

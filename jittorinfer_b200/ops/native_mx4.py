@@ -63,9 +63,9 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
-def _desc(x_rows: int, w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act: Optional[str]) -> "nat.Mx4Desc":
+def _desc(w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act: Optional[str]) -> "nat.Mx4Desc":
     d = nat.Mx4Desc()
-    d.x_rows, d.w, d.w_scales = x_rows, w.codes.data_ptr(), w.scales.data_ptr()
+    d.w, d.w_scales = w.codes.data_ptr(), w.scales.data_ptr()
     d.out, d.ldo, d.out_f32 = out.data_ptr(), out.stride(0), int(out.dtype == torch.float32)
     if residual is not None:
         d.residual, d.ldr, d.res_f32 = residual.data_ptr(), residual.stride(0), int(residual.dtype == torch.float32)
@@ -75,30 +75,20 @@ def _desc(x_rows: int, w: Mx4Weight, out: torch.Tensor, residual: Optional[torch
     return d
 
 
-_gemm_sizes: dict = {}        # (rows, n, k, gated, grouped) -> bytes of planes and of their scales, floats of part, ints of counters
+_scratch_bytes: dict = {}        # (rows, n, k, gated, grouped)
 
 
-def _sizes(*key: int):
-    if key not in _gemm_sizes:
-        if len(_gemm_sizes) > 4096:
-            _gemm_sizes.clear()
-        s = (C.c_longlong * 4)()
-        nat.load().jib_mx4_gemm_sizes(*key, s)
-        _gemm_sizes[key] = tuple(s)
-    return _gemm_sizes[key]
-
-
-def _tiled(d: "nat.Mx4Desc", x: torch.Tensor, rows: int, src: Optional[int], limit: Optional[int], count: Optional[int], what: str) -> None:
-    """bf16 activations as planes, then the tiled product.  ``src``, ``limit``, ``count``: addresses, of grouped rows."""
-    planes, scales, part, counters = _sizes(rows, d.N, d.K, d.gated, int(count is not None))
-    scratch = torch.empty(planes + scales + 4 * (part + counters), dtype=torch.uint8, device=x.device)
-    at = scratch.data_ptr()
-    L, stream = nat.load(), nat._stream()
-    at_scales, at_part = at + planes, at + planes + scales
-    at_counters = at_part + 4 * part
-    nat._ck(L.jib_mx4_planes(x.data_ptr(), x.stride(0), src, limit, at, at_scales, rows, d.K, at_counters, counters, stream), "mx4_planes")
-    d.x = at
-    nat._ck(L.jib_mx4_gemm(C.byref(d), at_scales, count, at_part, at_counters, stream), what)
+def _tiled(d: "nat.Mx4Desc", x: torch.Tensor, count: Optional[int], what: str) -> None:
+    """bf16 activations as planes, then the tiled product.  ``count``: address, of grouped rows."""
+    key = (d.T, d.N, d.K, d.gated, int(count is not None))
+    n = _scratch_bytes.get(key)
+    if n is None:
+        if len(_scratch_bytes) > 4096:
+            _scratch_bytes.clear()
+        n = _scratch_bytes[key] = nat.load().jib_mx4_gemm_scratch(*key)
+    scratch = torch.empty(n, dtype=torch.uint8, device=x.device)
+    d.x, d.ldx = x.data_ptr(), x.stride(0)
+    nat._ck(nat.load().jib_mx4_gemm(C.byref(d), count, scratch.data_ptr(), nat._stream()), what)
 
 
 def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dtype: torch.dtype, act: Optional[str]) -> torch.Tensor:
@@ -108,9 +98,9 @@ def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dty
         residual = residual.contiguous()
     if x.shape[0]:
         with _on(x):
-            d = _desc(x.shape[0], w, out, residual, act)
+            d = _desc(w, out, residual, act)
             if x.dtype == torch.bfloat16:
-                _tiled(d, x, x.shape[0], None, None, None, "mx4_gemm")
+                _tiled(d, x, None, "mx4_gemm")
             else:
                 d.x, d.ldx = x.data_ptr(), x.stride(0)
                 nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), nat._stream()), "mx4_product_simt")
@@ -120,7 +110,7 @@ def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dty
 def _grouped_simt(x: torch.Tensor, w: Mx4Weight, seg: torch.Tensor, src: Optional[torch.Tensor], rows: int, act: Optional[str]) -> torch.Tensor:
     """fp32 rows sorted by expert: expert e's are seg[e] .. seg[e + 1] - 1; row r is computed from x[src[r]] (without ``src`` x[r])."""
     out = torch.empty(rows, w.n, dtype=x.dtype, device=x.device)
-    d = _desc(x.shape[0], w, out, None, act)
+    d = _desc(w, out, None, act)
     d.x, d.ldx, d.seg, d.src, d.batch, d.max_rows = x.data_ptr(), x.stride(0), seg.data_ptr(), nat._p(src), w.batch, rows
     nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), nat._stream()), "mx4_grouped_simt")
     return out
@@ -130,9 +120,9 @@ def _grouped(x: torch.Tensor, w: Mx4Weight, pad, src: Optional[int], pairs: int,
     """bf16 rows in the padded order ``pad`` = (first, count, capacity); row r is computed from x[src[r]] (without ``src`` x[r])."""
     first, count, cap = pad
     out = torch.empty(cap, w.n, dtype=torch.bfloat16, device=x.device)
-    d = _desc(cap, w, out, None, act)
-    d.seg, d.batch, d.max_rows = first, w.batch, pairs
-    _tiled(d, x, cap, src, first + 4 * w.batch, count, "mx4_grouped")
+    d = _desc(w, out, None, act)
+    d.seg, d.src, d.batch, d.max_rows = first, src, w.batch, pairs
+    _tiled(d, x, count, "mx4_grouped")
     return out
 
 

@@ -404,10 +404,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
             const float2 wt = *(const float2 *) (wtab + slot * 8 + t2);
             const int e0 = __shfl_sync(0xffffffffu, h.top, 4 * t2), e1 = __shfl_sync(0xffffffffu, h.top, 4 * t2 + 4);
             const float w0 = wt.x * mx4::pow2_normal(e0 - BIAS - 14), w1 = wt.y * mx4::pow2_normal(e1 - BIAS - 14);
+            // (a token that has not chosen this expert takes nothing from it, were its weights NaN)
+            const int chosen = mask[slot] >> t2;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[m][i] += y[m][i] * r[2 * m + (i >> 1)] * (i & 1 ? w1 : w0);
+                for (int i = 0; i < 4; ++i)
+                    if (chosen & (i & 1 ? 2 : 1)) acc[m][i] += y[m][i] * r[2 * m + (i >> 1)] * (i & 1 ? w1 : w0);
         }
         float * mine = red + (gr & 1) * (L::RED / 4) + warp * L::SUMS * 32 + lane;
 #pragma unroll

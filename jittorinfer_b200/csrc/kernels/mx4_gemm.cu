@@ -49,23 +49,66 @@ struct Args {
     int * counters;                          // zeros, one a tile
     int * status;
     long long ldo, ldr, x_rows;
-    int T, N, R, C, E, bn, m_tiles, t_tiles, splits, stages, slots, cps, wide, gated, act, out_f32, res_f32;
+    int T, N, R, C, E, bn, m_tiles, t_tiles, splits, stages, slots, cps, gated, act, out_f32, res_f32;
 };
 
 __device__ __forceinline__ void st_cols4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_mxf8f6f4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t) accumulate)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t) accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t) accumulate)
+            : "memory");
 }
-// E2M1 x E4M3 with E8M0 scales, 128 x n, the scales in byte k of their words.
-__device__ __forceinline__ uint32_t idesc_e2m1_e4m3(int n, uint32_t k) {
-    return k << 4 | 5u << 7 | 0u << 10 | (uint32_t) (n >> 3) << 17 | 1u << 23 | (uint32_t) (BM >> 4) << 24 | k << 29;
+// The products so far done: an arrival at the barrier, of a pair at both CTAs' barriers at that place.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t * bar) {
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t) 3)
+                     : "memory");
+    else mma_commit(bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void alloc_all(uint32_t * slot) {
+    if (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        tmem_alloc(slot, 512);
+        tmem_relinquish();
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void free_all(uint32_t at) {
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(512) : "memory");
+    else tmem_dealloc(at, 512);
+}
+// An arrival at a barrier of the pair's first CTA.  What it tells of is in tensor memory (waited for, and fenced by tcgen05.fence) or came through a barrier of its
+// own: no other write waits for it.  (As a release for the cluster it took the scale warps 2 thousand cycles a stage.)
+template <bool PAIR>
+__device__ __forceinline__ void arrive_first(uint64_t * bar) {
+    if (PAIR) {
+        uint32_t at;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(bar)));
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
+    } else mbar_arrive(bar);
+}
+__device__ __forceinline__ void both_here() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+// E2M1 x E4M3 with E8M0 scales, m x n, the scales in byte k of their words.
+__device__ __forceinline__ uint32_t idesc_e2m1_e4m3(int m, int n, uint32_t k) {
+    return k << 4 | 5u << 7 | 0u << 10 | (uint32_t) (n >> 3) << 17 | 1u << 23 | (uint32_t) (m >> 4) << 24 | k << 29;
 }
 
 // A place in a ring of n and the parity of its round (divisions by the number of stages took the issuing thread as long as the products).
@@ -91,7 +134,7 @@ __device__ __forceinline__ void sums16(uint32_t at, int other, uint32_t (&v)[16]
     }
 }
 
-// What item i is: row tile m, first row of x, how many, chunks c0 .. c1 - 1, matrix, tile (for sums that meet).
+// What item i is: row tile m (of a pair: the first of two), first row of x, how many, chunks c0 .. c1 - 1, matrix, tile (for sums that meet).
 struct Item {
     int m, row0, rows, c0, c1, e, tile, split;
 };
@@ -129,6 +172,9 @@ __device__ __forceinline__ Item item_of(const Args & g, const int * first_tile, 
     return t;
 }
 
+template <bool PAIR>
+__device__ __forceinline__ int row_tile(int m, int rank) { return PAIR ? 2 * m + rank : m; }
+
 // How many chunks item i has.
 __device__ __forceinline__ int chunks_of(const Args & g, int i) {
     if (g.splits == 1) return g.C;
@@ -136,6 +182,7 @@ __device__ __forceinline__ int chunks_of(const Args & g, int i) {
     return (split + 1) * g.C / g.splits - split * g.C / g.splits;
 }
 
+template <bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Args g) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ int first_tile[MAX_E + 1], last_s;
@@ -146,22 +193,21 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
     uint64_t * full = bars, * empty = full + MAX_STAGES, * sl_full = empty + MAX_STAGES, * sf_full = sl_full + MAX_SLOTS, * sf_empty = sf_full + MAX_SLOTS,
              * acc_full = sf_empty + MAX_SLOTS, * acc_empty = acc_full + 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = g.stages, Q = g.slots, bn = g.bn, cps = g.cps;
-    uint8_t * scale_slots = tiles + S * cps * stage_bytes(bn);
-    const int SB = stage_bytes(bn), QB = slot_bytes(bn), plane = bn * 128, mn = g.wide ? 2 * bn : bn, sfc = scale_cols(mn), slab = 4 + (g.wide ? sfc : 2 * sfc);
+        const int rank = PAIR ? blockIdx.x & 1 : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x, xn = PAIR ? bn / 2 : bn;            // rows of x in this CTA's shared memory
+    const int SB = stage_bytes(xn), QB = slot_bytes(bn), plane = xn * 128, mn = PAIR ? bn : 2 * bn, sfc = scale_cols(mn), slab = PAIR ? 4 + 2 * sfc : 4 + sfc;
+    uint8_t * scale_slots = tiles + S * cps * SB;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < Q; ++i) { mbar_init(&sl_full[i], 1); mbar_init(&sf_full[i], 4); mbar_init(&sf_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 8); }
+        for (int i = 0; i < Q; ++i) { mbar_init(&sl_full[i], 1); mbar_init(&sf_full[i], PAIR ? 8 : 4); mbar_init(&sf_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], PAIR ? 16 : 8); }
         fence_barrier_init();
         prefetch_tmap(&tm_w);
         prefetch_tmap(&tm_x);
     }
-    if (warp == 2) {
-        tmem_alloc(&tmem_slot, 512);
-        tmem_relinquish();
-    }
+    if (warp == 2) alloc_all<PAIR>(&tmem_slot);
     tc_fence_before();
     __syncthreads();
+    if (PAIR) both_here();                   // barriers are arrived at from the other CTA
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     PDL_TRIGGER_TOP();
@@ -195,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             Ring r;
             bool ok = true;
 #pragma unroll 1
-            for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+            for (int i = first; i < items && ok; i += step) {
                 const Item t = item_of(g, first_tile, experts, i);
 #pragma unroll 1
                 for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(S)) {
@@ -205,9 +251,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 #pragma unroll 1
                     for (int j = 0; j < n; ++j) {
                         uint8_t * st = tiles + (s * cps + j) * SB;
-                        tma_load_3d(st, &tm_w, &full[s], 0, t.m * BM, t.e * g.C + c0 + j);
-                        tma_load_3d(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0, 0);
-                        tma_load_3d(st + A_BYTES + plane, &tm_x, &full[s], (c0 + j) * 128, t.row0, 1);
+                        tma_load_3d(st, &tm_w, &full[s], 0, row_tile<PAIR>(t.m, rank) * BM, t.e * g.C + c0 + j);
+                        tma_load_3d(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 0);
+                        tma_load_3d(st + A_BYTES + plane, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 1);
                     }
                 }
             }
@@ -221,9 +267,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             Ring r;
             bool ok = true;
 #pragma unroll 1
-            for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+            for (int i = first; i < items && ok; i += step) {
                 const Item t = item_of(g, first_tile, experts, i);
-                const int w_rows = min(BM, g.R - t.m * BM);
+                const int m0 = row_tile<PAIR>(t.m, rank) * BM, w_rows = max(0, min(BM, g.R - m0));      // (a pair's second tile may lie behind the last row)
 #pragma unroll 1
                 for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(Q)) {
                     const int q = r.at, n = min(cps, t.c1 - c0);
@@ -232,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 #pragma unroll 1
                     for (int c = c0; c < c0 + n; ++c) {
                         uint8_t * sc = scale_slots + (q * cps + c - c0) * QB;
-                        mx4::bulk_load(sc, g.w_scales + ((size_t) (t.e * g.C + c) * g.R + t.m * BM) * 4, w_rows * 4, &sl_full[q]);
+                        if (!PAIR || w_rows > 0) mx4::bulk_load(sc, g.w_scales + ((size_t) (t.e * g.C + c) * g.R + m0) * 4, w_rows * 4, &sl_full[q]);
                         mx4::bulk_load(sc + SA_BYTES, g.x_scales + ((size_t) c * g.x_rows + t.row0) * 4, bn * 4, &sl_full[q]);
                         mx4::bulk_load(sc + SA_BYTES + bn * 4, g.x_scales + ((size_t) (g.C + c) * g.x_rows + t.row0) * 4, bn * 4, &sl_full[q]);
                     }
@@ -243,14 +289,14 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (elect_one()) {
+        if ((!PAIR || rank == 0) && elect_one()) {
             Ring r, rq;
             int j = 0;
             bool ok = true;
             const uint64_t desc0 = desc_k_sw128(smem_u32(tiles));
-            const uint32_t id0 = idesc_e2m1_e4m3(mn, 0), lo = (uint32_t) plane >> 4;
+            const uint32_t id0 = idesc_e2m1_e4m3(PAIR ? 2 * BM : BM, mn, 0), lo = (uint32_t) plane >> 4;
 #pragma unroll 1
-            for (int i = blockIdx.x; i < items && ok; i += gridDim.x, ++j) {
+            for (int i = first; i < items && ok; i += step, ++j) {
                 const int n = chunks_of(g, i);
                 const int buf = j & 1;
                 if (!mbar_wait(&acc_empty[buf], (j >> 1 & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 62, i); break; }
@@ -270,23 +316,23 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     for (int j = 0; j < min(cps, n - c0); ++j) {
                         const uint64_t a = desc0 + (uint32_t) ((r.at * cps + j) * SB >> 4), b = a + (A_BYTES >> 4);
                         const uint32_t sf = sf0 + (rq.at * cps + j) * slab;
-                        if (g.wide) {
+                        if (!PAIR) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) mma_mxf8f6f4(acc, a + 2 * k, b + 2 * k, id0 + (k << 4) + ((uint32_t) k << 29), sf, sf + 4, more || k != 0);
+                            for (int k = 0; k < 4; ++k) mma_mxf8f6f4<PAIR>(acc, a + 2 * k, b + 2 * k, id0 + (k << 4) + ((uint32_t) k << 29), sf, sf + 4, more || k != 0);
                         } else {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 const uint32_t id = id0 + (k << 4) + ((uint32_t) k << 29);
-                                mma_mxf8f6f4(acc, a + 2 * k, b + 2 * k, id, sf, sf + 4, more || k != 0);
-                                mma_mxf8f6f4(acc, a + 2 * k, b + lo + 2 * k, id, sf, sf + 4 + sfc, true);
+                                mma_mxf8f6f4<PAIR>(acc, a + 2 * k, b + 2 * k, id, sf, sf + 4, more || k != 0);
+                                mma_mxf8f6f4<PAIR>(acc, a + 2 * k, b + lo + 2 * k, id, sf, sf + 4 + sfc, true);
                             }
                         }
                         more = true;
                     }
-                    mma_commit(&empty[r.at]);
-                    mma_commit(&sf_empty[rq.at]);
+                    commit<PAIR>(&empty[r.at]);
+                    commit<PAIR>(&sf_empty[rq.at]);
                 }
-                mma_commit(&acc_full[buf]);
+                commit<PAIR>(&acc_full[buf]);
             }
         }
         __syncwarp();
@@ -296,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         Ring r, rs;
         bool ok = true;
 #pragma unroll 1
-        for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+        for (int i = first; i < items && ok; i += step) {
             const int n = chunks_of(g, i);
 #pragma unroll 1
             for (int c0 = 0; c0 < n; c0 += cps, r.next(Q), rs.next(S)) {
@@ -310,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     const uint32_t dst = mine + (q * cps + c) * slab;
                     st_cols4(dst, sc[0], sc[32], sc[64], sc[96]);
 #pragma unroll 1
-                    for (int p = 0; p < 2 - g.wide; ++p) {
+                    for (int p = 0; p < (PAIR ? 2 : 1); ++p) {
                         const uint32_t * sx = sc + SA_BYTES / 4 + p * bn;
                         for (int j = 0; j < sfc; j += 4) {
                             uint32_t v[4];
@@ -325,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                 if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 67, i); break; }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sf_full[q]);
+                if (lane == 0) arrive_first<PAIR>(&sf_full[q]);
             }
         }
     } else if (warp >= 8) {
@@ -334,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         const uint32_t mine = tmem + ((uint32_t) q << 21);
         int j = 0;
 #pragma unroll 1
-        for (int i = blockIdx.x; i < items; i += gridDim.x, ++j) {
+        for (int i = first; i < items; i += step, ++j) {
             const Item t = item_of(g, first_tile, experts, i);
             const int buf = j & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], j >> 1 & 1))) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 65, i); break; }
@@ -342,12 +388,12 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             const uint32_t acc = mine + buf * mn;
             bool finish = true;
             float * part = g.part + ((size_t) t.tile * g.splits * bn) * BM + q * 32 + lane;
-            if (g.splits > 1) {
+            if (!PAIR && g.splits > 1) {
                 float * to = part + (size_t) t.split * bn * BM;
 #pragma unroll 1
                 for (int c = 16 * half; c < t.rows; c += 32) {
                     uint32_t v[16];
-                    sums16(acc + c, g.wide ? bn : 0, v);
+                    sums16(acc + c, PAIR ? 0 : bn, v);
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
                         if (c + k < t.rows) __stcg(to + (size_t) (c + k) * BM, __uint_as_float(v[k]));
@@ -363,11 +409,11 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                 asm volatile("bar.sync 1, 256;" ::: "memory");
             }
             // lane = row n of the tile (of pairs: 16 of the gate, 16 of the up matrix), 16 rows of x at a time
-            const int n = g.gated ? t.m * 64 + q * 16 + (lane & 15) : t.m * BM + q * 32 + lane;
+            const int m = row_tile<PAIR>(t.m, rank), n = g.gated ? m * 64 + q * 16 + (lane & 15) : m * BM + q * 32 + lane;
 #pragma unroll 1
             for (int c = 16 * half; c < t.rows && finish; c += 32) {
                 float y[16];
-                if (g.splits > 1) {
+                if (!PAIR && g.splits > 1) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) y[k] = 0.f;
 #pragma unroll 1
@@ -385,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     }
                 } else {
                     uint32_t v[16];
-                    sums16(acc + c, g.wide ? bn : 0, v);
+                    sums16(acc + c, PAIR ? 0 : bn, v);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) y[k] = __uint_as_float(v[k]);
                 }
@@ -424,12 +470,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            if (lane == 0) arrive_first<PAIR>(&acc_empty[buf]);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 2) tmem_dealloc(tmem, 512);
+    if (PAIR) both_here();                   // neither leaves while the other arrives at its barriers or multiplies its rows
+    if (warp == 2) free_all<PAIR>(tmem);
 }
 
 // ---- bf16 rows as two E4M3 planes ------------------------------------------------------------------------------------------------
@@ -612,26 +659,56 @@ int planes_map(CUtensorMap * out, const void * planes, long long rows, long long
                : JIB_E_TENSORMAP;
 }
 
-// Up to this many rows of x the planes are one operand (two buffers of sums and the scales fit in tensor memory).
+// Up to this many rows of x the planes are one operand (two buffers of sums and the scales fit in tensor memory); above, pairs of CTAs work on a tile.
 constexpr int MAX_WIDE = 96;
 
-// Rows of x in a tile and splits of K of a dense product.  What a chunk costs is its traffic with shared memory: 128 bytes written a row of either operand and
-// plane, and as many read by each instruction: in rows of x (512 bytes) w, and for the weights' tile 64, 96 where it is read for each plane.  1531 rows to
-// 2 x 10944, K 2048: 137 us with 192 rows, 139 us with 128.  Where the tiles leave SMs idle, K is split, four chunks a split at least.
-void shape_of(long long T, int m_tiles, int C, int * bn, int * splits) {
-    const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
+int sm_count() { return jib::sm_count() > 0 ? jib::sm_count() : 148; }
+
+// Pairs of CTAs that run at a time (0: not one).
+int pair_count() {
+    static std::atomic<int> known[jib::MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= jib::MAX_DEVICES) return 0;
+    int n = known[dev].load();
+    if (n == 0) {
+        static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
+        if (!jib::ensure_dyn_smem(mx4_gemm_kernel<true>, MOST_SMEM - 5120, attr_done)) return 0;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(sm_count() / 2 * 2);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = MOST_SMEM - 5120;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, mx4_gemm_kernel<true>, &cfg) != cudaSuccess) n = 0;
+        known[dev].store(n);
+    }
+    return n;
+}
+
+// Rows of x in a tile and splits of K of a dense product.  What a chunk costs a CTA is its traffic with shared memory: 128 bytes written a row of either operand
+// and plane, and as many read by each instruction.  In rows of x (512 bytes): w + 64 with the planes as one operand; in a pair w / 2 + 96, or w for its
+// products where that is more.  Where the tiles leave SMs idle, K is split, four chunks a split at least.
+void shape_of(long long T, int R, int C, int * bn, int * splits) {
+    const int sms = sm_count(), pairs = R > BM ? pair_count() : 0;
+    const long long m_tiles = (R + BM - 1) / BM;
     long long best = -1;
-    for (int w = T > 16 ? 32 : 16; w <= MAX_BN; w += 32) {
-        const long long tiles = (long long) m_tiles * ((T + w - 1) / w), cost = (tiles + sms - 1) / sms * (w + (w <= MAX_WIDE ? 64 : 96));
+    for (int w = T > 16 ? 32 : 16; w <= (pairs > 0 ? MAX_BN : MAX_WIDE); w += 32) {
+        const bool pair = w > MAX_WIDE;
+        const long long tiles = (pair ? (m_tiles + 1) / 2 : m_tiles) * ((T + w - 1) / w), at_once = pair ? pairs : sms;
+        const long long cost = (tiles + at_once - 1) / at_once * (!pair ? w + 64 : w > w / 2 + 96 ? w : w / 2 + 96);
         if (best < 0 || cost <= best) { best = cost; *bn = w; }
         if (w >= T) break;
         if (w == 16) w = 0;
     }
-    const long long tiles = (long long) m_tiles * ((T + *bn - 1) / *bn);
+    const long long tiles = m_tiles * ((T + *bn - 1) / *bn);
     int s = (int) (sms / tiles);
     if (s > C / 4) s = C / 4;
     if (s > 16) s = 16;
-    *splits = s < 1 ? 1 : s;
+    *splits = s < 1 || *bn > MAX_WIDE ? 1 : s;
 }
 
 // What a product needs besides its operands: planes and their scales; sums and counters of splits.
@@ -639,12 +716,12 @@ struct Scratch {
     long long scales, part, counters, bytes;             // (planes come first)
     int bn = 0, splits = 1, tiles = 0;                   // of a dense product
     Scratch(long long rows, int N, int K, bool gated, bool grouped) {
-        const int C = mx4::chunks(K), m_tiles = (mx4::rows_of(N, gated) + BM - 1) / BM;
+        const int C = mx4::chunks(K), R = mx4::rows_of(N, gated), m_tiles = (R + BM - 1) / BM;
         scales = 2 * rows * C * 128;
         part = scales + 2ll * C * scale_rows_of(rows) * 4;
         counters = part;
         if (!grouped) {
-            shape_of(rows, m_tiles, C, &bn, &splits);
+            shape_of(rows, R, C, &bn, &splits);
             if (splits > 1) {
                 tiles = (int) (m_tiles * ((rows + bn - 1) / bn));
                 counters = part + 4ll * tiles * splits * bn * BM;
@@ -676,7 +753,7 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
     if (((uintptr_t) d->x | (uintptr_t) (d->ldx * 2) | (uintptr_t) scratch | (uintptr_t) d->w_scales) & 15) return JIB_E_ALIGN;
     const Scratch sc(d->T, d->N, d->K, d->gated != 0, d->seg != nullptr);
     uint8_t * planes = (uint8_t *) scratch, * x_scales = planes + sc.scales;
-    const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148;
+    const int sms = sm_count();
     Args g;
     g.w_scales = d->w_scales; g.x_scales = x_scales; g.out = d->out; g.residual = d->residual; g.seg = d->seg; g.count = count;
     g.part = (float *) (planes + sc.part); g.counters = (int *) (planes + sc.counters); g.status = d->status; g.ldo = d->ldo; g.ldr = d->ldr; g.x_rows = scale_rows_of(d->T);
@@ -688,7 +765,8 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
         // an expert's rows on average and twice their spread: most experts then take one tile
         const float avg = (float) d->max_rows / d->batch;
         const int w = ((int) (avg + 2.f * sqrtf(avg)) + 31) / 32 * 32;
-        g.bn = w < 32 ? 32 : w > MAX_BN ? MAX_BN : w;
+        const int most = g.R > BM && pair_count() > 0 ? MAX_BN : MAX_WIDE;
+        g.bn = w < 32 ? 32 : w > most ? most : w;
         g.splits = 1;
         g.t_tiles = 1;
         items = sms;
@@ -698,26 +776,34 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
         g.t_tiles = (d->T + g.bn - 1) / g.bn;
         items = (long long) g.m_tiles * g.t_tiles * g.splits;
     }
+    const bool pair = g.bn > MAX_WIDE;
+    const int at_once = pair ? pair_count() : sms, xn = pair ? g.bn / 2 : g.bn;
+    if (pair) {
+        g.m_tiles = (g.m_tiles + 1) / 2;
+        items = d->seg != nullptr ? at_once : (long long) g.m_tiles * g.t_tiles;
+    }
     if (items > 0x3fffffff) return JIB_E_ARG;
     g.cps = g.bn <= 64 ? 2 : 1;
-    g.wide = g.bn <= MAX_WIDE;
-    g.slots = (512 - (g.wide ? 4 : 2) * g.bn) / (g.cps * (4 + (g.wide ? scale_cols(2 * g.bn) : 2 * scale_cols(g.bn))));
+    g.slots = pair ? (512 - 2 * g.bn) / (4 + 2 * scale_cols(g.bn)) : (512 - 4 * g.bn) / (g.cps * (4 + scale_cols(2 * g.bn)));
     if (g.slots > MAX_SLOTS) g.slots = MAX_SLOTS;
-    g.stages = (MOST_SMEM - 5120 - 1024 - g.slots * g.cps * slot_bytes(g.bn)) / (g.cps * stage_bytes(g.bn));        // (5 KB: barriers and tables)
+    g.stages = (MOST_SMEM - 5120 - 1024 - g.slots * g.cps * slot_bytes(g.bn)) / (g.cps * stage_bytes(xn));        // (5 KB: barriers and tables)
     if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
+    const size_t smem = g.cps * (g.stages * stage_bytes(xn) + g.slots * slot_bytes(g.bn)) + 1024;
     CUtensorMap mw, mx;
     int rc = weights_map(&mw, d->w, g.R, (long long) g.C * d->batch);
     if (rc) return rc;
-    rc = planes_map(&mx, planes, d->T, (long long) g.C * 128, g.bn);
+    rc = planes_map(&mx, planes, d->T, (long long) g.C * 128, xn);
     if (rc) return rc;
     static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
-    if (!jib::ensure_dyn_smem(mx4_gemm_kernel, MOST_SMEM - 5120, attr_done)) return JIB_E_LAUNCH;
+    if (!pair && !jib::ensure_dyn_smem(mx4_gemm_kernel<false>, MOST_SMEM - 5120, attr_done)) return JIB_E_LAUNCH;
     // a thread keeps its eight columns and walks down the rows
     const int nx = (g.C * 16 + 255) / 256, th = ((g.C * 16 + nx - 1) / nx + 31) / 32 * 32;
     const long long ny = (d->T + ROWS - 1) / ROWS, most = ((long long) sms * 4096 / th + nx - 1) / nx;
     JIB_LAUNCH((planes_kernel), dim3(nx, (unsigned) (ny < most ? ny : most < 65535 ? most : 65535)), th, 0, (cudaStream_t) stream, (const bf16 *) d->x, d->ldx, d->src,
                d->seg != nullptr ? d->seg + d->batch : nullptr, planes, x_scales, (long long) d->T, g.x_rows, d->K, g.C, g.counters, sc.tiles);
-    JIB_LAUNCH((mx4_gemm_kernel), (unsigned) (items < sms ? items : sms), THREADS, g.cps * (g.stages * stage_bytes(g.bn) + g.slots * slot_bytes(g.bn)) + 1024, (cudaStream_t) stream, mw, mx, g);
+    const unsigned grid = (unsigned) (items < at_once ? items : at_once);
+    if (pair) (void) jib::launch_pdl_pairs(mx4_gemm_kernel<true>, grid, dim3(THREADS), smem, (cudaStream_t) stream, mw, mx, g);
+    else JIB_LAUNCH((mx4_gemm_kernel<false>), grid, THREADS, smem, (cudaStream_t) stream, mw, mx, g);
     return launched();
 }
 

@@ -85,10 +85,8 @@ inline int warm_enabled() {
 constexpr int WARM_MAX_ROWS = 256;
 inline int warm_for(long long rows) { return (warm_enabled() && rows <= WARM_MAX_ROWS) ? 1 : 0; }
 
-// cluster_z > 1: consecutive blockIdx.z values form a thread-block cluster of that size.
 template <typename... P, typename... A>
-inline cudaError_t launch_pdl_cluster(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster_z,
-                                      A &&... args) {
+inline cudaError_t launch_pdl_cluster_dim(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, dim3 cluster, A &&... args) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = grid;
@@ -102,16 +100,29 @@ inline cudaError_t launch_pdl_cluster(void (*kern)(P...), dim3 grid, dim3 block,
         attr[n].val.programmaticStreamSerializationAllowed = 1;
         ++n;
     }
-    if (cluster_z > 1) {
+    if (cluster.x * cluster.y * cluster.z > 1) {
         attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = 1;
-        attr[n].val.clusterDim.y = 1;
-        attr[n].val.clusterDim.z = (unsigned) cluster_z;
+        attr[n].val.clusterDim.x = cluster.x;
+        attr[n].val.clusterDim.y = cluster.y;
+        attr[n].val.clusterDim.z = cluster.z;
         ++n;
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
+}
+
+// cluster_z > 1: consecutive blockIdx.z values form a thread-block cluster of that size.
+template <typename... P, typename... A>
+inline cudaError_t launch_pdl_cluster(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster_z,
+                                      A &&... args) {
+    return launch_pdl_cluster_dim(kern, grid, block, smem, stream, dim3(1, 1, (unsigned) cluster_z), std::forward<A>(args)...);
+}
+
+// `pairs` pairs of CTAs, consecutive in blockIdx.x (cta_group::2 wants them there).
+template <typename... P, typename... A>
+inline cudaError_t launch_pdl_pairs(void (*kern)(P...), unsigned pairs, dim3 block, size_t smem, cudaStream_t stream, A &&... args) {
+    return launch_pdl_cluster_dim(kern, dim3(2 * pairs), block, smem, stream, dim3(2), std::forward<A>(args)...);
 }
 
 template <typename... P, typename... A>

@@ -106,6 +106,18 @@ __device__ __forceinline__ void arrive_first(uint64_t * bar) {
     } else mbar_arrive(bar);
 }
 __device__ __forceinline__ void both_here() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+// A tile to this CTA's shared memory, told to the barrier of the pair's first CTA.
+template <bool PAIR>
+__device__ __forceinline__ void load(void * dst, const CUtensorMap * m, uint64_t * bar, int x, int y, int z) {
+    if (PAIR) {
+        uint32_t at;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(bar)));
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+            ::"r"(smem_u32(dst)), "l"(m), "r"(at), "r"(x), "r"(y), "r"(z)
+            : "memory");
+    } else tma_load_3d(dst, m, bar, x, y, z);
+}
 // E2M1 x E4M3 with E8M0 scales, m x n, the scales in byte k of their words.
 __device__ __forceinline__ uint32_t idesc_e2m1_e4m3(int m, int n, uint32_t k) {
     return k << 4 | 5u << 7 | 0u << 10 | (uint32_t) (n >> 3) << 17 | 1u << 23 | (uint32_t) (m >> 4) << 24 | k << 29;
@@ -247,18 +259,19 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                 for (int c0 = t.c0; c0 < t.c1; c0 += cps, r.next(S)) {
                     const int s = r.at, n = min(cps, t.c1 - c0);
                     if (!mbar_wait(&empty[s], r.round ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 61, i); ok = false; break; }
-                    mbar_expect_tx(&full[s], n * (A_BYTES / 2 + 2 * plane));      // (codes count as they are in memory)
+                    // (codes count as they are in memory; a pair's first CTA waits for both CTAs' tiles)
+                    if (rank == 0) mbar_expect_tx(&full[s], n * (PAIR ? 2 : 1) * (A_BYTES / 2 + 2 * plane));
 #pragma unroll 1
                     for (int j = 0; j < n; ++j) {
                         uint8_t * st = tiles + (s * cps + j) * SB;
-                        tma_load_3d(st, &tm_w, &full[s], 0, row_tile<PAIR>(t.m, rank) * BM, t.e * g.C + c0 + j);
-                        tma_load_3d(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 0);
-                        tma_load_3d(st + A_BYTES + plane, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 1);
+                        load<PAIR>(st, &tm_w, &full[s], 0, row_tile<PAIR>(t.m, rank) * BM, t.e * g.C + c0 + j);
+                        load<PAIR>(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 0);
+                        load<PAIR>(st + A_BYTES + plane, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 1);
                     }
                 }
             }
             // copies in flight end before the memory is given back (the last round's; a stage that was not asked for is not waited for long)
-            if (!ok)
+            if (!ok && rank == 0)
                 for (int i = 0; i < S; ++i) mbar_wait(&full[i], i < r.at ? r.round : r.round ^ 1);
         }
         __syncwarp();
@@ -305,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                 bool more = false;
 #pragma unroll 1
                 for (int c0 = 0; c0 < n; c0 += cps, r.next(S), rq.next(Q)) {
-                    if (!mbar_wait(&sf_full[rq.at], rq.round)) {      // the stage's tiles are there too
+                    if (!mbar_wait(&sf_full[rq.at], rq.round) || (PAIR && !mbar_wait(&full[r.at], r.round))) {      // (of a CTA alone the stage's tiles are there too)
                         jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 63, i);
                         ok = false;
                         break;
@@ -337,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         }
         __syncwarp();
     } else if (warp >= 4 && warp < 8) {
-        // scales to tensor memory; these warps also wait for the stage's tiles, so that the issuing thread waits once a stage
+        // scales to tensor memory; of a CTA alone these warps also wait for the stage's tiles, so that the issuing thread waits once a stage
         const uint32_t mine = sf0 + ((uint32_t) (warp & 3) << 21);
         Ring r, rs;
         bool ok = true;
@@ -367,8 +380,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     }
                 }
                 tmem_st_wait();
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[rs.at], rs.round));
-                if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 67, i); break; }
+                if (!PAIR) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&full[rs.at], rs.round));
+                    if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 67, i); break; }
+                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_first<PAIR>(&sf_full[q]);

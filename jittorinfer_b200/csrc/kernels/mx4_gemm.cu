@@ -367,16 +367,19 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                 for (int c = 0; c < min(cps, n - c0); ++c) {
                     const uint32_t * sc = (const uint32_t *) (scale_slots + (q * cps + c) * QB) + lane;
                     const uint32_t dst = mine + (q * cps + c) * slab;
-                    st_cols4(dst, sc[0], sc[32], sc[64], sc[96]);
-#pragma unroll 1
-                    for (int p = 0; p < (PAIR ? 2 : 1); ++p) {
-                        const uint32_t * sx = sc + SA_BYTES / 4 + p * bn;
-                        for (int j = 0; j < sfc; j += 4) {
-                            uint32_t v[4];
+                    constexpr int P = PAIR ? 2 : 1;
+                    uint32_t w[4], v[P][8];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) v[k] = (j + k) * 32 + lane < mn ? sx[(j + k) * 32] : 0u;
-                            st_cols4(dst + 4 + p * sfc + j, v[0], v[1], v[2], v[3]);
-                        }
+                    for (int k = 0; k < 4; ++k) w[k] = sc[k * 32];
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[p][k] = k * 32 + lane < mn ? sc[SA_BYTES / 4 + p * bn + k * 32] : 0u;
+                    st_cols4(dst, w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        st_cols4(dst + 4 + p * sfc, v[p][0], v[p][1], v[p][2], v[p][3]);
+                        if (sfc > 4) st_cols4(dst + 8 + p * sfc, v[p][4], v[p][5], v[p][6], v[p][7]);
                     }
                 }
                 tmem_st_wait();

@@ -4,15 +4,17 @@
 // The weights go to the tensor cores as they are: the tensor map of type 16U4_ALIGN16B spreads 4-bit codes over bytes in shared memory and
 // tcgen05.mma.kind::mxf8f6f4 takes them as E2M1 with their block's scale, 128 rows a tile.  So no instruction touches a weight.  Its other operand can have 8
 // bits at most; a bf16 activation is the sum of two E4M3 numbers, the first its value rounded to four significant bits, the second what is left, each
-// with a scale for 32 columns.  That sum is the bf16 value down to 2^-11 of the block's largest magnitude and within 2^-21 of the largest below.  Two
-// instructions multiply both planes into one accumulator; at twice the rate of bf16 that costs what a bf16 product costs.  Up to 96 rows of x both planes are one
-// operand of twice the rows, and the sums of the two meet in the epilogue: the weights' tile, the larger operand then, is read once.
+// with a scale for 32 columns.  That sum is the bf16 value down to 2^-11 of the block's largest magnitude and within 2^-21 of the largest below.  At
+// twice the rate of bf16 both planes cost what a bf16 product costs.
 //
-// A stage is a chunk of 128 columns (two for up to 64 rows of x: the issuing thread's waits cost as much as the products of a small chunk): codes (16 KB
-// in shared memory, 8 KB from memory) and both planes of up to 192 rows of x.  Scales have a longer ring of their own:
-// four warps move them from shared memory to tensor memory (column j of an operand: lane l of every quarter holds the four scale bytes of row 32 j + l)
-// while the stage they belong to is still on its way.  With few tiles K is split among CTAs; their sums meet in memory, and the one that comes last
-// adds them up in the order of K.
+// Up to 96 rows of x a CTA works alone, and both planes are one operand of twice the rows; the sums of the two meet in the epilogue.  Above, two CTAs
+// (cta_group::2) share a tile of 256 weights by up to 192 rows of x, of which each keeps half: the products are bound by their traffic with shared memory,
+// and the rows of x are half of it.  1531 rows by 2 x 10944 x 2048: 132 us with tiles of one CTA, 102 us with pairs (1.34 PFLOP/s).
+//
+// A stage is one to three chunks of 128 columns: codes (16 KB in shared memory, 8 KB from memory) and planes.  Scales have a ring of their own: one thread asks
+// for them, four warps move them to tensor memory (column j of an operand: lane l of every quarter holds the four scale bytes of row 32 j + l), well
+// ahead of the products.  Eight warps take the sums of the last tile while the products of the next run.  With few tiles K is split among CTAs; their sums
+// meet in memory, and the one that comes last adds them up in the order of K.
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                 bool more = false;
 #pragma unroll 1
                 for (int c0 = 0; c0 < n; c0 += cps, r.next(S), rq.next(Q)) {
-                    if (!mbar_wait(&sf_full[rq.at], rq.round) || (PAIR && !mbar_wait(&full[r.at], r.round))) {      // (of a CTA alone the stage's tiles are there too)
+                    if (!mbar_wait(&sf_full[rq.at], rq.round) || !mbar_wait(&full[r.at], r.round)) {
                         jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 63, i);
                         ok = false;
                         break;
@@ -350,15 +352,15 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         }
         __syncwarp();
     } else if (warp >= 4 && warp < 8) {
-        // scales to tensor memory; of a CTA alone these warps also wait for the stage's tiles, so that the issuing thread waits once a stage
+        // scales to tensor memory
         const uint32_t mine = sf0 + ((uint32_t) (warp & 3) << 21);
-        Ring r, rs;
+        Ring r;
         bool ok = true;
 #pragma unroll 1
         for (int i = first; i < items && ok; i += step) {
             const int n = chunks_of(g, i);
 #pragma unroll 1
-            for (int c0 = 0; c0 < n; c0 += cps, r.next(Q), rs.next(S)) {
+            for (int c0 = 0; c0 < n; c0 += cps, r.next(Q)) {
                 const int q = r.at;
                 ok = __all_sync(0xffffffffu, mbar_wait(&sl_full[q], r.round));
                 if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 64, i); break; }
@@ -383,10 +385,6 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     }
                 }
                 tmem_st_wait();
-                if (!PAIR) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&full[rs.at], rs.round));
-                    if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 67, i); break; }
-                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_first<PAIR>(&sf_full[q]);
@@ -801,7 +799,9 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
         items = d->seg != nullptr ? at_once : (long long) g.m_tiles * g.t_tiles;
     }
     if (items > 0x3fffffff) return JIB_E_ARG;
-    g.cps = g.bn <= 64 ? 2 : 1;
+    // Chunks of a stage: its waits and commits take the issuing thread as long as a few products.  8 rows by 12288 x 5120: 21 us with one, 16.5 with two, 14.3
+    // with three; 17 rows of the 66-expert layer 122 and 96 us with one and two, 107 with three (16 and 11 chunks are no multiple); 515 rows 191 and 160.
+    g.cps = g.bn <= 16 ? 3 : g.bn <= MAX_WIDE ? 2 : 1;
     g.slots = pair ? (512 - 2 * g.bn) / (4 + 2 * scale_cols(g.bn)) : (512 - 4 * g.bn) / (g.cps * (4 + scale_cols(2 * g.bn)));
     if (g.slots > MAX_SLOTS) g.slots = MAX_SLOTS;
     g.stages = (MOST_SMEM - 5120 - 1024 - g.slots * g.cps * slot_bytes(g.bn)) / (g.cps * stage_bytes(xn));        // (5 KB: barriers and tables)

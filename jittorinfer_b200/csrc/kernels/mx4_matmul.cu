@@ -21,7 +21,7 @@ constexpr int BOXES = 3, BOX_BYTES = (BM + MAX_BN) * 16;         // scales of tw
 constexpr int SMEM = STAGES * STAGE_BYTES + BOXES * BOX_BYTES + 1024 + 256;
 constexpr int SLAB = 12;                                         // columns of the scales of 128 columns of K: 4 of A, 8 of B
 constexpr int SF0 = 2 * MAX_BN;                                  // two accumulators, then the scales of each stage
-constexpr int THREADS = 384;                                     // producer, issuer, one idle, producer of scales; four scale warps; four epilogue warps
+constexpr int THREADS = 512;                                     // producer, issuer, one idle, producer of scales; four scale warps; eight epilogue warps
 static_assert(SF0 + STAGES * 2 * SLAB <= 512, "tensor memory");
 
 struct Args {
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&sf_full[i], 4); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 8); }
         for (int i = 0; i < BOXES; ++i) { mbar_init(&box_full[i], 1); mbar_init(&box_empty[i], 4); }
         fence_barrier_init();
         prefetch_tmap(&tm_as);
@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
         __syncwarp();
     } else if (warp == 1) {
         if (elect_one()) {
+            const uint64_t desc0 = desc_k_sw128(smem_u32(tiles));
             const uint32_t id0 = idesc_mxf4(g.bn, 0), id1 = idesc_mxf4(g.bn, 2);
             int it = 0, j = 0;
             bool ok = true;
@@ -113,11 +114,11 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
                     const uint32_t ph = it / STAGES & 1;
                     if (!mbar_wait(&full[s], ph) || !mbar_wait(&sf_full[s], ph)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 43, item); ok = false; break; }
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(tiles + s * STAGE_BYTES), b_addr = a_addr + A_BYTES, sf = tmem + SF0 + s * 2 * SLAB;
+                    const uint64_t a = desc0 + (uint32_t) (s * STAGE_BYTES >> 4), b = a + (A_BYTES >> 4);       // (descriptors count in 16 bytes)
+                    const uint32_t sf = tmem + SF0 + s * 2 * SLAB;
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        mma_mxf4(acc, desc_k_sw128(a_addr + q * 32), desc_k_sw128(b_addr + q * 32), q & 1 ? id1 : id0, sf + q / 2 * SLAB,
-                                 sf + q / 2 * SLAB + 4, (kb | q) != 0);
+                        mma_mxf4(acc, a + 2 * q, b + 2 * q, q & 1 ? id1 : id0, sf + q / 2 * SLAB, sf + q / 2 * SLAB + 4, (kb | q) != 0);
                     mma_commit(&empty[s]);
                 }
                 mma_commit(&acc_full[buf]);
@@ -186,24 +187,28 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(&sf_full[s]);
             }
     } else if (warp >= 8) {
+        // two warps a quarter of the rows, they take every second 16 tokens
         const uint32_t mine = tmem + ((uint32_t) (warp & 3) << 21);
+        const int half = (warp - 8) >> 2;
         int j = 0;
         for (int item = blockIdx.x; item < g.items; item += gridDim.x, ++j) {
             const int n = item % g.m_tiles * BM + (warp & 3) * 32 + lane, t0 = item / g.m_tiles * g.bn, buf = j & 1, cols = min(g.bn, g.T - t0);
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], j >> 1 & 1))) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 45, item); break; }
             tc_fence_after();
-            for (int c = 0; c < cols; c += 16) {
+            for (int c = 16 * half; c < cols; c += 32) {
                 uint32_t v[16];
                 tmem_ld16(mine + buf * MAX_BN + c, v);
                 tmem_ld_wait();
-                if (n < g.N)
+                if (n >= g.N) continue;
+                bf16 * to = (bf16 *) g.out + (long long) (t0 + c) * g.ldo + n;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (c + i >= cols) break;
-                        const long long at = (long long) (t0 + c + i) * g.ldo + n;
-                        if (g.out_f32) ((float *) g.out)[at] = __uint_as_float(v[i]);
-                        else ((bf16 *) g.out)[at] = __float2bfloat16(__uint_as_float(v[i]));
+                for (int i = 0; i < 16; ++i) {
+                    if (c + i < cols) {
+                        if (g.out_f32) ((float *) g.out)[(long long) (t0 + c + i) * g.ldo + n] = __uint_as_float(v[i]);
+                        else *to = __float2bfloat16(__uint_as_float(v[i]));
                     }
+                    to += g.ldo;
+                }
             }
             tc_fence_before();
             __syncwarp();

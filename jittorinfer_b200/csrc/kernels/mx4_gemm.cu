@@ -19,6 +19,7 @@
 #include <math.h>
 
 #include "jib_kernels.h"
+#include "mx4_pair.cuh"
 #include "mx4_stream.cuh"
 #include "pdl.cuh"
 #include "sm100.cuh"
@@ -73,52 +74,6 @@ __device__ __forceinline__ void mma_mxf8f6f4(uint32_t d, uint64_t a, uint64_t b,
             "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
             ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t) accumulate)
             : "memory");
-}
-// The products so far done: an arrival at the barrier, of a pair at both CTAs' barriers at that place.
-template <bool PAIR>
-__device__ __forceinline__ void commit(uint64_t * bar) {
-    if (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t) 3)
-                     : "memory");
-    else mma_commit(bar);
-}
-template <bool PAIR>
-__device__ __forceinline__ void alloc_all(uint32_t * slot) {
-    if (PAIR) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-        tmem_alloc(slot, 512);
-        tmem_relinquish();
-    }
-}
-template <bool PAIR>
-__device__ __forceinline__ void free_all(uint32_t at) {
-    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(512) : "memory");
-    else tmem_dealloc(at, 512);
-}
-// An arrival at a barrier of the pair's first CTA.  What it tells of is in tensor memory (waited for, and fenced by tcgen05.fence) or came through a barrier of its
-// own: no other write waits for it.  (As a release for the cluster it took the scale warps 2 thousand cycles a stage.)
-template <bool PAIR>
-__device__ __forceinline__ void arrive_first(uint64_t * bar) {
-    if (PAIR) {
-        uint32_t at;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(bar)));
-        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
-    } else mbar_arrive(bar);
-}
-__device__ __forceinline__ void both_here() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
-// A tile to this CTA's shared memory, told to the barrier of the pair's first CTA.
-template <bool PAIR>
-__device__ __forceinline__ void load(void * dst, const CUtensorMap * m, uint64_t * bar, int x, int y, int z) {
-    if (PAIR) {
-        uint32_t at;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(bar)));
-        asm volatile(
-            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-            ::"r"(smem_u32(dst)), "l"(m), "r"(at), "r"(x), "r"(y), "r"(z)
-            : "memory");
-    } else tma_load_3d(dst, m, bar, x, y, z);
 }
 // E2M1 x E4M3 with E8M0 scales, m x n, the scales in byte k of their words.
 __device__ __forceinline__ uint32_t idesc_e2m1_e4m3(int m, int n, uint32_t k) {
@@ -218,10 +173,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         prefetch_tmap(&tm_w);
         prefetch_tmap(&tm_x);
     }
-    if (warp == 2) alloc_all<PAIR>(&tmem_slot);
+    if (warp == 2) mx4::alloc_all<PAIR>(&tmem_slot);
     tc_fence_before();
     __syncthreads();
-    if (PAIR) both_here();                   // barriers are arrived at from the other CTA
+    if (PAIR) mx4::both_here();                   // barriers are arrived at from the other CTA
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     PDL_TRIGGER_TOP();
@@ -266,9 +221,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 #pragma unroll 1
                     for (int j = 0; j < n; ++j) {
                         uint8_t * st = tiles + (s * cps + j) * SB;
-                        load<PAIR>(st, &tm_w, &full[s], 0, row_tile<PAIR>(t.m, rank) * BM, t.e * g.C + c0 + j);
-                        load<PAIR>(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 0);
-                        load<PAIR>(st + A_BYTES + plane, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 1);
+                        mx4::load<PAIR>(st, &tm_w, &full[s], 0, row_tile<PAIR>(t.m, rank) * BM, t.e * g.C + c0 + j);
+                        mx4::load<PAIR>(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 0);
+                        mx4::load<PAIR>(st + A_BYTES + plane, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 1);
                     }
                 }
             }
@@ -344,10 +299,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                         }
                         more = true;
                     }
-                    commit<PAIR>(&empty[r.at]);
-                    commit<PAIR>(&sf_empty[rq.at]);
+                    mx4::commit<PAIR>(&empty[r.at]);
+                    mx4::commit<PAIR>(&sf_empty[rq.at]);
                 }
-                commit<PAIR>(&acc_full[buf]);
+                mx4::commit<PAIR>(&acc_full[buf]);
             }
         }
         __syncwarp();
@@ -387,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_first<PAIR>(&sf_full[q]);
+                if (lane == 0) mx4::arrive_first<PAIR>(&sf_full[q]);
             }
         }
     } else if (warp >= 8) {
@@ -486,13 +441,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) arrive_first<PAIR>(&acc_empty[buf]);
+            if (lane == 0) mx4::arrive_first<PAIR>(&acc_empty[buf]);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (PAIR) both_here();                   // neither leaves while the other arrives at its barriers or multiplies its rows
-    if (warp == 2) free_all<PAIR>(tmem);
+    if (PAIR) mx4::both_here();                   // neither leaves while the other arrives at its barriers or multiplies its rows
+    if (warp == 2) mx4::free_all<PAIR>(tmem);
 }
 
 // ---- bf16 rows as two E4M3 planes ------------------------------------------------------------------------------------------------
@@ -680,29 +635,10 @@ constexpr int MAX_WIDE = 96;
 
 int sm_count() { return jib::sm_count() > 0 ? jib::sm_count() : 148; }
 
-// Pairs of CTAs that run at a time (0: not one).
 int pair_count() {
     static std::atomic<int> known[jib::MAX_DEVICES];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= jib::MAX_DEVICES) return 0;
-    int n = known[dev].load();
-    if (n == 0) {
-        static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
-        if (!jib::ensure_dyn_smem(mx4_gemm_kernel<true>, MOST_SMEM - 5120, attr_done)) return 0;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(sm_count() / 2 * 2);
-        cfg.blockDim = dim3(THREADS);
-        cfg.dynamicSmemBytes = MOST_SMEM - 5120;
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = 2;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&n, mx4_gemm_kernel<true>, &cfg) != cudaSuccess) n = 0;
-        known[dev].store(n);
-    }
-    return n;
+    static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
+    return mx4::pair_count(mx4_gemm_kernel<true>, THREADS, MOST_SMEM - 5120, known, attr_done);
 }
 
 // Rows of x in a tile and splits of K of a dense product.  What a chunk costs a CTA is its traffic with shared memory: 128 bytes written a row of either operand

@@ -7,6 +7,7 @@
 // memory ahead of their stage.  (Read from global memory by those warps, stage by stage, they took 1200 clocks a stage, three times the products.)
 #include "sm100.cuh"
 #include "jib_kernels.h"
+#include "mx4_pair.cuh"
 #include "pdl.cuh"
 #include "tma_host.cuh"
 
@@ -15,14 +16,21 @@ namespace {
 using namespace sm100;
 typedef __nv_bfloat16 bf16;
 
-constexpr int BM = 128, MAX_BN = 208, STAGES = 4, KS = 256;       // weights a tile, tokens at most, stages, columns a stage
-constexpr int A_BYTES = BM * 128, B_BYTES = MAX_BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int BOXES = 3, BOX_BYTES = (BM + MAX_BN) * 16;         // scales of two stages
-constexpr int SMEM = STAGES * STAGE_BYTES + BOXES * BOX_BYTES + 1024 + 256;
+constexpr int BM = 128, KS = 256;                                // weights a tile, columns a stage
+constexpr int A_BYTES = BM * 128;
+constexpr int BOXES = 3;
 constexpr int SLAB = 12;                                         // columns of the scales of 128 columns of K: 4 of A, 8 of B
-constexpr int SF0 = 2 * MAX_BN;                                  // two accumulators, then the scales of each stage
-constexpr int THREADS = 512;                                     // producer, issuer, one idle, producer of scales; four scale warps; eight epilogue warps
-static_assert(SF0 + STAGES * 2 * SLAB <= 512, "tensor memory");
+constexpr int THREADS = 640;                                     // producer, issuer, one idle, producer of scales; eight scale warps; eight epilogue warps
+
+template <bool PAIR>
+struct Shape {
+    static constexpr int MAX_BN = PAIR ? 192 : 208, STAGES = PAIR ? 5 : 4;         // tokens of a tile at most
+    static constexpr int STAGE_BYTES = A_BYTES + (PAIR ? MAX_BN / 2 : MAX_BN) * 128;
+    static constexpr int BOX_BYTES = (BM + MAX_BN) * 16;                           // scales of two stages
+    static constexpr int SMEM = STAGES * STAGE_BYTES + BOXES * BOX_BYTES + 1024 + 256;
+    static constexpr int SF0 = 2 * MAX_BN;                                         // two accumulators, then the scales of each stage
+    static_assert(SF0 + STAGES * 2 * SLAB <= 512 && SMEM <= 227 * 1024, "tensor memory, shared memory");
+};
 
 struct Args {
     void * out;
@@ -34,21 +42,33 @@ struct Args {
 __device__ __forceinline__ void st_cols4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t) accumulate)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t) accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t) accumulate)
+            : "memory");
 }
-// E2M1 x E2M1 with E8M0 scales, 128 x n, the scales in bytes `half` and `half` + 1 of their words.
-__device__ __forceinline__ uint32_t idesc_mxf4(int n, uint32_t half) {
-    return half << 4 | 1u << 7 | 1u << 10 | (uint32_t) (n >> 3) << 17 | 1u << 23 | (uint32_t) (BM >> 4) << 24 | half << 29;
+// E2M1 x E2M1 with E8M0 scales, m x n, the scales in bytes `half` and `half` + 1 of their words.
+__device__ __forceinline__ uint32_t idesc_mxf4(int m, int n, uint32_t half) {
+    return half << 4 | 1u << 7 | 1u << 10 | (uint32_t) (n >> 3) << 17 | 1u << 23 | (uint32_t) (m >> 4) << 24 | half << 29;
 }
 
+template <bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                                                                 const __grid_constant__ CUtensorMap tm_as, const __grid_constant__ CUtensorMap tm_bs, const Args g) {
+    using S = Shape<PAIR>;
+    constexpr int STAGES = S::STAGES, STAGE_BYTES = S::STAGE_BYTES, BOX_BYTES = S::BOX_BYTES, SF0 = S::SF0, MAX_BN = S::MAX_BN;
     extern __shared__ uint8_t smem_raw[];
     uint8_t * tiles = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
     uint8_t * boxes = tiles + STAGES * STAGE_BYTES;
@@ -56,22 +76,23 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
              * acc_empty = acc_full + 2, * box_full = acc_empty + 2, * box_empty = box_full + BOXES;
     uint32_t * tmem_slot = (uint32_t *) (box_empty + BOXES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // of a pair each CTA has 128 rows of weights and keeps half of the tokens
+    const int rank = PAIR ? blockIdx.x & 1 : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const int rows = PAIR ? 2 * BM : BM, an = PAIR ? g.bn / 2 : g.bn;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&sf_full[i], 4); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 8); }
-        for (int i = 0; i < BOXES; ++i) { mbar_init(&box_full[i], 1); mbar_init(&box_empty[i], 4); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&sf_full[i], PAIR ? 8 : 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], PAIR ? 16 : 8); }
+        for (int i = 0; i < BOXES; ++i) { mbar_init(&box_full[i], 1); mbar_init(&box_empty[i], 8); }
         fence_barrier_init();
         prefetch_tmap(&tm_as);
         prefetch_tmap(&tm_bs);
         prefetch_tmap(&tm_a);
         prefetch_tmap(&tm_b);
     }
-    if (warp == 2) {
-        tmem_alloc(tmem_slot, 512);
-        tmem_relinquish();
-    }
+    if (warp == 2) mx4::alloc_all<PAIR>(tmem_slot);
     tc_fence_before();
     __syncthreads();
+    if (PAIR) mx4::both_here();              // barriers are arrived at from the other CTA
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     PDL_TRIGGER_TOP();
@@ -82,29 +103,29 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
         if (elect_one()) {
             int it = 0;
             bool ok = true;
-            for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
-                const int n0 = item % g.m_tiles * BM, t0 = item / g.m_tiles * g.bn;
+            for (int item = first; item < g.items && ok; item += step) {
+                const int n0 = item % g.m_tiles * rows + rank * BM, t0 = item / g.m_tiles * g.bn;
                 for (int kb = 0; kb < n_stages; ++kb, ++it) {
                     const int s = it % STAGES;
                     if (!mbar_wait(&empty[s], (it / STAGES & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 41, item); ok = false; break; }
                     uint8_t * st = tiles + s * STAGE_BYTES;
-                    mbar_expect_tx(&full[s], A_BYTES + g.bn * 128);
-                    tma_load_2d(st, &tm_b, &full[s], kb * 128, n0);
-                    tma_load_2d(st + A_BYTES, &tm_a, &full[s], kb * 128, t0);
+                    if (rank == 0) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * (A_BYTES + an * 128));
+                    mx4::load<PAIR>(st, &tm_b, &full[s], kb * 128, n0);
+                    mx4::load<PAIR>(st + A_BYTES, &tm_a, &full[s], kb * 128, t0 + rank * an);
                 }
             }
             // copies in flight end before the memory is given back
-            if (!ok)
+            if (!ok && rank == 0)
                 for (int i = it - STAGES < 0 ? 0 : it - STAGES; i < it; ++i) mbar_wait(&full[i % STAGES], i / STAGES & 1);
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (elect_one()) {
+        if (rank == 0 && elect_one()) {
             const uint64_t desc0 = desc_k_sw128(smem_u32(tiles));
-            const uint32_t id0 = idesc_mxf4(g.bn, 0), id1 = idesc_mxf4(g.bn, 2);
+            const uint32_t id0 = idesc_mxf4(rows, g.bn, 0), id1 = idesc_mxf4(rows, g.bn, 2);
             int it = 0, j = 0;
             bool ok = true;
-            for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x, ++j) {
+            for (int item = first; item < g.items && ok; item += step, ++j) {
                 const int buf = j & 1;
                 if (!mbar_wait(&acc_empty[buf], (j >> 1 & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 42, item); break; }
                 tc_fence_after();
@@ -118,10 +139,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
                     const uint32_t sf = tmem + SF0 + s * 2 * SLAB;
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        mma_mxf4(acc, a + 2 * q, b + 2 * q, q & 1 ? id1 : id0, sf + q / 2 * SLAB, sf + q / 2 * SLAB + 4, (kb | q) != 0);
-                    mma_commit(&empty[s]);
+                        mma_mxf4<PAIR>(acc, a + 2 * q, b + 2 * q, q & 1 ? id1 : id0, sf + q / 2 * SLAB, sf + q / 2 * SLAB + 4, (kb | q) != 0);
+                    mx4::commit<PAIR>(&empty[s]);
                 }
-                mma_commit(&acc_full[buf]);
+                mx4::commit<PAIR>(&acc_full[buf]);
             }
         }
         __syncwarp();
@@ -129,8 +150,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
         if (elect_one()) {
             int it = 0;
             bool ok = true;
-            for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
-                const int n0 = item % g.m_tiles * BM, t0 = item / g.m_tiles * g.bn;
+            for (int item = first; item < g.items && ok; item += step) {
+                const int n0 = item % g.m_tiles * rows + rank * BM, t0 = item / g.m_tiles * g.bn;
                 for (int kb = 0; kb < n_stages; kb += 2, ++it) {
                     const int s = it % BOXES;
                     if (!mbar_wait(&box_empty[s], (it / BOXES & 1) ^ 1)) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 46, item); ok = false; break; }
@@ -143,35 +164,31 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
                 for (int i = it - BOXES < 0 ? 0 : it - BOXES; i < it; ++i) mbar_wait(&box_full[i % BOXES], i / BOXES & 1);
         }
         __syncwarp();
-    } else if (warp >= 4 && warp < 8) {
-        // scales of a stage: eight bytes a row
+    } else if (warp >= 4 && warp < 12) {
+        // scales of a stage, eight bytes a row: four warps take the even stages of a tile, four the odd ones
         const uint32_t mine = tmem + ((uint32_t) (warp & 3) << 21) + SF0;
-        const int valid = g.K / 32;
-        int it = 0, box = -1;
+        const int valid = g.K / 32, odd = (warp - 4) >> 2;
+        int it = odd, box = 0;
         bool ok = true;
-        for (int item = blockIdx.x; item < g.items && ok; item += gridDim.x)
-            for (int kb = 0; kb < n_stages; ++kb, ++it) {
+        for (int item = first; item < g.items && ok; item += step, it -= n_stages & 1)
+            for (int kb = odd; kb < n_stages + odd; kb += 2, it += 2, ++box) {          // (the odd ones' last turn may have a box and no stage)
                 const int s = it % STAGES, n = valid - kb * 8;
-                if ((kb & 1) == 0) {
-                    ++box;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&box_full[box % BOXES], box / BOXES & 1));
-                    if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 47, item); break; }
-                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&box_full[box % BOXES], box / BOXES & 1));
+                if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 47, item); break; }
                 // bytes behind the last block: 1 (the codes there are zero)
-                const uint64_t keep = n >= 8 ? ~0ull : (1ull << (8 * n)) - 1, ones = 0x7f7f7f7f7f7f7f7full & ~keep;
-                const uint8_t * rows = boxes + box % BOXES * BOX_BYTES + (kb & 1) * 8 + lane * 16;
+                const uint64_t keep = n >= 8 ? ~0ull : n <= 0 ? 0ull : (1ull << (8 * n)) - 1, ones = 0x7f7f7f7f7f7f7f7full & ~keep;
+                const uint8_t * at = boxes + box % BOXES * BOX_BYTES + odd * 8 + lane * 16;
                 uint2 v[12];
 #pragma unroll
                 for (int j = 0; j < 12; ++j) {
                     uint64_t w = 0;
-                    if (j < 4 || (j - 4) * 32 + lane < g.bn) w = *(const uint64_t *) (rows + j * 512);
+                    if (j < 4 || (j - 4) * 32 + lane < g.bn) w = *(const uint64_t *) (at + j * 512);
                     w = (w & keep) | ones;
                     v[j] = make_uint2((uint32_t) w, (uint32_t) (w >> 32));
                 }
-                if ((kb & 1) != 0 || kb == n_stages - 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&box_empty[box % BOXES]);
-                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&box_empty[box % BOXES]);
+                if (kb >= n_stages) continue;
                 ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (it / STAGES & 1) ^ 1));
                 if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 44, item); break; }
                 tc_fence_after();
@@ -184,15 +201,15 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sf_full[s]);
+                if (lane == 0) mx4::arrive_first<PAIR>(&sf_full[s]);
             }
-    } else if (warp >= 8) {
+    } else if (warp >= 12) {
         // two warps a quarter of the rows, they take every second 16 tokens
         const uint32_t mine = tmem + ((uint32_t) (warp & 3) << 21);
-        const int half = (warp - 8) >> 2;
+        const int half = (warp - 12) >> 2;
         int j = 0;
-        for (int item = blockIdx.x; item < g.items; item += gridDim.x, ++j) {
-            const int n = item % g.m_tiles * BM + (warp & 3) * 32 + lane, t0 = item / g.m_tiles * g.bn, buf = j & 1, cols = min(g.bn, g.T - t0);
+        for (int item = first; item < g.items; item += step, ++j) {
+            const int n = item % g.m_tiles * rows + rank * BM + (warp & 3) * 32 + lane, t0 = item / g.m_tiles * g.bn, buf = j & 1, cols = min(g.bn, g.T - t0);
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], j >> 1 & 1))) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 45, item); break; }
             tc_fence_after();
             for (int c = 16 * half; c < cols; c += 32) {
@@ -212,12 +229,19 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_matmul_kernel(const __grid_con
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            if (lane == 0) mx4::arrive_first<PAIR>(&acc_empty[buf]);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 2) tmem_dealloc(tmem, 512);
+    if (PAIR) mx4::both_here();              // neither leaves while the other arrives at its barriers or multiplies its rows
+    if (warp == 2) mx4::free_all<PAIR>(tmem);
+}
+
+int pair_count() {
+    static std::atomic<int> known[jib::MAX_DEVICES];
+    static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
+    return mx4::pair_count(mx4_matmul_kernel<true>, THREADS, Shape<true>::SMEM, known, attr_done);
 }
 
 }  // namespace
@@ -228,22 +252,29 @@ extern "C" JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_sc
     if (T <= 0) return 0;
     if (N <= 0 || K <= 0 || K % 32 || a_ld < K / 32 || b_ld < K / 32) return JIB_E_ARG;
     if (((uintptr_t) a_scales | (uintptr_t) b_scales | (uintptr_t) a_ld | (uintptr_t) b_ld) & 15) return JIB_E_ALIGN;
-    // The width of a token tile: the one whose rounds over the machine cost least (a tile's fixed part is worth some 24 tokens).
-    const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148, m_tiles = (N + BM - 1) / BM;
+    // The width of a token tile, of a CTA alone or a pair: whose rounds over the machine cost least.  A stage costs its traffic with shared memory: 128 bytes of
+    // each row written and read, of a pair half of the tokens'.
+    const int sms = jib::sm_count() > 0 ? jib::sm_count() : 148, tiles_n = (N + BM - 1) / BM, pairs = N > BM ? pair_count() : 0;
     int bn = 16;
+    bool pair = false;
     long long best = -1;
-    for (int w = 16; w <= MAX_BN; w += 16) {
-        const long long tiles = (long long) m_tiles * ((T + w - 1) / w), cost = (tiles + sms - 1) / sms * (w + 24);
-        if (best < 0 || cost <= best) { best = cost; bn = w; }
+    for (int w = 16; w <= Shape<false>::MAX_BN; w += 16) {
+        const long long tt = (T + w - 1) / w, cost = (tiles_n * tt + sms - 1) / sms * (w + BM);
+        if (best < 0 || cost <= best) { best = cost; bn = w; pair = false; }
+        if (pairs > 0 && w % 32 == 0 && w <= Shape<true>::MAX_BN) {
+            const long long both = ((tiles_n + 1) / 2 * tt + pairs - 1) / pairs * (w / 2 + BM);
+            if (both < best) { best = both; bn = w; pair = true; }
+        }
         if (w >= T) break;
     }
+    const int m_tiles = pair ? (tiles_n + 1) / 2 : tiles_n, at_once = pair ? pairs : sms;
     Args g;
     g.out = out; g.ldo = ldo; g.status = status; g.T = T; g.N = N; g.K = K; g.bn = bn; g.out_f32 = out_f32; g.m_tiles = m_tiles;
     const long long items = (long long) m_tiles * ((T + bn - 1) / bn);
     if (items > 0x3fffffff) return JIB_E_ARG;
     g.items = (int) items;
     CUtensorMap ma, mb;
-    int rc = jib::tma_rows_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a_codes, T, K / 2, K / 2, bn);
+    int rc = jib::tma_rows_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a_codes, T, K / 2, K / 2, pair ? bn / 2 : bn);
     if (rc) return rc;
     rc = jib::tma_rows_map(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, b_codes, N, K / 2, K / 2, BM);
     if (rc) return rc;
@@ -252,8 +283,13 @@ extern "C" JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_sc
     if (rc) return rc;
     rc = jib::tma_bytes_map(&mbs, b_scales, N, b_ld, 16, BM);
     if (rc) return rc;
-    static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
-    if (!jib::ensure_dyn_smem(mx4_matmul_kernel, SMEM, attr_done)) return JIB_E_LAUNCH;
-    JIB_LAUNCH((mx4_matmul_kernel), (unsigned) (items < sms ? items : sms), THREADS, SMEM, (cudaStream_t) stream, ma, mb, mas, mbs, g);
+    const unsigned grid = (unsigned) (items < at_once ? items : at_once);
+    if (pair) {
+        (void) jib::launch_pdl_pairs(mx4_matmul_kernel<true>, grid, dim3(THREADS), Shape<true>::SMEM, (cudaStream_t) stream, ma, mb, mas, mbs, g);
+    } else {
+        static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
+        if (!jib::ensure_dyn_smem(mx4_matmul_kernel<false>, Shape<false>::SMEM, attr_done)) return JIB_E_LAUNCH;
+        JIB_LAUNCH((mx4_matmul_kernel<false>), grid, THREADS, Shape<false>::SMEM, (cudaStream_t) stream, ma, mb, mas, mbs, g);
+    }
     return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH;
 }

@@ -458,11 +458,11 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
 }
-__device__ __forceinline__ float e4m3_value(uint32_t w, int i) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t) (w >> (8 * i) & 0xff), __NV_E4M3)));
+__device__ __forceinline__ float2 e4m3_values(uint32_t two) {
+    return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) two, __NV_E4M3)));
 }
 
-constexpr int ROWS = 2;                             // of a thread's columns, their loads in flight together
+constexpr int ROWS = 4;                             // of a thread's columns, their loads in flight together
 
 __global__ void __launch_bounds__(256) planes_kernel(const bf16 * __restrict__ x, long long ldx, const int * __restrict__ src, const int * __restrict__ limit,
                                                      uint8_t * __restrict__ planes, uint8_t * __restrict__ scales, long long rows, long long scale_rows, int K, int C,
@@ -503,9 +503,10 @@ __global__ void __launch_bounds__(256) planes_kernel(const bf16 * __restrict__ x
             hi.x = e4m3x4(z[0], z[1], z[2], z[3]);
             hi.y = e4m3x4(z[4], z[5], z[6], z[7]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                z[j] = (z[j] - e4m3_value(hi.x, j)) * 16.f;
-                z[4 + j] = (z[4 + j] - e4m3_value(hi.y, j)) * 16.f;
+            for (int j = 0; j < 8; j += 2) {
+                const float2 f = e4m3_values((j < 4 ? hi.x : hi.y) >> (j & 2) * 8);
+                z[j] = (z[j] - f.x) * 16.f;
+                z[j + 1] = (z[j + 1] - f.y) * 16.f;
             }
             lo.x = e4m3x4(z[0], z[1], z[2], z[3]);
             lo.y = e4m3x4(z[4], z[5], z[6], z[7]);

@@ -103,6 +103,14 @@ __device__ __forceinline__ void sums16(uint32_t at, int other, uint32_t (&v)[16]
     }
 }
 
+// Named barrier 1 of the eight epilogue warps, and their decision: true when `ok` is for every thread.
+__device__ __forceinline__ bool all_of_256(bool ok) {
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((uint32_t) ok) : "memory");
+    return all != 0;
+}
+
 // What item i is: row tile m (of a pair: the first of two), first row of x, how many, chunks c0 .. c1 - 1, matrix, tile (for sums that meet).
 struct Item {
     int m, row0, rows, c0, c1, e, tile, split;
@@ -354,7 +362,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         for (int i = first; i < items; i += step, ++j) {
             const Item t = item_of(g, first_tile, experts, i);
             const int buf = j & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], j >> 1 & 1))) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 65, i); break; }
+            bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], j >> 1 & 1));
+            if (!PAIR && g.splits > 1) ok = all_of_256(ok);          // (they meet below)
+            if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 65, i); break; }
             tc_fence_after();
             const uint32_t acc = mine + buf * mn;
             bool finish = true;
@@ -655,7 +665,6 @@ void shape_of(long long T, int R, int C, int * bn, int * splits) {
         const long long cost = (tiles + at_once - 1) / at_once * (!pair ? w + 64 : w > w / 2 + 96 ? w : w / 2 + 96);
         if (best < 0 || cost <= best) { best = cost; *bn = w; }
         if (w >= T) break;
-        if (w == 16) w = 0;
     }
     const long long tiles = m_tiles * ((T + *bn - 1) / *bn);
     int s = (int) (sms / tiles);

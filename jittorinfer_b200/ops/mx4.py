@@ -344,7 +344,7 @@ def mx4_moe_layer(x: torch.Tensor, w_router: torch.Tensor, bias: Optional[torch.
         raise ValueError(f"mx4_moe_layer: router {tuple(w_router.shape)} {w_router.dtype} and {n_shared} shared experts for {wgu.batch} of width {x.shape[1]}")
     if bias is not None and (tuple(bias.shape) != (E,) or bias.dtype != torch.float32 or bias.device != x.device):
         raise ValueError(f"mx4_moe_layer: bias {tuple(bias.shape)} {bias.dtype} for {E} experts")
-    if not 1 <= k <= E or n_group < 1 or E % n_group or not 1 <= topk_group <= n_group:
+    if k < 1 or n_group < 1 or E % n_group or not 1 <= topk_group <= n_group or k > topk_group * (E // n_group):
         raise ValueError(f"mx4_moe_layer: {k} of {E} experts in {topk_group} of {n_group} groups")
     n = _native(x)
     if n:

@@ -216,7 +216,6 @@ def moe_layer(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, w
     T, d = x.shape
     if T == 0:
         return torch.empty_like(x)
-    w_router, bias = w_router.contiguous(), None if bias is None else bias.contiguous()
     if k + n_shared > MAX_CHOICES or wgu.batch > MAX_EXPERTS or n_group > 32:
         raise ValueError(f"mx4_moe_layer: {k} + {n_shared} of {wgu.batch} experts in {n_group} groups; at most {MAX_CHOICES} of {MAX_EXPERTS} in 32")
     with _on(x):

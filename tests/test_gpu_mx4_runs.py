@@ -72,6 +72,18 @@ def test_an_expert_that_is_not_a_number_touches_only_those_who_chose_it(nat, T):
 
 
 @pytest.mark.parametrize("T", [3, 20])
+@pytest.mark.parametrize("gate", [(2, 1, 1, 1.0, False, False), (2, 4, 2, 1.0, True, True)])
+def test_a_row_that_is_not_a_number_in_a_layer(nat, T, gate):
+    wgu, wd, *_ = experts(8, 128, 64)
+    x, router = randn(T, 128, seed=1, dtype=torch.bfloat16), randn(8, 128, seed=3, scale=0.1)
+    clean = ops.mx4_moe_layer(x, router, None, *gate, wgu, wd)
+    x[1, 7] = float("nan")
+    got = ops.mx4_moe_layer(x, router, None, *gate, wgu, wd)
+    others = torch.arange(T, device=DEV) != 1
+    assert torch.equal(got[others], clean[others]) and bool(got[1].isnan().all())
+
+
+@pytest.mark.parametrize("T", [3, 20])
 def test_router_and_rows_with_strides(nat, T):
     E, d, F = 8, 128, 64
     wgu, wd, *_ = experts(E, d, F)

@@ -131,6 +131,7 @@ def refusals():
         "experts without a router row": lambda: layer(n_shared=1),
         "more choices than experts": lambda: layer(k=5),
         "uneven groups": lambda: layer(n_group=3),
+        "more choices than the kept groups have": lambda: layer(n_group=4, topk_group=1),
         "bias": lambda: layer(bias=torch.zeros(3)),
     }
 

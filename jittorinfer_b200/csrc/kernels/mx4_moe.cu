@@ -45,7 +45,7 @@ struct MoeArgs {
                                              // [slots][8], pieces done of each 64 rows
     int * status;
     long long ldr;
-    int T, max_slots, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act, gw, depth1, depth2, warm;
+    int T, max_slots, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act, gw, depth1, depth2;
     float scale;
 };
 
@@ -103,9 +103,6 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     if (threadIdx.x < 4 * KNOWN) drawn[threadIdx.x] = -1;
     __syncthreads();
     PDL_TRIGGER_TOP();
-    if (g.warm && g.logits != nullptr && warp == 0)      // the choice's code (33 KB) comes to the SM while the launch before this one runs
-        gate_token(nullptr, nullptr, nullptr, nullptr, 0, g.E - g.n_shared, g.k, g.n_group, g.topk_group, g.scale, g.norm, g.sigmoid, g.n_shared, g.group_top2,
-                   red, red + MAX_E, ids_s, wts_s, true);
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
     if (warp % g.gw == 0 && lane < AHEAD) drawn[warp / g.gw * KNOWN + lane] = (long long) lane << 32 | atomicAdd(g.sync, 1);
     if (threadIdx.x == THREADS - 1) {
@@ -130,8 +127,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     __syncthreads();
     if (warp == 0) {
         int n = 0;
-#pragma unroll 1
-        for (int e = lane; e < MAX_E; e += 32) {
+#pragma unroll 4
+        for (int e = lane; e < (g.E + 31) / 32 * 32; e += 32) {
             const bool hit = slot_of[e] != 0;
             const unsigned m = __ballot_sync(0xffffffffu, hit);
             const int s = n + __popc(m & ((1u << lane) - 1));
@@ -140,15 +137,23 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
             n += __popc(m);
         }
         if (lane == 0) word[0] = n;
-        __syncwarp();
-        if (lane < g.T)
-#pragma unroll 1
-            for (int j = 0; j < kk; ++j) {
-                const int e = ids_s[lane * kk + j];
-                if ((unsigned) e >= (unsigned) g.E) continue;
-                wtab[slot_of[e] * 8 + lane] += wts_s[lane * kk + j];
-                atomicOr(&mask[slot_of[e]], 1 << lane);
+    }
+    __syncthreads();
+    // a thread a choice; of an expert that a token chose several times the first adds the weights up, in their order
+    for (int i = threadIdx.x; i < g.T * kk; i += THREADS) {
+        const int e = ids_s[i], t = i / kk;
+        if ((unsigned) e >= (unsigned) g.E) continue;
+        float w = 0.f;
+        bool repeated = false;
+#pragma unroll 4
+        for (int j = t * kk; j < (t + 1) * kk; ++j)
+            if (ids_s[j] == e) {
+                w += wts_s[j];
+                repeated |= j < i;
             }
+        if (repeated) continue;
+        wtab[slot_of[e] * 8 + t] = w;
+        atomicOr(&mask[slot_of[e]], 1 << t);
     }
     __syncthreads();
     const int slots = word[0], C1 = mx4::chunks(g.d), C2 = mx4::chunks(g.F), RB1 = g.F / 16, G = gridDim.x, U = slots * RB1;
@@ -460,12 +465,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
 // the next launch counts.
 __global__ void __launch_bounds__(GATE_NT) mx4_prepare_kernel(const bf16 * __restrict__ x, long long ldx, const float * __restrict__ w_router,
                                                               float * __restrict__ logits, uint4 * __restrict__ xf, int * __restrict__ sync, int n_sync, int T,
-                                                              int d, int E, int warm) {
+                                                              int d, int E) {
     __shared__ float red[GATE_NT / 32][GATE_TG];
     const bool router = (int) blockIdx.x < E;
     PDL_TRIGGER_TOP();
-    // the code and this expert's row come to the SM; x is not there yet, the router's first values stand in for it
-    if (warm && router) router_rows((const bf16 *) w_router, w_router, nullptr, 0.f, nullptr, logits, 0, 1, 1, d, E, blockIdx.x, red, nullptr, true);
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
     for (int i = blockIdx.x * GATE_NT + threadIdx.x; i < n_sync; i += gridDim.x * GATE_NT) sync[i] = 0;
     if (router) {
@@ -550,8 +553,7 @@ JIB_EXPORT int jib_mx4_moe_prepare(const void * x, long long ldx, const float * 
     if (w_router == nullptr) E = 0;
     if (T < 1 || T > MAX_T || E < 0 || E > MAX_E || d % 32 || d > GATE_MAXC * GATE_NT * 8 || (E > 0 && ldx != d)) return JIB_E_ARG;
     if (((uintptr_t) x | (uintptr_t) (ldx * 2) | (uintptr_t) xf) & 15) return JIB_E_ALIGN;
-    JIB_LAUNCH((mx4_prepare_kernel), E + 8, GATE_NT, 0, (cudaStream_t) stream, (const bf16 *) x, ldx, w_router, logits, (uint4 *) xf, sync, n_sync, T, d, E,
-               jib::warm_for(T));
+    JIB_LAUNCH((mx4_prepare_kernel), E + 8, GATE_NT, 0, (cudaStream_t) stream, (const bf16 *) x, ldx, w_router, logits, (uint4 *) xf, sync, n_sync, T, d, E);
     return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH;
 }
 
@@ -574,7 +576,6 @@ JIB_EXPORT int jib_mx4_moe(const jib_mx4_moe_desc * m, void * stream) {
     a.ldr = m->ldr; a.gu_factors = m->gu_factors; a.down_factors = m->down_factors;
     a.T = m->T; a.d = m->d; a.F = m->F; a.E = m->E; a.k = m->k; a.n_group = m->n_group; a.topk_group = m->topk_group; a.norm = m->norm; a.sigmoid = m->sigmoid;
     a.n_shared = m->n_shared; a.group_top2 = m->group_top2; a.act = m->act; a.scale = m->scale;
-    a.warm = jib::warm_enabled();
     return launch(a, (cudaStream_t) stream);
 }
 

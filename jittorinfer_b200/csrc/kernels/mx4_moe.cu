@@ -182,22 +182,27 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
         };
         // Asks for this warp's next chunks: of unit after unit the chunks wg, wg + gw .., at most two units ahead; and for the exponents of a unit's rows.
         int ia = 0, ka = wg, at = 0, ua = 0;
-        long long src = -1;                 // the first chunk's row among all
+        const uint8_t * codes = nullptr, * factors = nullptr;           // of this lane's next 16 bytes (NULL: of a unit not begun)
+        const size_t step = (size_t) g.gw * R1;
         auto ask = [&] {
-            if (src < 0 && ua < U) ua = unit(ia);
+            if (codes == nullptr && ua < U) ua = unit(ia);
             if (ua < U && ka < C1) {
-                if (src < 0) {
+                if (codes == nullptr) {
                     const int slot = ua / RB1, rb = ua - slot * RB1, e = expert_of[slot];
-                    src = (long long) e * C1 * R1 + rb * 32;
+                    const size_t row = ((size_t) e * C1 + wg) * R1 + rb * 32;
+                    codes = g.gu + row * mx4::CODES + lane * 16;
+                    factors = g.gu_factors + row * mx4::SCALES + lane * 16;
                     if (lane < 8 && wg < 1)
                         mx4::copy16(smem_u32(rows_of + (ia % KNOWN) * 32 + lane * 4), g.gu_exp + (size_t) e * R1 + rb * 32 + lane * 4, policy);
                 }
-                mx4::copy_chunk(ring_s + at * mx4::SLOT, g.gu, g.gu_factors, (size_t) (src + (long long) ka * R1), policy);
+                mx4::copy_chunk(ring_s + at * mx4::SLOT, codes, factors, policy);
                 at = at + 1 == depth ? 0 : at + 1;
+                codes += step * mx4::CODES;
+                factors += step * mx4::SCALES;
                 ka += g.gw;
                 if (ka >= C1) {
                     ka = wg;
-                    src = -1;
+                    codes = nullptr;
                     ++ia;
                 }
             }
@@ -326,7 +331,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     auto first_row = [&](const Place & x) { return x.gr * 64 + pair * 32 < g.d ? x.gr * 64 + pair * 32 : 0; };      // (rows behind the last: any)
     auto ask = [&] {
         if (xa.p < xa.end) {
-            mx4::copy_chunk(ring_s + at * mx4::SLOT, g.down, g.down_factors, ((size_t) expert_of[xa.slot] * C2 + xa.c) * g.d + first_row(xa), policy);
+            const size_t row = ((size_t) expert_of[xa.slot] * C2 + xa.c) * g.d + first_row(xa);
+            mx4::copy_chunk(ring_s + at * mx4::SLOT, g.down + row * mx4::CODES + lane * 16, g.down_factors + row * mx4::SCALES + lane * 16, policy);
             at = at + 1 == depth ? 0 : at + 1;
             advance(xa);
         }

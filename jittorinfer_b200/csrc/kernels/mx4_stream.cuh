@@ -30,12 +30,13 @@ constexpr int SLOT = 32 * (CODES + SCALES);      // 32 rows of a chunk in shared
 __device__ __forceinline__ void copy16(uint32_t dst, const void * src, uint64_t policy) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
-// 32 rows of a chunk: row `row` of codes and factors on.
-__device__ __forceinline__ void copy_chunk(uint32_t dst, const uint8_t * codes, const uint8_t * factors, size_t row, uint64_t policy) {
+// 32 rows of a chunk: this lane's first 16 bytes of codes and factors (of the first eight lanes).
+__device__ __forceinline__ void copy_chunk(uint32_t dst, const uint8_t * codes, const uint8_t * factors, uint64_t policy) {
     const int lane = threadIdx.x & 31;
+    dst += lane * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) copy16(dst + (i * 32 + lane) * 16, codes + row * CODES + (i * 32 + lane) * 16, policy);
-    if (lane < 8) copy16(dst + 32 * CODES + lane * 16, factors + row * SCALES + lane * 16, policy);
+    for (int i = 0; i < 4; ++i) copy16(dst + i * 512, codes + i * 512, policy);
+    if (lane < 8) copy16(dst + 32 * CODES, factors, policy);
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // All but the last n groups of copies are there (n: 0 .. 3).

@@ -159,7 +159,7 @@ __device__ __forceinline__ int chunks_of(const Args & g, int i) {
     return (split + 1) * g.C / g.splits - split * g.C / g.splits;
 }
 
-template <bool PAIR>
+template <bool PAIR, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Args g) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ int first_tile[MAX_E + 1], last_s;
@@ -170,8 +170,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
     uint64_t * full = bars, * empty = full + MAX_STAGES, * sl_full = empty + MAX_STAGES, * sf_full = sl_full + MAX_SLOTS, * sf_empty = sf_full + MAX_SLOTS,
              * acc_full = sf_empty + MAX_SLOTS, * acc_empty = acc_full + 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = g.stages, Q = g.slots, bn = g.bn, cps = g.cps;
-        const int rank = PAIR ? blockIdx.x & 1 : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x, xn = PAIR ? bn / 2 : bn;            // rows of x in this CTA's shared memory
-    const int SB = stage_bytes(xn), QB = slot_bytes(bn), plane = xn * 128, mn = PAIR ? bn : 2 * bn, sfc = scale_cols(mn), slab = PAIR ? 4 + 2 * sfc : 4 + sfc;
+        const int rank = PAIR ? blockIdx.x & 1 : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    // rows of x in this CTA's shared memory: of a pair half of them, or, WIDE, all of one plane
+    const int xn = PAIR ? bn / 2 : bn, SB = stage_bytes(xn), QB = slot_bytes(bn), plane = xn * 128;
+    const int mn = WIDE ? 2 * bn : bn, sfc = scale_cols(mn), slab = WIDE ? 4 + sfc : 4 + 2 * sfc;
     uint8_t * scale_slots = tiles + S * cps * SB;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
@@ -230,8 +232,12 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     for (int j = 0; j < n; ++j) {
                         uint8_t * st = tiles + (s * cps + j) * SB;
                         mx4::load<PAIR>(st, &tm_w, &full[s], 0, row_tile<PAIR>(t.m, rank) * BM, t.e * g.C + c0 + j);
-                        mx4::load<PAIR>(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 0);
-                        mx4::load<PAIR>(st + A_BYTES + plane, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 1);
+                        if (PAIR && WIDE) {
+                            mx4::load<PAIR>(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0, rank);
+                        } else {
+                            mx4::load<PAIR>(st + A_BYTES, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 0);
+                            mx4::load<PAIR>(st + A_BYTES + plane, &tm_x, &full[s], (c0 + j) * 128, t.row0 + rank * xn, 1);
+                        }
                     }
                 }
             }
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     for (int j = 0; j < min(cps, n - c0); ++j) {
                         const uint64_t a = desc0 + (uint32_t) ((r.at * cps + j) * SB >> 4), b = a + (A_BYTES >> 4);
                         const uint32_t sf = sf0 + (rq.at * cps + j) * slab;
-                        if (!PAIR) {
+                        if (WIDE) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) mma_mxf8f6f4<PAIR>(acc, a + 2 * k, b + 2 * k, id0 + (k << 4) + ((uint32_t) k << 29), sf, sf + 4, more || k != 0);
                         } else {
@@ -332,7 +338,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                 for (int c = 0; c < min(cps, n - c0); ++c) {
                     const uint32_t * sc = (const uint32_t *) (scale_slots + (q * cps + c) * QB) + lane;
                     const uint32_t dst = mine + (q * cps + c) * slab;
-                    constexpr int P = PAIR ? 2 : 1;
+                    constexpr int P = WIDE ? 1 : 2;
                     uint32_t w[4], v[P][8];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) w[k] = sc[k * 32];
@@ -374,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 #pragma unroll 1
                 for (int c = 16 * half; c < t.rows; c += 32) {
                     uint32_t v[16];
-                    sums16(acc + c, PAIR ? 0 : bn, v);
+                    sums16(acc + c, WIDE ? bn : 0, v);
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
                         if (c + k < t.rows) __stcg(to + (size_t) (c + k) * BM, __uint_as_float(v[k]));
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
                     }
                 } else {
                     uint32_t v[16];
-                    sums16(acc + c, PAIR ? 0 : bn, v);
+                    sums16(acc + c, WIDE ? bn : 0, v);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) y[k] = __uint_as_float(v[k]);
                 }
@@ -641,22 +647,23 @@ int planes_map(CUtensorMap * out, const void * planes, long long rows, long long
                : JIB_E_TENSORMAP;
 }
 
-// Up to this many rows of x the planes are one operand (two buffers of sums and the scales fit in tensor memory); above, pairs of CTAs work on a tile.
+// Up to this many rows of x the planes are one operand (two buffers of sums and the scales fit in tensor memory).
 constexpr int MAX_WIDE = 96;
 
 int sm_count() { return jib::sm_count() > 0 ? jib::sm_count() : 148; }
 
+template <bool WIDE>
 int pair_count() {
     static std::atomic<int> known[jib::MAX_DEVICES];
     static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
-    return mx4::pair_count(mx4_gemm_kernel<true>, THREADS, MOST_SMEM - 5120, known, attr_done);
+    return mx4::pair_count(mx4_gemm_kernel<true, WIDE>, THREADS, MOST_SMEM - 5120, known, attr_done);
 }
 
 // Rows of x in a tile and splits of K of a dense product.  What a chunk costs a CTA is its traffic with shared memory: 128 bytes written a row of either operand
 // and plane, and as many read by each instruction.  In rows of x (512 bytes): w + 64 with the planes as one operand; in a pair w / 2 + 96, or w for its
 // products where that is more.  Where the tiles leave SMs idle, K is split, four chunks a split at least.
 void shape_of(long long T, int R, int C, int * bn, int * splits) {
-    const int sms = sm_count(), pairs = R > BM ? pair_count() : 0;
+    const int sms = sm_count(), pairs = R > BM ? pair_count<false>() : 0;
     const long long m_tiles = (R + BM - 1) / BM;
     long long best = -1;
     for (int w = T > 16 ? 32 : 16; w <= (pairs > 0 ? MAX_BN : MAX_WIDE); w += 32) {
@@ -727,7 +734,7 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
         // an expert's rows on average and twice their spread: most experts then take one tile
         const float avg = (float) d->max_rows / d->batch;
         const int w = ((int) (avg + 2.f * sqrtf(avg)) + 31) / 32 * 32;
-        const int most = g.R > BM && pair_count() > 0 ? MAX_BN : MAX_WIDE;
+        const int most = g.R > BM && pair_count<false>() > 0 ? MAX_BN : MAX_WIDE;
         g.bn = w < 32 ? 32 : w > most ? most : w;
         g.splits = 1;
         g.t_tiles = 1;
@@ -738,8 +745,9 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
         g.t_tiles = (d->T + g.bn - 1) / g.bn;
         items = (long long) g.m_tiles * g.t_tiles * g.splits;
     }
-    const bool pair = g.bn > MAX_WIDE;
-    const int at_once = pair ? pair_count() : sms, xn = pair ? g.bn / 2 : g.bn;
+    // pairs: tiles of more rows, and experts' tiles (of the 66-expert layer 17 rows take 95.5 us alone, 92 in pairs, 515 rows 159 and 143)
+    const bool wide = g.bn <= MAX_WIDE, pair = !wide || (d->seg != nullptr && g.R > BM && pair_count<true>() > 0);
+    const int at_once = !pair ? sms : wide ? pair_count<true>() : pair_count<false>(), xn = pair ? g.bn / 2 : g.bn;
     if (pair) {
         g.m_tiles = (g.m_tiles + 1) / 2;
         items = d->seg != nullptr ? at_once : (long long) g.m_tiles * g.t_tiles;
@@ -748,7 +756,7 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
     // Chunks of a stage: its waits and commits take the issuing thread as long as a few products.  8 rows by 12288 x 5120: 21 us with one, 16.5 with two, 14.3
     // with three; 17 rows of the 66-expert layer 122 and 96 us with one and two, 107 with three (16 and 11 chunks are no multiple); 515 rows 191 and 160.
     g.cps = g.bn <= 16 ? 3 : g.bn <= MAX_WIDE ? 2 : 1;
-    g.slots = pair ? (512 - 2 * g.bn) / (4 + 2 * scale_cols(g.bn)) : (512 - 4 * g.bn) / (g.cps * (4 + scale_cols(2 * g.bn)));
+    g.slots = !wide ? (512 - 2 * g.bn) / (4 + 2 * scale_cols(g.bn)) : (512 - 4 * g.bn) / (g.cps * (4 + scale_cols(2 * g.bn)));
     if (g.slots > MAX_SLOTS) g.slots = MAX_SLOTS;
     g.stages = (MOST_SMEM - 5120 - 1024 - g.slots * g.cps * slot_bytes(g.bn)) / (g.cps * stage_bytes(xn));        // (5 KB: barriers and tables)
     if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
@@ -756,18 +764,19 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
     CUtensorMap mw, mx;
     int rc = weights_map(&mw, d->w, g.R, (long long) g.C * d->batch);
     if (rc) return rc;
-    rc = planes_map(&mx, planes, d->T, (long long) g.C * 128, xn);
+    rc = planes_map(&mx, planes, d->T, (long long) g.C * 128, wide ? g.bn : xn);
     if (rc) return rc;
     static std::atomic<unsigned char> attr_done[jib::MAX_DEVICES];
-    if (!pair && !jib::ensure_dyn_smem(mx4_gemm_kernel<false>, MOST_SMEM - 5120, attr_done)) return JIB_E_LAUNCH;
+    if (!pair && !jib::ensure_dyn_smem(mx4_gemm_kernel<false, true>, MOST_SMEM - 5120, attr_done)) return JIB_E_LAUNCH;
     // a thread keeps its eight columns and walks down the rows
     const int nx = (g.C * 16 + 255) / 256, th = ((g.C * 16 + nx - 1) / nx + 31) / 32 * 32;
     const long long ny = (d->T + ROWS - 1) / ROWS, most = ((long long) sms * 4096 / th + nx - 1) / nx;
     JIB_LAUNCH((planes_kernel), dim3(nx, (unsigned) (ny < most ? ny : most < 65535 ? most : 65535)), th, 0, (cudaStream_t) stream, (const bf16 *) d->x, d->ldx, d->src,
                d->seg != nullptr ? d->seg + d->batch : nullptr, planes, x_scales, (long long) d->T, g.x_rows, d->K, g.C, g.counters, sc.tiles);
     const unsigned grid = (unsigned) (items < at_once ? items : at_once);
-    if (pair) (void) jib::launch_pdl_pairs(mx4_gemm_kernel<true>, grid, dim3(THREADS), smem, (cudaStream_t) stream, mw, mx, g);
-    else JIB_LAUNCH((mx4_gemm_kernel<false>), grid, THREADS, smem, (cudaStream_t) stream, mw, mx, g);
+    if (pair && wide) (void) jib::launch_pdl_pairs(mx4_gemm_kernel<true, true>, grid, dim3(THREADS), smem, (cudaStream_t) stream, mw, mx, g);
+    else if (pair) (void) jib::launch_pdl_pairs(mx4_gemm_kernel<true, false>, grid, dim3(THREADS), smem, (cudaStream_t) stream, mw, mx, g);
+    else JIB_LAUNCH((mx4_gemm_kernel<false, true>), grid, THREADS, smem, (cudaStream_t) stream, mw, mx, g);
     return launched();
 }
 

@@ -7,9 +7,11 @@
 // with a scale for 32 columns.  That sum is the bf16 value down to 2^-11 of the block's largest magnitude and within 2^-21 of the largest below.  At
 // twice the rate of bf16 both planes cost what a bf16 product costs.
 //
-// Up to 96 rows of x a CTA works alone, and both planes are one operand of twice the rows; the sums of the two meet in the epilogue.  Above, two CTAs
-// (cta_group::2) share a tile of 256 weights by up to 192 rows of x, of which each keeps half: the products are bound by their traffic with shared memory,
-// and the rows of x are half of it.  1531 rows by 2 x 10944 x 2048: 132 us with tiles of one CTA, 102 us with pairs (1.34 PFLOP/s).
+// Up to 96 rows of x (WIDE) both planes are one operand of twice the rows, and the sums of the two meet in the epilogue.  Dense tiles then belong to one CTA,
+// experts' tiles to two (PAIR, cta_group::2: 256 weights, each CTA keeps one plane).  Above 96 rows two CTAs share 256 weights by up to 192 rows of x, of
+// which each keeps half: the products are bound by their traffic with shared memory, and the rows of x are half of it.  1531 rows by 2 x 10944 x 2048:
+// 132 us with tiles of one CTA, 102 us with pairs (1.34 PFLOP/s).  Bounds: few rows, the weights' stream and a stage's fixed cost (8 rows by 12288 x 5120
+// 14.1 us, 2.4 TB/s); many, the tensor cores (79 cycles an instruction of 256 x 192 x 32).
 //
 // A stage is one to three chunks of 128 columns: codes (16 KB in shared memory, 8 KB from memory) and planes.  Scales have a ring of their own: one thread asks
 // for them, four warps move them to tensor memory (column j of an operand: lane l of every quarter holds the four scale bytes of row 32 j + l), well
@@ -467,7 +469,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 }
 
 // ---- bf16 rows as two E4M3 planes ------------------------------------------------------------------------------------------------
-// Four lanes a block of 32 columns.  Scale 2^e with e = floor(log2 max) - 7, at least -123: the largest magnitude becomes 128 .. 256, rounded to hi; what is left, at
+// Four lanes a block of 32 columns; a thread keeps its eight columns and walks down the rows.  Bound by memory and two dependent loads with src (4 thousand
+// rows of 2048 columns gathered from 515: 12 us).  Scale 2^e with e = floor(log2 max) - 7, at least -123: the largest magnitude becomes 128 .. 256, rounded to hi; what is left, at
 // most 8, times 16 is rounded to lo, whose scale is 2^(e - 4).  src: row r is x[src[r]] (zeros where that is negative); limit: rows from *limit on are
 // left alone.
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
@@ -540,7 +543,7 @@ __global__ void __launch_bounds__(256) planes_kernel(const bf16 * __restrict__ x
 
 // ---- pairs by expert, each expert's rows at a multiple of PAD -------------------------------------------------------------------------
 // first[e] and count[e] of the padded order (first[E]: its end), the token of each of its rows (-1: none) and the row of each pair (-1: an id outside the experts).
-// One CTA: counts, their sums, places, with a table for each warp (tokens that choose alike would queue for one).  Which of its warp's rows a pair gets is left
+// 4 thousand pairs: 7 us; by the framework's own sort and a launch that spreads its places 18.  One CTA: counts, their sums, places, with a table for each warp (tokens that choose alike would queue for one).  Which of its warp's rows a pair gets is left
 // to chance; what is computed from a row does not depend on where it stands.
 constexpr int SORT_NT = 1024, SORT_AHEAD = 4;
 

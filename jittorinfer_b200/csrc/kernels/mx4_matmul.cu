@@ -2,9 +2,13 @@
 //
 // tcgen05.mma.kind::mxf4.block_scale multiplies E2M1 codes and applies the blocks' scales itself, 64 columns an instruction: nothing is
 // expanded.  b (the weights) is operand A of the instruction, 128 rows a tile, a's rows are its columns, up to 208 a tile: so few tokens cost
-// a narrow tile.  The scales live in tensor memory: column j of a slab holds, in lane l of every quarter, the four scale bytes of row 32 j + l
-// for 128 columns of K.  They come in boxes of 16 bytes a row (512 columns, two stages) in a ring of their own, and four warps move them to tensor
-// memory ahead of their stage.  (Read from global memory by those warps, stage by stage, they took 1200 clocks a stage, three times the products.)
+// a narrow tile.  Where it costs less, two CTAs (PAIR, cta_group::2) share 256 weights by up to 192 tokens, of which each keeps half.
+//
+// The scales live in tensor memory: column j of a slab holds, in lane l of every quarter, the four scale bytes of row 32 j + l for 128 columns of K.  They
+// come in boxes of 16 bytes a row (512 columns, two stages) in a ring of their own, and eight warps, four a stage in turn, move them to tensor
+// memory ahead of their stage.  (Read from global memory by those warps, stage by stage, they took 1200 clocks a stage, three times the products; four
+// warps for them took longer than the products of a pair.)  2048 x 5120 by 12288, quantising included: 91 us with four warps for scales and four for
+// results, 81 with eight for results, 67 with eight for scales and pairs (3.85 PFLOP/s; pairs alone 86); bound by the scales' way and shared memory.
 #include "sm100.cuh"
 #include "jib_kernels.h"
 #include "mx4_pair.cuh"

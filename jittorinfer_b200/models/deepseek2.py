@@ -305,6 +305,8 @@ class DeepSeek2Model:
                 raise ValueError(f"layer {il}: missing tensors {missing}")
             if self.ffn_format is not None:
                 self._lay_out_ffn(L)
+        if self.ffn_format is not None and self.device.type == "cuda":
+            torch.cuda.empty_cache()          # what held the weights before they were quantised: the cache is sized from free memory
 
     def cache_bytes_per_token(self) -> int:
         return self.hp.n_layer * self.hp.kv_row * torch.empty(0, dtype=self.dtype).element_size()

@@ -345,7 +345,8 @@ JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, void * stream);
 // The same on the tensor cores, bf16 activations (mx4_gemm.cu): as planes first; grouped rows at padded places.
 JIB_EXPORT long long jib_mx4_gemm_scratch(long long rows, int N, int K, int gated, int grouped);
 JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, int * count, int * row_src, int * pair_row, void * stream);
-JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, void * stream);
+JIB_EXPORT int jib_mx4_gemm_joins(int N, int gated);
+JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, void * next, int ready, void * stream);
 // A mixture-of-experts layer for up to 8 tokens (mx4_moe.cu).
 typedef struct jib_mx4_moe_desc {
     const void * residual;                 // NULL, or bf16 [T][d], rows ldr elements apart

@@ -36,6 +36,7 @@ constexpr int BM = 128, MAX_BN = 192, MAX_STAGES = 8, MAX_SLOTS = 8, MAX_E = 256
 constexpr int A_BYTES = BM * 128, SA_BYTES = BM * 4;
 constexpr int THREADS = 512;                       // producer, issuer, one idle, producer of scales; four scale warps; eight epilogue warps
 constexpr int MOST_SMEM = 227 * 1024;
+constexpr int STAGED = 72, STAGED_BYTES = 2 * 16 * STAGED * 2;          // 64 hidden units of a row and room between rows; two times 16 rows
 // Rows of the planes' scales: a tile reads up to MAX_BN behind the last one, 16 bytes (four rows) at a time.
 __host__ __device__ inline long long scale_rows_of(long long rows) { return (rows + MAX_BN + 31) / 32 * 32; }
 
@@ -53,8 +54,9 @@ struct Args {
     float * part;                            // [tile][split][bn][128]
     int * counters;                          // zeros, one a tile
     int * status;
-    long long ldo, ldr, x_rows;
-    int T, N, R, C, E, bn, m_tiles, t_tiles, splits, stages, slots, cps, gated, act, out_f32, res_f32;
+    uint8_t * h_planes, * h_scales;          // the result as planes and scales for the next product (NULL: as it is, to out); rows h_rows, h_C chunks
+    long long ldo, ldr, x_rows, h_rows;
+    int T, N, R, C, E, bn, m_tiles, t_tiles, splits, stages, slots, cps, h_C, gated, act, out_f32, res_f32;
 };
 
 __device__ __forceinline__ void st_cols4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -90,6 +92,48 @@ struct Ring {
         if (++at == n) { at = 0; round ^= 1; }
     }
 };
+
+// ---- bf16 values as two E4M3 numbers ----------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
+__device__ __forceinline__ float2 e4m3_values(uint32_t two) {
+    return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) two, __NV_E4M3)));
+}
+
+// Four lanes a block of 32 columns, eight of them each.  Scale 2^e with e = floor(log2 max) - 7, at least -123: the largest magnitude becomes 128 .. 256, rounded
+// to hi; what is left, at most 8, times 16 is rounded to lo, whose scale is 2^(e - 4).  Returns e + 127, or 255 for a block with an infinity or NaN.
+__device__ __forceinline__ int to_planes(uint4 in, uint2 & hi, uint2 & lo) {
+    const uint32_t w[4] = {in.x, in.y, in.z, in.w};
+    float z[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = __bfloat1622float2(*(const __nv_bfloat162 *) &w[j]);
+        z[2 * j] = f.x;
+        z[2 * j + 1] = f.y;
+        top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int field = (int) (top >> 23), byte = field == 255 ? 255 : max(field - 7, 4);
+    const float unit = field == 255 ? 0.f : __uint_as_float((uint32_t) (254 - byte) << 23);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] = field == 255 ? 0.f : z[j] * unit;
+    hi.x = e4m3x4(z[0], z[1], z[2], z[3]);
+    hi.y = e4m3x4(z[4], z[5], z[6], z[7]);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const float2 f = e4m3_values((j < 4 ? hi.x : hi.y) >> (j & 2) * 8);
+        z[j] = (z[j] - f.x) * 16.f;
+        z[j + 1] = (z[j + 1] - f.y) * 16.f;
+    }
+    lo.x = e4m3x4(z[0], z[1], z[2], z[3]);
+    lo.y = e4m3x4(z[4], z[5], z[6], z[7]);
+    return byte;
+}
+__device__ __forceinline__ uint8_t low_scale(int byte) { return (uint8_t) (byte == 255 ? 255 : byte - 4); }
 
 // Sixteen columns of sums; with the planes side by side the other plane's stand `other` columns on.
 __device__ __forceinline__ void sums16(uint32_t at, int other, uint32_t (&v)[16]) {
@@ -365,13 +409,14 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
         // two warps a quarter of the rows, they take every second 16 rows of x
         const int q = warp & 3, half = (warp - 8) >> 2;
         const uint32_t mine = tmem + ((uint32_t) q << 21);
+        bf16 * staged = (bf16 *) (scale_slots + Q * cps * QB) + half * 16 * STAGED;
         int j = 0;
 #pragma unroll 1
         for (int i = first; i < items; i += step, ++j) {
             const Item t = item_of(g, first_tile, experts, i);
             const int buf = j & 1;
             bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], j >> 1 & 1));
-            if (!PAIR && g.splits > 1) ok = all_of_256(ok);          // (they meet below)
+            if (g.h_planes != nullptr || (!PAIR && g.splits > 1)) ok = all_of_256(ok);          // (they meet below)
             if (!ok) { jib_report(g.status, JIB_ERR_WAIT_TIMEOUT, 65, i); break; }
             tc_fence_after();
             const uint32_t acc = mine + buf * mn;
@@ -424,6 +469,33 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 #pragma unroll
                     for (int k = 0; k < 16; ++k) y[k] = __uint_as_float(v[k]);
                 }
+                if (PAIR && g.h_planes != nullptr) {
+                    // four warps: 16 rows of 64 units, in bf16, through shared memory; then a thread eight units of a row
+                    bf16 * at = staged + (lane >> 4) * STAGED + q * 16 + (lane & 15);
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? y[k + 1] : y[k], 16);
+                        const float v = mx4::gated(lane < 16 ? y[k] : other, lane < 16 ? other : y[k + 1], g.act);
+                        at[k * STAGED] = __float2bfloat16(n < g.N ? v : 0.f);
+                    }
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+                    const int id = threadIdx.x & 127, row = id >> 3, col = m * 64 + (id & 7) * 8;
+                    uint2 hi, lo;
+                    const int byte = to_planes(*(const uint4 *) (staged + row * STAGED + (id & 7) * 8), hi, lo);
+                    if (c + row < t.rows && col < g.h_C * 128) {
+                        const long long r = t.row0 + c + row, width = g.h_C * 128;
+                        *(uint2 *) (g.h_planes + r * width + col) = hi;
+                        *(uint2 *) (g.h_planes + (g.h_rows + r) * width + col) = lo;
+                        if ((id & 3) == 0) {
+                            const long long rows = scale_rows_of(g.h_rows);
+                            uint8_t * sc = g.h_scales + ((col >> 7) * rows + r) * 4 + (col >> 5 & 3);
+                            sc[0] = (uint8_t) byte;
+                            sc[g.h_C * rows * 4] = low_scale(byte);
+                        }
+                    }
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+                    continue;
+                }
                 if (g.gated) {
                     // a gate's lane takes the even rows of x, the up matrix's lane 16 above it the odd ones
                     bf16 * to = (bf16 *) g.out + (long long) (t.row0 + c + (lane >> 4)) * g.ldo + n;
@@ -469,18 +541,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
 }
 
 // ---- bf16 rows as two E4M3 planes ------------------------------------------------------------------------------------------------
-// Four lanes a block of 32 columns; a thread keeps its eight columns and walks down the rows.  Bound by memory and two dependent loads with src (4 thousand
-// rows of 2048 columns gathered from 515: 12 us).  Scale 2^e with e = floor(log2 max) - 7, at least -123: the largest magnitude becomes 128 .. 256, rounded to hi; what is left, at
-// most 8, times 16 is rounded to lo, whose scale is 2^(e - 4).  src: row r is x[src[r]] (zeros where that is negative); limit: rows from *limit on are
-// left alone.
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return lo | hi << 16;
-}
-__device__ __forceinline__ float2 e4m3_values(uint32_t two) {
-    return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) two, __NV_E4M3)));
-}
-
+// A thread keeps its eight columns and walks down the rows.  Bound by memory and two dependent loads with src (4 thousand rows of 2048 columns gathered from
+// 515: 12 us).  src: row r is x[src[r]] (zeros where that is negative); limit: rows from *limit on are left alone.
 constexpr int ROWS = 4;                             // of a thread's columns, their loads in flight together
 
 __global__ void __launch_bounds__(256) planes_kernel(const bf16 * __restrict__ x, long long ldx, const int * __restrict__ src, const int * __restrict__ limit,
@@ -501,41 +563,16 @@ __global__ void __launch_bounds__(256) planes_kernel(const bf16 * __restrict__ x
         }
 #pragma unroll
         for (int h = 0; h < ROWS; ++h) {
-            const uint32_t w[4] = {in[h].x, in[h].y, in[h].z, in[h].w};
-            float z[8];
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = __bfloat1622float2(*(const __nv_bfloat162 *) &w[j]);
-                z[2 * j] = f.x;
-                z[2 * j + 1] = f.y;
-                top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-            }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (r0 + h >= most || k >= C * 128) continue;
-            const int field = (int) (top >> 23), byte = field == 255 ? 255 : max(field - 7, 4);          // e + 127
-            const float unit = field == 255 ? 0.f : __uint_as_float((uint32_t) (254 - byte) << 23);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = field == 255 ? 0.f : z[j] * unit;
             uint2 hi, lo;
-            hi.x = e4m3x4(z[0], z[1], z[2], z[3]);
-            hi.y = e4m3x4(z[4], z[5], z[6], z[7]);
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const float2 f = e4m3_values((j < 4 ? hi.x : hi.y) >> (j & 2) * 8);
-                z[j] = (z[j] - f.x) * 16.f;
-                z[j + 1] = (z[j + 1] - f.y) * 16.f;
-            }
-            lo.x = e4m3x4(z[0], z[1], z[2], z[3]);
-            lo.y = e4m3x4(z[4], z[5], z[6], z[7]);
+            const int byte = to_planes(in[h], hi, lo);
+            if (r0 + h >= most || k >= C * 128) continue;
             uint8_t * to = planes + (r0 + h) * (long long) (C * 128) + k;
             *(uint2 *) to = hi;
             *(uint2 *) (to + rows * (long long) (C * 128)) = lo;
             if ((k >> 3 & 3) == 0) {
                 uint8_t * sc = scales + ((long long) (k >> 7) * scale_rows + r0 + h) * 4 + (k >> 5 & 3);
                 sc[0] = (uint8_t) byte;
-                sc[(long long) C * scale_rows * 4] = (uint8_t) (byte == 255 ? 255 : byte - 4);
+                sc[(long long) C * scale_rows * 4] = low_scale(byte);
             }
         }
     }
@@ -710,6 +747,9 @@ extern "C" {
 // Bytes that jib_mx4_gemm needs for `rows` rows.
 JIB_EXPORT long long jib_mx4_gemm_scratch(long long rows, int N, int K, int gated, int grouped) { return Scratch(rows, N, K, gated != 0, grouped != 0).bytes; }
 
+// Whether a grouped product can hand its results to the next one as planes.
+JIB_EXPORT int jib_mx4_gemm_joins(int N, int gated) { return gated && mx4::rows_of(N, true) > BM && pair_count<true>() > 0 && pair_count<false>() > 0; }
+
 // ids [n / k][k]; first: E + 1 ints, count: E, row_src: room for n pairs and PAD - 1 more rows of each expert that has any, pair_row: n.
 JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, int * count, int * row_src, int * pair_row, void * stream) {
     if (E < 1 || E > MAX_E || n < 1 || k < 1) return JIB_E_ARG;
@@ -718,10 +758,13 @@ JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, i
 }
 
 // The tiled product of bf16 rows d->x: as planes, then multiplied.  Grouped: d->seg = first, count, d->src = row_src of jib_mx4_sort (NULL: x in that order), T
-// rows at most.  scratch: jib_mx4_gemm_scratch(T, ..) bytes.
-JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, void * stream) {
+// rows at most.  scratch: jib_mx4_gemm_scratch(T, ..) bytes; ready: it holds the planes already (then d->x is not read).  next (grouped pairs of more than one
+// tile of weights, see jib_mx4_gemm_joins): the scratch of a product of the results, which go there as planes and not to d->out.
+JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, void * next, int ready, void * stream) {
     if (d->T <= 0) return 0;
-    if (d->N <= 0 || d->K <= 0 || d->K % 32 || d->batch < 1 || d->batch > MAX_E || (d->seg != nullptr && (count == nullptr || d->residual != nullptr))) return JIB_E_ARG;
+    if (d->N <= 0 || d->K <= 0 || d->K % 32 || d->batch < 1 || d->batch > MAX_E || (d->seg != nullptr && (count == nullptr || d->residual != nullptr)) ||
+        (next != nullptr && (!jib_mx4_gemm_joins(d->N, d->gated) || d->seg == nullptr || !d->gated || ((uintptr_t) next & 15))) || (ready && d->seg == nullptr))
+        return JIB_E_ARG;
     if (((uintptr_t) d->x | (uintptr_t) (d->ldx * 2) | (uintptr_t) scratch | (uintptr_t) d->w_scales) & 15) return JIB_E_ALIGN;
     const Scratch sc(d->T, d->N, d->K, d->gated != 0, d->seg != nullptr);
     uint8_t * planes = (uint8_t *) scratch, * x_scales = planes + sc.scales;
@@ -731,6 +774,7 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
     g.part = (float *) (planes + sc.part); g.counters = (int *) (planes + sc.counters); g.status = d->status; g.ldo = d->ldo; g.ldr = d->ldr; g.x_rows = scale_rows_of(d->T);
     g.T = d->T; g.N = d->N; g.R = mx4::rows_of(d->N, d->gated != 0); g.C = mx4::chunks(d->K); g.E = d->batch;
     g.gated = d->gated; g.act = d->act; g.out_f32 = d->out_f32; g.res_f32 = d->res_f32;
+    g.h_planes = (uint8_t *) next; g.h_rows = d->T; g.h_C = mx4::chunks(d->N); g.h_scales = g.h_planes + 2ll * d->T * g.h_C * 128;
     g.m_tiles = (g.R + BM - 1) / BM;
     long long items;
     if (d->seg != nullptr) {
@@ -761,9 +805,10 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
     g.cps = g.bn <= 16 ? 3 : g.bn <= MAX_WIDE ? 2 : 1;
     g.slots = !wide ? (512 - 2 * g.bn) / (4 + 2 * scale_cols(g.bn)) : (512 - 4 * g.bn) / (g.cps * (4 + scale_cols(2 * g.bn)));
     if (g.slots > MAX_SLOTS) g.slots = MAX_SLOTS;
-    g.stages = (MOST_SMEM - 5120 - 1024 - g.slots * g.cps * slot_bytes(g.bn)) / (g.cps * stage_bytes(xn));        // (5 KB: barriers and tables)
+    const int staged = next != nullptr ? STAGED_BYTES : 0;
+    g.stages = (MOST_SMEM - 5120 - 1024 - staged - g.slots * g.cps * slot_bytes(g.bn)) / (g.cps * stage_bytes(xn));        // (5 KB: barriers and tables)
     if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
-    const size_t smem = g.cps * (g.stages * stage_bytes(xn) + g.slots * slot_bytes(g.bn)) + 1024;
+    const size_t smem = g.cps * (g.stages * stage_bytes(xn) + g.slots * slot_bytes(g.bn)) + staged + 1024;
     CUtensorMap mw, mx;
     int rc = weights_map(&mw, d->w, g.R, (long long) g.C * d->batch);
     if (rc) return rc;
@@ -774,7 +819,8 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
     // a thread keeps its eight columns and walks down the rows
     const int nx = (g.C * 16 + 255) / 256, th = ((g.C * 16 + nx - 1) / nx + 31) / 32 * 32;
     const long long ny = (d->T + ROWS - 1) / ROWS, most = ((long long) sms * 4096 / th + nx - 1) / nx;
-    JIB_LAUNCH((planes_kernel), dim3(nx, (unsigned) (ny < most ? ny : most < 65535 ? most : 65535)), th, 0, (cudaStream_t) stream, (const bf16 *) d->x, d->ldx, d->src,
+    if (!ready)
+        JIB_LAUNCH((planes_kernel), dim3(nx, (unsigned) (ny < most ? ny : most < 65535 ? most : 65535)), th, 0, (cudaStream_t) stream, (const bf16 *) d->x, d->ldx, d->src,
                d->seg != nullptr ? d->seg + d->batch : nullptr, planes, x_scales, (long long) d->T, g.x_rows, d->K, g.C, g.counters, sc.tiles);
     const unsigned grid = (unsigned) (items < at_once ? items : at_once);
     if (pair && wide) (void) jib::launch_pdl_pairs(mx4_gemm_kernel<true, true>, grid, dim3(THREADS), smem, (cudaStream_t) stream, mw, mx, g);

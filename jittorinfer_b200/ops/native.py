@@ -174,7 +174,8 @@ def load():
     sig("jib_mx4_gemm_scratch", ll, i, i, i, i)
     L.jib_mx4_gemm_scratch.restype = ll
     sig("jib_mx4_sort", ip, i, i, i, ip, ip, ip, ip, vp)
-    sig("jib_mx4_gemm", C.POINTER(Mx4Desc), ip, vp, vp)
+    sig("jib_mx4_gemm_joins", i, i)
+    sig("jib_mx4_gemm", C.POINTER(Mx4Desc), ip, vp, vp, i, vp)
     sig("jib_mx4_moe_sizes", i, i, i, i, i, C.POINTER(ll))
     sig("jib_mx4_moe_prepare", vp, ll, fp, fp, vp, ip, i, i, i, i, vp)
     sig("jib_mx4_moe", C.POINTER(Mx4MoeDesc), vp)

@@ -78,17 +78,14 @@ def _desc(w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act
 _scratch_bytes: dict = {}        # (rows, n, k, gated, grouped)
 
 
-def _tiled(d: "nat.Mx4Desc", x: torch.Tensor, count: Optional[int], what: str) -> None:
-    """bf16 activations as planes, then the tiled product.  ``count``: address, of grouped rows."""
-    key = (d.T, d.N, d.K, d.gated, int(count is not None))
+def _scratch(rows: int, w: Mx4Weight, grouped: bool, device) -> torch.Tensor:
+    key = (rows, w.n, w.k, int(w.gated), int(grouped))
     n = _scratch_bytes.get(key)
     if n is None:
         if len(_scratch_bytes) > 4096:
             _scratch_bytes.clear()
         n = _scratch_bytes[key] = nat.load().jib_mx4_gemm_scratch(*key)
-    scratch = torch.empty(n, dtype=torch.uint8, device=x.device)
-    d.x, d.ldx = x.data_ptr(), x.stride(0)
-    nat._ck(nat.load().jib_mx4_gemm(C.byref(d), count, scratch.data_ptr(), nat._stream()), what)
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dtype: torch.dtype, act: Optional[str]) -> torch.Tensor:
@@ -100,7 +97,9 @@ def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dty
         with _on(x):
             d = _desc(w, out, residual, act)
             if x.dtype == torch.bfloat16:
-                _tiled(d, x, None, "mx4_gemm")
+                scratch = _scratch(x.shape[0], w, False, x.device)
+                d.x, d.ldx = x.data_ptr(), x.stride(0)
+                nat._ck(nat.load().jib_mx4_gemm(C.byref(d), None, scratch.data_ptr(), None, 0, nat._stream()), "mx4_gemm")
             else:
                 d.x, d.ldx = x.data_ptr(), x.stride(0)
                 nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), nat._stream()), "mx4_product_simt")
@@ -116,14 +115,22 @@ def _grouped_simt(x: torch.Tensor, w: Mx4Weight, seg: torch.Tensor, src: Optiona
     return out
 
 
-def _grouped(x: torch.Tensor, w: Mx4Weight, pad, src: Optional[int], pairs: int, act: Optional[str]) -> torch.Tensor:
-    """bf16 rows in the padded order ``pad`` = (first, count, capacity); row r is computed from x[src[r]] (without ``src`` x[r])."""
+def _grouped(x: torch.Tensor, wgu: Mx4Weight, wd: Mx4Weight, pad, src: int, pairs: int, act: str) -> torch.Tensor:
+    """The experts' results, bf16 rows in the padded order ``pad`` = (first, count, capacity); row r is computed from x[src[r]].  Hidden units go from product to
+    product as planes where the first can write them."""
     first, count, cap = pad
-    out = torch.empty(cap, w.n, dtype=torch.bfloat16, device=x.device)
-    d = _desc(w, out, None, act)
-    d.seg, d.src, d.batch, d.max_rows = first, src, w.batch, pairs
-    _tiled(d, x, count, "mx4_grouped")
-    return out
+    L, stream = nat.load(), nat._stream()
+    scratch, then = _scratch(cap, wgu, True, x.device), _scratch(cap, wd, True, x.device)
+    joined = L.jib_mx4_gemm_joins(wgu.n, 1)
+    h = torch.empty(0 if joined else cap, wgu.n, dtype=torch.bfloat16, device=x.device)
+    y = torch.empty(cap, wd.n, dtype=torch.bfloat16, device=x.device)
+    d = _desc(wgu, h, None, act)
+    d.T, d.x, d.ldx, d.seg, d.src, d.batch, d.max_rows = cap, x.data_ptr(), x.stride(0), first, src, wgu.batch, pairs
+    nat._ck(L.jib_mx4_gemm(C.byref(d), count, scratch.data_ptr(), then.data_ptr() if joined else None, 0, stream), "mx4_grouped")
+    d = _desc(wd, y, None, None)
+    d.x, d.ldx, d.seg, d.batch, d.max_rows = h.data_ptr(), wgu.n, first, wd.batch, pairs
+    nat._ck(L.jib_mx4_gemm(C.byref(d), count, then.data_ptr(), None, joined, stream), "mx4_grouped")
+    return y
 
 
 def matmul(a: Mx4Tensor, b: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -200,8 +207,7 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act, n_shared=0):
             count, row_src, pair_row = first + 4 * (E + 1), first + 4 * (2 * E + 1), first + 4 * (2 * E + 1 + cap)
             nat._ck(nat.load().jib_mx4_sort(ids.data_ptr(), n, k, E, first, count, row_src, pair_row, nat._stream()), "mx4_sort")
             routed = T * (k - n_shared) * E // (E - n_shared)       # the rows were there no shared experts: what the tiles are chosen for
-            h = _grouped(x, wgu, (first, count, cap), row_src, routed, act)
-            y = _grouped(h, wd, (first, count, cap), None, routed, None)
+            y = _grouped(x, wgu, wd, (first, count, cap), row_src, routed, act)
             return nat.moe_combine(y, table[2 * E + 1 + cap:].view(T, k), wts, None, None if residual is None else residual.contiguous())
         seg, src, dest = nat.moe_permute(ids, 0, E)
         h = _grouped_simt(x, wgu, seg, src, n, act)

@@ -11,7 +11,7 @@ from . import native as nat
 from .mx4 import COLS, MX4_MAX_EXPERTS as MAX_EXPERTS, Mx4Tensor, Mx4Weight, scale_rows
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-FEW_TOKENS = 8                               # tokens of a layer in two launches (8 of the 66-expert layer: 68 us, as tiles 76; 9, as two tiles of 8: 98 and 93)
+FEW_TOKENS = 8                               # tokens of a layer in two launches (8 of the 66-expert layer: 66 us, as tiles 71; 9, with a second tile of 8 here: 98 and 73)
 PAD = 32                                     # rows of an expert are padded to in grouped products (csrc/kernels/mx4_gemm.cu)
 MAX_CHOICES = 32                             # of a token: what the gate takes (csrc/kernels/moe.cu)
 _NO_SWITCH = contextlib.nullcontext()

@@ -55,6 +55,29 @@ def test_layers_of_many_rows(nat, T, E, k, choice):
     assert torch.equal(ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd), ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd))
 
 
+@pytest.mark.parametrize("T", [1, 8, 9, 300])
+def test_choices_that_are_no_expert_leave_the_residual(nat, T):
+    wgu, wd, *_ = experts(4, 160, 96)
+    x, res = randn(T, 160, seed=1, dtype=torch.bfloat16), randn(T, 160, seed=2, dtype=torch.bfloat16)
+    ids = torch.full((T, 3), -1, dtype=torch.int32, device=DEV)
+    ids[:, 1] = 4
+    wts = torch.rand(T, 3, generator=gen(3), device=DEV)
+    assert torch.equal(ops.mx4_moe_ffn(x, res, ids, wts, wgu, wd), res)
+    assert not bool(ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd).any())
+
+
+@pytest.mark.parametrize("F", [32, 64, 96, 160, 256, 288])
+def test_hidden_units_of_every_width_between_the_products(nat, F):
+    """Widths at which a tile of weights ends inside, at and behind a chunk of hidden units."""
+    T, E, k, d = 40, 5, 2, 96
+    wgu, wd, gv, uv, dv = experts(E, d, F, seed=F)
+    x = randn(T, d, seed=F, dtype=torch.bfloat16)
+    ids = torch.rand(T, E, generator=gen(F), device=DEV).argsort(-1)[:, :k].int()
+    wts = torch.rand(T, k, generator=gen(F + 2), device=DEV)
+    want, lim = layer_want(x, ids, wts, gv, uv, dv)
+    within(ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd), want, lim)
+
+
 @pytest.mark.parametrize("T", [3, 20])
 def test_an_expert_that_is_not_a_number_touches_only_those_who_chose_it(nat, T):
     wgu, wd, *_ = experts(4, 128, 64)

@@ -212,8 +212,8 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act, n_shared=0):
         seg, src, dest = nat.moe_permute(ids, 0, E)
         h = _grouped_simt(x, wgu, seg, src, n, act)
         y = _grouped_simt(h, wd, seg, None, n, None)
-        ok = (dest >= 0).to(wts.dtype) * wts
-        out = (y[dest.clamp(min=0).long()] * ok[..., None]).sum(1)
+        # a choice without an expert has no row: what stands in its place, and its weight, may be no number
+        out = torch.where((dest >= 0)[..., None], y[dest.clamp(min=0).long()] * wts[..., None], 0.0).sum(1)
         return out if residual is None else out + residual
 
 

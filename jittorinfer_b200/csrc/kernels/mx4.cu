@@ -137,16 +137,20 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t * __rest
 // Where row r of a matrix stands: of a pair's member `first` of `step` 2, in blocks of 16 rows that alternate.
 __device__ __forceinline__ int packed_row(int r, int step, int first) { return step == 1 ? r : (r / 16 * 2 + first) * 16 + r % 16; }
 
-// Exponents of the rows: the largest scale of a row (1 for one without a number) less 127 and TOP.  One warp a row.
-__global__ void __launch_bounds__(128) row_exponent_kernel(const uint8_t * __restrict__ scales, long long ld_s, int * __restrict__ exps, int N, int K, int R, int step,
-                                                           int first) {
+// Whether a block's codes are all 0 or -0.
+__device__ __forceinline__ bool no_value(uint4 v) { return ((v.x | v.y | v.z | v.w) & 0x77777777u) == 0u; }
+
+// Exponents of the rows: the largest scale of a block with a value (1 for a row without one) less 127 and TOP.  (A block of zeros can have any scale.)  One
+// warp a row.
+__global__ void __launch_bounds__(128) row_exponent_kernel(const uint4 * __restrict__ codes, const uint8_t * __restrict__ scales, long long ld_s,
+                                                           int * __restrict__ exps, int N, int K, int R, int step, int first) {
     const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5), m = blockIdx.y;
     if (r >= R / step) return;
     int top = -1;
     if (r < N)
         for (int i = lane; i < K / 32; i += 32) {
             const int e = scales[((size_t) m * N + r) * ld_s + i];
-            if (e != 255) top = max(top, e);
+            if (e != 255 && !no_value(codes[((size_t) m * N + r) * (K / 32) + i])) top = max(top, e);
         }
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) exps[(size_t) m * R + packed_row(r, step, first)] = (top < 0 ? 127 : top) - 127 - mx4::TOP;
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t * __restrict__ 
     int e = 0, f = 0;
     if (r < N && b < K / 32) {
         e = scales[((size_t) m * N + r) * ld_s + b];
-        f = e == 255 ? 31 : max(0, 15 + e - 127 - exps[(size_t) m * R + row]);
+        f = e == 255 ? 31 : min(max(0, 15 + e - 127 - exps[(size_t) m * R + row]), 30);        // (above 15 + TOP only for a block of zeros)
         if (e != 255) v = ((const uint4 *) codes)[((size_t) m * N + r) * (K / 32) + b];
     }
     out[at] = v;
@@ -300,7 +304,7 @@ JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long l
     const long long n = (long long) mx4::chunks(K) * (R / step) * 4;
     if ((n + 255) / 256 > 0x7fffffffll) return JIB_E_ARG;
     cudaStream_t s = (cudaStream_t) stream;
-    row_exponent_kernel<<<dim3((R / step + 3) / 4, batch), 128, 0, s>>>((const uint8_t *) scales, ld_s, exps, N, K, R, step, first);
+    row_exponent_kernel<<<dim3((R / step + 3) / 4, batch), 128, 0, s>>>((const uint4 *) codes, (const uint8_t *) scales, ld_s, exps, N, K, R, step, first);
     pack_kernel<<<dim3((unsigned) ((n + 255) / 256), batch), 256, 0, s>>>((const uint8_t *) codes, (const uint8_t *) scales, ld_s, exps, (uint4 *) out,
                                                                          (uint8_t *) out_scales, (uint8_t *) factors, N, K, R, step, first);
     return launched();

@@ -9,9 +9,10 @@
 // holds the 32 columns 32 t .. of rows g and g + 8, that is 16 bytes and one scale each, and step s of the chunk's eight multiplies its columns 4 s
 // .. 4 s + 3.  Decoding is one conversion instruction a byte (E2M1 pair to fp16 pair) and one product with the block's scale.  (Masks and shifts to
 // bf16 took eleven integer instructions for eight weights; 16 warps of an SM decoded and multiplied 38 weights a clock so, 66 with the
-// conversion.)  fp16 cannot hold every scale, so a factor is relative to the largest scale of its row: the upper byte of 2^(13 - (largest -
-// scale)) in fp16, exact up to 27 binades below the largest and 0 beyond, where a weight is less than 2^-25 of the row's largest; and a row has an
-// exponent (int) that its sum is multiplied with.  A block without a number (scale 255) has codes 0 and a factor of infinity.
+// conversion.)  fp16 cannot hold every scale, so a factor is relative to the largest scale of its row's blocks with a value: the upper byte of 2^(13 -
+// (largest - scale)) in fp16, exact up to 27 binades below the largest and 0 beyond, where a weight is less than 2^-24 of the row's largest (6 2^-28
+// of a value that is half its scale at least); and a row has an exponent (int) that its sum is multiplied with.  A block without a number (scale 255)
+// has codes 0 and a factor of infinity.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>

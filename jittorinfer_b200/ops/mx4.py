@@ -180,8 +180,9 @@ def _unpack(w: Mx4Weight, member: int) -> torch.Tensor:
     out = scaled(torch.where(e == 255, nan, _pow2(e - 127)))
     unit = _pow2(rows(w.exps[:, None, :, None]))
     again = scaled(torch.where(f == 31, nan, torch.where(f > 0, _pow2(f - 15), torch.zeros_like(nan))) * unit)
-    lost = rows(w.exps[:, None, :, None]).double()          # scales more than 27 binades below the largest are 0 in the second form
-    same = (out == again) | (out.isnan() & again.isnan()) | (out.abs() <= 6 * _pow2((lost - 14).int()).reshape(w.matrices, w.n, 1))
+    largest = out.nan_to_num(0.0).abs().amax(-1, keepdim=True)
+    lost = (again == 0) & (out.abs() < 2.0 ** -24 * largest)          # scales more than 27 binades below the largest are 0 in the second form
+    same = (out == again) | (out.isnan() & again.isnan()) | lost
     if not bool(same.all()):
         raise RuntimeError("the two forms of a packed weight's scales differ")
     out = out.float()

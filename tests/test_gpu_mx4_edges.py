@@ -56,3 +56,23 @@ def test_choices_outside_beside_what_is_not_a_number(nat, dtype, T):
     got = ops.mx4_moe_ffn(x, None, ids, wts, wgu, ops.mx4_weight(q))
     assert bool(got[0].isnan().all()) and not bool(got[1].any())
     within(got[1:], want[1:], lim[1:])
+
+
+# ---- scales far apart in a row ----------------------------------------------------------------------------------------------------
+@BOTH
+@pytest.mark.parametrize("T", [1, 3, 8, 20])
+def test_blocks_of_zeros_with_a_large_scale(nat, dtype, T):
+    """A block without a value says nothing of its row, whatever its scale."""
+    E, d, F, k = 4, 128, 96, 2
+    q = [ops.mx4_quantize(randn(*s, seed=i, scale=0.05)) for i, s in enumerate(((E, F, d), (E, F, d), (E, d, F)))]
+    for t, at in zip(q, (0, 3, 1)):
+        t.codes[..., 16 * at:16 * at + 16] = torch.tensor([0x80, 0x08, 0x00, 0x88], dtype=torch.uint8, device=DEV).repeat(4)
+        t.scales[..., at] = 254
+    gv, uv, dv = (mx4._dequantize(t, torch.float64) for t in q)
+    wgu, wd = ops.mx4_weight(q[0], q[1]), ops.mx4_weight(q[2])
+    assert all(torch.equal(a, b) for a, b in zip((*wgu.values(torch.float64), *wd.values(torch.float64)), (gv, uv, dv)))
+    x = randn(T, d, seed=7, dtype=dtype)
+    ids = torch.rand(T, E, generator=gen(T), device=DEV).argsort(-1)[:, :k].int()
+    wts = torch.rand(T, k, generator=gen(8), device=DEV)
+    want, lim = moe_want(x, None, ids, wts, gv, uv, dv)
+    within(ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd), want, lim)

@@ -322,8 +322,8 @@ JIB_EXPORT int jib_selective_scan(const jib_scan * m, int single, int f32, void 
 // type: 0 bf16, 1 fp16, 2 fp32.
 JIB_EXPORT int jib_mx4_quantize(const void * x, int type, long long ld, void * codes, void * scales, long long ld_s, int rows, int cols, void * stream);
 JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long long ld_s, void * out, int type, long long rows, int cols, void * stream);
-JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, void * out, void * out_scales, void * factors, int * exps, int batch, int N,
-                            int K, int step, int first, void * stream);
+JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, void * out, void * out_scales, void * factors, int * exps, int * lost, int batch,
+                            int N, int K, int step, int first, void * stream);
 // out[t][n] = sum_k a[t][k] b[n][k], both in 4 bits; scale rows are multiples of 16 bytes apart, all is 16-byte aligned.
 JIB_EXPORT int jib_mx4_matmul(const void * a_codes, const void * a_scales, long long a_ld, const void * b_codes, const void * b_scales, long long b_ld,
                               void * out, long long ldo, int out_f32, int T, int N, int K, int * status, void * stream);

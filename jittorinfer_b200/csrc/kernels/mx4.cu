@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(128) row_exponent_kernel(const uint4 * __restr
 // A thread moves 32 columns of a row: 16 bytes and a scale.
 __global__ void __launch_bounds__(256) pack_kernel(const uint8_t * __restrict__ codes, const uint8_t * __restrict__ scales, long long ld_s,
                                                    const int * __restrict__ exps, uint4 * __restrict__ out, uint8_t * __restrict__ out_scales,
-                                                   uint8_t * __restrict__ factors, int N, int K, int R, int step, int first) {
+                                                   uint8_t * __restrict__ factors, int * __restrict__ lost, int N, int K, int R, int step, int first) {
     const int C = mx4::chunks(K), rows = R / step, m = blockIdx.y;
     const long long id = (long long) blockIdx.x * blockDim.x + threadIdx.x;
     if (id >= (long long) C * rows * 4) return;
@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t * __restrict__ 
         e = scales[((size_t) m * N + r) * ld_s + b];
         f = e == 255 ? 31 : min(max(0, 15 + e - 127 - exps[(size_t) m * R + row]), 30);        // (above 15 + TOP only for a block of zeros)
         if (e != 255) v = ((const uint4 *) codes)[((size_t) m * N + r) * (K / 32) + b];
+        if (lost != nullptr && f == 0 && !no_value(v)) *lost = 1;
     }
     out[at] = v;
     out_scales[at] = (uint8_t) e;
@@ -294,9 +295,9 @@ JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long 
 }
 
 // Row-major codes and scales of `batch` matrices [N][K] to the order that the products read: out, out_scales, factors and exps of all (of pairs, with step 2, the
-// member `first`).
-JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, void * out, void * out_scales, void * factors, int * exps, int batch, int N,
-                            int K, int step, int first, void * stream) {
+// member `first`).  lost (or NULL): set to 1 where a weight's factor is 0 and the weight is not.
+JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, void * out, void * out_scales, void * factors, int * exps, int * lost, int batch,
+                            int N, int K, int step, int first, void * stream) {
     if (batch <= 0) return 0;
     if (N <= 0 || K <= 0 || K % 32 || ld_s < K / 32 || batch > 65535 || step < 1 || step > 2 || first < 0 || first >= step) return JIB_E_ARG;
     if (((uintptr_t) codes | (uintptr_t) out) & 15) return JIB_E_ALIGN;
@@ -306,7 +307,7 @@ JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long l
     cudaStream_t s = (cudaStream_t) stream;
     row_exponent_kernel<<<dim3((R / step + 3) / 4, batch), 128, 0, s>>>((const uint4 *) codes, (const uint8_t *) scales, ld_s, exps, N, K, R, step, first);
     pack_kernel<<<dim3((unsigned) ((n + 255) / 256), batch), 256, 0, s>>>((const uint8_t *) codes, (const uint8_t *) scales, ld_s, exps, (uint4 *) out,
-                                                                         (uint8_t *) out_scales, (uint8_t *) factors, N, K, R, step, first);
+                                                                         (uint8_t *) out_scales, (uint8_t *) factors, lost, N, K, R, step, first);
     return launched();
 }
 

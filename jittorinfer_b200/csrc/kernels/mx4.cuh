@@ -11,8 +11,8 @@
 // bf16 took eleven integer instructions for eight weights; 16 warps of an SM decoded and multiplied 38 weights a clock so, 66 with the
 // conversion.)  fp16 cannot hold every scale, so a factor is relative to the largest scale of its row's blocks with a value: the upper byte of 2^(13 -
 // (largest - scale)) in fp16, exact up to 27 binades below the largest and 0 beyond, where a weight is less than 2^-24 of the row's largest (6 2^-28
-// of a value that is half its scale at least); and a row has an exponent (int) that its sum is multiplied with.  A block without a number (scale 255)
-// has codes 0 and a factor of infinity.
+// of a value that is half its scale at least): layers of weights that have such rows run as tiled products.  A row has an exponent (int) that its sum
+// is multiplied with.  A block without a number (scale 255) has codes 0 and a factor of infinity.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>

@@ -99,12 +99,14 @@ class Mx4Tensor:
 class Mx4Weight:
     """A matrix [n, k], or ``batch`` of them, or as many gated pairs, in the order in which the products read it.  On the GPU ``codes`` and ``scales`` hold
     chunks of 128 columns, rows within them (of a pair 16 of each matrix in turn), ``factors`` and ``exps`` the scales again as the products of a few
-    tokens need them; elsewhere ``plain`` holds the tensors."""
-    __slots__ = ("n", "k", "batch", "gated", "codes", "scales", "factors", "exps", "plain")
+    tokens need them; ``far`` says that some weights of a batch lie too far below their row's largest scale for the latter, which then do not read it;
+    elsewhere ``plain`` holds the tensors."""
+    __slots__ = ("n", "k", "batch", "gated", "codes", "scales", "factors", "exps", "far", "plain")
 
     def __init__(self, n, k, batch, gated):
         self.n, self.k, self.batch, self.gated = n, k, batch, gated
         self.codes = self.scales = self.factors = self.exps = self.plain = None
+        self.far = False
 
     @property
     def device(self) -> torch.device:

@@ -168,7 +168,7 @@ def load():
     sig("jib_mla_flash", vp, vp, ll, ip, i, ip, ip, i, i, i, f, i, i, i, fp, fp, vp, ip, vp)
     sig("jib_mx4_quantize", vp, i, ll, vp, vp, ll, i, i, vp)
     sig("jib_mx4_dequantize", vp, vp, ll, vp, i, ll, i, vp)
-    sig("jib_mx4_pack", vp, vp, ll, vp, vp, vp, ip, i, i, i, i, i, vp)
+    sig("jib_mx4_pack", vp, vp, ll, vp, vp, vp, ip, ip, i, i, i, i, i, vp)
     sig("jib_mx4_matmul", vp, vp, ll, vp, vp, ll, vp, ll, i, i, i, i, ip, vp)
     sig("jib_mx4_product_simt", C.POINTER(Mx4Desc), vp)
     sig("jib_mx4_gemm_scratch", ll, i, i, i, i)

@@ -51,10 +51,13 @@ def pack(w: Mx4Weight, q: Mx4Tensor, up: Optional[Mx4Tensor]) -> None:
     w.scales = torch.empty(E, w.chunks, R, COLS // 32, dtype=torch.uint8, device=q.device)
     w.factors = torch.empty_like(w.scales)
     w.exps = torch.empty(E, R, dtype=torch.int32, device=q.device)
+    lost = torch.zeros(1, dtype=torch.int32, device=q.device) if w.batch else None
     with _on(q.codes):
         for m, t in enumerate(members):
             nat._ck(nat.load().jib_mx4_pack(t.codes.data_ptr(), t.scales.data_ptr(), t.scales.stride(-2), w.codes.data_ptr(), w.scales.data_ptr(),
-                                            w.factors.data_ptr(), w.exps.data_ptr(), E, w.n, w.k, len(members), m, nat._stream()), "mx4_pack")
+                                            w.factors.data_ptr(), w.exps.data_ptr(), nat._p(lost), E, w.n, w.k, len(members), m, nat._stream()), "mx4_pack")
+        # (read once, when weights are laid out; a graph that does so cannot say yet)
+        w.far = lost is not None and (torch.cuda.is_current_stream_capturing() or bool(lost.item()))
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -148,9 +151,9 @@ def matmul(a: Mx4Tensor, b: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
 _few_sizes: dict = {}        # (tokens, width, hidden, experts, choices) -> bytes of xf and h, floats of part, ints of sync, or None
 
 
-def _few(x: torch.Tensor, wgu: Mx4Weight, k: int):
+def _few(x: torch.Tensor, wgu: Mx4Weight, wd: Mx4Weight, k: int):
     """The buffers' sizes where a layer of few tokens runs as two launches."""
-    if x.dtype != torch.bfloat16 or x.shape[0] > FEW_TOKENS:
+    if x.dtype != torch.bfloat16 or x.shape[0] > FEW_TOKENS or wgu.far or wd.far:
         return None
     key = (x.shape[0], wgu.k, wgu.n, wgu.batch, k)
     if key not in _few_sizes:
@@ -194,7 +197,7 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act, n_shared=0):
     if wgu.batch > MAX_EXPERTS:
         raise ValueError(f"mx4_moe_ffn: {wgu.batch} experts, at most {MAX_EXPERTS}")
     with _on(x):
-        sizes = _few(x, wgu, k)
+        sizes = _few(x, wgu, wd, k)
         if sizes is not None:
             m = nat.Mx4MoeDesc()
             m.ids, m.wts, m.k = ids.data_ptr(), wts.data_ptr(), k
@@ -226,7 +229,7 @@ def moe_layer(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, w
         raise ValueError(f"mx4_moe_layer: {k} + {n_shared} of {wgu.batch} experts in {n_group} groups; at most {MAX_CHOICES} of {MAX_EXPERTS} in 32")
     with _on(x):
         x = x if x.stride(0) == d else x.contiguous()
-        sizes = _few(x, wgu, k + n_shared)
+        sizes = _few(x, wgu, wd, k + n_shared)
         if sizes is not None:
             if residual is not None and residual.stride(1) != 1:
                 residual = residual.contiguous()

@@ -76,3 +76,47 @@ def test_blocks_of_zeros_with_a_large_scale(nat, dtype, T):
     wts = torch.rand(T, k, generator=gen(8), device=DEV)
     want, lim = moe_want(x, None, ids, wts, gv, uv, dv)
     within(ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd), want, lim)
+
+
+def rescaled(q, add):
+    return ops.Mx4Tensor(q.codes, (q.scales.int() + add).to(torch.uint8))
+
+
+@BOTH
+@pytest.mark.parametrize("T", [1, 8, 9])
+@pytest.mark.parametrize("apart", [20, 60])
+def test_blocks_far_below_the_largest_of_their_row(nat, dtype, T, apart):
+    """The large blocks meet zeros, in x and in the hidden units: what is left are the small ones."""
+    E, d, F, k = 4, 160, 96, 2
+    qs = [ops.mx4_quantize(randn(*s, seed=i, scale=0.05)) for i, s in enumerate(((E, F, d), (E, F, d), (E, d, F)))]
+    adds = [torch.tensor([0] * 5, device=DEV), torch.tensor([apart] + [0] * 4, device=DEV), torch.tensor([apart, 0, 0], device=DEV)]
+    qs = [rescaled(q, a) for q, a in zip(qs, adds)]
+    gv, uv, dv = (mx4._dequantize(q, torch.float64) for q in qs)
+    x = randn(T, d, seed=7, dtype=dtype)
+    x[:, :32] = 0                                    # up: the large block
+    qs[0].codes[:, :32] = 0                          # gate: no hidden units where the down matrix is large
+    gv[:, :32] = 0
+    wgu, wd = ops.mx4_weight(qs[0], qs[1]), ops.mx4_weight(qs[2])
+    ids = torch.rand(T, E, generator=gen(T), device=DEV).argsort(-1)[:, :k].int()
+    wts = torch.rand(T, k, generator=gen(8), device=DEV)
+    want, lim = moe_want(x, None, ids, wts, gv, uv, dv)
+    got = ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd)
+    assert float(want.abs().min()) > 0 and float(lim.max()) < 0.05 * float(want.abs().max())
+    within(got, want, lim)
+
+
+def test_weights_laid_out_while_capturing(nat):
+    E, d, F, T = 4, 128, 96, 3
+    q = [ops.mx4_quantize(randn(*s, seed=i, scale=0.05)) for i, s in enumerate(((E, F, d), (E, F, d), (E, d, F)))]
+    x, ids, wts = randn(T, d, seed=7, dtype=torch.bfloat16), torch.tensor([[0, 1], [3, 1], [2, 2]], dtype=torch.int32, device=DEV), torch.rand(T, 2, generator=gen(8), device=DEV)
+    want, lim = moe_want(x, None, ids, wts, *(mx4._dequantize(t, torch.float64) for t in q))
+    ops.mx4_moe_ffn(x, None, ids, wts, ops.mx4_weight(q[0], q[1]), ops.mx4_weight(q[2]))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ops.mx4_moe_ffn(x, None, ids, wts, ops.mx4_weight(q[0], q[1]), ops.mx4_weight(q[2]))
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    within(got, want, lim)
+    del g

@@ -422,7 +422,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (chosen & (i & 1 ? 2 : 1)) acc[m][i] += y[m][i] * r[2 * m + (i >> 1)] * (i & 1 ? w1 : w0);
+                    // (the factors first: either alone may take y out of fp32's range where the result is well inside)
+                    if (chosen & (i & 1 ? 2 : 1)) acc[m][i] += y[m][i] * (r[2 * m + (i >> 1)] * (i & 1 ? w1 : w0));
         }
         float * mine = red + (gr & 1) * (L::RED / 4) + warp * L::SUMS * 32 + lane;
 #pragma unroll

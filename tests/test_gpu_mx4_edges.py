@@ -120,3 +120,24 @@ def test_weights_laid_out_while_capturing(nat):
     torch.cuda.synchronize()
     within(got, want, lim)
     del g
+
+
+@BOTH
+@pytest.mark.parametrize("T", [1, 8, 9])
+@pytest.mark.parametrize("first,second", [(-50, 120), (30, -110)])
+def test_large_down_weights_of_small_hidden_units(nat, dtype, T, first, second):
+    """Results of ordinary size whose factors are near the ends of fp32: no step in between may leave it."""
+    E, d, F, k = 4, 128, 96, 2
+    q = [ops.mx4_quantize(randn(*s, seed=i, scale=0.05)) for i, s in enumerate(((E, F, d), (E, F, d), (E, d, F)))]
+    q = [rescaled(t, a) for t, a in zip(q, (first, first, second))]
+    q[0].codes &= 0x77                               # positive: a large z passes as it is
+    gv, uv, dv = (mx4._dequantize(t, torch.float64) for t in q)
+    x = randn(T, d, seed=7, dtype=dtype).abs()
+    ids = torch.rand(T, E, generator=gen(T), device=DEV).argsort(-1)[:, :k].int()
+    wts = torch.rand(T, k, generator=gen(8), device=DEV)
+    want, lim = moe_want(x, None, ids, wts, gv, uv, dv)
+    # the hidden units' limit has 1e-30 for fp32's smallest numbers, which here would be all of it: from 2^-100 on they are 2^49 steps of 2^-149 and more
+    lim = lim - sum(wts[:, j, None].double() * 1e-30 * dv[ids[:, j].long()].abs().sum(-1) for j in range(k)) * (1 + 2.0 ** -8 * (dtype == torch.bfloat16))
+    assert float((lim / want.abs()).median()) < 0.2
+    got = ops.mx4_moe_ffn(x, None, ids, wts, ops.mx4_weight(q[0], q[1]), ops.mx4_weight(q[2]))
+    within(got, want, lim.clamp(min=0) + 2.0 ** -20 * want.abs())

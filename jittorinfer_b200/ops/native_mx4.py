@@ -228,7 +228,8 @@ def moe_layer(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, w
     if k + n_shared > MAX_CHOICES or wgu.batch > MAX_EXPERTS or n_group > 32:
         raise ValueError(f"mx4_moe_layer: {k} + {n_shared} of {wgu.batch} experts in {n_group} groups; at most {MAX_CHOICES} of {MAX_EXPERTS} in 32")
     with _on(x):
-        x = x if x.stride(0) == d else x.contiguous()
+        if x.stride(0) != d:           # (a single row counts as contiguous whatever its stride)
+            x = x.clone(memory_format=torch.contiguous_format) if T > 1 else x.as_strided((1, d), (d, 1))
         sizes = _few(x, wgu, wd, k + n_shared)
         if sizes is not None:
             if residual is not None and residual.stride(1) != 1:

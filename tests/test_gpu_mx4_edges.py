@@ -141,3 +141,20 @@ def test_large_down_weights_of_small_hidden_units(nat, dtype, T, first, second):
     assert float((lim / want.abs()).median()) < 0.2
     got = ops.mx4_moe_ffn(x, None, ids, wts, ops.mx4_weight(q[0], q[1]), ops.mx4_weight(q[2]))
     within(got, want, lim.clamp(min=0) + 2.0 ** -20 * want.abs())
+
+
+# ---- rows, strides and sizes ------------------------------------------------------------------------------------------------------
+@BOTH
+@pytest.mark.parametrize("T", [1, 2])
+def test_a_row_of_a_wider_tensor(nat, dtype, T):
+    """One token's stride is any: PyTorch calls its row contiguous."""
+    E, d, F = 8, 128, 64
+    wgu, wd, *_ = experts(E, d, F)
+    x, res = randn(T, 3 * d, seed=1, dtype=dtype), randn(T, 2 * d, seed=2, dtype=dtype)
+    router = randn(E, d, seed=3, scale=0.1)
+    args = (router, None, 2, 1, 1, 1.0, True, False, wgu, wd)
+    want = ops.mx4_moe_layer(x[:, d:2 * d].clone(), *args, residual=res[:, d:].clone())
+    got = ops.mx4_moe_layer(x[:, d:2 * d], *args, residual=res[:, d:])
+    assert torch.equal(got, want)
+    ids, wts = torch.zeros(T, 1, dtype=torch.int32, device=DEV), torch.ones(T, 1, device=DEV)
+    assert torch.equal(ops.mx4_moe_ffn(x[:, d:2 * d], res[:, d:], ids, wts, wgu, wd), ops.mx4_moe_ffn(x[:, d:2 * d].clone(), res[:, d:].clone(), ids, wts, wgu, wd))

@@ -918,6 +918,7 @@ static bool gate_args_ok(int E, int k, int n_group, int n_shared) {
 static int router_of(const void * g, const float * w_router, float * logits, int T, int d, int E, void * stream) {
     if (g == nullptr) return 0;
     if (d % 8 || d > GATE_MAXC * GATE_NT * 8) return JIB_E_ARG;
+    if (((uintptr_t) g | (uintptr_t) w_router) & 15) return JIB_E_ALIGN;          // (read 16 bytes at a time)
     return launch_router((const bf16 *) g, w_router, logits, T, d, E, (cudaStream_t) stream);
 }
 
@@ -962,6 +963,7 @@ int jib_moe_route_fused(const void * g, const float * w_router, const float * bi
     if (T > ROUTE_MAX_T || counter == nullptr || E_local > MAX_E || E_local < 1) return JIB_E_ARG;
     if (E > MAX_E || k + n_shared > 32 || n_shared < 0 || k > E || d % 8 || d > GATE_MAXC * GATE_NT * 8 || n_group > 32 || (n_group > 1 && E % n_group)) return JIB_E_ARG;
     if (norm_w != nullptr && g_out == nullptr) return JIB_E_ARG;
+    if (((uintptr_t) g | (uintptr_t) w_router | (uintptr_t) norm_w | (uintptr_t) g_out) & 15) return JIB_E_ALIGN;
     JIB_LAUNCH((moe_route_fused_kernel), E, GATE_NT, 0, (cudaStream_t) stream, (const bf16 *) g, w_router, bias, logits, ids, wts, seg,
                src_token, dest, counter, T, d, E, k, n_group, topk_group, scale, norm, sigmoid, n_shared, group_top2, expert_base, E_local,
                norm_w, eps, (bf16 *) g_out, route_warm() ? 1 : 0);

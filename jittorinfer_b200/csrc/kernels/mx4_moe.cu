@@ -560,7 +560,7 @@ JIB_EXPORT int jib_mx4_moe_prepare(const void * x, long long ldx, const float * 
                                    void * stream) {
     if (w_router == nullptr) E = 0;
     if (T < 1 || T > MAX_T || E < 0 || E > MAX_E || d % 32 || d > GATE_MAXC * GATE_NT * 8 || (E > 0 && ldx != d)) return JIB_E_ARG;
-    if (((uintptr_t) x | (uintptr_t) (ldx * 2) | (uintptr_t) xf) & 15) return JIB_E_ALIGN;
+    if (((uintptr_t) x | (uintptr_t) (ldx * 2) | (uintptr_t) xf | (uintptr_t) w_router) & 15) return JIB_E_ALIGN;
     JIB_LAUNCH((mx4_prepare_kernel), E + 8, GATE_NT, 0, (cudaStream_t) stream, (const bf16 *) x, ldx, w_router, logits, (uint4 *) xf, sync, n_sync, T, d, E);
     return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH;
 }

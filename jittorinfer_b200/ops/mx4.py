@@ -351,7 +351,7 @@ def mx4_moe_layer(x: torch.Tensor, w_router: torch.Tensor, bias: Optional[torch.
         raise ValueError(f"mx4_moe_layer: {k} of {E} experts in {topk_group} of {n_group} groups")
     n = _native(x)
     if n:
-        return n.moe_layer(x, w_router.contiguous(), bias if bias is None else bias.contiguous(), k, n_group, topk_group, scale, norm, sigmoid, wgu, wd,
+        return n.moe_layer(x, w_router, bias if bias is None else bias.contiguous(), k, n_group, topk_group, scale, norm, sigmoid, wgu, wd,
                            n_shared, group_top2, residual, act)
     ids, wts = ref.moe_gate(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, n_shared, group_top2)
     return _moe_plain(x, residual, ids, wts, wgu, wd, act)

@@ -66,6 +66,12 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
+def _vectors(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and 16-byte aligned."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _desc(w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act: Optional[str]) -> "nat.Mx4Desc":
     d = nat.Mx4Desc()
     d.w, d.w_scales = w.codes.data_ptr(), w.scales.data_ptr()
@@ -228,6 +234,7 @@ def moe_layer(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, w
     if k + n_shared > MAX_CHOICES or wgu.batch > MAX_EXPERTS or n_group > 32:
         raise ValueError(f"mx4_moe_layer: {k} + {n_shared} of {wgu.batch} experts in {n_group} groups; at most {MAX_CHOICES} of {MAX_EXPERTS} in 32")
     with _on(x):
+        w_router = _vectors(w_router)
         if x.stride(0) != d:           # (a single row counts as contiguous whatever its stride)
             x = x.clone(memory_format=torch.contiguous_format) if T > 1 else x.as_strided((1, d), (d, 1))
         sizes = _few(x, wgu, wd, k + n_shared)

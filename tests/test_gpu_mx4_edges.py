@@ -158,3 +158,19 @@ def test_a_row_of_a_wider_tensor(nat, dtype, T):
     assert torch.equal(got, want)
     ids, wts = torch.zeros(T, 1, dtype=torch.int32, device=DEV), torch.ones(T, 1, device=DEV)
     assert torch.equal(ops.mx4_moe_ffn(x[:, d:2 * d], res[:, d:], ids, wts, wgu, wd), ops.mx4_moe_ffn(x[:, d:2 * d].clone(), res[:, d:].clone(), ids, wts, wgu, wd))
+
+
+def behind(t, elements):
+    """A contiguous copy that begins so many elements behind an aligned address."""
+    at = torch.zeros(t.numel() + 8, dtype=t.dtype, device=t.device)[elements:elements + t.numel()].view(t.shape)
+    return at.copy_(t)
+
+
+@BOTH
+@pytest.mark.parametrize("T", [1, 3, 20])
+def test_a_router_at_an_odd_address(nat, dtype, T):
+    E, d, F = 8, 128, 64
+    wgu, wd, *_ = experts(E, d, F)
+    x, router = randn(T, d, seed=1, dtype=dtype), randn(E, d, seed=3, scale=0.1)
+    args = (None, 2, 1, 1, 1.0, True, False, wgu, wd)
+    assert torch.equal(ops.mx4_moe_layer(behind(x, 1), behind(router, 1), *args), ops.mx4_moe_layer(x, router, *args))

@@ -1,0 +1,81 @@
+"""What the expert layers over 4-bit weights hand to their launches when tensors are views, and what the launches refuse: addresses only, nothing is computed."""
+import contextlib
+import ctypes as C
+import types
+
+import pytest
+import torch
+
+from jittorinfer_b200 import build
+from jittorinfer_b200.ops import mx4, native, native_mx4
+
+E, D, F, K = 8, 64, 32, 2
+ALIGN = -2                     # JIB_E_ALIGN
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """(name, arguments) of the launches; the library is not called."""
+    seen = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: seen.append((name, a)) or int(name in ("jib_mx4_moe_sizes", "jib_mx4_gemm_scratch"))
+
+    def launched(rc, what):
+        pass
+    monkeypatch.setattr(native, "load", lambda: Lib())
+    monkeypatch.setattr(native, "_ck", launched)
+    monkeypatch.setattr(native, "_stream", lambda: 0)
+    monkeypatch.setattr(native, "workspace", lambda dev: types.SimpleNamespace(status=torch.zeros(4, dtype=torch.int32)))
+    monkeypatch.setattr(native_mx4, "_on", lambda t: contextlib.nullcontext())
+    monkeypatch.setattr(native_mx4, "_few_sizes", {})
+    monkeypatch.setattr(native_mx4, "_scratch_bytes", {})
+    return seen
+
+
+def packed(n, k, gated):
+    w = mx4.Mx4Weight(n, k, E, gated)
+    w.codes = w.scales = w.factors = w.exps = torch.zeros(64, dtype=torch.uint8)
+    return w
+
+
+def view(rows, cols, dtype, offset):
+    """Contiguous rows that begin `offset` elements behind an aligned address."""
+    return torch.zeros(rows * cols + 8, dtype=dtype)[offset:offset + rows * cols].view(rows, cols)
+
+
+def layer(T, router, residual=None):
+    return native_mx4.moe_layer(torch.zeros(T, D, dtype=torch.bfloat16), router, None, K, 1, 1, 1.0, False, False, packed(F, D, True), packed(D, F, False), 0, False,
+                                residual, "silu")
+
+
+@pytest.mark.parametrize("T,launch,at", [(3, "jib_mx4_moe_prepare", 2), (20, "jib_moe_gate", 1)])
+@pytest.mark.parametrize("offset", [0, 1, 3])
+def test_a_router_at_an_odd_address_is_copied(calls, T, launch, at, offset):
+    router = view(E, D, torch.float32, offset)
+    layer(T, router)
+    given = next(a[at] for name, a in calls if name == launch)
+    assert given % 16 == 0 and (given == router.data_ptr()) == (offset == 0)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return C.CDLL(build.build_kernels())
+
+
+P = C.c_void_p
+ALL = 1 << 20                  # an aligned address that is not read
+
+
+@pytest.mark.parametrize("odd", [0, 1])
+def test_a_router_at_an_odd_address_is_refused(lib, odd):
+    a = [P(ALL), P(ALL)]
+    a[odd] = P(ALL + 4)
+    x, w = a
+    f, z = C.c_float(1.0), C.c_longlong(D)
+    assert lib.jib_mx4_moe_prepare(x, z, w, P(ALL), P(ALL), P(ALL), 4, 3, D, E, None) == ALIGN
+    for T in (3, 20):
+        assert lib.jib_moe_gate(x, w, None, None, P(ALL), P(ALL), P(ALL), T, D, E, K, 1, 1, f, 0, 0, 0, 0, 0, None) == ALIGN
+        assert lib.jib_moe_gate_sort(x, w, None, None, P(ALL), P(ALL), P(ALL), T, D, E, K, 1, 1, f, 0, 0, 0, 0, 0, 0, E, P(ALL), P(ALL), P(ALL), P(ALL), None) == ALIGN
+    assert lib.jib_moe_route_fused(x, w, None, P(ALL), P(ALL), P(ALL), P(ALL), P(ALL), P(ALL), P(ALL), 3, D, E, K, 1, 1, f, 0, 0, 0, 0, 0, E, None, f, None, None) == ALIGN

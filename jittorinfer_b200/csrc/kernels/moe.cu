@@ -1008,6 +1008,7 @@ int jib_moe_combine(const void * y, const int * dest, const float * wts, const v
                     int k, int d, void * stream) {
     if (T <= 0) return 0;
     if (d % 8) return JIB_E_ARG;
+    if (((uintptr_t) y | (uintptr_t) shared | (uintptr_t) residual | (uintptr_t) out) & 15) return JIB_E_ALIGN;          // (rows go 16 bytes at a time)
     JIB_LAUNCH((moe_combine_kernel), T, 256, 0, (cudaStream_t) stream, (const bf16 *) y, dest, wts, (const bf16 *) shared, (const bf16 *) residual,
                                                               (bf16 *) out, k, d, jib::warm_for(T));
     return launched();
@@ -1018,6 +1019,7 @@ int jib_moe_combine_norm(const void * y, const int * dest, const float * wts, co
                          const float * norm_w, void * out, void * out_norm, int T, int k, int d, float eps, void * stream) {
     if (T <= 0) return 0;
     if (d % 8 || norm_w == nullptr || out_norm == nullptr) return JIB_E_ARG;
+    if (((uintptr_t) y | (uintptr_t) shared | (uintptr_t) residual | (uintptr_t) norm_w | (uintptr_t) out | (uintptr_t) out_norm) & 15) return JIB_E_ALIGN;
     const int nv = d / 8;
     cudaStream_t s = (cudaStream_t) stream;
 #define JIB_CN(NT, MAXV)                                                                                                         \

@@ -217,7 +217,7 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act, n_shared=0):
             nat._ck(nat.load().jib_mx4_sort(ids.data_ptr(), n, k, E, first, count, row_src, pair_row, nat._stream()), "mx4_sort")
             routed = T * (k - n_shared) * E // (E - n_shared)       # the rows were there no shared experts: what the tiles are chosen for
             y = _grouped(x, wgu, wd, (first, count, cap), row_src, routed, act)
-            return nat.moe_combine(y, table[2 * E + 1 + cap:].view(T, k), wts, None, None if residual is None else residual.contiguous())
+            return nat.moe_combine(y, table[2 * E + 1 + cap:].view(T, k), wts, None, None if residual is None else _vectors(residual))
         seg, src, dest = nat.moe_permute(ids, 0, E)
         h = _grouped_simt(x, wgu, seg, src, n, act)
         y = _grouped_simt(h, wd, seg, None, n, None)

@@ -174,3 +174,16 @@ def test_a_router_at_an_odd_address(nat, dtype, T):
     x, router = randn(T, d, seed=1, dtype=dtype), randn(E, d, seed=3, scale=0.1)
     args = (None, 2, 1, 1, 1.0, True, False, wgu, wd)
     assert torch.equal(ops.mx4_moe_layer(behind(x, 1), behind(router, 1), *args), ops.mx4_moe_layer(x, router, *args))
+
+
+@BOTH
+@pytest.mark.parametrize("T", [1, 3, 9, 20])
+def test_a_residual_at_an_odd_address(nat, dtype, T):
+    E, d, F = 8, 128, 64
+    wgu, wd, *_ = experts(E, d, F)
+    x, res, router = randn(T, d, seed=1, dtype=dtype), randn(T, d, seed=2, dtype=dtype), randn(E, d, seed=3, scale=0.1)
+    ids, wts = torch.randint(0, E, (T, 2), generator=gen(3), device=DEV, dtype=torch.int32), torch.rand(T, 2, generator=gen(4), device=DEV)
+    args = (router, None, 2, 1, 1, 1.0, True, False, wgu, wd)
+    for at in (1, 4):
+        assert torch.equal(ops.mx4_moe_layer(x, *args, residual=behind(res, at)), ops.mx4_moe_layer(x, *args, residual=res))
+        assert torch.equal(ops.mx4_moe_ffn(x, behind(res, at), behind(ids, 1), behind(wts, 1), wgu, wd), ops.mx4_moe_ffn(x, res, ids, wts, wgu, wd))

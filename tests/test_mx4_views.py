@@ -79,3 +79,18 @@ def test_a_router_at_an_odd_address_is_refused(lib, odd):
         assert lib.jib_moe_gate(x, w, None, None, P(ALL), P(ALL), P(ALL), T, D, E, K, 1, 1, f, 0, 0, 0, 0, 0, None) == ALIGN
         assert lib.jib_moe_gate_sort(x, w, None, None, P(ALL), P(ALL), P(ALL), T, D, E, K, 1, 1, f, 0, 0, 0, 0, 0, 0, E, P(ALL), P(ALL), P(ALL), P(ALL), None) == ALIGN
     assert lib.jib_moe_route_fused(x, w, None, P(ALL), P(ALL), P(ALL), P(ALL), P(ALL), P(ALL), P(ALL), 3, D, E, K, 1, 1, f, 0, 0, 0, 0, 0, E, None, f, None, None) == ALIGN
+
+
+@pytest.mark.parametrize("offset", [0, 1, 4])
+def test_a_residual_at_an_odd_address_is_copied_for_the_weighted_sum(calls, offset):
+    residual = view(20, D, torch.bfloat16, offset)
+    layer(20, torch.zeros(E, D), residual)
+    given = next(a[4] for name, a in calls if name == "jib_moe_combine")
+    assert given % 16 == 0 and (given == residual.data_ptr()) == (offset == 0)
+
+
+@pytest.mark.parametrize("odd", range(4))
+def test_rows_at_an_odd_address_are_refused_by_the_weighted_sum(lib, odd):
+    y, shared, residual, out = (P(ALL + 2 * (i == odd)) for i in range(4))
+    assert lib.jib_moe_combine(y, P(ALL), P(ALL), shared, residual, out, 20, K, D, None) == ALIGN
+    assert lib.jib_moe_combine_norm(y, P(ALL), P(ALL), shared, residual, P(ALL), out, P(ALL), 20, K, D, C.c_float(1e-6), None) == ALIGN

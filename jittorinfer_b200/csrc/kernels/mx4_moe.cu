@@ -105,7 +105,11 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_moe_kernel(const MoeArgs g) {
     __syncthreads();
     PDL_TRIGGER_TOP();
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
-    if (warp % g.gw == 0 && lane < AHEAD) drawn[warp / g.gw * KNOWN + lane] = (long long) lane << 32 | atomicAdd(g.sync, 1);
+    if (warp % g.gw == 0) {
+        // one draw for all: a group stops at its first unit that is none, so its units have to ascend, and lanes' own draws come in any order
+        const int unit0 = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(g.sync, AHEAD) : 0, 0);
+        if (lane < AHEAD) drawn[warp / g.gw * KNOWN + lane] = (long long) lane << 32 | (unit0 + lane);
+    }
     if (threadIdx.x == THREADS - 1) {
         word[1] = 0;
         mbar_expect_tx(acts_full, L::frags(g.d));

@@ -187,3 +187,19 @@ def test_a_residual_at_an_odd_address(nat, dtype, T):
     for at in (1, 4):
         assert torch.equal(ops.mx4_moe_layer(x, *args, residual=behind(res, at)), ops.mx4_moe_layer(x, *args, residual=res))
         assert torch.equal(ops.mx4_moe_ffn(x, behind(res, at), behind(ids, 1), behind(wts, 1), wgu, wd), ops.mx4_moe_ffn(x, res, ids, wts, wgu, wd))
+
+
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 66, 8), (3, 5, 2), (8, 256, 8)])
+@pytest.mark.parametrize("F", [32, 64, 96, 448])
+def test_few_units_over_many_groups(nat, T, E, k, F):
+    """Where the units of gate and up end within a group's first draws, again and again: every run gives every unit's part."""
+    d = 64
+    wgu, wd, gv, uv, dv = experts(E, d, F, seed=F)
+    x = randn(T, d, seed=T, dtype=torch.bfloat16)
+    ids = torch.rand(T, E, generator=gen(T), device=DEV).argsort(-1)[:, :k].int()
+    wts = torch.rand(T, k, generator=gen(8), device=DEV)
+    want, lim = moe_want(x, None, ids, wts, gv, uv, dv)
+    first = ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd)
+    within(first, want, lim)
+    assert all(torch.equal(ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd), first) for _ in range(30))
+    nat.check_status()

@@ -346,7 +346,8 @@ JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, void * stream);
 JIB_EXPORT long long jib_mx4_gemm_scratch(long long rows, int N, int K, int gated, int grouped);
 JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, int * count, int * row_src, int * pair_row, void * stream);
 JIB_EXPORT int jib_mx4_gemm_joins(int N, int gated);
-JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, void * next, int ready, void * stream);
+JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, long long scratch_bytes, void * next, long long next_bytes, int ready,
+                            void * stream);
 // A mixture-of-experts layer for up to 8 tokens (mx4_moe.cu).
 typedef struct jib_mx4_moe_desc {
     const void * residual;                 // NULL, or bf16 [T][d], rows ldr elements apart
@@ -361,7 +362,7 @@ typedef struct jib_mx4_moe_desc {
     float * part;                          // scratch
     int * sync;                            // zeros
     int * status;
-    long long ldr;
+    long long ldr, part_floats;            // (what there is room for)
     int T, d, F, E, k, n_group, topk_group, norm, sigmoid, n_shared, group_top2, act;
     float scale;
 } jib_mx4_moe_desc;

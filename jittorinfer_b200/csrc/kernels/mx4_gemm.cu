@@ -727,7 +727,7 @@ struct Scratch {
     Scratch(long long rows, int N, int K, bool gated, bool grouped) {
         const int C = mx4::chunks(K), R = mx4::rows_of(N, gated), m_tiles = (R + BM - 1) / BM;
         scales = 2 * rows * C * 128;
-        part = scales + 2ll * C * scale_rows_of(rows) * 4;
+        part = planes(rows, C);
         counters = part;
         if (!grouped) {
             shape_of(rows, R, C, &bn, &splits);
@@ -738,6 +738,7 @@ struct Scratch {
         }
         bytes = counters + 4ll * tiles;
     }
+    static long long planes(long long rows, int C) { return 2 * rows * C * 128 + 2ll * C * scale_rows_of(rows) * 4; }
 };
 
 }  // namespace
@@ -758,15 +759,17 @@ JIB_EXPORT int jib_mx4_sort(const int * ids, int n, int k, int E, int * first, i
 }
 
 // The tiled product of bf16 rows d->x: as planes, then multiplied.  Grouped: d->seg = first, count, d->src = row_src of jib_mx4_sort (NULL: x in that order), T
-// rows at most.  scratch: jib_mx4_gemm_scratch(T, ..) bytes; ready: it holds the planes already (then d->x is not read).  next (grouped pairs of more than one
+// rows at most.  scratch: jib_mx4_gemm_scratch(T, ..) bytes on this device at least; ready: it holds the planes already (then d->x is not read).  next (grouped pairs of more than one
 // tile of weights, see jib_mx4_gemm_joins): the scratch of a product of the results, which go there as planes and not to d->out.
-JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, void * next, int ready, void * stream) {
+JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * scratch, long long scratch_bytes, void * next, long long next_bytes, int ready,
+                            void * stream) {
     if (d->T <= 0) return 0;
     if (d->N <= 0 || d->K <= 0 || d->K % 32 || d->batch < 1 || d->batch > MAX_E || (d->seg != nullptr && (count == nullptr || d->residual != nullptr)) ||
         (next != nullptr && (!jib_mx4_gemm_joins(d->N, d->gated) || d->seg == nullptr || !d->gated || ((uintptr_t) next & 15))) || (ready && d->seg == nullptr))
         return JIB_E_ARG;
     if (((uintptr_t) d->x | (uintptr_t) (d->ldx * 2) | (uintptr_t) scratch | (uintptr_t) d->w_scales) & 15) return JIB_E_ALIGN;
     const Scratch sc(d->T, d->N, d->K, d->gated != 0, d->seg != nullptr);
+    if (scratch_bytes < sc.bytes || (next != nullptr && next_bytes < Scratch::planes(d->T, mx4::chunks(d->N)))) return JIB_E_SCRATCH;
     uint8_t * planes = (uint8_t *) scratch, * x_scales = planes + sc.scales;
     const int sms = sm_count();
     Args g;

@@ -580,6 +580,7 @@ JIB_EXPORT int jib_mx4_moe(const jib_mx4_moe_desc * m, void * stream) {
         return JIB_E_ARG;
     if (((uintptr_t) m->gu | (uintptr_t) m->down | (uintptr_t) m->gu_factors | (uintptr_t) m->down_factors | (uintptr_t) m->gu_exp | (uintptr_t) m->h | (uintptr_t) m->xf | (uintptr_t) m->part | (uintptr_t) m->sync | (uintptr_t) m->down_exp) & 15)
         return JIB_E_ALIGN;
+    if (m->part_floats < sizes[2]) return JIB_E_SCRATCH;          // (goes by the device's SMs)
     MoeArgs a;
     a.xf = (const uint4 *) m->xf; a.residual = (const bf16 *) m->residual; a.logits = m->logits; a.bias = m->bias; a.ids = m->ids; a.wts = m->wts;
     a.gu = (const uint8_t *) m->gu; a.down = (const uint8_t *) m->down; a.gu_exp = m->gu_exp; a.down_exp = m->down_exp;

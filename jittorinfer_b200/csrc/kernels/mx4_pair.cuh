@@ -71,14 +71,14 @@ __device__ __forceinline__ void load(void * dst, const CUtensorMap * m, uint64_t
     } else tma_load_2d(dst, m, bar, x, y);
 }
 
-// Pairs of CTAs that run at a time (0: not one); known: zeros, of each device.
+// Pairs of CTAs that run at a time (0: not one); known: zeros, of each device.  An answer stands, that there are none too: sizes of buffers go by it.
 template <typename... P>
 int pair_count(void (*kern)(P...), int threads, int smem, std::atomic<int> (&known)[jib::MAX_DEVICES], std::atomic<unsigned char> (&attr_done)[jib::MAX_DEVICES]) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= jib::MAX_DEVICES) return 0;
     int n = known[dev].load();
     if (n == 0) {
-        if (!jib::ensure_dyn_smem(kern, smem, attr_done)) return 0;
+        const bool ready = jib::ensure_dyn_smem(kern, smem, attr_done);
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2);
         cfg.blockDim = dim3(threads);
@@ -89,10 +89,13 @@ int pair_count(void (*kern)(P...), int threads, int smem, std::atomic<int> (&kno
         attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
-        known[dev].store(n);
+        if (!ready || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+            n = 0;
+            (void) cudaGetLastError();           // (else the next launch would be blamed)
+        }
+        known[dev].store(n > 0 ? n : -1);
     }
-    return n;
+    return n > 0 ? n : 0;
 }
 
 }  // namespace mx4

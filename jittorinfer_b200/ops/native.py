@@ -110,7 +110,7 @@ class Mx4Desc(C.Structure):
 class Mx4MoeDesc(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("residual", "logits", "bias", "ids", "wts", "gu", "down", "gu_factors", "down_factors", "gu_exp", "down_exp",
                                           "xf", "h", "out", "part", "sync", "status")] + \
-               [(n, C.c_longlong) for n in ("ldr",)] + \
+               [(n, C.c_longlong) for n in ("ldr", "part_floats")] + \
                [(n, C.c_int) for n in ("T", "d", "F", "E", "k", "n_group", "topk_group", "norm", "sigmoid", "n_shared", "group_top2", "act")] + [("scale", C.c_float)]
 
 
@@ -175,7 +175,7 @@ def load():
     L.jib_mx4_gemm_scratch.restype = ll
     sig("jib_mx4_sort", ip, i, i, i, ip, ip, ip, ip, vp)
     sig("jib_mx4_gemm_joins", i, i)
-    sig("jib_mx4_gemm", C.POINTER(Mx4Desc), ip, vp, vp, i, vp)
+    sig("jib_mx4_gemm", C.POINTER(Mx4Desc), ip, vp, ll, vp, ll, i, vp)
     sig("jib_mx4_moe_sizes", i, i, i, i, i, C.POINTER(ll))
     sig("jib_mx4_moe_prepare", vp, ll, fp, fp, vp, ip, i, i, i, i, vp)
     sig("jib_mx4_moe", C.POINTER(Mx4MoeDesc), vp)

@@ -84,16 +84,16 @@ def _desc(w: Mx4Weight, out: torch.Tensor, residual: Optional[torch.Tensor], act
     return d
 
 
-_scratch_bytes: dict = {}        # (rows, n, k, gated, grouped)
+_scratch_bytes: dict = {}        # (rows, n, k, gated, grouped, device): tiles and splits go by a device's SMs
 
 
 def _scratch(rows: int, w: Mx4Weight, grouped: bool, device) -> torch.Tensor:
-    key = (rows, w.n, w.k, int(w.gated), int(grouped))
+    key = (rows, w.n, w.k, int(w.gated), int(grouped), device)
     n = _scratch_bytes.get(key)
     if n is None:
         if len(_scratch_bytes) > 4096:
             _scratch_bytes.clear()
-        n = _scratch_bytes[key] = nat.load().jib_mx4_gemm_scratch(*key)
+        n = _scratch_bytes[key] = nat.load().jib_mx4_gemm_scratch(*key[:5])
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
@@ -108,7 +108,7 @@ def product(x: torch.Tensor, w: Mx4Weight, residual: Optional[torch.Tensor], dty
             if x.dtype == torch.bfloat16:
                 scratch = _scratch(x.shape[0], w, False, x.device)
                 d.x, d.ldx = x.data_ptr(), x.stride(0)
-                nat._ck(nat.load().jib_mx4_gemm(C.byref(d), None, scratch.data_ptr(), None, 0, nat._stream()), "mx4_gemm")
+                nat._ck(nat.load().jib_mx4_gemm(C.byref(d), None, scratch.data_ptr(), scratch.numel(), None, 0, 0, nat._stream()), "mx4_gemm")
             else:
                 d.x, d.ldx = x.data_ptr(), x.stride(0)
                 nat._ck(nat.load().jib_mx4_product_simt(C.byref(d), nat._stream()), "mx4_product_simt")
@@ -135,10 +135,10 @@ def _grouped(x: torch.Tensor, wgu: Mx4Weight, wd: Mx4Weight, pad, src: int, pair
     y = torch.empty(cap, wd.n, dtype=torch.bfloat16, device=x.device)
     d = _desc(wgu, h, None, act)
     d.T, d.x, d.ldx, d.seg, d.src, d.batch, d.max_rows = cap, x.data_ptr(), x.stride(0), first, src, wgu.batch, pairs
-    nat._ck(L.jib_mx4_gemm(C.byref(d), count, scratch.data_ptr(), then.data_ptr() if joined else None, 0, stream), "mx4_grouped")
+    nat._ck(L.jib_mx4_gemm(C.byref(d), count, scratch.data_ptr(), scratch.numel(), then.data_ptr() if joined else None, then.numel(), 0, stream), "mx4_grouped")
     d = _desc(wd, y, None, None)
     d.x, d.ldx, d.seg, d.batch, d.max_rows = h.data_ptr(), wgu.n, first, wd.batch, pairs
-    nat._ck(L.jib_mx4_gemm(C.byref(d), count, then.data_ptr(), None, joined, stream), "mx4_grouped")
+    nat._ck(L.jib_mx4_gemm(C.byref(d), count, then.data_ptr(), then.numel(), None, 0, joined, stream), "mx4_grouped")
     return y
 
 
@@ -154,17 +154,17 @@ def matmul(a: Mx4Tensor, b: Mx4Tensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
-_few_sizes: dict = {}        # (tokens, width, hidden, experts, choices) -> bytes of xf and h, floats of part, ints of sync, or None
+_few_sizes: dict = {}        # (tokens, width, hidden, experts, choices, device) -> bytes of xf and h, floats of part, ints of sync, or None
 
 
 def _few(x: torch.Tensor, wgu: Mx4Weight, wd: Mx4Weight, k: int):
     """The buffers' sizes where a layer of few tokens runs as two launches."""
     if x.dtype != torch.bfloat16 or x.shape[0] > FEW_TOKENS or wgu.far or wd.far:
         return None
-    key = (x.shape[0], wgu.k, wgu.n, wgu.batch, k)
+    key = (x.shape[0], wgu.k, wgu.n, wgu.batch, k, x.device)
     if key not in _few_sizes:
         s = (C.c_longlong * 4)()
-        _few_sizes[key] = tuple(s) if nat.load().jib_mx4_moe_sizes(*key, s) else None
+        _few_sizes[key] = tuple(s) if nat.load().jib_mx4_moe_sizes(*key[:5], s) else None
     return _few_sizes[key]
 
 
@@ -176,7 +176,7 @@ def _few_layer(x, residual, wgu: Mx4Weight, wd: Mx4Weight, sizes, act: str, m, w
     E = w_router.shape[0] if w_router is not None else 0
     scratch = torch.empty(xf + h + 4 * (part + sync + T * E), dtype=torch.uint8, device=x.device)
     m.out, m.xf = out.data_ptr(), scratch.data_ptr()
-    m.h, m.part, m.sync = m.xf + xf, m.xf + xf + h, m.xf + xf + h + 4 * part
+    m.h, m.part, m.sync, m.part_floats = m.xf + xf, m.xf + xf + h, m.xf + xf + h + 4 * part, part
     if E:
         m.logits = m.sync + 4 * sync
     if residual is not None:

@@ -94,3 +94,32 @@ def test_rows_at_an_odd_address_are_refused_by_the_weighted_sum(lib, odd):
     y, shared, residual, out = (P(ALL + 2 * (i == odd)) for i in range(4))
     assert lib.jib_moe_combine(y, P(ALL), P(ALL), shared, residual, out, 20, K, D, None) == ALIGN
     assert lib.jib_moe_combine_norm(y, P(ALL), P(ALL), shared, residual, P(ALL), out, P(ALL), 20, K, D, C.c_float(1e-6), None) == ALIGN
+
+
+# ---- sizes of buffers -------------------------------------------------------------------------------------------------------------
+def test_sizes_are_asked_for_on_each_device(calls):
+    """Tiles, splits and partial sums go by a device's SMs."""
+    w, down = packed(F, D, True), packed(D, F, False)
+    for dev in ("cpu", "meta"):
+        for _ in range(2):
+            native_mx4._scratch(20, w, True, torch.device(dev))
+            native_mx4._few(torch.zeros(3, D, dtype=torch.bfloat16, device=dev), w, down, K)
+    assert [name for name, _ in calls] == ["jib_mx4_gemm_scratch", "jib_mx4_moe_sizes"] * 2
+
+
+def test_a_buffer_that_is_too_small_is_refused(lib):
+    SCRATCH = -6               # JIB_E_SCRATCH
+    need = lib.jib_mx4_gemm_scratch
+    need.restype, need.argtypes = C.c_longlong, [C.c_longlong] + [C.c_int] * 4
+    d = native.Mx4Desc()
+    d.x, d.w, d.w_scales, d.out, d.status, d.ldx, d.ldo, d.T, d.N, d.K, d.batch, d.max_rows = ALL, ALL, ALL, ALL, ALL, 2048, 512, 40, 512, 2048, 1, 40
+    n = need(40, 512, 2048, 0, 0)
+    assert n > 2 * 40 * 2048 + 4 * 40 * 512             # planes of x and, K being split, sums
+    assert lib.jib_mx4_gemm(C.byref(d), None, P(ALL), C.c_longlong(n - 1), None, C.c_longlong(0), 0, None) == SCRATCH
+    m, sizes = native.Mx4MoeDesc(), (C.c_longlong * 4)()
+    assert lib.jib_mx4_moe_sizes(3, D, F, E, K, sizes) == 1
+    for name, kind in m._fields_:
+        if kind is C.c_void_p:
+            setattr(m, name, ALL)
+    m.T, m.d, m.F, m.E, m.k, m.n_group, m.topk_group, m.scale, m.part_floats = 3, D, F, E, K, 1, 1, 1.0, sizes[2] - 1
+    assert lib.jib_mx4_moe(C.byref(m), None) == SCRATCH

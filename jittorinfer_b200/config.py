@@ -98,6 +98,8 @@ class ServerConfig:
             raise ValueError("ffn_format must be empty or mxfp4")
         if self.ffn_format and self.world_size > 1:
             raise ValueError("ffn_format runs on one GPU: tp_size and ep_size must be 1")
+        if self.ffn_format and self.split_mode == "LLAMA_SPLIT_MODE_LAYER" and self.layer_split_gpus > 1:
+            raise ValueError("ffn_format runs on one GPU: layer_split_gpus must be 0 or 1")
         if self.tp_size not in (1, 2, 4, 8) or self.ep_size not in (1, 2, 4, 8):
             raise ValueError("tp_size / ep_size must be 1, 2, 4 or 8")       # reference: llama-model.cpp:467-476
         if self.ep_size > 1 and self.tp_size > 1 and self.ep_size != self.tp_size:

@@ -31,8 +31,10 @@ def build_from_config(cfg, device=None, world: int = 1, rank: int = 0):
                   check_tensors=bool(getattr(cfg, "check_tensors", False)), ffn_format=getattr(cfg, "ffn_format", "") or None)
     hp_known = preset(cfg.random_init) if cfg.random_init else None
     folder = is_folder_model(cfg.model) and not cfg.random_init
-    if world == 1 and device.type == "cuda" and not folder and (hp_known is None or hasattr(hp_known, "kv_row")) and cfg.split_mode == "LLAMA_SPLIT_MODE_LAYER" and not common["ffn_format"]:
+    if world == 1 and device.type == "cuda" and not folder and (hp_known is None or hasattr(hp_known, "kv_row")) and cfg.split_mode == "LLAMA_SPLIT_MODE_LAYER":
         n = int(getattr(cfg, "layer_split_gpus", 1))
+        if n <= 0 and common["ffn_format"]:          # automatic: the one GPU that these weights run on
+            n = 1
         if n <= 0:          # automatic, as the reference spreads layers over all devices by free memory (src/llama-model.cpp:495-540)
             if hp_known is None:
                 from ..gguf.io import GGUFReader

@@ -118,6 +118,9 @@ class DeepSeek2Model:
             raise ValueError(f"ffn_format {ffn_format!r}: None or \"mxfp4\"")
         if ffn_format is not None and (spec.sharded or self.split):
             raise ValueError("ffn_format runs on one GPU: no tensor, expert or layer parallelism")
+        if ffn_format is not None and (hp.n_expert > ops.MX4_MAX_EXPERTS or hp.n_expert_used > ops.MX4_MAX_CHOICES or hp.n_group > ops.MX4_MAX_GROUPS):
+            raise ValueError(f"ffn_format: {hp.n_expert_used} of {hp.n_expert} experts in {hp.n_group} groups; at most {ops.MX4_MAX_CHOICES} of "
+                             f"{ops.MX4_MAX_EXPERTS} in {ops.MX4_MAX_GROUPS}")
         self.ffn_format = ffn_format
         self.out_device = self.layer_dev[-1]
         self._cur_dev = self.device
@@ -192,7 +195,7 @@ class DeepSeek2Model:
         if L.w_gate_sh is not None:
             E, F, d = gate.shape
             ns = L.w_gate_sh.shape[0] // F
-            if L.w_gate_sh.shape[0] == ns * F and E + ns <= ops.MX4_MAX_EXPERTS:
+            if L.w_gate_sh.shape[0] == ns * F and E + ns <= ops.MX4_MAX_EXPERTS and self.hp.n_expert_used + ns <= ops.MX4_MAX_CHOICES:
                 def rows(q, s):
                     return ops.Mx4Tensor(*(torch.cat([a, b.reshape(ns, F, -1)]) for a, b in ((q.codes, s.codes), (q.scales, s.scales))))
 

@@ -13,8 +13,8 @@ import os
 import torch
 
 from . import reference as ref
-from .mx4 import (MX4_MAX_EXPERTS, Mx4Tensor, Mx4Weight, mx4_dequantize, mx4_gateup, mx4_linear, mx4_matmul, mx4_moe_ffn, mx4_moe_layer,  # noqa: F401
-                  mx4_quantize, mx4_weight)
+from .mx4 import (MX4_MAX_CHOICES, MX4_MAX_EXPERTS, MX4_MAX_GROUPS, Mx4Tensor, Mx4Weight, mx4_dequantize, mx4_gateup, mx4_linear, mx4_matmul,  # noqa: F401
+                  mx4_moe_ffn, mx4_moe_layer, mx4_quantize, mx4_weight)
 from .specs import ExpertRoute
 
 _FORCE_TORCH = os.environ.get("JITTORINFER_OPS", "").lower() == "torch"

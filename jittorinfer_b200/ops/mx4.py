@@ -16,7 +16,7 @@ from . import reference as ref
 BLOCK = 32                     # columns that share a scale
 COLS = 128                     # columns of a packed chunk (csrc/kernels/mx4.cuh)
 ACTS = ("silu", "gelu_tanh")
-MX4_MAX_EXPERTS = 256          # of a layer: what the gate and the sort take (csrc/kernels/moe.cu)
+MX4_MAX_EXPERTS, MX4_MAX_CHOICES, MX4_MAX_GROUPS = 256, 32, 32          # of a layer, of a token: what the gate and the sort take (csrc/kernels/moe.cu)
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 

@@ -8,12 +8,11 @@ from typing import Optional
 import torch
 
 from . import native as nat
-from .mx4 import COLS, MX4_MAX_EXPERTS as MAX_EXPERTS, Mx4Tensor, Mx4Weight, scale_rows
+from .mx4 import COLS, MX4_MAX_CHOICES as MAX_CHOICES, MX4_MAX_EXPERTS as MAX_EXPERTS, MX4_MAX_GROUPS as MAX_GROUPS, Mx4Tensor, Mx4Weight, scale_rows
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 FEW_TOKENS = 8                               # tokens of a layer in two launches (8 of the 66-expert layer: 66 us, as tiles 71; 9, with a second tile of 8 here: 98 and 73)
 PAD = 32                                     # rows of an expert are padded to in grouped products (csrc/kernels/mx4_gemm.cu)
-MAX_CHOICES = 32                             # of a token: what the gate takes (csrc/kernels/moe.cu)
 _NO_SWITCH = contextlib.nullcontext()
 _current = nat._device or torch.cuda.current_device
 
@@ -231,8 +230,8 @@ def moe_layer(x, w_router, bias, k, n_group, topk_group, scale, norm, sigmoid, w
     T, d = x.shape
     if T == 0:
         return torch.empty_like(x)
-    if k + n_shared > MAX_CHOICES or wgu.batch > MAX_EXPERTS or n_group > 32:
-        raise ValueError(f"mx4_moe_layer: {k} + {n_shared} of {wgu.batch} experts in {n_group} groups; at most {MAX_CHOICES} of {MAX_EXPERTS} in 32")
+    if k + n_shared > MAX_CHOICES or wgu.batch > MAX_EXPERTS or n_group > MAX_GROUPS:
+        raise ValueError(f"mx4_moe_layer: {k} + {n_shared} of {wgu.batch} experts in {n_group} groups; at most {MAX_CHOICES} of {MAX_EXPERTS} in {MAX_GROUPS}")
     with _on(x):
         w_router = _vectors(w_router)
         if x.stride(0) != d:           # (a single row counts as contiguous whatever its stride)

@@ -201,6 +201,8 @@ def moe_ffn(x, residual, ids, wts, wgu, wd, act, n_shared=0):
         raise ValueError(f"mx4_moe_ffn: {T} tokens of {k} choices in one call")
     if wgu.batch > MAX_EXPERTS:
         raise ValueError(f"mx4_moe_ffn: {wgu.batch} experts, at most {MAX_EXPERTS}")
+    if k == 0:
+        return torch.zeros_like(x) if residual is None else residual.clone(memory_format=torch.contiguous_format)
     with _on(x):
         sizes = _few(x, wgu, wd, k)
         if sizes is not None:

@@ -203,3 +203,14 @@ def test_few_units_over_many_groups(nat, T, E, k, F):
     within(first, want, lim)
     assert all(torch.equal(ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd), first) for _ in range(30))
     nat.check_status()
+
+
+@BOTH
+@pytest.mark.parametrize("T", [3, 20])
+def test_no_choices(nat, dtype, T):
+    wgu, wd, *_ = experts(4, 128, 64)
+    x, res = randn(T, 128, seed=1, dtype=dtype), randn(T, 128, seed=2, dtype=dtype)
+    none = torch.zeros(T, 0, dtype=torch.int32, device=DEV), torch.zeros(T, 0, device=DEV)
+    got = ops.mx4_moe_ffn(x, res, *none, wgu, wd)
+    assert torch.equal(got, res) and got.data_ptr() != res.data_ptr()
+    assert not bool(ops.mx4_moe_ffn(x, None, *none, wgu, wd).any())

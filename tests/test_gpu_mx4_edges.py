@@ -5,7 +5,7 @@ import torch
 
 from jittorinfer_b200 import ops
 from jittorinfer_b200.ops import mx4
-from test_gpu_mx4 import DEV, experts, gen, moe_want, randn, within
+from test_gpu_mx4 import DEV, experts, gen, moe_want, product_limit, randn, weights, within
 
 pytestmark = pytest.mark.gpu
 BOTH = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -214,3 +214,18 @@ def test_no_choices(nat, dtype, T):
     got = ops.mx4_moe_ffn(x, res, *none, wgu, wd)
     assert torch.equal(got, res) and got.data_ptr() != res.data_ptr()
     assert not bool(ops.mx4_moe_ffn(x, None, *none, wgu, wd).any())
+
+
+def test_more_fp32_rows_than_a_grid_is_high(nat):
+    T = 8 * 65535 + 77
+    q, w = weights(16, 32, seed=1)
+    x = randn(T, 32, seed=2)
+    want = x.double() @ w.T
+    within(ops.mx4_linear(x, ops.mx4_weight(q)), want, product_limit(x, w, want, torch.float32))
+    wgu, wd, *_ = experts(2, 32, 32)
+    x = x[:T // 2 + 50]                              # two choices each
+    ids = torch.randint(0, 2, (x.shape[0], 2), generator=gen(3), device=DEV, dtype=torch.int32)
+    wts = torch.rand(x.shape[0], 2, generator=gen(4), device=DEV)
+    got = ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd)
+    assert torch.equal(got[:999], ops.mx4_moe_ffn(x[:999], None, ids[:999], wts[:999], wgu, wd))
+    assert torch.equal(got[-999:], ops.mx4_moe_ffn(x[-999:], None, ids[-999:], wts[-999:], wgu, wd))

@@ -229,3 +229,15 @@ def test_more_fp32_rows_than_a_grid_is_high(nat):
     got = ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd)
     assert torch.equal(got[:999], ops.mx4_moe_ffn(x[:999], None, ids[:999], wts[:999], wgu, wd))
     assert torch.equal(got[-999:], ops.mx4_moe_ffn(x[-999:], None, ids[-999:], wts[-999:], wgu, wd))
+
+
+@pytest.mark.parametrize("T", [1, 12, 70])
+def test_no_value_of_an_infinite_row_is_finite(nat, T):
+    """On the tensor cores the block of an infinity is NaN, and so is NaN times a weight of 0."""
+    (q, w), (u, _) = weights(40, 256, seed=9), weights(40, 256, seed=10)
+    x = randn(T, 256, seed=10, dtype=torch.bfloat16)
+    clean = ops.mx4_linear(x, ops.mx4_weight(q)), ops.mx4_gateup(x, ops.mx4_weight(q, u))
+    for bad in ("inf", "-inf", "nan"):
+        x[0, 200] = float(bad)
+        for got, was in zip((ops.mx4_linear(x, ops.mx4_weight(q)), ops.mx4_gateup(x, ops.mx4_weight(q, u))), clean):
+            assert not bool(got[0].isfinite().any()) and torch.equal(got[1:], was[1:])

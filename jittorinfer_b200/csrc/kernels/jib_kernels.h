@@ -143,8 +143,9 @@ JIB_EXPORT int jib_moe_permute(const int * ids, int T, int k, int expert_base, i
 JIB_EXPORT int jib_moe_tile_list(const int * seg, int E_local, int bn, int * out, int cap, void * stream);
 JIB_EXPORT int jib_moe_permute_multi(const int * ids, int T, int k, int expert_base, int E_local, int * seg, int * src_token, int * dest,
                                      int * tmp, const float * wts, float * row_wts, void * stream);
+// rows: of y, which dest points into.
 JIB_EXPORT int jib_moe_combine(const void * y, const int * dest, const float * wts, const void * shared, const void * residual,
-                               void * out, int T, int k, int d, void * stream);
+                               void * out, int T, int k, int d, int rows, void * stream);
 // The same followed by RMSNorm(out) * norm_w (fp32 weights, as jib_rmsnorm) in one launch; bitwise the two-launch results.
 JIB_EXPORT int jib_moe_combine_norm(const void * y, const int * dest, const float * wts, const void * shared, const void * residual,
                                     const float * norm_w, void * out, void * out_norm, int T, int k, int d, float eps, void * stream);

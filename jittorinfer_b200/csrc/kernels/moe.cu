@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(256) tile_list_kernel(const int * __restrict__
 // dry: the same instructions with row 0 in place of the sorted-row indices (which are not valid yet) and no stores.
 __device__ __noinline__ void moe_combine_row(const bf16 * __restrict__ y, const int * __restrict__ dest, const float * __restrict__ wts,
                                              const bf16 * __restrict__ shared, const bf16 * __restrict__ residual, bf16 * __restrict__ out,
-                                             int k, int d, bool dry) {
+                                             int k, int d, int rows, bool dry) {
     const int t = blockIdx.x;
     for (int i = threadIdx.x; i < d / 8; i += blockDim.x) {
         float acc[8];
@@ -727,7 +727,7 @@ __device__ __noinline__ void moe_combine_row(const bf16 * __restrict__ y, const 
         for (int j = 0; j < 8; ++j) acc[j] = 0.f;
         for (int j = 0; j < k; ++j) {
             const int row = dry ? 0 : dest[(size_t) t * k + j];
-            JIB_BC(row < (int) gridDim.x * k, 14, row);
+            JIB_BC(row < rows, 14, row);
             if (row < 0) continue;
             const float w = wts[(size_t) t * k + j];
             const uint4 raw = ((const uint4 *) (y + (size_t) row * d))[i];
@@ -769,13 +769,13 @@ __device__ __noinline__ void moe_combine_row(const bf16 * __restrict__ y, const 
 
 __global__ void moe_combine_kernel(const bf16 * __restrict__ y, const int * __restrict__ dest, const float * __restrict__ wts,
                                    const bf16 * __restrict__ shared, const bf16 * __restrict__ residual, bf16 * __restrict__ out, int k,
-                                   int d, int warm) {
+                                   int d, int rows, int warm) {
     JIB_KS(12, 0);
     PDL_TRIGGER_TOP();
-    if (warm) moe_combine_row(y, dest, wts, shared, residual, out, k, d, true);
+    if (warm) moe_combine_row(y, dest, wts, shared, residual, out, k, d, rows, true);
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
     JIB_KS(12, 1);
-    moe_combine_row(y, dest, wts, shared, residual, out, k, d, false);
+    moe_combine_row(y, dest, wts, shared, residual, out, k, d, rows, false);
     JIB_KS(12, 9);
 }
 
@@ -1004,13 +1004,14 @@ int jib_moe_permute_multi(const int * ids, int T, int k, int expert_base, int E_
     return launched();
 }
 
+// rows: of y (T k of them, or more where experts' rows are padded).
 int jib_moe_combine(const void * y, const int * dest, const float * wts, const void * shared, const void * residual, void * out, int T,
-                    int k, int d, void * stream) {
+                    int k, int d, int rows, void * stream) {
     if (T <= 0) return 0;
     if (d % 8) return JIB_E_ARG;
     if (((uintptr_t) y | (uintptr_t) shared | (uintptr_t) residual | (uintptr_t) out) & 15) return JIB_E_ALIGN;          // (rows go 16 bytes at a time)
     JIB_LAUNCH((moe_combine_kernel), T, 256, 0, (cudaStream_t) stream, (const bf16 *) y, dest, wts, (const bf16 *) shared, (const bf16 *) residual,
-                                                              (bf16 *) out, k, d, jib::warm_for(T));
+                                                              (bf16 *) out, k, d, rows, jib::warm_for(T));
     return launched();
 }
 

@@ -161,7 +161,7 @@ def load():
     sig("jib_moe_route_fused", vp, fp, fp, fp, ip, fp, ip, ip, ip, ip, i, i, i, i, i, i, f, i, i, i, i, i, i, fp, f, vp, vp)
     sig("jib_moe_permute_multi", ip, i, i, i, i, ip, ip, ip, ip, fp, fp, vp)
     sig("jib_moe_tile_list", ip, i, i, ip, i, vp)
-    sig("jib_moe_combine", vp, ip, fp, vp, vp, vp, i, i, i, vp)
+    sig("jib_moe_combine", vp, ip, fp, vp, vp, vp, i, i, i, i, vp)
     sig("jib_moe_combine_norm", vp, ip, fp, vp, vp, fp, vp, vp, i, i, i, f, vp)
     sig("jib_mla_attention", vp, vp, ip, i, ip, ip, i, i, i, i, i, i, f, i, i, i, fp, fp, vp, vp)
     sig("jib_mla_combine", fp, fp, i, i, i, i, vp, vp)
@@ -703,7 +703,7 @@ def moe_combine(y, dest, wts, shared, residual, norm=None):
                                         out.data_ptr(), normed.data_ptr(), T, k, d, float(norm[1]), _stream()), "moe_combine_norm")
         return out, normed
     _ck(load().jib_moe_combine(y.data_ptr(), dest.data_ptr(), wts.data_ptr(), _p(shared), _p(residual), out.data_ptr(), T, k, d,
-                               _stream()), "moe_combine")
+                               y.shape[0], _stream()), "moe_combine")
     return out
 
 

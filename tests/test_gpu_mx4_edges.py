@@ -1,9 +1,13 @@
 """4-bit operators where their inputs end: choices without an expert, rows of one token, memory that nobody wrote, scales far apart, strides and
 addresses of views.  Limits as in the tests of the single operators."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
-from jittorinfer_b200 import ops
+from jittorinfer_b200 import build, ops
 from jittorinfer_b200.ops import mx4
 from test_gpu_mx4 import DEV, experts, gen, moe_want, product_limit, randn, weights, within
 
@@ -241,3 +245,24 @@ def test_no_value_of_an_infinite_row_is_finite(nat, T):
         x[0, 200] = float(bad)
         for got, was in zip((ops.mx4_linear(x, ops.mx4_weight(q)), ops.mx4_gateup(x, ops.mx4_weight(q, u))), clean):
             assert not bool(got[0].isfinite().any()) and torch.equal(got[1:], was[1:])
+
+
+def test_padded_rows_are_within_the_bounds_of_the_checking_build(nat):
+    """The build that checks indexes counts the rows that there are, not the choices: an expert's rows are padded."""
+    checked = build.KERNELS_SO.replace(".so", "_bc.so")
+    if not os.path.exists(checked):
+        pytest.skip("the checking build is not there")
+    code = """
+import torch
+from jittorinfer_b200 import ops
+from jittorinfer_b200.ops import native
+assert native.load().jib_bounds_check_enabled() == 1
+w = ops.mx4_quantize(torch.randn(8, 64, 64, device="cuda"))
+x = torch.randn(20, 64, device="cuda").bfloat16()
+ids = torch.arange(40, device="cuda", dtype=torch.int32).view(20, 2) % 8
+out = ops.mx4_moe_ffn(x, None, ids, torch.ones(20, 2, device="cuda"), ops.mx4_weight(w, w), ops.mx4_weight(w))
+native.check_status()
+"""
+    env = dict(os.environ, JITTORINFER_KERNELS_SO=checked, PYTHONPATH=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

@@ -92,7 +92,7 @@ def test_a_residual_at_an_odd_address_is_copied_for_the_weighted_sum(calls, offs
 @pytest.mark.parametrize("odd", range(4))
 def test_rows_at_an_odd_address_are_refused_by_the_weighted_sum(lib, odd):
     y, shared, residual, out = (P(ALL + 2 * (i == odd)) for i in range(4))
-    assert lib.jib_moe_combine(y, P(ALL), P(ALL), shared, residual, out, 20, K, D, None) == ALIGN
+    assert lib.jib_moe_combine(y, P(ALL), P(ALL), shared, residual, out, 20, K, D, 20 * K, None) == ALIGN
     assert lib.jib_moe_combine_norm(y, P(ALL), P(ALL), shared, residual, P(ALL), out, P(ALL), 20, K, D, C.c_float(1e-6), None) == ALIGN
 
 

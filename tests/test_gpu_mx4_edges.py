@@ -266,3 +266,59 @@ native.check_status()
     env = dict(os.environ, JITTORINFER_KERNELS_SO=checked, PYTHONPATH=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ---- activations with loud columns ------------------------------------------------------------------------------------------------
+def planes_loss(x):
+    """What two planes of 8 bits may lose of bf16 activations: nothing down to 2^-11 of a block's largest, below at most 2^-21 of it (the second plane's
+    smallest step, rounded) or the value."""
+    b = x.double().abs().reshape(x.shape[0], -1, 32)
+    top = b.amax(-1, keepdim=True)
+    return torch.where(b < 2.0 ** -11 * top, torch.minimum(b, 2.0 ** -21 * top), 0.0).reshape(x.shape)
+
+
+def loud(T, K, by, dtype=torch.bfloat16):
+    x = randn(T, K, seed=T)
+    x[:, ::37] *= by
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("T", [1, 9, 40, 150])
+@pytest.mark.parametrize("by", [2.0 ** 4, 2.0 ** 9, 2.0 ** 14, 2.0 ** 24])
+def test_products_of_loud_columns(nat, T, by):
+    N, K = 200, 416
+    (q, w), (u, v) = weights(N, K, seed=1, scale=0.05), weights(N, K, seed=2, scale=0.05)
+    x = loud(T, K, by)
+    want = x.double() @ w.T
+    within(ops.mx4_linear(x, ops.mx4_weight(q), out_dtype=torch.float32), want, product_limit(x, w, want, torch.float32) + planes_loss(x) @ w.abs().T)
+    z, y = want, x.double() @ v.T
+    want = mx4._act(z, "silu") * y
+    lost, half = planes_loss(x), 2.0 ** -8
+    dz, dy = (K * 2.0 ** -23 * (x.double().abs() @ m.abs().T) + lost @ m.abs().T for m in (w, v))
+    within(ops.mx4_gateup(x, ops.mx4_weight(q, u)), want, (1.13 * dz * (y.abs() + dy) + mx4._act(z, "silu").abs() * dy) + (2.0 ** -20 + half) * want.abs() + 1e-30)
+
+
+@pytest.mark.parametrize("T", [1, 8, 9, 60])
+@pytest.mark.parametrize("by", [2.0 ** 4, 2.0 ** 9, 2.0 ** 14])
+def test_layers_of_loud_columns(nat, T, by):
+    """The few-token form keeps x to 2^-39 of a row's largest and hidden units in fp16; the tiled one has two planes of both."""
+    E, d, F, k = 6, 160, 96, 2
+    wgu, wd, gv, uv, dv = experts(E, d, F, seed=5)
+    x = loud(T, d, by)
+    ids = torch.rand(T, E, generator=gen(T), device=DEV).argsort(-1)[:, :k].int()
+    wts = torch.rand(T, k, generator=gen(8), device=DEV)
+    half = 2.0 ** -8
+    lost = torch.maximum(planes_loss(x), 2.0 ** -39 * x.double().abs().amax(-1, keepdim=True))
+    want, lim = torch.zeros(T, d, dtype=torch.float64, device=DEV), torch.zeros(T, d, dtype=torch.float64, device=DEV)
+    for e in range(E):
+        share = (wts.double() * (ids == e)).sum(-1, keepdim=True)
+        z, y = x.double() @ gv[e].T, x.double() @ uv[e].T
+        dz, dy = (d * 2.0 ** -23 * (x.double().abs() @ m[e].abs().T) + lost @ m[e].abs().T for m in (gv, uv))
+        h = mx4._act(z, "silu") * y
+        dh = (1.13 * dz * (y.abs() + dy) + mx4._act(z, "silu").abs() * dy) + (2.0 ** -20 + half) * h.abs() + 1e-30
+        dh = dh + torch.maximum(planes_loss(h * (1 + half)), 2.0 ** -25 * h.abs().amax(-1, keepdim=True))          # (fp16: half a step of 2^-24 of the largest)
+        r = h @ dv[e].T
+        want += share * r
+        lim += share * (dh @ dv[e].abs().T + F * 2.0 ** -23 * ((h.abs() + dh) @ dv[e].abs().T) + half * r.abs())
+    lim = lim * (1 + half) + (half + (k + 1) * 2.0 ** -23) * want.abs() + 1e-30
+    within(ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd), want, lim)

@@ -170,13 +170,13 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t * __restrict__ 
     int e = 0, f = 0;
     if (r < N && b < K / 32) {
         e = scales[((size_t) m * N + r) * ld_s + b];
-        f = e == 255 ? 31 : min(max(0, 15 + e - 127 - exps[(size_t) m * R + row]), 30);        // (above 15 + TOP only for a block of zeros)
+        if (factors != nullptr) f = e == 255 ? 31 : min(max(0, 15 + e - 127 - exps[(size_t) m * R + row]), 30);        // (above 15 + TOP only for a block of zeros)
         if (e != 255) v = ((const uint4 *) codes)[((size_t) m * N + r) * (K / 32) + b];
         if (lost != nullptr && f == 0 && !no_value(v)) *lost = 1;
     }
     out[at] = v;
     out_scales[at] = (uint8_t) e;
-    factors[at] = (uint8_t) (f << 2);
+    if (factors != nullptr) factors[at] = (uint8_t) (f << 2);
 }
 
 // ---- the product of fp32 activations, on CUDA cores ------------------------------------------------------------------
@@ -296,17 +296,19 @@ JIB_EXPORT int jib_mx4_dequantize(const void * codes, const void * scales, long 
 }
 
 // Row-major codes and scales of `batch` matrices [N][K] to the order that the products read: out, out_scales, factors and exps of all (of pairs, with step 2, the
-// member `first`).  lost (or NULL): set to 1 where a weight's factor is 0 and the weight is not.
+// member `first`).  factors and exps NULL: not made.  lost (or NULL): set to 1 where a weight's factor is 0 and the weight is not.
 JIB_EXPORT int jib_mx4_pack(const void * codes, const void * scales, long long ld_s, void * out, void * out_scales, void * factors, int * exps, int * lost, int batch,
                             int N, int K, int step, int first, void * stream) {
     if (batch <= 0) return 0;
-    if (N <= 0 || K <= 0 || K % 32 || ld_s < K / 32 || batch > 65535 || step < 1 || step > 2 || first < 0 || first >= step) return JIB_E_ARG;
+    if (N <= 0 || K <= 0 || K % 32 || ld_s < K / 32 || batch > 65535 || step < 1 || step > 2 || first < 0 || first >= step ||
+        (factors == nullptr) != (exps == nullptr) || (lost != nullptr && factors == nullptr))
+        return JIB_E_ARG;
     if (((uintptr_t) codes | (uintptr_t) out) & 15) return JIB_E_ALIGN;
     const int R = mx4::rows_of(N, step == 2);
     const long long n = (long long) mx4::chunks(K) * (R / step) * 4;
     if ((n + 255) / 256 > 0x7fffffffll) return JIB_E_ARG;
     cudaStream_t s = (cudaStream_t) stream;
-    row_exponent_kernel<<<dim3((R / step + 3) / 4, batch), 128, 0, s>>>((const uint4 *) codes, (const uint8_t *) scales, ld_s, exps, N, K, R, step, first);
+    if (exps != nullptr) row_exponent_kernel<<<dim3((R / step + 3) / 4, batch), 128, 0, s>>>((const uint4 *) codes, (const uint8_t *) scales, ld_s, exps, N, K, R, step, first);
     pack_kernel<<<dim3((unsigned) ((n + 255) / 256), batch), 256, 0, s>>>((const uint8_t *) codes, (const uint8_t *) scales, ld_s, exps, (uint4 *) out,
                                                                          (uint8_t *) out_scales, (uint8_t *) factors, lost, N, K, R, step, first);
     return launched();

@@ -98,8 +98,8 @@ class Mx4Tensor:
 
 class Mx4Weight:
     """A matrix [n, k], or ``batch`` of them, or as many gated pairs, in the order in which the products read it.  On the GPU ``codes`` and ``scales`` hold
-    chunks of 128 columns, rows within them (of a pair 16 of each matrix in turn), ``factors`` and ``exps`` the scales again as the products of a few
-    tokens need them; ``far`` says that some weights of a batch lie too far below their row's largest scale for the latter, which then do not read it;
+    chunks of 128 columns, rows within them (of a pair 16 of each matrix in turn), ``factors`` and ``exps`` of a batch the scales again as expert layers of a
+    few tokens need them; ``far`` says that some of its weights lie too far below their row's largest scale for those, which then do not read it;
     elsewhere ``plain`` holds the tensors."""
     __slots__ = ("n", "k", "batch", "gated", "codes", "scales", "factors", "exps", "far", "plain")
 
@@ -127,7 +127,7 @@ class Mx4Weight:
 
     def nbytes(self) -> int:
         if self.codes is not None:
-            return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.factors, self.exps))
+            return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.factors, self.exps) if t is not None)
         return sum(p.nbytes() for p in self.plain)
 
     def values(self, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, ...]:
@@ -177,16 +177,16 @@ def _unpack(w: Mx4Weight, member: int) -> torch.Tensor:
 
     def scaled(s):
         return (v * s[..., None]).reshape(w.matrices, w.n, -1)[..., :w.k]
-    e, f = rows(w.scales).int(), rows(w.factors).int() >> 2
+    e = rows(w.scales).int()
     nan = torch.full(e.shape, float("nan"), dtype=torch.float64, device=w.device)
     out = scaled(torch.where(e == 255, nan, _pow2(e - 127)))
-    unit = _pow2(rows(w.exps[:, None, :, None]))
-    again = scaled(torch.where(f == 31, nan, torch.where(f > 0, _pow2(f - 15), torch.zeros_like(nan))) * unit)
-    largest = out.nan_to_num(0.0).abs().amax(-1, keepdim=True)
-    lost = (again == 0) & (out.abs() < 2.0 ** -24 * largest)          # scales more than 27 binades below the largest are 0 in the second form
-    same = (out == again) | (out.isnan() & again.isnan()) | lost
-    if not bool(same.all()):
-        raise RuntimeError("the two forms of a packed weight's scales differ")
+    if w.factors is not None:
+        f, unit = rows(w.factors).int() >> 2, _pow2(rows(w.exps[:, None, :, None]))
+        again = scaled(torch.where(f == 31, nan, torch.where(f > 0, _pow2(f - 15), torch.zeros_like(nan))) * unit)
+        largest = out.nan_to_num(0.0).abs().amax(-1, keepdim=True)
+        lost = (again == 0) & (out.abs() < 2.0 ** -24 * largest)          # scales more than 27 binades below the largest are 0 in the second form
+        if not bool(((out == again) | (out.isnan() & again.isnan()) | lost).all()):
+            raise RuntimeError("the two forms of a packed weight's scales differ")
     out = out.float()
     return out if w.batch else out[0]
 

@@ -48,13 +48,15 @@ def pack(w: Mx4Weight, q: Mx4Tensor, up: Optional[Mx4Tensor]) -> None:
     E, R, members = w.matrices, w.rows, (q,) if up is None else (q, up)
     w.codes = torch.empty(E, w.chunks, R, COLS // 2, dtype=torch.uint8, device=q.device)
     w.scales = torch.empty(E, w.chunks, R, COLS // 32, dtype=torch.uint8, device=q.device)
-    w.factors = torch.empty_like(w.scales)
-    w.exps = torch.empty(E, R, dtype=torch.int32, device=q.device)
-    lost = torch.zeros(1, dtype=torch.int32, device=q.device) if w.batch else None
+    lost = None
+    if w.batch:                    # only layers of experts have a form for a few tokens
+        w.factors = torch.empty_like(w.scales)
+        w.exps = torch.empty(E, R, dtype=torch.int32, device=q.device)
+        lost = torch.zeros(1, dtype=torch.int32, device=q.device)
     with _on(q.codes):
         for m, t in enumerate(members):
             nat._ck(nat.load().jib_mx4_pack(t.codes.data_ptr(), t.scales.data_ptr(), t.scales.stride(-2), w.codes.data_ptr(), w.scales.data_ptr(),
-                                            w.factors.data_ptr(), w.exps.data_ptr(), nat._p(lost), E, w.n, w.k, len(members), m, nat._stream()), "mx4_pack")
+                                            nat._p(w.factors), nat._p(w.exps), nat._p(lost), E, w.n, w.k, len(members), m, nat._stream()), "mx4_pack")
         # (read once, when weights are laid out; a graph that does so cannot say yet)
         w.far = lost is not None and (torch.cuda.is_current_stream_capturing() or bool(lost.item()))
 

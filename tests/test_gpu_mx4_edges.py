@@ -322,3 +322,11 @@ def test_layers_of_loud_columns(nat, T, by):
         lim += share * (dh @ dv[e].abs().T + F * 2.0 ** -23 * ((h.abs() + dh) @ dv[e].abs().T) + half * r.abs())
     lim = lim * (1 + half) + (half + (k + 1) * 2.0 ** -23) * want.abs() + 1e-30
     within(ops.mx4_moe_ffn(x, None, ids, wts, wgu, wd), want, lim)
+
+
+def test_only_experts_have_factors(nat):
+    q = ops.mx4_quantize(randn(3, 40, 224, seed=1))
+    one, batch = ops.mx4_weight(ops.Mx4Tensor(q.codes[1], q.scales[1])), ops.mx4_weight(q)
+    assert one.factors is None and one.exps is None and batch.factors is not None and not batch.far
+    assert one.nbytes() == 2 * 64 * (64 + 4) and batch.nbytes() == 3 * 64 * (2 * (64 + 4 + 4) + 4)         # two chunks of 64 laid-out rows
+    assert torch.equal(one.values()[0], batch.values()[0][1])

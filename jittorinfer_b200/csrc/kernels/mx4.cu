@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t * __restrict__ 
 constexpr int ST = 8;
 
 template <bool PAIR>
-__global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
+__global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d, unsigned first_tile) {
     PDL_TRIGGER_TOP();
     pdl_wait();      // inputs come from earlier kernels; nothing is written before this point
     constexpr int M = PAIR ? 2 : 1;
@@ -196,61 +196,60 @@ __global__ void __launch_bounds__(128) product_kernel(const jib_mx4_desc d) {
         base = d.seg[e];
         rows = d.seg[e + 1] - base;
     }
-#pragma unroll 1
-    for (long long t0 = (long long) blockIdx.y * ST; t0 < rows; t0 += (long long) gridDim.y * ST) {
-        const int nt = (int) (rows - t0 < ST ? rows - t0 : ST);
-        const float * xr[ST];
+    const long long t0 = (long long) (first_tile + blockIdx.y) * ST;
+    if (t0 >= rows) return;
+    const int nt = (int) (rows - t0 < ST ? rows - t0 : ST);
+    const float * xr[ST];
 #pragma unroll
-        for (int j = 0; j < ST; ++j) {
-            const long long r = base + t0 + (j < nt ? j : 0);
-            xr[j] = (const float *) d.x + (d.src != nullptr ? (long long) d.src[r] : r) * d.ldx;
-        }
-        float acc[M][2][ST] = {};
-        for (int c = 0; c < C; ++c) {
-            const int k = c * mx4::COLS + 32 * t;
-            if (k >= d.K) continue;
+    for (int j = 0; j < ST; ++j) {
+        const long long r = base + t0 + (j < nt ? j : 0);
+        xr[j] = (const float *) d.x + (d.src != nullptr ? (long long) d.src[r] : r) * d.ldx;
+    }
+    float acc[M][2][ST] = {};
+    for (int c = 0; c < C; ++c) {
+        const int k = c * mx4::COLS + 32 * t;
+        if (k >= d.K) continue;
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const size_t row = ((size_t) e * C + c) * R + (b * M + m) * 16 + h * 8 + g;
-                    const uint4 q = ((const uint4 *) d.w)[row * 4 + t];
-                    const uint32_t s = d.w_scales[row * 4 + t], word[4] = {q.x, q.y, q.z, q.w};
-                    const float unit = s == 255 ? __uint_as_float(0x7fffffffu) : mx4::pow2((int) s - 127);
+            for (int h = 0; h < 2; ++h) {
+                const size_t row = ((size_t) e * C + c) * R + (b * M + m) * 16 + h * 8 + g;
+                const uint4 q = ((const uint4 *) d.w)[row * 4 + t];
+                const uint32_t s = d.w_scales[row * 4 + t], word[4] = {q.x, q.y, q.z, q.w};
+                const float unit = s == 255 ? __uint_as_float(0x7fffffffu) : mx4::pow2((int) s - 127);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float w = code_value(word[i] >> (4 * j)) * unit;
+                    for (int j = 0; j < 8; ++j) {
+                        const float w = code_value(word[i] >> (4 * j)) * unit;
 #pragma unroll
-                            for (int n = 0; n < ST; ++n)
-                                if (n < nt) acc[m][h][n] += w * xr[n][k + 8 * i + j];
-                        }
-                }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < ST; ++j) {
-                float s[M];
-#pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    s[m] = acc[m][h][j];
-                    s[m] += __shfl_xor_sync(0xffffffffu, s[m], 1);
-                    s[m] += __shfl_xor_sync(0xffffffffu, s[m], 2);
-                }
-                const int n = b * 16 + 8 * h + g;
-                if (t != 0 || j >= nt || n >= d.N) continue;
-                const long long r = base + t0 + j;
-                float y = PAIR ? mx4::gated(s[0], s[M - 1], d.act) : s[0];
-                if (d.residual != nullptr) {
-                    const long long ri = r * d.ldr + n;
-                    y += d.res_f32 ? ((const float *) d.residual)[ri] : to_f(((const bf16 *) d.residual)[ri]);
-                }
-                if (d.out_f32) ((float *) d.out)[r * d.ldo + n] = y;
-                else ((bf16 *) d.out)[r * d.ldo + n] = __float2bfloat16(y);
+                        for (int n = 0; n < ST; ++n)
+                            if (n < nt) acc[m][h][n] += w * xr[n][k + 8 * i + j];
+                    }
             }
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < ST; ++j) {
+            float s[M];
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                s[m] = acc[m][h][j];
+                s[m] += __shfl_xor_sync(0xffffffffu, s[m], 1);
+                s[m] += __shfl_xor_sync(0xffffffffu, s[m], 2);
+            }
+            const int n = b * 16 + 8 * h + g;
+            if (t != 0 || j >= nt || n >= d.N) continue;
+            const long long r = base + t0 + j;
+            float y = PAIR ? mx4::gated(s[0], s[M - 1], d.act) : s[0];
+            if (d.residual != nullptr) {
+                const long long ri = r * d.ldr + n;
+                y += d.res_f32 ? ((const float *) d.residual)[ri] : to_f(((const bf16 *) d.residual)[ri]);
+            }
+            if (d.out_f32) ((float *) d.out)[r * d.ldo + n] = y;
+            else ((bf16 *) d.out)[r * d.ldo + n] = __float2bfloat16(y);
+        }
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? 0 : JIB_E_LAUNCH; }
@@ -318,11 +317,15 @@ JIB_EXPORT int jib_mx4_product_simt(const jib_mx4_desc * d, void * stream) {
     if (d->T <= 0) return 0;
     if (d->N <= 0 || d->K <= 0 || d->K % 32 || d->batch < 1 || d->batch > 65535) return JIB_E_ARG;
     const long long rows = d->seg != nullptr ? d->max_rows : d->T;
-    const long long tiles = (rows + ST - 1) / ST;
-    const dim3 grid(((d->N + 15) / 16 + 3) / 4, (unsigned) (tiles < 65535 ? tiles : 65535), d->batch);          // (the kernel strides on)
     cudaStream_t s = (cudaStream_t) stream;
-    if (d->gated) JIB_LAUNCH((product_kernel<true>), grid, 128, 0, s, *d);
-    else JIB_LAUNCH((product_kernel<false>), grid, 128, 0, s, *d);
+    // A grid is 65535 tiles of rows high at most.  (A kernel that strides on took 432 us for a row of 10944 by 2048 instead of 393; rows along the grid's other
+    // side 713 for 300 by 2048 x 2048 instead of 646.)
+    const long long tiles = (rows + ST - 1) / ST;
+    for (long long t = 0; t < tiles; t += 65535) {
+        const dim3 grid(((d->N + 15) / 16 + 3) / 4, (unsigned) (tiles - t < 65535 ? tiles - t : 65535), d->batch);
+        if (d->gated) JIB_LAUNCH((product_kernel<true>), grid, 128, 0, s, *d, (unsigned) t);
+        else JIB_LAUNCH((product_kernel<false>), grid, 128, 0, s, *d, (unsigned) t);
+    }
     return launched();
 }
 

@@ -5,7 +5,8 @@
 // tcgen05.mma.kind::mxf8f6f4 takes them as E2M1 with their block's scale, 128 rows a tile.  So no instruction touches a weight.  Its other operand can have 8
 // bits at most; a bf16 activation is the sum of two E4M3 numbers, the first its value rounded to four significant bits, the second what is left, each
 // with a scale for 32 columns.  That sum is the bf16 value down to 2^-11 of the block's largest magnitude and within 2^-21 of the largest below.  At
-// twice the rate of bf16 both planes cost what a bf16 product costs.
+// twice the rate of bf16 both planes cost what a bf16 product costs.  (Hidden units on their way to the next product are rounded to bf16, whose eight
+// bits the planes then hold.)
 //
 // Up to 96 rows of x (WIDE) both planes are one operand of twice the rows, and the sums of the two meet in the epilogue.  Dense tiles then belong to one CTA,
 // experts' tiles to two (PAIR, cta_group::2: 256 weights, each CTA keeps one plane).  Above 96 rows two CTAs share 256 weights by up to 192 rows of x, of
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm_kernel(const __grid_const
     uint64_t * full = bars, * empty = full + MAX_STAGES, * sl_full = empty + MAX_STAGES, * sf_full = sl_full + MAX_SLOTS, * sf_empty = sf_full + MAX_SLOTS,
              * acc_full = sf_empty + MAX_SLOTS, * acc_empty = acc_full + 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = g.stages, Q = g.slots, bn = g.bn, cps = g.cps;
-        const int rank = PAIR ? blockIdx.x & 1 : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const int rank = PAIR ? blockIdx.x & 1 : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
     // rows of x in this CTA's shared memory: of a pair half of them, or, WIDE, all of one plane
     const int xn = PAIR ? bn / 2 : bn, SB = stage_bytes(xn), QB = slot_bytes(bn), plane = xn * 128;
     const int mn = WIDE ? 2 * bn : bn, sfc = scale_cols(mn), slab = WIDE ? 4 + sfc : 4 + 2 * sfc;
@@ -804,7 +805,8 @@ JIB_EXPORT int jib_mx4_gemm(const jib_mx4_desc * d, const int * count, void * sc
     }
     if (items > 0x3fffffff) return JIB_E_ARG;
     // Chunks of a stage: its waits and commits take the issuing thread as long as a few products.  8 rows by 12288 x 5120: 21 us with one, 16.5 with two, 14.3
-    // with three; 17 rows of the 66-expert layer 122 and 96 us with one and two, 107 with three (16 and 11 chunks are no multiple); 515 rows 191 and 160.
+    // with three; 17 rows of the 66-expert layer (16 and 11 chunks) 122 and 96 us with one and two, 107 with three; 515 rows 191 and 160.  The rule goes by the
+    // tile's width alone: numbers of chunks that three divides were not measured.
     g.cps = g.bn <= 16 ? 3 : g.bn <= MAX_WIDE ? 2 : 1;
     g.slots = !wide ? (512 - 2 * g.bn) / (4 + 2 * scale_cols(g.bn)) : (512 - 4 * g.bn) / (g.cps * (4 + scale_cols(2 * g.bn)));
     if (g.slots > MAX_SLOTS) g.slots = MAX_SLOTS;

@@ -2,8 +2,8 @@
 // choice of experts, gate and up products, activation, down products, weighted sum, residual.
 //
 // The reference runs router, choice, sorting, grouped products and the weighted sum as some dozen launches
-// (src/llama-graph-ffn.cpp:145-260); the bf16 path here takes five.  Width 2048, 64 experts of 1408, 6 chosen + 2 shared, norm included: 1 token 34.6 us, 8
-// tokens 66 (bf16: 43 and 120); alone, 8 tokens read their 170 MB of weights at 2.5 TB/s over the whole layer, at 3.4 TB/s within its two loops.
+// (src/llama-graph-ffn.cpp:145-260); the bf16 path here takes five.  Width 2048, 64 experts of 1408, 6 chosen + 2 shared, norm included: 1 token 33.7 us, 8
+// tokens 66 (bf16: 43 and 119); alone, 8 tokens read their 170 MB of weights at 2.5 TB/s over the whole layer, at 3.4 TB/s within its two loops.
 //
 // The layer is bound by the stream of the chosen experts' weights, and on the way by instructions: a weight has 2.8 issue slots at the memory's rate.  So
 // the second launch is two plain loops over chunks and a meeting of its CTAs in between; every warp is alike, and keeps a ring of weights of its

@@ -1,9 +1,9 @@
 // What the products of a few rows of activations with packed 4-bit weights share: 32 rows of a chunk of weights times tiles of 8 rows of activations by
 // mma, the copies that bring chunks, and the order in which a warp reads activations.
 //
-// Up to 16 rows the stream of weights counts, 4096 weights in 2176 bytes, and the instructions on its way: at the memory's rate an SM gets 43
+// Up to 8 rows, one tile, the stream of weights counts, 4096 weights in 2176 bytes, and the instructions on its way: at the memory's rate an SM gets 43
 // weights a clock, 2.8 issue slots (of 32 lanes) a weight.  A weight is decoded once for all rows.  The mma bound it in the end: 14 clocks each
-// on a quarter of an SM, 70 weights a clock and SM for one tile, 35 for two.
+// on a quarter of an SM, 70 weights a clock and SM.  (A second tile halves that; more rows run as tiled products.)
 //
 // Activations are fp16, each row scaled by a power of two to a largest magnitude in [2^14, 2^15): exact for bf16 values down to 2^-29 of
 // the row's largest, and within 2^-39 of it below.  They are read as fragments of B: for a chunk, a tile of 8 rows and two steps 2 p, 2 p + 1, lane 4 n + t

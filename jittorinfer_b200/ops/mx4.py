@@ -1,9 +1,15 @@
 """Microscaled 4-bit floating point: tensors, weights laid out for the products, and the operators over them.
 
 A value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) times the power of two that its block of 32 columns shares (E8M0, a
-byte less 127; 255 makes the block NaN).  Activations stay bf16 (or fp32) in ``mx4_linear``, ``mx4_gateup`` and the MoE layers;
+byte less 127; 255 makes the block NaN).  Activations are bf16 (or fp32) in ``mx4_linear``, ``mx4_gateup`` and the MoE layers;
 ``mx4_matmul`` multiplies two 4-bit operands.  CUDA tensors go to the kernels in ``csrc/kernels/mx4*.cu``, CPU tensors to plain PyTorch; fp32
 activations are multiplied in fp32.
+
+What the kernels do to bf16 activations.  Tiled products take them as two planes of 8 bits: a value is exact down to 2^-11 of the largest magnitude among its
+32 columns and within 2^-21 of that below.  Layers of up to 8 tokens take them as fp16 scaled by a power of two: exact down to 2^-29 of a row's
+largest magnitude and within 2^-39 of it below; hidden units have 11 bits each, and sixteen neighbours that are all below 2^-24 of a token's largest in an
+expert count as 0.  Sums are fp32.
+A row with an infinity or NaN gives results that are not finite, and no other row's.
 """
 from __future__ import annotations
 
@@ -324,9 +330,11 @@ def _moe_plain(x, residual, ids, wts, wgu, wd, act):
 
 def mx4_moe_ffn(x: torch.Tensor, residual: Optional[torch.Tensor], ids: torch.Tensor, wts: torch.Tensor, wgu: Mx4Weight, wd: Mx4Weight,
                 act: str = "silu") -> torch.Tensor:
-    """residual + sum over the choices of a token of wts * down(act(gate) * up), x's dtype; the hidden units are rounded to x's dtype.
+    """residual + sum over the choices of a token of wts * down(act(gate) * up), x's dtype.
 
-    ``ids`` int32, ``wts`` fp32 [tokens, k]; an id outside the experts counts for nothing.  ``residual`` may be None.  Up to 8 bf16 tokens run as two launches."""
+    ``ids`` int32, ``wts`` fp32 [tokens, k]; an id outside the experts counts for nothing, its weight neither.  ``residual`` may be None.  Up to 8 bf16 tokens
+    run as two launches, unless weights lie more than 27 binades below the largest scale of their row.  More tokens' hidden units and each expert's result
+    before the weighted sum are rounded to x's dtype."""
     _check_moe(x, wgu, wd, residual, act, "mx4_moe_ffn")
     if ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape != wts.shape or ids.dtype != torch.int32 or wts.dtype != torch.float32 or \
             ids.device != x.device or wts.device != x.device:
@@ -339,7 +347,8 @@ def mx4_moe_layer(x: torch.Tensor, w_router: torch.Tensor, bias: Optional[torch.
                   sigmoid: bool, wgu: Mx4Weight, wd: Mx4Weight, n_shared: int = 0, group_top2: bool = False,
                   residual: Optional[torch.Tensor] = None, act: str = "silu") -> torch.Tensor:
     """A whole MoE layer: router, choice of experts, their products, weighted sum and residual.  The gate's arguments are those of ``moe_gate``; the
-    last ``n_shared`` experts of the weights take every token with weight 1.  Up to 8 bf16 tokens run as two launches."""
+    last ``n_shared`` experts of the weights take every token with weight 1.  On the GPU at most 32 choices, shared ones among them, of 256 experts in 32
+    groups.  Launches and roundings as in ``mx4_moe_ffn``."""
     _check_moe(x, wgu, wd, residual, act, "mx4_moe_layer")
     E = w_router.shape[0] if w_router.dim() == 2 else -1
     if w_router.dim() != 2 or w_router.shape[1] != x.shape[1] or E + n_shared != wgu.batch or n_shared < 0 or w_router.dtype != torch.float32 or \
